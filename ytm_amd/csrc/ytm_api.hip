@@ -83,11 +83,16 @@ namespace {
 
 thread_local std::string g_error;
 
-int fail(int code, const std::string& msg) {
+}  // namespace
+
+int ytm::fail(int code, const std::string& msg) {
   if (code == YTM_EHIP) (void)hipGetLastError();  // or this thread's next launch would report it again
   g_error = msg;
   return code;
 }
+using ytm::fail;
+
+namespace {
 
 // Waits for stream s; a failure is not left for this thread's next launch to report.
 hipError_t settle(hipStream_t s) {

@@ -11,6 +11,9 @@
 
 namespace ytm {
 
+// Records a failure of this thread for ytm_last_error and returns its status code.
+int fail(int code, const std::string& msg);
+
 // Device memory of the current device, kept between calls (ytm_memory.hip).  Blocks come with
 // whatever they held before; a block is freed once nothing on the GPU uses it any more.
 hipError_t pool_alloc(void** p, size_t bytes);
