@@ -41,7 +41,11 @@ enum {
     YTM_DTYPE_I32 = 5,
     YTM_DTYPE_I64 = 6,
     YTM_DTYPE_F32 = 7,
-    YTM_DTYPE_F64 = 8
+    YTM_DTYPE_F64 = 8,
+    /* of the answering operators alone: */
+    YTM_DTYPE_F16 = 9,
+    YTM_DTYPE_BF16 = 10,
+    YTM_DTYPE_BITS = 11 /* uint32 words, bit b of word j = clause 32 j + b */
 };
 
 /* Model hyperparameters, resolved on the host exactly as src/cutm/base.py:60-121,129-152
@@ -263,6 +267,61 @@ int ytm_get_bias(ytm_model *m, float *out);
 int ytm_binarize(const void *X, int x_dtype, int64_t n, const void *thresholds, int int_thresholds, int nthr,
                  int kind, int edge_bins, uint32_t *out);
 int ytm_collapse_bins(const uint32_t *B, int64_t rows, int64_t width, int kind, int edge_bins, int64_t *out);
+
+/* ---- From clause outputs to an answer (not in the reference): class sums through weights
+ * held in 4 bits, scores shaped by history, bias and grammar, and the choice of an answer.
+ *
+ * Unlike the calls above these take DEVICE pointers and put their work on `stream` (a
+ * hipStream_t of the current device, NULL the default one) without waiting for it: what they
+ * read must stay until the stream has passed, and results are there once it has.  They allocate
+ * nothing and may be captured into a graph.  Rows may be any distance apart (strides in
+ * elements, of codes in bytes); a row's elements follow one another.  Their errors are those
+ * of their arguments and of the launch.  Sums are made in f32 and rounded once; results do not
+ * depend on the order in which blocks run.
+ *
+ * ytm_readout: out[n][o] = sum over clauses c of x[n][c] * value(code[o][c]) * scale[o][c / group]
+ * for N rows (at most 65535), C clauses and K outputs.  x: YTM_DTYPE_BITS (clause outputs,
+ * (N, ceil(C/32)) words; bits past C are ignored), F32, F16 or BF16 (N, C).  codes: E2M1 floats (codes 0..7
+ * are 0, 0.5, 1, 1.5, 2, 3, 4, 6; 8..15 their negatives), two a byte, the even clause in the
+ * low half, 16 ceil(C/32) bytes an output, each output's at a multiple of 16 bytes (codes
+ * past C are ignored).  scales: (K, ceil(C/group)), group a multiple of 32.  scales and out: F32, F16 or
+ * BF16.  workspace: device memory of ytm_readout_workspace's bytes at a multiple of 16 bytes,
+ * for the time of the call's work (NULL where that is 0). */
+int ytm_readout_workspace(int x_dtype, int64_t N, int64_t C, int64_t K, int64_t *bytes);
+int ytm_readout(const void *x, int x_dtype, int64_t x_stride, int64_t N, int64_t C, const uint8_t *codes,
+                int64_t code_stride, const void *scales, int scale_dtype, int64_t scale_stride, int64_t group,
+                int64_t K, void *out, int out_dtype, int64_t out_stride, void *workspace, int64_t workspace_bytes,
+                void *stream);
+
+/* ytm_adjust_scores: for row n (at most 65535 rows) and answer v of V (at most 8388608), with h
+ * the first lengths[n] (NULL: T) entries of tokens[n] (N, T), c the number of h's entries from
+ * prompt[n] on (NULL: 0) that are v:
+ *   s = score; if v is in h: s = s > 0 ? s / repetition[n] : s * repetition[n];
+ *   s = s - frequency[n] * c - presence[n] * (c > 0); s = s + bias[v];
+ *   s = -inf if bit v % 32 of allowed word v / 32 is 0.
+ * Entries outside 0..V-1 stand for no answer.  Anything NULL is left out; bias_stride or
+ * allowed_stride 0: one row for all.  A lengths[n] above T counts as T.  scores and out: F32,
+ * F16 or BF16, each its own; out may be scores itself. */
+int ytm_adjust_scores(const void *scores, int dtype, int64_t stride, int64_t N, int64_t V, const int32_t *tokens,
+                      int64_t token_stride, int64_t T, const int32_t *lengths, const int32_t *prompt,
+                      const float *repetition, const float *frequency, const float *presence, const float *bias,
+                      int64_t bias_stride, const uint32_t *allowed, int64_t allowed_stride, void *out, int out_dtype,
+                      int64_t out_stride, void *stream);
+
+/* ytm_choose: one of V (at most 8388608) answers for each row.  With z = score / temperature[n]
+ * (NULL: 1; 0 or less: temperature 1 and top_k 1; a NaN score counts as -inf, +inf as the
+ * largest float) and the answers in the order of z descending, then index ascending, the filters keep
+ * a first part of that order, the first answer always among it:
+ *   min_p: z >= max z + log(min_p[n]);  top_k: the first top_k[n] of these (0 or less: all);
+ *   top_p: of these, with masses exp(z - max z), those before which less than top_p[n] of the mass
+ *   stands (1 or more: all).
+ * tokens[n] = the index of the largest z + noise[n][v] (NULL: of z) of the kept answers, the
+ * lowest of equal ones, and logprobs[n] = z of it - log of the kept answers' sum of exp(z).
+ * With standard Gumbel noise -log(-log(u)) that is a draw from softmax(z) over the kept
+ * answers.  Noise is finite.  -1 and -inf where no score is above -inf. */
+int ytm_choose(const void *scores, int dtype, int64_t stride, int64_t N, int64_t V, const float *temperature,
+               const int32_t *top_k, const float *top_p, const float *min_p, const float *noise, int64_t noise_stride,
+               int32_t *tokens, float *logprobs, void *stream);
 
 #ifdef __cplusplus
 }

@@ -98,7 +98,16 @@ SIGNATURES = {
     "ytm_binarize": (ctypes.c_int, [_P, ctypes.c_int, _I64, _P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                     _P]),
     "ytm_collapse_bins": (ctypes.c_int, [_P, _I64, _I64, ctypes.c_int, ctypes.c_int, _P]),
+    "ytm_readout_workspace": (ctypes.c_int, [ctypes.c_int, _I64, _I64, _I64, ctypes.POINTER(_I64)]),
+    "ytm_readout": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _I64, _P, ctypes.c_int, _I64, _I64, _I64, _P,
+                                   ctypes.c_int, _I64, _P, _I64, _P]),
+    "ytm_adjust_scores": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P,
+                                         _I64, _P, _I64, _P, ctypes.c_int, _I64, _P]),
+    "ytm_choose": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P]),
 }
+
+# Element types of the answering operators (YTM_DTYPE_* of include/ytm.h).
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_BITS = 7, 9, 10, 11
 
 # Element types of ytm_binarize (YTM_DTYPE_* of include/ytm.h).
 DTYPES = {"uint8": 0, "int8": 1, "uint16": 2, "int16": 3, "uint32": 4, "int32": 5, "int64": 6, "float32": 7,
