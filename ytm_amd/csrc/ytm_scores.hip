@@ -107,6 +107,18 @@ hipError_t launch_adjust_out(int out_dtype, const AdjustArgs& a, int64_t N, hipS
 // order, ended by a cut, the last answer kept.  The answer drawn is the largest z + noise of the
 // kept ones.  Masses exp(z - max) are whole numbers of 2^-40, so that sums in any order are the
 // same; 2^23 of them stay below 2^63.
+//
+// A block takes a row.  What it needs of the row depends on the filters:
+//  - none: one pass, a running maximum and sum of exponentials beside the largest z + noise;
+//  - top_k up to kMaxSeek: the k-th largest of the threads' own maxima over a part of the row is
+//    no larger than the k-th largest score, so the scores that reach it hold the first k; they
+//    go to a list in LDS in the one pass over the row and are sorted there, and everything else
+//    (min_p, top_p, the noise) looks at the list alone;
+//  - min_p without top_k: the same with the bound that the row's maximum gives, after a pass for it;
+//  - otherwise: a histogram of counts and masses over max - z finds the slice of 1/64 in which the
+//    cut lies, and that slice's answers, sorted, the cut;
+//  - where a list overflows (thousands of equal scores): the cut's key eight bits at a time, from
+//    histograms over the whole row.
 struct ChooseArgs {
   const void* scores;
   int64_t stride;
@@ -120,10 +132,18 @@ struct ChooseArgs {
   float* logprobs;
 };
 
+typedef unsigned long long u64;
+
 constexpr int kChooseThreads = 1024;
 constexpr int kChooseWaves = kChooseThreads / kWave;
 constexpr int kDigits = 256;
 constexpr float kMass = 1099511627776.0f;  // 2^40
+constexpr int kPack = 8;                   // scores a thread takes at once
+constexpr int kRound = kPack * kChooseThreads;
+constexpr int kList = 4096;
+constexpr int kMaxSeek = 256;  // a quarter of the threads, so that few maxima share a thread
+constexpr int kBins = 2048;
+constexpr float kBinsPerUnit = 64.0f;
 
 // Floats as whole numbers of the same order (no -0.0, no NaN).
 __device__ __forceinline__ uint32_t key_of(float z) {
@@ -135,19 +155,44 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 constexpr uint32_t kNone = 0x007FFFFFu;  // key of -inf
 
+__device__ __forceinline__ float scaled(float score, float t) {
+  const float z = score / t;
+  return (z != z ? -INFINITY : fminf(z, FLT_MAX)) + 0.0f;
+}
+
 template <typename In>
 struct Row {
   const In* in;
   float t;
-  __device__ __forceinline__ float operator()(int i) const {
-    float z = to_float(in[i]) / t;
-    z = z != z ? -INFINITY : fminf(z, FLT_MAX);
-    return z + 0.0f;
-  }
+  __device__ __forceinline__ float operator()(int i) const { return scaled(to_float(in[i]), t); }
 };
 
-__device__ __forceinline__ unsigned long long mass_of(float z, float best) {
-  return (unsigned long long)(expf(z - best) * kMass);
+__device__ __forceinline__ u64 mass_of(float z, float best) { return (u64)(expf(z - best) * kMass); }
+
+__device__ __forceinline__ u64 drawn_of(float z, int i, const float* noise) {
+  float y = noise ? z + noise[i] : z;
+  y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
+  return (u64)key_of(y) << 32 | (uint32_t)~i;
+}
+
+// kPack elements from in[i], -inf past V.  Rows start anywhere; the loads need no alignment.
+template <typename In>
+__device__ __forceinline__ void load_pack(const In* in, int i, int V, float past, float (&v)[kPack]) {
+  if (i + kPack <= V) {
+    In raw[kPack];
+    __builtin_memcpy(raw, in + i, sizeof raw);
+#pragma unroll
+    for (int j = 0; j < kPack; ++j) v[j] = to_float(raw[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPack; ++j) v[j] = i + j < V ? to_float(in[i + j]) : past;
+  }
+}
+__device__ __forceinline__ float most(const float (&v)[kPack]) {  // NaN only where all are
+  float m = v[0];
+#pragma unroll
+  for (int j = 1; j < kPack; ++j) m = fmaxf(m, v[j]);
+  return m;
 }
 
 // The last answer kept: all of a larger key are, and of its own key those up to its index.
@@ -158,16 +203,21 @@ struct Cut {
 };
 
 struct ChooseShared {
-  unsigned long long hist[kDigits];
-  unsigned long long part[kChooseWaves];
-  unsigned long long above, in;
+  u64 list[kList];
+  u64 mass[kBins];
+  uint32_t count[kBins];
+  u64 part[kChooseWaves];
+  double sums[kChooseWaves];
+  float tops[kChooseWaves];
+  u64 above, in;
+  uint32_t listed;
   int digit;
   int found;
 };
 
-__device__ __forceinline__ unsigned long long block_max(unsigned long long v, ChooseShared& sh) {
+__device__ __forceinline__ u64 block_max(u64 v, ChooseShared& sh) {
   for (int d = 32; d; d >>= 1) {
-    const unsigned long long o = __shfl_xor(v, d);
+    const u64 o = __shfl_xor(v, d);
     v = o > v ? o : v;
   }
   __syncthreads();
@@ -177,7 +227,7 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long v, Ch
   return v;
 }
 
-__device__ __forceinline__ unsigned long long block_sum(unsigned long long v, ChooseShared& sh) {
+__device__ __forceinline__ u64 block_sum(u64 v, ChooseShared& sh) {
   for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
   __syncthreads();
   if (threadIdx.x % kWave == 0) sh.part[threadIdx.x / kWave] = v;
@@ -185,6 +235,49 @@ __device__ __forceinline__ unsigned long long block_sum(unsigned long long v, Ch
   v = 0;
   for (int w = 0; w < kChooseWaves; ++w) v += sh.part[w];
   return v;
+}
+
+// Sum of the v of this thread and those before it.
+__device__ __forceinline__ u64 block_upto(u64 v, ChooseShared& sh) {
+  for (int d = 1; d < kWave; d <<= 1) {
+    const u64 o = __shfl_up(v, d);
+    if ((int)(threadIdx.x % kWave) >= d) v += o;
+  }
+  __syncthreads();
+  if (threadIdx.x % kWave == kWave - 1) sh.part[threadIdx.x / kWave] = v;
+  __syncthreads();
+  for (int w = 0; w < (int)threadIdx.x / kWave; ++w) v += sh.part[w];
+  return v;
+}
+
+// The first wave finds the highest bin at which the bins from the top on (bin 0 first where
+// RISING), after `before`, reach `target`; sh.digit is it or -1, sh.above what comes before it,
+// sh.in what it holds.
+template <int BINS, bool RISING, typename T>
+__device__ __forceinline__ void find_bin(const T* bins, u64 before, u64 target, ChooseShared& sh) {
+  __syncthreads();
+  if (threadIdx.x < kWave) {
+    constexpr int kEach = BINS / kWave;
+    const auto at = [&](int j) { return (u64)bins[RISING ? j : BINS - 1 - j]; };
+    u64 own = 0;
+    for (int j = 0; j < kEach; ++j) own += at(kEach * threadIdx.x + j);
+    u64 upto = own;
+    for (int d = 1; d < kWave; d <<= 1) {
+      const u64 o = __shfl_up(upto, d);
+      if ((int)threadIdx.x >= d) upto += o;
+    }
+    const u64 reached = __ballot(before + upto >= target);
+    if (threadIdx.x == 0) sh.digit = -1;
+    if (reached && (int)threadIdx.x == __ffsll(reached) - 1) {
+      u64 sum = before + upto - own;
+      int j = kEach * threadIdx.x;
+      while (sum + at(j) < target) sum += at(j++);
+      sh.digit = RISING ? j : BINS - 1 - j;
+      sh.above = sum;
+      sh.in = at(j);
+    }
+  }
+  __syncthreads();
 }
 
 // Index of the r-th (from 1) answer of key `key`, in index order.
@@ -195,7 +288,7 @@ __device__ int tie_index(const Row<In>& row, int V, uint32_t key, int r, ChooseS
   for (int first = 0; first < V; first += kChooseThreads) {
     const int i = first + threadIdx.x;
     const bool tie = i < V && key_of(row(i)) == key;
-    const unsigned long long mine = __ballot(tie);
+    const u64 mine = __ballot(tie);
     __syncthreads();
     if (threadIdx.x % kWave == 0) sh.part[threadIdx.x / kWave] = __popcll(mine);
     __syncthreads();
@@ -216,57 +309,385 @@ __device__ int tie_index(const Row<In>& row, int V, uint32_t key, int r, ChooseS
 // weighed, reach `target`; leaves it where they never do.  The key is found eight bits at a time
 // from a histogram.
 template <bool MASS, typename In>
-__device__ void raise_cut(const Row<In>& row, int V, float best, unsigned long long target, Cut& cut,
-                          ChooseShared& sh) {
+__device__ void raise_cut(const Row<In>& row, int V, float best, u64 target, Cut& cut, ChooseShared& sh) {
   uint32_t prefix = 0u, mask = 0u;
-  unsigned long long above = 0;
+  u64 above = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < kDigits; i += kChooseThreads) sh.hist[i] = 0;
+    for (int i = threadIdx.x; i < kDigits; i += kChooseThreads) sh.mass[i] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < V; i += kChooseThreads) {
       const float z = row(i);
       const uint32_t key = key_of(z);
       if (cut.keeps(key, i) && (key & mask) == prefix)
-        atomicAdd(&sh.hist[key >> shift & 255u], MASS ? mass_of(z, best) : 1ull);
+        atomicAdd(&sh.mass[key >> shift & 255u], MASS ? mass_of(z, best) : 1ull);
     }
-    __syncthreads();
-    if (threadIdx.x < kWave) {  // lane l takes the digits 255 - 4 l and the three below
-      unsigned long long own = 0;
-      for (int j = 0; j < 4; ++j) own += sh.hist[kDigits - 1 - 4 * threadIdx.x - j];
-      unsigned long long upto = own;
-      for (int d = 1; d < kWave; d <<= 1) {
-        const unsigned long long o = __shfl_up(upto, d);
-        if ((int)threadIdx.x >= d) upto += o;
-      }
-      const unsigned long long reached = __ballot(above + upto >= target);
-      if (threadIdx.x == 0) sh.digit = -1;
-      if (reached && (int)threadIdx.x == __ffsll(reached) - 1) {
-        unsigned long long sum = above + upto - own;
-        int j = kDigits - 1 - 4 * threadIdx.x;
-        while (sum + sh.hist[j] < target) sum += sh.hist[j--];
-        sh.digit = j;
-        sh.above = sum;
-        sh.in = sh.hist[j];
-      }
-    }
-    __syncthreads();
+    find_bin<kDigits, false>(sh.mass, above, target, sh);
     if (sh.digit < 0) return;
     above = sh.above;
     prefix |= (uint32_t)sh.digit << shift;
     mask |= 255u << shift;
   }
   // `above` comes before the answers of key `prefix`, which have `in` together
-  const unsigned long long need = target - above;
-  const unsigned long long each = MASS ? mass_of(value_of(prefix), best) : 1ull;
-  const unsigned long long in = sh.in;
+  const u64 need = target - above;
+  const u64 each = MASS ? mass_of(value_of(prefix), best) : 1ull;
+  const u64 in = sh.in;
   int last = prefix == cut.key ? cut.last : V - 1;
   if (each && need + each <= in) {  // some of them are left out
-    const unsigned long long r = (need + each - 1) / each;
+    const u64 r = (need + each - 1) / each;
     last = tie_index(row, V, prefix, (int)(r < 1 ? 1 : r), sh);
   }
   cut.key = prefix;
   cut.last = last;
   __syncthreads();
+}
+
+// target of a cut by mass: the first answer at which masses add up to it is the last kept.
+__device__ __forceinline__ u64 share_of(float p, u64 total) {
+  const double target = ceil((double)p * (double)total);
+  return target > 1.0 ? (u64)target : 1ull;
+}
+
+__device__ __forceinline__ void answer(const ChooseArgs& a, int64_t n, u64 drawn, float z, float best, u64 mass) {
+  if (threadIdx.x == 0) {
+    a.tokens[n] = (int)~(uint32_t)drawn;
+    a.logprobs[n] = (z - best) - logf((float)mass * (1.0f / kMass));
+  }
+}
+__device__ __forceinline__ void no_answer(const ChooseArgs& a, int64_t n) {
+  if (threadIdx.x == 0) {
+    a.tokens[n] = -1;
+    a.logprobs[n] = -INFINITY;
+  }
+}
+
+// Sorts list[0 .. size) (size a power of two from 128 on) descending.  A wave's pairs at
+// distances up to 64 lie in 128 places of its own, so the block waits only at longer ones.
+__device__ __forceinline__ void sort_list(u64* list, int size) {
+  for (int k = 2; k <= size; k <<= 1)
+    for (int j = k >> 1; j; j >>= 1) {
+      if (j >= kWave || j == k >> 1) __syncthreads();
+      for (int p = threadIdx.x; p < size / 2; p += kChooseThreads) {
+        const int i = 2 * p - (p & (j - 1));
+        const u64 x = list[i], y = list[i + j];
+        if ((x < y) == ((i & k) == 0)) {
+          list[i] = y;
+          list[i + j] = x;
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  __syncthreads();
+}
+
+// Sorts the list's `count` entries (descending; zeros follow them).
+__device__ __forceinline__ void order_list(int count, ChooseShared& sh) {
+  int size = 2 * kWave;
+  while (size < count) size <<= 1;
+  __syncthreads();
+  for (int i = count + threadIdx.x; i < size; i += kChooseThreads) sh.list[i] = 0;
+  sort_list(sh.list, size);
+}
+
+__device__ __forceinline__ void put(u64 entry, ChooseShared& sh) {
+  const uint32_t at = atomicAdd(&sh.listed, 1u);
+  if (at < kList) sh.list[at] = entry;
+}
+
+// The answer from a list (of key of score, ~index) that holds every answer the filters may keep.
+__device__ void from_list(const ChooseArgs& a, int64_t n, int count, float t, int k, ChooseShared& sh) {
+  for (int i = threadIdx.x; i < count; i += kChooseThreads) {
+    const u64 e = sh.list[i];
+    sh.list[i] = (u64)key_of(scaled(value_of((uint32_t)(e >> 32)), t)) << 32 | (uint32_t)e;
+  }
+  order_list(count, sh);
+  const uint32_t top = (uint32_t)(sh.list[0] >> 32);
+  if (count == 0 || top <= kNone) return no_answer(a, n);
+  const float best = value_of(top);
+  uint32_t least = kNone + 1u;
+  if (a.min_p && a.min_p[n] > 0.0f) {
+    const float z = best + logf(a.min_p[n]);
+    const uint32_t key = key_of((z <= best ? z : best) + 0.0f);
+    if (key > least) least = key;
+  }
+  if (k > 0 && k < count) count = k;
+  const float p = a.top_p ? a.top_p[n] : 1.0f;
+  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
+  u64 total = 0, drawn = 0, sum = 0;
+  for (int i = threadIdx.x; i < count; i += kChooseThreads) {
+    const uint32_t key = (uint32_t)(sh.list[i] >> 32);
+    if (key >= least) total += mass_of(value_of(key), best);
+  }
+  total = block_sum(total, sh);
+  const u64 target = p >= 1.0f ? ~0ull : share_of(p, total);
+  u64 before = 0;
+  for (int first = 0; first < count; first += kChooseThreads) {
+    const int i = first + threadIdx.x;
+    const u64 e = i < count ? sh.list[i] : 0;
+    const uint32_t key = (uint32_t)(e >> 32);
+    const u64 mass = key >= least ? mass_of(value_of(key), best) : 0;
+    const u64 upto = before + block_upto(mass, sh);
+    if (key >= least && (upto - mass < target || i == 0)) {
+      sum += mass;
+      const u64 d = drawn_of(value_of(key), (int)~(uint32_t)e, noise);
+      drawn = d > drawn ? d : drawn;
+    }
+    if (first + kChooseThreads < count) {  // what this round holds
+      __syncthreads();
+      if (threadIdx.x == kChooseThreads - 1) sh.above = upto;
+      __syncthreads();
+      before = sh.above;
+    }
+  }
+  sum = block_sum(sum, sh);
+  drawn = block_max(drawn, sh);
+  const int at = (int)~(uint32_t)drawn;
+  // z of the answer drawn: its noise taken off again would not be exact
+  for (int i = threadIdx.x; i < count; i += kChooseThreads)
+    if ((uint32_t)~sh.list[i] == (uint32_t)at) sh.tops[0] = value_of((uint32_t)(sh.list[i] >> 32));
+  __syncthreads();
+  answer(a, n, drawn, sh.tops[0], best, sum);
+}
+
+// Every answer may be drawn.  Sums are kept in double: a float's would lose what many small terms
+// add up to.
+template <typename In>
+__device__ void from_all(const ChooseArgs& a, int64_t n, const Row<In>& row, ChooseShared& sh) {
+  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
+  float top = -INFINITY;
+  double sum = 0.0;
+  u64 drawn = 0;
+  for (int i = kPack * threadIdx.x; i < a.V; i += kRound) {
+    float z[kPack], g[kPack];
+    load_pack(row.in, i, a.V, -INFINITY, z);
+    if (noise) load_pack(noise, i, a.V, 0.0f, g);
+    float here = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kPack; ++j) {
+      z[j] = scaled(z[j], row.t);
+      here = fmaxf(here, z[j]);
+    }
+    if (here > top) {
+      sum *= (double)expf(top - here);  // 0 the first time
+      top = here;
+    }
+    if (top == -INFINITY) continue;
+    float part = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPack; ++j) {
+      part += expf(z[j] - top);
+      float y = noise ? z[j] + g[j] : z[j];
+      y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
+      const u64 d = z[j] > -INFINITY ? (u64)key_of(y) << 32 | (uint32_t)~(i + j) : 0;
+      drawn = d > drawn ? d : drawn;
+    }
+    sum += (double)part;
+  }
+  for (int d = 32; d; d >>= 1) {
+    const float o = __shfl_xor(top, d);
+    const double s = __shfl_xor(sum, d);
+    const float m = fmaxf(top, o);
+    if (m > -INFINITY) sum = sum * (double)expf(top - m) + s * (double)expf(o - m);
+    top = m;
+  }
+  if (threadIdx.x % kWave == 0) {
+    sh.tops[threadIdx.x / kWave] = top;
+    sh.sums[threadIdx.x / kWave] = sum;
+  }
+  drawn = block_max(drawn, sh);  // waits for the others' too
+  if (drawn == 0) return no_answer(a, n);
+  float best = -INFINITY;
+  for (int w = 0; w < kChooseWaves; ++w) best = fmaxf(best, sh.tops[w]);
+  sum = 0.0;
+  for (int w = 0; w < kChooseWaves; ++w) sum += sh.sums[w] * (double)expf(sh.tops[w] - best);
+  if (threadIdx.x == 0) {
+    const int i = (int)~(uint32_t)drawn;
+    a.tokens[n] = i;
+    a.logprobs[n] = (row(i) - best) - logf((float)sum);
+  }
+}
+
+// The cut from histograms over max - z; false where a slice holds more than the list.
+template <typename In>
+__device__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, float best, int k, float p, Cut cut,
+                          ChooseShared& sh) {
+  const auto bin_of = [&](float z) { return (int)fminf((best - z) * kBinsPerUnit, (float)(kBins - 1)); };
+  for (int i = threadIdx.x; i < kBins; i += kChooseThreads) {
+    sh.mass[i] = 0;
+    sh.count[i] = 0;
+  }
+  __syncthreads();
+  for (int i = kPack * threadIdx.x; i < a.V; i += kRound) {
+    float v[kPack];
+    load_pack(row.in, i, a.V, -INFINITY, v);
+#pragma unroll
+    for (int j = 0; j < kPack; ++j) {
+      const float z = scaled(v[j], row.t);
+      if (key_of(z) < cut.key) continue;
+      const int b = bin_of(z);
+      atomicAdd(&sh.mass[b], mass_of(z, best));
+      atomicAdd(&sh.count[b], 1u);
+    }
+  }
+  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
+  u64 total = 0;  // of what top_k leaves
+  u64 drawn = 0, sum = 0;
+  int listed = -1, count = 0;  // the slice in the list
+  // puts the answers of slice b into the list in their order, and the largest z + noise of those before it
+  // into `drawn`
+  const auto gather = [&](int b) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    drawn = 0;
+    for (int i = kPack * threadIdx.x; i < a.V; i += kRound) {
+      float v[kPack];
+      load_pack(row.in, i, a.V, -INFINITY, v);
+#pragma unroll
+      for (int j = 0; j < kPack; ++j) {
+        const float z = scaled(v[j], row.t);
+        if (key_of(z) < cut.key) continue;
+        const int at = bin_of(z);
+        if (at == b) put((u64)key_of(z) << 32 | (uint32_t)~(i + j), sh);
+        if (at < b) {
+          const u64 d = drawn_of(z, i + j, noise);
+          drawn = d > drawn ? d : drawn;
+        }
+      }
+    }
+    __syncthreads();
+    listed = b;
+    count = (int)sh.listed;
+    order_list(count, sh);
+  };
+  // the number of the list's first answers whose masses reach `target` (all where they never do), and their sum
+  const auto upto = [&](int most_, u64 target) {
+    u64 before = 0;
+    int kept = 0;
+    sum = 0;
+    for (int first = 0; first < most_; first += kChooseThreads) {
+      const int i = first + threadIdx.x;
+      const u64 mass = i < most_ ? mass_of(value_of((uint32_t)(sh.list[i] >> 32)), best) : 0;
+      const u64 up = before + block_upto(mass, sh);
+      const bool keep = i < most_ && (up - mass < target || i == 0);
+      kept += (int)block_sum(keep ? 1 : 0, sh);
+      sum += block_sum(keep ? mass : 0, sh);
+      before += block_sum(mass, sh);
+    }
+    return kept;
+  };
+  int kept = 0;  // of the list
+  u64 above = 0;
+  int end = kBins;  // slices from here on are left out
+  find_bin<kBins, true>(sh.count, 0, k > 0 ? (u64)k : ~0ull, sh);
+  if (sh.digit >= 0) {
+    end = sh.digit;
+    if (sh.in > kList) return false;
+    const int r = k - (int)sh.above;
+    gather(end);
+    u64 m = 0;
+    for (int i = threadIdx.x; i < end; i += kChooseThreads) m += sh.mass[i];
+    above = block_sum(m, sh);
+    kept = upto(r, ~0ull);
+    total = above + sum;
+  } else {
+    u64 m = 0;
+    for (int i = threadIdx.x; i < kBins; i += kChooseThreads) m += sh.mass[i];
+    total = block_sum(m, sh);
+  }
+  if (p < 1.0f) {
+    const u64 target = share_of(p, total);
+    find_bin<kBins, true>(sh.mass, 0, target, sh);
+    const int b = sh.digit;
+    if (b >= 0 && b < end) {  // in a slice that top_k leaves whole
+      above = sh.above;
+      if (sh.count[b] > kList) return false;
+      gather(b);
+      kept = upto(count, target - above);
+    } else if (listed >= 0) {
+      kept = upto(kept, target - above);
+    }
+  }
+  if (listed < 0) {  // nothing is cut off
+    gather(kBins);
+    above = total;
+    sum = 0;
+  }
+  for (int i = threadIdx.x; i < kept; i += kChooseThreads) {
+    const u64 e = sh.list[i];
+    const u64 d = drawn_of(value_of((uint32_t)(e >> 32)), (int)~(uint32_t)e, noise);
+    drawn = d > drawn ? d : drawn;
+  }
+  drawn = block_max(drawn, sh);
+  answer(a, n, drawn, row((int)~(uint32_t)drawn), best, above + sum);
+  return true;
+}
+
+// Passes over the whole row for each step: right for every row, and what is left for lists
+// that overflow.
+template <typename In>
+__device__ void from_row(const ChooseArgs& a, int64_t n, const Row<In>& row, float best, int k, float p, Cut cut,
+                         ChooseShared& sh) {
+  const int V = a.V;
+  if (k > 0 && k < V) raise_cut<false>(row, V, best, (u64)k, cut, sh);
+  if (p < 1.0f) {
+    u64 m = 0;
+    for (int i = threadIdx.x; i < V; i += kChooseThreads) {
+      const float z = row(i);
+      if (cut.keeps(key_of(z), i)) m += mass_of(z, best);
+    }
+    raise_cut<true>(row, V, best, share_of(p, block_sum(m, sh)), cut, sh);
+  }
+  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
+  u64 m = 0, drawn = 0;
+  for (int i = threadIdx.x; i < V; i += kChooseThreads) {
+    const float z = row(i);
+    if (!cut.keeps(key_of(z), i)) continue;
+    m += mass_of(z, best);
+    const u64 d = drawn_of(z, i, noise);
+    drawn = d > drawn ? d : drawn;
+  }
+  m = block_sum(m, sh);
+  drawn = block_max(drawn, sh);
+  answer(a, n, drawn, row((int)~(uint32_t)drawn), best, m);
+}
+
+// A score from which on z may equal that of one at `score`: two scores' quotients by t are
+// equal only within a rounding of them, below the smallest normal float or at the largest.
+__device__ __forceinline__ float with_equals(float score, float t) {
+  score = fminf(score, FLT_MAX);
+  const float lower = score - fabsf(score) * 0x1p-22f - t * 0x1p-124f;
+  return t < 1.0f ? fminf(lower, FLT_MAX * t * (1.0f - 0x1p-20f)) : lower;
+}
+
+// Lists the row's scores from `least` on (those above -inf); whether they fit.
+template <typename In>
+__device__ bool list_from(const In* in, int V, float least, ChooseShared& sh) {
+  __syncthreads();
+  if (threadIdx.x == 0) sh.listed = 0;
+  __syncthreads();
+  for (int i = kPack * threadIdx.x; i < V; i += kRound) {
+    float v[kPack];
+    load_pack(in, i, V, -INFINITY, v);
+    if (!(most(v) >= least)) continue;
+#pragma unroll
+    for (int j = 0; j < kPack; ++j)
+      if (v[j] >= least && v[j] > -INFINITY) put((u64)key_of(v[j] + 0.0f) << 32 | (uint32_t)~(i + j), sh);
+  }
+  __syncthreads();
+  return sh.listed <= kList;
+}
+
+// The threads' maxima over the row's first `rounds` rounds.
+template <typename In>
+__device__ float own_most(const In* in, int V, int rounds) {
+  float top = -INFINITY;
+  const int end = V < (int64_t)rounds * kRound ? V : rounds * kRound;
+  for (int i = kPack * threadIdx.x; i < end; i += kRound) {
+    float v[kPack];
+    load_pack(in, i, V, -INFINITY, v);
+    top = fmaxf(top, most(v));
+  }
+  return top;
 }
 
 template <typename In>
@@ -280,55 +701,43 @@ __global__ __launch_bounds__(kChooseThreads) void choose_kernel(ChooseArgs a) {
     t = 1.0f;
     k = 1;
   }
+  if (k >= V) k = 0;
+  const float p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
+  const bool bounded = a.min_p && a.min_p[n] > 0.0f;
   const Row<In> row{(const In*)a.scores + n * a.stride, t};
-  unsigned long long v = 0;
-  for (int i = threadIdx.x; i < V; i += kChooseThreads) {
-    const unsigned long long key = key_of(row(i));
-    v = key > v ? key : v;
-  }
-  const uint32_t top = (uint32_t)block_max(v, sh);
-  if (top <= kNone) {
-    if (threadIdx.x == 0) {
-      a.tokens[n] = -1;
-      a.logprobs[n] = -INFINITY;
+  if (k <= 0 && p >= 1.0f && !bounded) return from_all(a, n, row, sh);
+  if (k > 0 && k <= kMaxSeek) {
+    const int rounds = (V + kRound - 1) / kRound;
+    const uint32_t own = key_of(own_most(row.in, V, (rounds + 3) / 4) + 0.0f);
+    // the upper 16 bits of the k-th largest
+    uint32_t prefix = 0u;
+    u64 above = 0;
+    for (int shift = 24; shift >= 16; shift -= 8) {
+      for (int i = threadIdx.x; i < kDigits; i += kChooseThreads) sh.count[i] = 0;
+      __syncthreads();
+      if (shift == 24 || own >> 24 == prefix >> 24) atomicAdd(&sh.count[own >> shift & 255u], 1u);
+      find_bin<kDigits, false>(sh.count, above, (u64)k, sh);
+      prefix |= (uint32_t)sh.digit << shift;
+      above = sh.above;
+      __syncthreads();
     }
-    return;
+    if (list_from(row.in, V, prefix > kNone ? with_equals(value_of(prefix), t) : -INFINITY, sh))
+      return from_list(a, n, (int)sh.listed, t, k, sh);
   }
-  const float best = value_of(top);
+  const float own = own_most(row.in, V, (V + kRound - 1) / kRound);
+  const float best = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), t);
+  if (best == -INFINITY) return no_answer(a, n);
   Cut cut{kNone + 1u, V - 1};
-  if (a.min_p && a.min_p[n] > 0.0f) {
+  if (bounded) {
     const float least = best + logf(a.min_p[n]);
     const uint32_t key = key_of((least <= best ? least : best) + 0.0f);
     if (key > cut.key) cut.key = key;
+    if (k <= 0 && list_from(row.in, V, with_equals(least * t, t), sh))
+      return from_list(a, n, (int)sh.listed, t, k, sh);
   }
-  if (k > 0 && k < V) raise_cut<false>(row, V, best, (unsigned long long)k, cut, sh);
-  if (a.top_p && !(a.top_p[n] >= 1.0f)) {
-    unsigned long long m = 0;
-    for (int i = threadIdx.x; i < V; i += kChooseThreads) {
-      const float z = row(i);
-      if (cut.keeps(key_of(z), i)) m += mass_of(z, best);
-    }
-    const double target = ceil((double)a.top_p[n] * (double)block_sum(m, sh));
-    raise_cut<true>(row, V, best, target > 1.0 ? (unsigned long long)target : 1ull, cut, sh);
-  }
-  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
-  unsigned long long m = 0, drawn = 0;
-  for (int i = threadIdx.x; i < V; i += kChooseThreads) {
-    const float z = row(i);
-    if (!cut.keeps(key_of(z), i)) continue;
-    m += mass_of(z, best);
-    float y = noise ? z + noise[i] : z;
-    y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
-    const unsigned long long w = (unsigned long long)key_of(y) << 32 | (uint32_t)~i;
-    drawn = w > drawn ? w : drawn;
-  }
-  m = block_sum(m, sh);
-  drawn = block_max(drawn, sh);
-  if (threadIdx.x == 0) {
-    const int i = (int)~(uint32_t)drawn;
-    a.tokens[n] = i;
-    a.logprobs[n] = (row(i) - best) - logf((float)m * (1.0f / kMass));
-  }
+  if ((k > 0 || p < 1.0f) && from_bins(a, n, row, best, k, p, cut, sh)) return;
+  __syncthreads();
+  from_row(a, n, row, best, k, p, cut, sh);
 }
 
 }  // namespace
