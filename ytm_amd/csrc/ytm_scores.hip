@@ -175,19 +175,52 @@ __device__ __forceinline__ u64 drawn_of(float z, int i, const float* noise) {
   return (u64)key_of(y) << 32 | (uint32_t)~i;
 }
 
-// kPack elements from in[i], -inf past V.  Rows start anywhere; the loads need no alignment.
+// kPack elements of a row from element i on, as they are in memory: loads that need no alignment
+// and no branch, so that several are on their way at once.  A pack that would pass the row's end
+// V is taken from V - kPack, and the elements before i are not its own.
 template <typename In>
-__device__ __forceinline__ void load_pack(const In* in, int i, int V, float past, float (&v)[kPack]) {
-  if (i + kPack <= V) {
-    In raw[kPack];
-    __builtin_memcpy(raw, in + i, sizeof raw);
+struct Pack {
+  In raw[kPack];
+  __device__ __forceinline__ int load(const In* in, int i, int V) {
+    const int at = i + kPack <= V ? i : V - kPack;
+    if (V >= kPack) {
+      __builtin_memcpy(raw, in + at, sizeof raw);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPack; ++j) raw[j] = at + j >= 0 ? in[at + j] : In{};
+    }
+    return at;
+  }
+  // the elements as floats, `past` for those not the pack's own
+  __device__ __forceinline__ void values(int i, int at, float past, float (&v)[kPack]) const {
 #pragma unroll
     for (int j = 0; j < kPack; ++j) v[j] = to_float(raw[j]);
-  } else {
+    if (at != i) {
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) v[j] = i + j < V ? to_float(in[i + j]) : past;
+      for (int j = 0; j < kPack; ++j) v[j] = at + j >= i && at + j >= 0 ? v[j] : past;
+    }
+  }
+};
+
+// f(first index, values) for this thread's packs of elements 0 .. end - 1, -inf where there are
+// none; `end` the row's length V or a multiple of kRound.  U packs are loaded before the first is
+// looked at.
+template <int U, typename In, typename F>
+__device__ __forceinline__ void each_pack(const In* in, int V, int end, F f) {
+  for (int first = kPack * threadIdx.x; first < end; first += U * kRound) {
+    Pack<In> pack[U];
+    int at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) at[u] = pack[u].load(in, first + u * kRound, V);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[kPack];
+      pack[u].values(first + u * kRound, at[u], -INFINITY, v);
+      f(at[u], v);
+    }
   }
 }
+
 __device__ __forceinline__ float most(const float (&v)[kPack]) {  // NaN only where all are
   float m = v[0];
 #pragma unroll
@@ -260,6 +293,7 @@ __device__ __forceinline__ void find_bin(const T* bins, u64 before, u64 target, 
     constexpr int kEach = BINS / kWave;
     const auto at = [&](int j) { return (u64)bins[RISING ? j : BINS - 1 - j]; };
     u64 own = 0;
+#pragma unroll 4
     for (int j = 0; j < kEach; ++j) own += at(kEach * threadIdx.x + j);
     u64 upto = own;
     for (int d = 1; d < kWave; d <<= 1) {
@@ -282,7 +316,7 @@ __device__ __forceinline__ void find_bin(const T* bins, u64 before, u64 target, 
 
 // Index of the r-th (from 1) answer of key `key`, in index order.
 template <typename In>
-__device__ int tie_index(const Row<In>& row, int V, uint32_t key, int r, ChooseShared& sh) {
+__device__ __forceinline__ int tie_index(const Row<In>& row, int V, uint32_t key, int r, ChooseShared& sh) {
   int seen = 0;
   if (threadIdx.x == 0) sh.found = V - 1;
   for (int first = 0; first < V; first += kChooseThreads) {
@@ -309,7 +343,7 @@ __device__ int tie_index(const Row<In>& row, int V, uint32_t key, int r, ChooseS
 // weighed, reach `target`; leaves it where they never do.  The key is found eight bits at a time
 // from a histogram.
 template <bool MASS, typename In>
-__device__ void raise_cut(const Row<In>& row, int V, float best, u64 target, Cut& cut, ChooseShared& sh) {
+__device__ __forceinline__ void raise_cut(const Row<In>& row, int V, float best, u64 target, Cut& cut, ChooseShared& sh) {
   uint32_t prefix = 0u, mask = 0u;
   u64 above = 0;
   for (int shift = 24; shift >= 0; shift -= 8) {
@@ -394,7 +428,7 @@ __device__ __forceinline__ void put(u64 entry, ChooseShared& sh) {
 }
 
 // The answer from a list (of key of score, ~index) that holds every answer the filters may keep.
-__device__ void from_list(const ChooseArgs& a, int64_t n, int count, float t, int k, ChooseShared& sh) {
+__device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, int count, float t, int k, ChooseShared& sh) {
   for (int i = threadIdx.x; i < count; i += kChooseThreads) {
     const u64 e = sh.list[i];
     sh.list[i] = (u64)key_of(scaled(value_of((uint32_t)(e >> 32)), t)) << 32 | (uint32_t)e;
@@ -451,36 +485,47 @@ __device__ void from_list(const ChooseArgs& a, int64_t n, int count, float t, in
 // Every answer may be drawn.  Sums are kept in double: a float's would lose what many small terms
 // add up to.
 template <typename In>
-__device__ void from_all(const ChooseArgs& a, int64_t n, const Row<In>& row, ChooseShared& sh) {
+__device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const Row<In>& row, ChooseShared& sh) {
   const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
   float top = -INFINITY;
   double sum = 0.0;
   u64 drawn = 0;
-  for (int i = kPack * threadIdx.x; i < a.V; i += kRound) {
-    float z[kPack], g[kPack];
-    load_pack(row.in, i, a.V, -INFINITY, z);
-    if (noise) load_pack(noise, i, a.V, 0.0f, g);
-    float here = -INFINITY;
+  for (int first = kPack * threadIdx.x; first < a.V; first += 2 * kRound) {
+    Pack<In> score[2];
+    Pack<float> more[2];
+    int at[2];
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) {
-      z[j] = scaled(z[j], row.t);
-      here = fmaxf(here, z[j]);
+    for (int u = 0; u < 2; ++u) {
+      at[u] = score[u].load(row.in, first + u * kRound, a.V);
+      if (noise) more[u].load(noise, first + u * kRound, a.V);
     }
-    if (here > top) {
-      sum *= (double)expf(top - here);  // 0 the first time
-      top = here;
-    }
-    if (top == -INFINITY) continue;
-    float part = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) {
-      part += expf(z[j] - top);
-      float y = noise ? z[j] + g[j] : z[j];
-      y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
-      const u64 d = z[j] > -INFINITY ? (u64)key_of(y) << 32 | (uint32_t)~(i + j) : 0;
-      drawn = d > drawn ? d : drawn;
+    for (int u = 0; u < 2; ++u) {
+      float z[kPack], g[kPack];
+      score[u].values(first + u * kRound, at[u], -INFINITY, z);
+      if (noise) more[u].values(first + u * kRound, at[u], 0.0f, g);
+      float here = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kPack; ++j) {
+        z[j] = scaled(z[j], row.t);
+        here = fmaxf(here, z[j]);
+      }
+      if (here > top) {
+        sum *= (double)expf(top - here);  // 0 the first time
+        top = here;
+      }
+      if (top == -INFINITY) continue;
+      float part = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kPack; ++j) {
+        part += expf(z[j] - top);
+        float y = noise ? z[j] + g[j] : z[j];
+        y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
+        const u64 d = z[j] > -INFINITY ? (u64)key_of(y) << 32 | (uint32_t)~(at[u] + j) : 0;
+        drawn = d > drawn ? d : drawn;
+      }
+      sum += (double)part;
     }
-    sum += (double)part;
   }
   for (int d = 32; d; d >>= 1) {
     const float o = __shfl_xor(top, d);
@@ -508,7 +553,7 @@ __device__ void from_all(const ChooseArgs& a, int64_t n, const Row<In>& row, Cho
 
 // The cut from histograms over max - z; false where a slice holds more than the list.
 template <typename In>
-__device__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, float best, int k, float p, Cut cut,
+__device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, float best, int k, float p, Cut cut,
                           ChooseShared& sh) {
   const auto bin_of = [&](float z) { return (int)fminf((best - z) * kBinsPerUnit, (float)(kBins - 1)); };
   for (int i = threadIdx.x; i < kBins; i += kChooseThreads) {
@@ -516,9 +561,7 @@ __device__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, fl
     sh.count[i] = 0;
   }
   __syncthreads();
-  for (int i = kPack * threadIdx.x; i < a.V; i += kRound) {
-    float v[kPack];
-    load_pack(row.in, i, a.V, -INFINITY, v);
+  each_pack<2>(row.in, a.V, a.V, [&](int, float(&v)[kPack]) {
 #pragma unroll
     for (int j = 0; j < kPack; ++j) {
       const float z = scaled(v[j], row.t);
@@ -527,7 +570,7 @@ __device__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, fl
       atomicAdd(&sh.mass[b], mass_of(z, best));
       atomicAdd(&sh.count[b], 1u);
     }
-  }
+  });
   const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
   u64 total = 0;  // of what top_k leaves
   u64 drawn = 0, sum = 0;
@@ -539,9 +582,7 @@ __device__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, fl
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     drawn = 0;
-    for (int i = kPack * threadIdx.x; i < a.V; i += kRound) {
-      float v[kPack];
-      load_pack(row.in, i, a.V, -INFINITY, v);
+    each_pack<2>(row.in, a.V, a.V, [&](int i, float(&v)[kPack]) {
 #pragma unroll
       for (int j = 0; j < kPack; ++j) {
         const float z = scaled(v[j], row.t);
@@ -553,7 +594,7 @@ __device__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, fl
           drawn = d > drawn ? d : drawn;
         }
       }
-    }
+    });
     __syncthreads();
     listed = b;
     count = (int)sh.listed;
@@ -625,7 +666,7 @@ __device__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, fl
 // Passes over the whole row for each step: right for every row, and what is left for lists
 // that overflow.
 template <typename In>
-__device__ void from_row(const ChooseArgs& a, int64_t n, const Row<In>& row, float best, int k, float p, Cut cut,
+__device__ __forceinline__ void from_row(const ChooseArgs& a, int64_t n, const Row<In>& row, float best, int k, float p, Cut cut,
                          ChooseShared& sh) {
   const int V = a.V;
   if (k > 0 && k < V) raise_cut<false>(row, V, best, (u64)k, cut, sh);
@@ -659,39 +700,72 @@ __device__ __forceinline__ float with_equals(float score, float t) {
   return t < 1.0f ? fminf(lower, FLT_MAX * t * (1.0f - 0x1p-20f)) : lower;
 }
 
-// Lists the row's scores from `least` on (those above -inf); whether they fit.
+// Lists the row's scores from `least` on (those above -inf) in an order of threads; whether they
+// fit.  A thread marks those of 16 packs in 128 bits, without a branch, and reads them again once
+// it knows its place in the list: few reach `least`.
 template <typename In>
-__device__ bool list_from(const In* in, int V, float least, ChooseShared& sh) {
-  __syncthreads();
-  if (threadIdx.x == 0) sh.listed = 0;
-  __syncthreads();
-  for (int i = kPack * threadIdx.x; i < V; i += kRound) {
-    float v[kPack];
-    load_pack(in, i, V, -INFINITY, v);
-    if (!(most(v) >= least)) continue;
+__device__ __forceinline__ bool list_from(const In* in, int V, float least, ChooseShared& sh) {
+  constexpr int kWords = 4, kPacks = 4;  // packs to a word of marks
+  uint32_t listed = 0;
+  least = fmaxf(least, -FLT_MAX);  // nothing where it is NaN: the largest is what is left of both
+  for (int start = 0; start < V; start += kWords * kPacks * kRound) {
+    uint32_t marks[kWords];
+    uint32_t own = 0;
 #pragma unroll
-    for (int j = 0; j < kPack; ++j)
-      if (v[j] >= least && v[j] > -INFINITY) put((u64)key_of(v[j] + 0.0f) << 32 | (uint32_t)~(i + j), sh);
+    for (int w = 0; w < kWords; ++w) {
+      const int first = start + w * kPacks * kRound + kPack * (int)threadIdx.x;
+      uint32_t m = 0;
+      if (first - kPack * (int)threadIdx.x < V) {
+        Pack<In> pack[kPacks];
+        int at[kPacks];
+#pragma unroll
+        for (int u = 0; u < kPacks; ++u) at[u] = pack[u].load(in, first + u * kRound, V);
+#pragma unroll
+        for (int u = 0; u < kPacks; ++u) {
+          float v[kPack];
+          pack[u].values(first + u * kRound, at[u], -INFINITY, v);
+#pragma unroll
+          for (int j = 0; j < kPack; ++j) m = m * 2 + (v[j] >= least ? 1u : 0u);
+        }
+      }
+      marks[w] = m;
+      own += __popc(m);
+    }
+    const uint32_t upto = (uint32_t)block_upto(own, sh);
+    uint32_t place = listed + upto - own;
+    __syncthreads();
+    if (threadIdx.x == kChooseThreads - 1) sh.listed = upto;
+    __syncthreads();
+    listed += sh.listed;
+    if (listed > kList) return false;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w)
+      for (uint32_t m = marks[w]; m;) {
+        const int b = __clz(m);  // pack b / kPack of the word, its element b % kPack
+        m &= ~(0x80000000u >> b);
+        const int i = start + (w * kPacks + b / kPack) * kRound + kPack * (int)threadIdx.x;
+        const int e = (i + kPack <= V ? i : V - kPack) + b % kPack;
+        sh.list[place++] = (u64)key_of(to_float(in[e]) + 0.0f) << 32 | (uint32_t)~e;
+      }
   }
   __syncthreads();
-  return sh.listed <= kList;
+  if (threadIdx.x == 0) sh.listed = listed;
+  __syncthreads();
+  return true;
 }
 
-// The threads' maxima over the row's first `rounds` rounds.
+// The largest of this thread's packs over the row's first `rounds` rounds.
 template <typename In>
-__device__ float own_most(const In* in, int V, int rounds) {
+__device__ __forceinline__ float own_most(const In* in, int V, int rounds) {
   float top = -INFINITY;
-  const int end = V < (int64_t)rounds * kRound ? V : rounds * kRound;
-  for (int i = kPack * threadIdx.x; i < end; i += kRound) {
-    float v[kPack];
-    load_pack(in, i, V, -INFINITY, v);
-    top = fmaxf(top, most(v));
-  }
+  each_pack<4>(in, V, V < (int64_t)rounds * kRound ? V : rounds * kRound,
+               [&](int, float(&v)[kPack]) { top = fmaxf(top, most(v)); });
   return top;
 }
 
 template <typename In>
-__global__ __launch_bounds__(kChooseThreads) void choose_kernel(ChooseArgs a) {
+__global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(4, 4))) void choose_kernel(
+    ChooseArgs a) {
   __shared__ ChooseShared sh;
   const int64_t n = blockIdx.x;
   const int V = a.V;

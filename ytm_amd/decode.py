@@ -27,6 +27,7 @@ import torch
 from ._lib import DTYPE_BF16, DTYPE_BITS, DTYPE_F16, DTYPE_F32, check, lib
 
 _FLOATS = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+_CLAUSES = {torch.int32: DTYPE_BITS, **_FLOATS}
 # E2M1 magnitudes of the codes 0..7, and the points between them
 _MAGNITUDES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], np.float32)
 _BETWEEN = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
@@ -80,67 +81,92 @@ def pack_outputs(outputs: np.ndarray, device: str | torch.device = "cuda") -> to
     return torch.from_numpy(packed.view("<i4")).to(device)
 
 
-def _operand(t, name: str, dims, device=None) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor):
+# Operators of a few microseconds: the checks are one condition each, and what is wrong is found out
+# where it fails.
+_Tensor = torch.Tensor
+_device_now = torch._C._cuda_getDevice
+_stream_of = torch._C._cuda_getCurrentRawStream
+
+
+def _refuse(t, name: str, dims: tuple, dtype, shape: str, device: int) -> None:
+    """Raises what is wrong with operand t (nothing where it only requires a gradient and none
+    is recorded)."""
+    if not isinstance(t, _Tensor):
         raise TypeError(f"{name} must be a torch tensor.")
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise ValueError(f"{name} must be on {'a GPU' if device is None else device}.")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a GPU.")
+    if device >= 0 and t.get_device() != device:
+        raise ValueError(f"{name} must be on cuda:{device}, not {t.device}.")
     if t.dim() not in dims:
         raise ValueError(f"{name} must have {' or '.join(map(str, dims))} dimensions.")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient; this operator has none.")
+    if dtype is not None and t.dtype not in (dtype if isinstance(dtype, (tuple, dict)) else (dtype,)):
+        names = dtype if isinstance(dtype, (tuple, dict)) else (dtype,)
+        raise TypeError(f"{name} must be {' or '.join(str(d).removeprefix('torch.') for d in names)}, not {t.dtype}.")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}'s rows must be contiguous.")
-    return t
+    if t.requires_grad:
+        if torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient; this operator has none.")
+    elif shape:
+        raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}.")
 
 
-def _float_type(t: torch.Tensor, name: str) -> int:
-    code = _FLOATS.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}.")
-    return code
+def _rows_of(t, name: str, types: dict) -> tuple[int, int, int, int]:
+    """(type code, rows, width, device) of an operator's first operand."""
+    if not (isinstance(t, _Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in types and not t.requires_grad
+            and (t.stride(1) == 1 or t.shape[1] < 2)):
+        _refuse(t, name, (2,), types, "", -1)
+    rows, width = t.shape
+    return types[t.dtype], rows, width, t.get_device()
 
 
-def _matrix(t, name: str, dtype: torch.dtype, rows: int, width: int, device) -> tuple[int | None, int]:
+def _matrix(t, name: str, dtype: torch.dtype, rows: int, width: int, device: int) -> tuple[int | None, int]:
     """(address, row stride; 0 for one row shared by all) of an optional operand (rows, width) or
     (width)."""
     if t is None:
         return None, 0
-    _operand(t, name, (1, 2), device)
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, not {t.dtype}.")
-    if t.shape[-1] != width or (t.dim() == 2 and t.shape[0] != rows):
-        raise ValueError(f"{name} must have shape ({rows}, {width}) or ({width},), not {tuple(t.shape)}.")
+    if isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == device and not t.requires_grad:
+        shape = t.shape
+        if shape == (rows, width):
+            if t.stride(1) == 1 or width < 2:
+                return t.data_ptr(), t.stride(0) if rows > 1 else 0
+        elif shape == (width,) and (t.stride(0) == 1 or width < 2):
+            return t.data_ptr(), 0
+    fits = isinstance(t, _Tensor) and tuple(t.shape) in ((rows, width), (width,))
+    _refuse(t, name, (1, 2), dtype, "" if fits else f"({rows}, {width}) or ({width},)", device)
     return t.data_ptr(), t.stride(0) if t.dim() == 2 and rows > 1 else 0
 
 
-def _per_row(t, name: str, dtype: torch.dtype, rows: int, device) -> int | None:
+def _per_row(t, name: str, dtype: torch.dtype, rows: int, device: int) -> int | None:
     if t is None:
         return None
-    _operand(t, name, (1,), device)
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, not {t.dtype}.")
-    if t.shape[0] != rows:
-        raise ValueError(f"{name} must have {rows} elements, not {t.shape[0]}.")
+    if not (isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == device and t.shape == (rows,)
+            and (t.stride(0) == 1 or rows < 2) and not t.requires_grad):
+        fits = isinstance(t, _Tensor) and tuple(t.shape) == (rows,)
+        _refuse(t, name, (1,), dtype, "" if fits else f"({rows},)", device)
     return t.data_ptr()
 
 
-def _result(out, name: str, shape: tuple[int, int], device) -> torch.Tensor:
+def _result(out, shape: tuple[int, int], device: int) -> tuple[torch.Tensor, int]:
+    """(the output tensor, its type code)"""
     if out is None:
-        return torch.empty(shape, dtype=torch.float32, device=device)
-    _operand(out, name, (2,), device)
-    if tuple(out.shape) != shape:
-        raise ValueError(f"{name} must have shape {shape}, not {tuple(out.shape)}.")
-    return out
+        return torch.empty(shape, dtype=torch.float32, device=torch.device("cuda", device)), DTYPE_F32
+    if not (isinstance(out, _Tensor) and out.get_device() == device and out.shape == shape and out.dtype in _FLOATS
+            and (out.stride(1) == 1 or shape[1] < 2) and not out.requires_grad):
+        fits = isinstance(out, _Tensor) and tuple(out.shape) == shape
+        _refuse(out, "out", (2,), _FLOATS, "" if fits else str(shape), device)
+    return out, _FLOATS[out.dtype]
 
 
-def _call(function, device: torch.device, *args) -> None:
+def _call(function, device: int, *args) -> None:
     """function(*args, current stream) with `device` current."""
-    if device.index == torch.cuda.current_device():
-        check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+    if device == _device_now():
+        rc = function(*args, _stream_of(device))
     else:
         with torch.cuda.device(device):
-            check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+            rc = function(*args, _stream_of(device))
+    if rc:
+        check(rc)
 
 
 def readout(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: int = 32, clauses: int | None = None,
@@ -150,39 +176,41 @@ def readout(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: i
     x: bits, int32 (N, ceil(C/32)) as pack_outputs gives them, C being `clauses` (default: every
     bit); or float32, float16 or bfloat16 (N, C), outputs averaged over models or patches.
     out: where the sums go, float32, float16 or bfloat16 (default: a new float32 tensor)."""
-    _operand(x, "x", (2,))
-    device = x.device
-    N, width = x.shape
-    if x.dtype == torch.int32:
-        x_type = DTYPE_BITS
+    x_type, N, width, device = _rows_of(x, "x", _CLAUSES)
+    if x_type == DTYPE_BITS:
         C = 32 * width if clauses is None else int(clauses)
-        if not -(-C // 32) == width:
+        if -(-C // 32) != width:
             raise ValueError(f"x must hold {-(-C // 32)} words of clause bits a row, not {width}.")
     else:
-        x_type = _float_type(x, "x")
         C = width
         if clauses is not None and int(clauses) != C:
             raise ValueError(f"x must have {clauses} columns, not {C}.")
-    _operand(codes, "codes", (2,), device)
-    _operand(scales, "scales", (2,), device)
-    if codes.dtype != torch.uint8:
-        raise TypeError("codes must be uint8.")
-    K, group = codes.shape[0], int(group)
+    group = int(group)
     if group < 32 or group % 32:
         raise ValueError("group must be a multiple of 32.")
-    if codes.shape[1] < 16 * -(-C // 32):
-        raise ValueError(f"codes must hold {16 * -(-C // 32)} bytes an output, not {codes.shape[1]}.")
-    if scales.shape[0] != K or scales.shape[1] != -(-C // group):
-        raise ValueError(f"scales must have shape ({K}, {-(-C // group)}), not {tuple(scales.shape)}.")
-    scale_type = _float_type(scales, "scales")
-    out = _result(out, "out", (N, K), device)
-    out_type = _float_type(out, "out")
+    if not (isinstance(codes, _Tensor) and codes.dtype is torch.uint8 and codes.get_device() == device
+            and codes.dim() == 2 and (codes.stride(1) == 1 or codes.shape[1] < 2)):
+        _refuse(codes, "codes", (2,), torch.uint8, "", device)
+    K, held = codes.shape
+    if held < 16 * -(-C // 32):
+        raise ValueError(f"codes must hold {16 * -(-C // 32)} bytes an output, not {held}.")
+    groups = -(-C // group)
+    if not (isinstance(scales, _Tensor) and scales.dtype in _FLOATS and scales.get_device() == device
+            and scales.shape == (K, groups) and (scales.stride(1) == 1 or groups < 2) and not scales.requires_grad):
+        fits = isinstance(scales, _Tensor) and tuple(scales.shape) == (K, groups)
+        _refuse(scales, "scales", (2,), _FLOATS, "" if fits else f"({K}, {groups})", device)
+    out, out_type = _result(out, (N, K), device)
     need = ctypes.c_int64()
-    check(lib.ytm_readout_workspace(x_type, N, C, K, ctypes.byref(need)))
-    workspace = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    rc = lib.ytm_readout_workspace(x_type, N, C, K, need)
+    if rc:
+        check(rc)
+    need = need.value
+    workspace = None
+    if need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
     _call(lib.ytm_readout, device, x.data_ptr(), x_type, x.stride(0), N, C, codes.data_ptr(), codes.stride(0),
-          scales.data_ptr(), scale_type, scales.stride(0), group, K, out.data_ptr(), out_type, out.stride(0),
-          None if workspace is None else workspace.data_ptr(), need.value)
+          scales.data_ptr(), _FLOATS[scales.dtype], scales.stride(0), group, K, out.data_ptr(), out_type,
+          out.stride(0), workspace.data_ptr() if need else None, need)
     return out
 
 
@@ -202,29 +230,26 @@ def adjust_scores(scores: torch.Tensor, tokens: torch.Tensor | None = None, leng
     where answer v may be given; the others get -inf, whatever their score.
     out: where the scores go, any of the three types, `scores` itself too (default: a new float32
     tensor)."""
-    _operand(scores, "scores", (2,))
-    device = scores.device
-    N, V = scores.shape
-    dtype = _float_type(scores, "scores")
+    dtype, N, V, device = _rows_of(scores, "scores", _FLOATS)
     T, said, token_stride = 0, None, 0
     if tokens is not None:
-        _operand(tokens, "tokens", (2,), device)
-        if tokens.dtype != torch.int32:
-            raise TypeError("tokens must be int32.")
-        if tokens.shape[0] != N:
-            raise ValueError(f"tokens must have {N} rows, not {tokens.shape[0]}.")
+        if not (isinstance(tokens, _Tensor) and tokens.dtype is torch.int32 and tokens.get_device() == device
+                and tokens.dim() == 2 and tokens.shape[0] == N and (tokens.stride(1) == 1 or tokens.shape[1] < 2)):
+            _refuse(tokens, "tokens", (2,), torch.int32, f"({N}, T)", device)
         T, said, token_stride = tokens.shape[1], tokens.data_ptr(), tokens.stride(0)
+        lengths = _per_row(lengths, "lengths", torch.int32, N, device)
+        prompt = _per_row(prompt, "prompt", torch.int32, N, device)
+        repetition = _per_row(repetition, "repetition", torch.float32, N, device)
+        frequency = _per_row(frequency, "frequency", torch.float32, N, device)
+        presence = _per_row(presence, "presence", torch.float32, N, device)
     elif not (lengths is None and prompt is None and repetition is None and frequency is None and presence is None):
         raise ValueError("lengths, prompt and penalties need tokens.")
-    bias_at, bias_stride = _matrix(bias, "bias", torch.float32, N, V, device)
-    allowed_at, allowed_stride = _matrix(allowed, "allowed", torch.int32, N, -(-V // 32), device)
-    out = _result(out, "out", (N, V), device)
+    bias, bias_stride = _matrix(bias, "bias", torch.float32, N, V, device)
+    allowed, allowed_stride = _matrix(allowed, "allowed", torch.int32, N, (V + 31) // 32, device)
+    out, out_type = _result(out, (N, V), device)
     _call(lib.ytm_adjust_scores, device, scores.data_ptr(), dtype, scores.stride(0), N, V, said, token_stride, T,
-          _per_row(lengths, "lengths", torch.int32, N, device), _per_row(prompt, "prompt", torch.int32, N, device),
-          _per_row(repetition, "repetition", torch.float32, N, device),
-          _per_row(frequency, "frequency", torch.float32, N, device),
-          _per_row(presence, "presence", torch.float32, N, device), bias_at, bias_stride, allowed_at, allowed_stride,
-          out.data_ptr(), _float_type(out, "out"), out.stride(0))
+          lengths, prompt, repetition, frequency, presence, bias, bias_stride, allowed, allowed_stride, out.data_ptr(),
+          out_type, out.stride(0))
     return out
 
 
@@ -238,16 +263,15 @@ def choose(scores: torch.Tensor, temperature: torch.Tensor | None = None, top_k:
     noise of these, the lowest of equal ones, the log probability that of a draw among them.
     noise: float32 (N, V) or (V,), finite; standard Gumbel draws -log(-log(u)) make the answer a
     draw, None the best one.  A row without a score above -inf gets -1 and -inf."""
-    _operand(scores, "scores", (2,))
-    device = scores.device
-    N, V = scores.shape
-    dtype = _float_type(scores, "scores")
-    noise_at, noise_stride = _matrix(noise, "noise", torch.float32, N, V, device)
-    tokens = torch.empty(N, dtype=torch.int32, device=device)
-    logprobs = torch.empty(N, dtype=torch.float32, device=device)
-    _call(lib.ytm_choose, device, scores.data_ptr(), dtype, scores.stride(0), N, V,
-          _per_row(temperature, "temperature", torch.float32, N, device),
-          _per_row(top_k, "top_k", torch.int32, N, device), _per_row(top_p, "top_p", torch.float32, N, device),
-          _per_row(min_p, "min_p", torch.float32, N, device), noise_at, noise_stride, tokens.data_ptr(),
-          logprobs.data_ptr())
+    dtype, N, V, device = _rows_of(scores, "scores", _FLOATS)
+    noise, noise_stride = _matrix(noise, "noise", torch.float32, N, V, device)
+    temperature = _per_row(temperature, "temperature", torch.float32, N, device)
+    top_k = _per_row(top_k, "top_k", torch.int32, N, device)
+    top_p = _per_row(top_p, "top_p", torch.float32, N, device)
+    min_p = _per_row(min_p, "min_p", torch.float32, N, device)
+    where = scores.device
+    tokens = torch.empty(N, dtype=torch.int32, device=where)
+    logprobs = torch.empty(N, dtype=torch.float32, device=where)
+    _call(lib.ytm_choose, device, scores.data_ptr(), dtype, scores.stride(0), N, V, temperature, top_k, top_p, min_p,
+          noise, noise_stride, tokens.data_ptr(), logprobs.data_ptr())
     return tokens, logprobs
