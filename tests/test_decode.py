@@ -80,7 +80,7 @@ def test_host_tensors_and_arrays_are_refused():
 # The C boundary refuses before anything is launched; addresses here are never read.
 P = 1 << 20
 READOUT = dict(x=P, x_dtype=7, x_stride=64, N=2, C=64, codes=P, code_stride=32, scales=P, scale_dtype=7, scale_stride=2,
-               group=32, K=3, out=P, out_dtype=7, out_stride=3, workspace=P, workspace_bytes=1 << 30, stream=None)
+               group=32, K=3, out=P, out_dtype=7, out_stride=3, workspace=None, workspace_bytes=0, stream=None)
 ADJUST = dict(scores=P, dtype=7, stride=8, N=2, V=8, tokens=P, token_stride=4, T=4, lengths=None, prompt=None,
               repetition=None, frequency=None, presence=None, bias=P, bias_stride=8, allowed=P, allowed_stride=1,
               out=P, out_dtype=7, out_stride=8, stream=None)
@@ -93,8 +93,11 @@ CHOOSE = dict(scores=P, dtype=7, stride=8, N=2, V=8, temperature=None, top_k=Non
         dict(x_dtype=8), dict(x_dtype=0), dict(scale_dtype=11), dict(out_dtype=11), dict(out_dtype=8), dict(N=-1),
         dict(N=65536), dict(C=-1), dict(K=-1), dict(C=1 << 31), dict(group=0), dict(group=16), dict(group=33),
         dict(x=None), dict(codes=None), dict(scales=None), dict(out=None), dict(codes=P + 8), dict(code_stride=40),
-        dict(code_stride=16), dict(scale_stride=1), dict(x_stride=63), dict(out_stride=2), dict(workspace=None),
-        dict(workspace_bytes=100), dict(workspace=P + 4))
+        dict(code_stride=16), dict(scale_stride=1), dict(x_stride=63), dict(out_stride=2),
+        dict(C=2097121, x_stride=1 << 30, code_stride=1 << 30, scale_stride=1 << 30), dict(K=(1 << 23) + 1, out_stride=1 << 24),
+        # a workspace that is missing, too small, at an odd address
+        *(dict(C=200000, x_stride=1 << 20, code_stride=1 << 20, scale_stride=1 << 20, **w) for w in (
+            {}, dict(workspace=P, workspace_bytes=100), dict(workspace=P + 2, workspace_bytes=1 << 30))))
 ] + [
     ("ytm_adjust_scores", ADJUST, w) for w in (
         dict(dtype=11), dict(out_dtype=8), dict(N=-1), dict(N=65536), dict(V=-1), dict(V=(1 << 23) + 1), dict(T=-1),
@@ -117,9 +120,11 @@ def test_nothing_to_do(function, base):
     assert getattr(_lib.lib, function)(*base.values()) == _lib.YTM_OK
 
 
-def test_workspace_refusals():
+def test_workspace():
     n = ctypes.c_int64(-1)
-    assert _lib.lib.ytm_readout_workspace(8, 1, 1, 1, ctypes.byref(n)) == _lib.YTM_EINVAL
-    assert _lib.lib.ytm_readout_workspace(7, -1, 1, 1, ctypes.byref(n)) == _lib.YTM_EINVAL
-    assert _lib.lib.ytm_readout_workspace(7, 1, 1, 1, None) == _lib.YTM_EINVAL
-    assert _lib.lib.ytm_readout_workspace(7, 0, 1, 1, ctypes.byref(n)) == _lib.YTM_OK and n.value == 0
+    ask = _lib.lib.ytm_readout_workspace
+    for wrong in ((8, 1, 1, 1, n), (7, -1, 1, 1, n), (7, 1, 2097121, 1, n), (7, 1, 1, -1, n), (7, 1, 1, 1, None)):
+        assert ask(*wrong) == _lib.YTM_EINVAL
+    for args in ((7, 0, 1000, 1), (7, 3, 0, 5), (7, 17, 100000, 10), (11, 1, 10000, 10000)):
+        assert ask(*args, n) == _lib.YTM_OK and n.value == 0
+    assert ask(7, 16, 20000, 10, n) == _lib.YTM_OK and n.value > 0

@@ -40,6 +40,9 @@ constexpr int64_t kDecodeRows = 65535;
 // Scores of a row: their masses, at most 2^40 each, add up below 2^63.
 constexpr int64_t kMaxScores = 1 << 23;
 
+// Clauses of a readout: fewer than 65536 steps of 32.
+constexpr int64_t kMaxClauses = 65535 * 32;
+
 inline bool decode_float(int dtype) {
   return dtype == YTM_DTYPE_F32 || dtype == YTM_DTYPE_F16 || dtype == YTM_DTYPE_BF16;
 }

@@ -1,5 +1,5 @@
 // ytm_readout.hip -- class sums from clause outputs through weights held in 4 bits: the entry
-// points ytm_readout and ytm_readout_workspace of include/ytm.h and their gfx950 kernels.
+// point ytm_readout of include/ytm.h and its gfx950 kernels.
 //
 //   out[n][o] = sum over groups q of scale[o][q] * sum over clauses c of q of x[n][c] value(code[o][c])
 //
@@ -11,7 +11,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <algorithm>
+#include <type_traits>
 
 #include "ytm_decode.h"
 #include "ytm_internal.h"
@@ -29,74 +29,116 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
 constexpr int kWave = 64;
-constexpr int kTile = 16;   // rows and outputs of a product
-constexpr int kStep = 32;   // clauses of a product
-constexpr int kChunk = 128; // clauses of a 16-byte load of codes by each lane
+constexpr int kTile = 16;    // rows and outputs of a product
+constexpr int kStep = 32;    // clauses of a product
+constexpr int kChunk = 128;  // clauses of a 16-byte load of codes by each lane, four products
+constexpr int kPieces = 16;  // of 8 clauses, in a chunk: a lane's part of a product's row operand
 
 struct ReadoutArgs {
   const void* x;
-  int x_dtype;
-  int64_t x_stride, N, C;
+  int64_t x_stride;
+  int N, C;
   const uint8_t* codes;
   int64_t code_stride;
   const void* scales;
-  int64_t scale_stride, group, K;
+  int scale_dtype;
+  int64_t scale_stride;
+  uint32_t inverse;  // (step + 1) * inverse >> 32 is the group of clauses 32 step ..
+  int K;
   void* out;
   int out_dtype;
   int64_t out_stride;
-  v4u* frag;
-  int64_t steps, row_tiles;
+  int chunks, part_chunks, out_tiles, row_tiles;
+  float* parts;
+};
+
+// What x is: its element, the number of 16-bit operands it is the sum of, whether these are float16.
+template <int X>
+struct Kind;
+template <>
+struct Kind<YTM_DTYPE_BITS> {
+  static constexpr int kPlanes = 1;
+  static constexpr bool kHalf = false;
+};
+template <>
+struct Kind<YTM_DTYPE_F16> {
+  static constexpr int kPlanes = 1;
+  static constexpr bool kHalf = true;
+};
+template <>
+struct Kind<YTM_DTYPE_BF16> {
+  static constexpr int kPlanes = 1;
+  static constexpr bool kHalf = false;
+};
+template <>
+struct Kind<YTM_DTYPE_F32> {
+  static constexpr int kPlanes = 3;
+  static constexpr bool kHalf = false;
 };
 
 // ------------------------------------------------------------------------------- row operands
-// The value of clause c in row n as float32 bits, whatever x's type.
-__device__ __forceinline__ float x_at(const ReadoutArgs& a, int64_t n, int64_t c) {
-  const int64_t i = n * a.x_stride;
-  switch (a.x_dtype) {
-    case YTM_DTYPE_BITS: return (float)(((const uint32_t*)a.x)[i + c / 32] >> (c % 32) & 1u);
-    case YTM_DTYPE_F16: return to_float(((const f16*)a.x)[i + c]);
-    case YTM_DTYPE_BF16: return to_float(((const bf16*)a.x)[i + c]);
-    default: return ((const float*)a.x)[i + c];
-  }
-}
-
-// Row operands frag[plane][step][row tile][lane], lane l holding 8 values (clauses 32 step +
-// 8 (l / 16) ...) of row l % 16, zero past the last clause or row.  Planes: one, or for float32
-// three whose sum it is, each cut (not rounded) to a bfloat16, so that nothing overflows; where
+// Eight clauses of a row as they are in memory, and as 16-bit operands: bits as 0 and 1, float32
+// as the sum of three bfloat16, each cut (not rounded) to one, so that nothing overflows; where
 // the first is infinite or NaN the others are zero.
-__global__ __launch_bounds__(256) void rows_kernel(ReadoutArgs a) {
-  const int64_t each = a.steps * a.row_tiles * kWave;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < each; i += (int64_t)gridDim.x * blockDim.x) {
-    const int l = (int)(i % kWave);
-    const int64_t n = i / kWave % a.row_tiles * kTile + l % 16;
-    const int64_t c0 = i / kWave / a.row_tiles * kStep + 8 * (l / 16);
-    v4u plane[3];
-    for (int p = 0; p < 3; ++p) plane[p] = v4u{0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float v = n < a.N && c0 + j < a.C ? x_at(a, n, c0 + j) : 0.0f;
-      const int sh = 16 * (j & 1);
-      if (a.x_dtype == YTM_DTYPE_F16) {
-        plane[0][j / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v) << sh;
-        continue;
-      }
-      const uint32_t hi = __float_as_uint(v) >> 16;
-      plane[0][j / 2] |= hi << sh;
-      if (a.x_dtype == YTM_DTYPE_F32 && (hi & 0x7F80u) != 0x7F80u) {
-        v -= __uint_as_float(hi << 16);
-        const uint32_t mid = __float_as_uint(v) >> 16;
-        plane[1][j / 2] |= mid << sh;
-        v -= __uint_as_float(mid << 16);
-        plane[2][j / 2] |= __float_as_uint(v) >> 16 << sh;
-      }
+template <int X>
+struct Piece {
+  v4u raw[X == YTM_DTYPE_F32 ? 2 : 1];
+
+  // clauses c .. c + 7 of row n; zero from clause C on
+  __device__ __forceinline__ void load(const ReadoutArgs& a, int n, int c) {
+    if (X == YTM_DTYPE_BITS) {
+      const uint32_t* words = (const uint32_t*)a.x + n * a.x_stride;
+      const uint32_t bits = c < a.C ? words[c / 32] >> (c % 32) & 255u : 0u;
+      raw[0][0] = a.C - c >= 8 ? bits : bits & ((1u << (a.C > c ? a.C - c : 0)) - 1u);
+      return;
     }
-    a.frag[i] = plane[0];
-    if (a.x_dtype == YTM_DTYPE_F32) {
-      a.frag[each + i] = plane[1];
-      a.frag[2 * each + i] = plane[2];
+    typedef typename std::conditional<X == YTM_DTYPE_F32, uint32_t, uint16_t>::type Bits;
+    const Bits* from = (const Bits*)a.x + n * a.x_stride + c;
+    if (c + 8 <= a.C) {
+      __builtin_memcpy(raw, from, sizeof raw);
+      return;
+    }
+    Bits e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = c + j < a.C ? from[j] : (Bits)0;
+    __builtin_memcpy(raw, e, sizeof raw);
+  }
+
+  __device__ __forceinline__ void operands(v4u (&plane)[Kind<X>::kPlanes]) const {
+    if (X == YTM_DTYPE_BITS) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t two = raw[0][0] >> (2 * q);
+        plane[0][q] = ((two & 1u) | (two & 2u) << 15) * 0x3F80u;  // 1.0 at either half
+      }
+      return;
+    }
+    if (X != YTM_DTYPE_F32) {
+      plane[0] = raw[0];
+      return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t part[3][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = 2 * q + h;
+        const uint32_t u = raw[j / 4 % (X == YTM_DTYPE_F32 ? 2 : 1)][j % 4];
+        const float v = __uint_as_float(u);
+        const uint32_t hi = u & 0xFFFF0000u;
+        const bool finite = (u & 0x7F800000u) != 0x7F800000u;
+        const float rest = finite ? v - __uint_as_float(hi) : 0.0f;
+        const uint32_t mid = __float_as_uint(rest) & 0xFFFF0000u;
+        part[0][h] = (u & 0x7FFFFFFFu) > 0x7F800000u ? u | 0x00400000u : u;  // a NaN stays one
+        part[1][h] = mid;
+        part[2][h] = __float_as_uint(rest - __uint_as_float(mid));
+      }
+#pragma unroll
+      for (int p = 0; p < Kind<X>::kPlanes; ++p)
+        plane[p][q] = __builtin_amdgcn_perm(part[p][1], part[p][0], 0x07060302u);
     }
   }
-}
+};
 
 // ------------------------------------------------------------------------------------ products
 template <bool HALF>
@@ -123,18 +165,63 @@ __device__ __forceinline__ v4f product(v4u x, v4u w, v4f d) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x), __builtin_bit_cast(v8bf, w), d, 0, 0, 0);
 }
 
-// A lane of group g = l / 16 holds codes of clauses 32 g .. 32 g + 31 in four words; after this
-// word s holds those of clauses 32 s + 8 g ..., so that a product's clauses are 32 in a row and
-// belong to one scale.  A 4 x 4 transposition in two exchanges of bits of (group, word).
+// A lane of group g = l / 16 holds a chunk's clauses 32 g .. 32 g + 31 in four words of codes, and
+// a product takes one word of each lane.  Where a scale holds for the whole chunk (GRAIN 128),
+// product s takes word s as it is: clauses 32 g + 8 s .., the row operands' alike.  Where it does
+// not (GRAIN 32), the words are exchanged first so that product s has clauses 32 s + 8 g ..:
+// a 4 x 4 transposition in two exchanges of bits of (group, word).
+template <int GRAIN>
 __device__ __forceinline__ v4u turn(v4u w) {
+  if (GRAIN == kChunk) return w;
   auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
   auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
   auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
   auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
   return v4u{c[0], c[1], d[0], d[1]};
 }
+// (step, lane group) of piece i (clauses 8 i ..) of a chunk, as 4 step + group.
+template <int GRAIN>
+__device__ __forceinline__ int place_of(int i) {
+  return GRAIN == kChunk ? 4 * (i % 4) + i / 4 : i;
+}
 
-__device__ __forceinline__ void store_out(const ReadoutArgs& a, int64_t n, int64_t o, float v) {
+// A chunk's codes of one output a lane, and a scale: that of the whole chunk (GRAIN 128), or of the
+// 32 clauses whose codes the lane holds, which turn() then hands to all.
+template <int GRAIN>
+struct Codes {
+  v4u w;
+  uint32_t scale;
+
+  // Chunks past the last take what the first holds: their rows are zero.
+  __device__ __forceinline__ void load(const ReadoutArgs& a, const uint8_t* codes, const char* scales, int chunk) {
+    const int g = threadIdx.x % kWave / 16;
+    const int at = chunk * (kChunk / 2) + g * 16;
+    const bool in = at < (a.C + 31) / 32 * 16;
+    w = *(const v4u*)(codes + (in ? at : 0));
+    const uint32_t step = (uint32_t)chunk * 4 + (GRAIN == kChunk ? 0 : g);
+    const uint32_t q = in || GRAIN == kChunk && chunk < a.chunks ? __umulhi(step + 1, a.inverse) : 0u;
+    if (a.scale_dtype == YTM_DTYPE_F32)
+      scale = ((const uint32_t*)scales)[q];
+    else
+      scale = ((const uint16_t*)scales)[q];
+  }
+  // scales of the four products
+  __device__ __forceinline__ void scaled(const ReadoutArgs& a, float (&f)[4]) const {
+    float v;
+    if (a.scale_dtype == YTM_DTYPE_F32)
+      v = __uint_as_float(scale);
+    else if (a.scale_dtype == YTM_DTYPE_BF16)
+      v = __uint_as_float(scale << 16);
+    else
+      v = (float)__builtin_bit_cast(_Float16, (uint16_t)scale);
+    const uint32_t u = __float_as_uint(v);
+    const v4u t = turn<GRAIN>(v4u{u, u, u, u});
+#pragma unroll
+    for (int s = 0; s < 4; ++s) f[s] = __uint_as_float(t[s]);
+  }
+};
+
+__device__ __forceinline__ void store_out(const ReadoutArgs& a, int n, int o, float v) {
   const int64_t i = n * a.out_stride + o;
   switch (a.out_dtype) {
     case YTM_DTYPE_F16: ((f16*)a.out)[i] = from_float<f16>(v); break;
@@ -143,86 +230,324 @@ __device__ __forceinline__ void store_out(const ReadoutArgs& a, int64_t n, int64
   }
 }
 
-// A block of four waves per tile of 16 outputs and 16 rows, the clauses split among the waves
-// chunk by chunk and their sums joined in LDS in the waves' order.  Lane l takes the codes of
-// output l % 16 as the second operand and gets sums of rows 4 (l / 16) .. + 3 of that output.
-// GRAIN: clauses after which sums are scaled, 32, 64 or 128, a divisor of the group.
-constexpr int kWaves = 4;
-template <int PLANES, bool HALF, int GRAIN, typename Scale>
-__global__ __launch_bounds__(kWaves* kWave) void readout_kernel(ReadoutArgs a) {
-  __shared__ v4f sums[kWaves][kWave];
-  const int l = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t o = blockIdx.x * (int64_t)kTile + l % 16;
-  const int64_t tile = blockIdx.y;
-  const bool real = o < a.K;
-  const uint8_t* codes = a.codes + (real ? o : 0) * a.code_stride;
-  const Scale* scales = (const Scale*)a.scales + (real ? o : 0) * a.scale_stride;
-  const int64_t bytes = (a.C + 31) / 32 * 16, chunks = (a.C + kChunk - 1) / kChunk;
-  const int64_t each = a.steps * a.row_tiles * kWave;
-  v4f total = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t t = wave; t < chunks; t += kWaves) {
-    const int64_t at = t * 64 + l / 16 * 16;
-    v4u w = {0u, 0u, 0u, 0u};
-    if (at < bytes) w = *(const v4u*)(codes + at);
-    w = turn(w);
-    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+// A chunk's products of NT row tiles, whose operands lie at from[((plane * steps + step) * stride + tile) *
+// kWave], and OB output tiles, added to the sums so far.
+template <int X, int GRAIN, int NT, int OB>
+__device__ __forceinline__ void add_chunk(const ReadoutArgs& a, const Codes<GRAIN> (&code)[OB], const v4u* from,
+                                          int plane, int step, int tile, v4f (&total)[NT][OB]) {
+  constexpr int kPlanes = Kind<X>::kPlanes;
+  constexpr bool kHalf = Kind<X>::kHalf;
+  v4u w[OB];
+  float scale[OB][4];
+  v4f sum[NT][OB];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int64_t c = t * kChunk + s * kStep;
-      if (c < a.C) {
-        const v4u b = codes_to_16<HALF>(w[s]);
-        const v4u* frag = a.frag + ((t * 4 + s) * a.row_tiles + tile) * kWave + l;
+  for (int b = 0; b < OB; ++b) {
+    w[b] = turn<GRAIN>(code[b].w);
+    code[b].scaled(a, scale[b]);
+  }
 #pragma unroll
-        for (int p = PLANES - 1; p >= 0; --p) sum = product<HALF>(frag[p * each], b, sum);
-        if ((s + 1) * kStep % GRAIN == 0 || c + kStep >= a.C) {
-          const float scale = to_float(scales[c / a.group]);
+  for (int s = 0; s < 4; ++s) {
+    v4u x[kPlanes][NT];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            total[r] += scale * sum[r];
-            sum[r] = 0.0f;
-          }
-        }
+    for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) x[p][n] = from[p * plane + s * step + n * tile];
+#pragma unroll
+    for (int b = 0; b < OB; ++b) {
+      const v4u y = codes_to_16<kHalf>(w[b][s]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (s * kStep % GRAIN == 0) sum[n][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int p = kPlanes - 1; p >= 0; --p) sum[n][b] = product<kHalf>(x[p][n], y, sum[n][b]);
       }
     }
-  }
-  sums[wave][l] = total;
-  __syncthreads();
-  if (wave == 0) {
-    for (int w = 1; w < kWaves; ++w) total += sums[w][l];
-    for (int r = 0; r < 4; ++r) {
-      const int64_t n = tile * kTile + l / 16 * 4 + r;
-      if (real && n < a.N) store_out(a, n, o, total[r]);
+    if ((s + 1) * kStep % GRAIN == 0) {
+#pragma unroll
+      for (int b = 0; b < OB; ++b)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) total[n][b][r] = __builtin_fmaf(scale[b][s], sum[n][b][r], total[n][b][r]);
     }
   }
 }
 
-int planes_of(int x_dtype) { return x_dtype == YTM_DTYPE_F32 ? 3 : 1; }
-int64_t steps_of(int64_t C) { return (C + kStep - 1) / kStep; }
-int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
+// Many rows: a block takes 16 NT RW rows and 16 OB WO outputs; its waves are WK groups, each with
+// chunks of clauses of its own, of WO x RW waves, each with NT tiles of rows and OB of outputs.  Lane l takes
+// the codes of output l % 16 as a product's second operand and gets sums of rows 4 (l / 16) .. + 3
+// of that output.  A group keeps a chunk of its rows' operands in LDS; the next chunk is in
+// registers or on its way, and the one after it is asked for before the products of this one, as
+// are the codes.  The groups' sums are joined in LDS in their order.
+template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
+__global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) {
+  constexpr int kPlanes = Kind<X>::kPlanes;
+  constexpr int kGroupThreads = kWave * RW * WO;
+  constexpr int kTiles = NT * RW;               // of rows
+  constexpr int kFrags = kPlanes * 4 * kTiles;  // operands of a buffer
+  constexpr int kEach = kPieces * kTile * kTiles / kGroupThreads;  // pieces a thread loads
+  static_assert(kPieces * kTile * kTiles % kGroupThreads == 0, "");
+  constexpr int kJoin = (WK - 1) * RW * WO * NT * OB;
+  __shared__ v4u lds[(2 * WK * kFrags > kJoin ? 2 * WK * kFrags : kJoin) * kWave];
 
-template <int PLANES, bool HALF, int GRAIN>
-void launch_scale(const ReadoutArgs& a, int scale_dtype, hipStream_t s) {
-  const dim3 grid((unsigned)tiles_of(a.K), (unsigned)a.row_tiles);
-  switch (scale_dtype) {
-    case YTM_DTYPE_F16: readout_kernel<PLANES, HALF, GRAIN, f16><<<grid, kWaves * kWave, 0, s>>>(a); break;
-    case YTM_DTYPE_BF16: readout_kernel<PLANES, HALF, GRAIN, bf16><<<grid, kWaves * kWave, 0, s>>>(a); break;
-    default: readout_kernel<PLANES, HALF, GRAIN, float><<<grid, kWaves * kWave, 0, s>>>(a); break;
+  // blocks of the same outputs one after the other on the same XCD, whose L2 then has the codes
+  const int slot = blockIdx.x / 8;
+  const int out_tile = slot / a.row_tiles * 8 + blockIdx.x % 8, row_tile = slot % a.row_tiles;
+  if (out_tile >= a.out_tiles) return;
+  const int l = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int group = wave / (RW * WO), wo = wave % (RW * WO) / RW, rw = wave % RW;
+  const int t = threadIdx.x % kGroupThreads;
+  const int first_row = row_tile * kTile * kTiles;
+  const int first_out = (out_tile * WO + wo) * OB * kTile + l % 16;
+
+  const uint8_t* codes[OB];
+  const char* scales[OB];
+#pragma unroll
+  for (int b = 0; b < OB; ++b) {  // outputs past the last take its codes and are not stored
+    const int o = first_out + b * kTile < a.K ? first_out + b * kTile : a.K - 1;
+    codes[b] = a.codes + o * a.code_stride;
+    scales[b] = (const char*)a.scales + o * a.scale_stride * (a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2);
+  }
+  struct Round {
+    Piece<X> piece[kEach];
+    Codes<GRAIN> code[OB];
+  };
+  const auto load = [&](int i, Round& to) {  // round i of this group
+    const int chunk = i * WK + group;
+#pragma unroll
+    for (int b = 0; b < OB; ++b) to.code[b].load(a, codes[b], scales[b], chunk);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {  // rows past the last take its clauses and are not stored
+      const int j = e * kGroupThreads + t;
+      const int n = first_row + j / kPieces;
+      to.piece[e].load(a, n < a.N ? n : a.N - 1, chunk * kChunk + j % kPieces * 8);
+    }
+  };
+  const auto keep = [&](const Round& of, int buffer) {
+    v4u* to = lds + (buffer * WK + group) * kFrags * kWave;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int j = e * kGroupThreads + t;
+      const int row = j / kPieces, place = place_of<GRAIN>(j % kPieces);
+      v4u plane[kPlanes];
+      of.piece[e].operands(plane);
+#pragma unroll
+      for (int p = 0; p < kPlanes; ++p)
+        to[((p * 4 + place / 4) * kTiles + row / kTile) * kWave + place % 4 * 16 + row % kTile] = plane[p];
+    }
+  };
+
+  v4f total[NT][OB];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int b = 0; b < OB; ++b) total[n][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto add = [&](const Codes<GRAIN>(&code)[OB], int buffer) {
+    add_chunk<X, GRAIN, NT, OB>(a, code, lds + ((buffer * WK + group) * kFrags + rw * NT) * kWave + l,
+                                4 * kTiles * kWave, kTiles * kWave, kWave, total);
+  };
+  const int rounds = (a.chunks + WK - 1) / WK;
+  Round even, odd;
+  load(0, even);
+  if (rounds > 1) load(1, odd);
+  keep(even, 0);
+  for (int i = 0; i < rounds; i += 2) {
+    __syncthreads();
+    Codes<GRAIN> now[OB];
+#pragma unroll
+    for (int b = 0; b < OB; ++b) now[b] = even.code[b];
+    if (i + 2 < rounds) load(i + 2, even);
+    add(now, 0);
+    if (i + 1 >= rounds) break;
+    keep(odd, 1);
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < OB; ++b) now[b] = odd.code[b];
+    if (i + 3 < rounds) load(i + 3, odd);
+    add(now, 1);
+    if (i + 2 < rounds) keep(even, 0);
+  }
+  v4f* join = (v4f*)lds;
+  if (WK > 1) {
+    __syncthreads();
+    if (group > 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int b = 0; b < OB; ++b)
+          join[(((group - 1) * RW * WO + wave % (RW * WO)) * NT * OB + n * OB + b) * kWave + l] = total[n][b];
+    }
+    __syncthreads();
+    if (group > 0) return;
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int b = 0; b < OB; ++b) {
+      v4f v = total[n][b];
+      for (int g = 0; g < WK - 1; ++g) v += join[((g * RW * WO + wave) * NT * OB + n * OB + b) * kWave + l];
+      const int o = first_out + b * kTile;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = first_row + (rw * NT + n) * kTile + l / 16 * 4 + r;
+        if (o < a.K && row < a.N) store_out(a, row, o, v[r]);
+      }
+    }
+}
+
+template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
+hipError_t launch_tile(ReadoutArgs a, hipStream_t s) {
+  a.row_tiles = (a.N + kTile * NT * RW - 1) / (kTile * NT * RW);
+  a.out_tiles = (a.K + kTile * OB * WO - 1) / (kTile * OB * WO);
+  const unsigned grid = (unsigned)((a.out_tiles + 7) / 8 * 8 * a.row_tiles);
+  tile_kernel<X, GRAIN, NT, RW, OB, WO, WK><<<grid, kWave * RW * WO * WK, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+// Few rows (up to 16): a block has 16 OB WO outputs and the clauses of one of the parts that the
+// grid's second axis counts, whose row operands lie in LDS from the start (without those of rows
+// that are not there), so that nothing waits between its first and last chunk.  WK waves share
+// an output tile's chunks; each loads kAhead of them before the first is looked at.  With more
+// than one part the sums go to the workspace, [part][row][output].
+template <int OB>
+constexpr int kAhead = OB == 1 ? 4 : 2;
+template <int X, int GRAIN, int OB, int WO, int WK>
+__global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
+  constexpr int kPlanes = Kind<X>::kPlanes;
+  constexpr int kDeep = kAhead<OB>;
+  extern __shared__ v4u held[];
+  __shared__ v4f join[WO * WK][OB][kWave];
+  const int l = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int wo = wave / WK, wk = wave % WK;
+  const int begin = blockIdx.y * a.part_chunks;
+  const int end = begin + a.part_chunks < a.chunks ? begin + a.part_chunks : a.chunks;
+  const int first_out = (blockIdx.x * WO + wo) * OB * kTile + l % 16;
+  const uint8_t* codes[OB];
+  const char* scales[OB];
+#pragma unroll
+  for (int b = 0; b < OB; ++b) {
+    const int o = first_out + b * kTile < a.K ? first_out + b * kTile : a.K - 1;
+    codes[b] = a.codes + o * a.code_stride;
+    scales[b] = (const char*)a.scales + o * a.scale_stride * (a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2);
+  }
+  Codes<GRAIN> code[kDeep][OB];
+  const auto load = [&](int chunk) {
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u)
+#pragma unroll
+      for (int b = 0; b < OB; ++b) code[u][b].load(a, codes[b], scales[b], chunk + u * WK);
+  };
+  if (begin < end) load(begin + wk);  // without clauses there are no codes either
+  const int count = (end - begin) * kPieces;
+  for (int n = 0; n < a.N; ++n)
+    for (int i = threadIdx.x; i < count; i += kWave * WO * WK) {
+      Piece<X> piece;
+      piece.load(a, n, begin * kChunk + 8 * i);
+      v4u plane[kPlanes];
+      piece.operands(plane);
+      const int place = i / kPieces * kPieces + place_of<GRAIN>(i % kPieces);
+#pragma unroll
+      for (int p = 0; p < kPlanes; ++p) held[(p * count + place) * a.N + n] = plane[p];
+    }
+  __syncthreads();
+  const v4u* from = held + l / 16 * a.N + (l % 16 < a.N ? l % 16 : 0);
+  v4f total[1][OB];
+#pragma unroll
+  for (int b = 0; b < OB; ++b) total[0][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int first = begin + wk; first < end; first += kDeep * WK) {
+    Codes<GRAIN> now[kDeep][OB];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u)
+#pragma unroll
+      for (int b = 0; b < OB; ++b) now[u][b] = code[u][b];
+    if (first + kDeep * WK < end) load(first + kDeep * WK);
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      const int chunk = first + u * WK;
+      if (chunk >= end) break;
+      add_chunk<X, GRAIN, 1, OB>(a, now[u], from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < OB; ++b) join[wave][b][l] = total[0][b];
+  __syncthreads();
+  if (wk > 0) return;
+#pragma unroll
+  for (int b = 0; b < OB; ++b) {
+    v4f v = total[0][b];
+    for (int w = 1; w < WK; ++w) v += join[wave + w][b][l];
+    const int o = first_out + b * kTile;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = l / 16 * 4 + r;
+      if (o >= a.K || n >= a.N) continue;
+      if (gridDim.y > 1)
+        a.parts[((int64_t)blockIdx.y * a.N + n) * a.K + o] = v[r];
+      else
+        store_out(a, n, o, v[r]);
+    }
   }
 }
 
-template <int PLANES, bool HALF>
-hipError_t launch_readout(const ReadoutArgs& a, int scale_dtype, hipStream_t s) {
-  const int64_t items = a.steps * a.row_tiles * kWave;
-  if (items) rows_kernel<<<(unsigned)std::min<int64_t>((items + 255) / 256, 4096), 256, 0, s>>>(a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  if (a.group % 128 == 0)
-    launch_scale<PLANES, HALF, 128>(a, scale_dtype, s);
-  else if (a.group % 64 == 0)
-    launch_scale<PLANES, HALF, 64>(a, scale_dtype, s);
-  else
-    launch_scale<PLANES, HALF, 32>(a, scale_dtype, s);
+// The parts' sums added in their order.
+__global__ __launch_bounds__(256) void parts_kernel(ReadoutArgs a, int parts) {
+  const int64_t each = (int64_t)a.N * a.K;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < each; i += (int64_t)gridDim.x * blockDim.x) {
+    float v = a.parts[i];
+    for (int p = 1; p < parts; ++p) v += a.parts[p * each + i];
+    store_out(a, (int)(i / a.K), (int)(i % a.K), v);
+  }
+}
+
+// A chunk's row operands take rows * kPlanes * 256 bytes of LDS; a part has as many chunks as
+// kHeldLimit takes, which leaves room for two blocks on a CU.
+constexpr int64_t kHeldLimit = 64 * 1024;
+int part_chunks_of(int planes, int N, int chunks) {
+  const int64_t most = kHeldLimit / ((int64_t)planes * N * kPieces * 16);
+  if (most >= chunks) return chunks > 0 ? chunks : 1;
+  const int64_t parts = (chunks + most - 1) / most;
+  return (int)((chunks + parts - 1) / parts);
+}
+int parts_of(int planes, int N, int chunks) {
+  const int each = part_chunks_of(planes, N, chunks);
+  return chunks > 0 ? (chunks + each - 1) / each : 1;
+}
+
+template <int X, int GRAIN, int OB, int WO, int WK>
+hipError_t launch_held(ReadoutArgs a, hipStream_t s) {
+  const int parts = parts_of(Kind<X>::kPlanes, a.N, a.chunks);
+  a.part_chunks = part_chunks_of(Kind<X>::kPlanes, a.N, a.chunks);
+  const size_t lds = (size_t)a.N * Kind<X>::kPlanes * (a.part_chunks < a.chunks ? a.part_chunks : a.chunks) * kPieces * 16;
+  const dim3 grid((unsigned)((a.K + kTile * OB * WO - 1) / (kTile * OB * WO)), (unsigned)parts);
+  held_kernel<X, GRAIN, OB, WO, WK><<<grid, kWave * WO * WK, lds, s>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || parts == 1) return e;
+  const int64_t blocks = ((int64_t)a.N * a.K + 255) / 256;
+  parts_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(a, parts);
   return hipGetLastError();
+}
+
+constexpr int kFewRows = 16;
+
+template <int X, int GRAIN>
+hipError_t launch_rows(const ReadoutArgs& a, hipStream_t s) {
+  constexpr bool kOne = Kind<X>::kPlanes == 1;
+  if (a.chunks == 0 || a.N <= kFewRows) {
+    if (parts_of(Kind<X>::kPlanes, a.N, a.chunks) > 1) return launch_held<X, GRAIN, 2, 4, 2>(a, s);
+    return a.K <= 4096 ? launch_held<X, GRAIN, 1, 1, 16>(a, s) : launch_held<X, GRAIN, 1, 1, 4>(a, s);
+  }
+  if (a.N <= 32) return launch_tile<X, GRAIN, 2, 1, 2, 4, kOne ? 2 : 1>(a, s);
+  if (a.N <= 64 || !kOne) return launch_tile<X, GRAIN, kOne ? 4 : 2, kOne ? 1 : 2, 2, 4, kOne ? 2 : 1>(a, s);
+  if constexpr (kOne) {
+    const bool narrow = (a.N + 95) / 96 * 96 < (a.N + 127) / 128 * 128;
+    if (narrow) return launch_tile<X, GRAIN, 3, 2, 2, 4, 1>(a, s);
+    return launch_tile<X, GRAIN, 4, 2, GRAIN == kChunk ? 3 : 2, 4, 1>(a, s);
+  }
+}
+
+template <int X>
+hipError_t launch_readout(const ReadoutArgs& a, int64_t group, hipStream_t s) {
+  return group % kChunk == 0 ? launch_rows<X, kChunk>(a, s) : launch_rows<X, kStep>(a, s);
 }
 
 }  // namespace
@@ -235,9 +560,12 @@ extern "C" {
 
 int ytm_readout_workspace(int x_dtype, int64_t N, int64_t C, int64_t K, int64_t* bytes) {
   if (!bytes || (x_dtype != YTM_DTYPE_BITS && !ytm::decode_float(x_dtype)) || N < 0 || C < 0 || K < 0 ||
-      N > ytm::kDecodeRows || C > INT32_MAX || K > INT32_MAX)
+      N > ytm::kDecodeRows || C > ytm::kMaxClauses || K > ytm::kMaxScores)
     return fail(YTM_EINVAL, "bad readout_workspace arguments");
-  *bytes = ytm::planes_of(x_dtype) * ytm::steps_of(C) * ytm::tiles_of(N) * ytm::kWave * 16;
+  *bytes = 0;
+  if (N == 0 || K == 0 || C == 0 || N > ytm::kFewRows) return YTM_OK;
+  const int parts = ytm::parts_of(x_dtype == YTM_DTYPE_F32 ? 3 : 1, (int)N, (int)((C + 127) / 128));
+  if (parts > 1) *bytes = parts * N * K * 4;
   return YTM_OK;
 }
 
@@ -249,8 +577,8 @@ int ytm_readout(const void* x, int x_dtype, int64_t x_stride, int64_t N, int64_t
     return fail(YTM_EINVAL, "readout takes bits, float32, float16 or bfloat16");
   if (!ytm::decode_float(scale_dtype) || !ytm::decode_float(out_dtype))
     return fail(YTM_EINVAL, "readout scales and sums are float32, float16 or bfloat16");
-  if (N < 0 || C < 0 || K < 0 || N > ytm::kDecodeRows || C > INT32_MAX || K > INT32_MAX)
-    return fail(YTM_EINVAL, "readout takes at most 65535 rows");
+  if (N < 0 || C < 0 || K < 0 || N > ytm::kDecodeRows || C > ytm::kMaxClauses || K > ytm::kMaxScores)
+    return fail(YTM_EINVAL, "readout takes at most 65535 rows, 2097120 clauses and 8388608 outputs");
   if (group < 32 || group % 32) return fail(YTM_EINVAL, "readout groups are multiples of 32 clauses");
   if (N == 0 || K == 0) return YTM_OK;
   if (!out || (C > 0 && (!x || !codes || !scales))) return fail(YTM_EINVAL, "bad readout arguments");
@@ -262,14 +590,21 @@ int ytm_readout(const void* x, int x_dtype, int64_t x_stride, int64_t N, int64_t
     return fail(YTM_EINVAL, "readout: rows overlap");
   int64_t need = 0;
   if (int rc = ytm_readout_workspace(x_dtype, N, C, K, &need)) return rc;
-  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
-    return fail(YTM_EINVAL, "readout: the workspace is too small or not at a multiple of 16 bytes");
-  ytm::ReadoutArgs a{x, x_dtype, x_stride, N, C, codes, code_stride, scales, scale_stride, group, K, out, out_dtype,
-                     out_stride, (ytm::v4u*)workspace, ytm::steps_of(C), ytm::tiles_of(N)};
+  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4))
+    return fail(YTM_EINVAL, "readout: the workspace is too small or not at a multiple of 4 bytes");
+  const int64_t steps = (C + 31) / 32, units = group / 32;
+  // (step + 1) * floor((2^32 - 1) / units) >> 32 is step / units while (step + 1) * units < 2^32
+  const uint32_t inverse = units >= steps ? 0u : (uint32_t)(0xFFFFFFFFu / units);
+  const ytm::ReadoutArgs a{x, x_stride, (int)N, (int)C, codes, code_stride, scales, scale_dtype, scale_stride, inverse,
+                           (int)K, out, out_dtype, out_stride, (int)((C + 127) / 128), 0, 0, 0, (float*)workspace};
   hipStream_t s = (hipStream_t)stream;
-  const hipError_t e = x_dtype == YTM_DTYPE_F16   ? ytm::launch_readout<1, true>(a, scale_dtype, s)
-                       : x_dtype == YTM_DTYPE_F32 ? ytm::launch_readout<3, false>(a, scale_dtype, s)
-                                                  : ytm::launch_readout<1, false>(a, scale_dtype, s);
+  hipError_t e;
+  switch (x_dtype) {
+    case YTM_DTYPE_BITS: e = ytm::launch_readout<YTM_DTYPE_BITS>(a, group, s); break;
+    case YTM_DTYPE_F16: e = ytm::launch_readout<YTM_DTYPE_F16>(a, group, s); break;
+    case YTM_DTYPE_BF16: e = ytm::launch_readout<YTM_DTYPE_BF16>(a, group, s); break;
+    default: e = ytm::launch_readout<YTM_DTYPE_F32>(a, group, s); break;
+  }
   if (e != hipSuccess) return fail(YTM_EHIP, std::string("readout failed: ") + hipGetErrorString(e));
   return YTM_OK;
 }

@@ -200,14 +200,15 @@ def readout(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: i
         fits = isinstance(scales, _Tensor) and tuple(scales.shape) == (K, groups)
         _refuse(scales, "scales", (2,), _FLOATS, "" if fits else f"({K}, {groups})", device)
     out, out_type = _result(out, (N, K), device)
-    need = ctypes.c_int64()
-    rc = lib.ytm_readout_workspace(x_type, N, C, K, need)
-    if rc:
-        check(rc)
-    need = need.value
-    workspace = None
-    if need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    need, workspace = 0, None
+    if N <= 16 and C * N > 4096:  # more rows, or rows that one block holds, need none
+        need = ctypes.c_int64()
+        rc = lib.ytm_readout_workspace(x_type, N, C, K, need)
+        if rc:
+            check(rc)
+        need = need.value
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
     _call(lib.ytm_readout, device, x.data_ptr(), x_type, x.stride(0), N, C, codes.data_ptr(), codes.stride(0),
           scales.data_ptr(), _FLOATS[scales.dtype], scales.stride(0), group, K, out.data_ptr(), out_type,
           out.stride(0), workspace.data_ptr() if need else None, need)
