@@ -285,7 +285,7 @@ int ytm_collapse_bins(const uint32_t *B, int64_t rows, int64_t width, int kind, 
  * are 0, 0.5, 1, 1.5, 2, 3, 4, 6; 8..15 their negatives), two a byte, the even clause in the
  * low half, 16 ceil(C/32) bytes an output, each output's at a multiple of 16 bytes (codes
  * past C are ignored).  scales: (K, ceil(C/group)), group a multiple of 32.  scales and out: F32, F16 or
- * BF16.  workspace: device memory of ytm_readout_workspace's bytes at a multiple of 4 bytes, for
+ * BF16.  Rows of x, codes and scales are at most 8 MiB apart.  workspace: device memory of ytm_readout_workspace's bytes at a multiple of 16 bytes, for
  * the time of the call's work (NULL where that is 0). */
 int ytm_readout_workspace(int x_dtype, int64_t N, int64_t C, int64_t K, int64_t *bytes);
 int ytm_readout(const void *x, int x_dtype, int64_t x_stride, int64_t N, int64_t C, const uint8_t *codes,

@@ -94,9 +94,10 @@ CHOOSE = dict(scores=P, dtype=7, stride=8, N=2, V=8, temperature=None, top_k=Non
         dict(N=65536), dict(C=-1), dict(K=-1), dict(C=1 << 31), dict(group=0), dict(group=16), dict(group=33),
         dict(x=None), dict(codes=None), dict(scales=None), dict(out=None), dict(codes=P + 8), dict(code_stride=40),
         dict(code_stride=16), dict(scale_stride=1), dict(x_stride=63), dict(out_stride=2),
-        dict(C=2097121, x_stride=1 << 30, code_stride=1 << 30, scale_stride=1 << 30), dict(K=(1 << 23) + 1, out_stride=1 << 24),
+        dict(C=2097121, x_stride=1 << 30, code_stride=1 << 30, scale_stride=1 << 30), dict(K=(1 << 23) + 1, out_stride=1 << 24), dict(code_stride=(8 << 20) + 16), dict(x_stride=(2 << 20) + 1),
+        dict(scale_stride=(2 << 20) + 1),
         # a workspace that is missing, too small, at an odd address
-        *(dict(C=200000, x_stride=1 << 20, code_stride=1 << 20, scale_stride=1 << 20, **w) for w in (
+        *(dict(C=200000, x_stride=200000, code_stride=100000, scale_stride=6250, **w) for w in (
             {}, dict(workspace=P, workspace_bytes=100), dict(workspace=P + 2, workspace_bytes=1 << 30))))
 ] + [
     ("ytm_adjust_scores", ADJUST, w) for w in (
@@ -125,6 +126,7 @@ def test_workspace():
     ask = _lib.lib.ytm_readout_workspace
     for wrong in ((8, 1, 1, 1, n), (7, -1, 1, 1, n), (7, 1, 2097121, 1, n), (7, 1, 1, -1, n), (7, 1, 1, 1, None)):
         assert ask(*wrong) == _lib.YTM_EINVAL
-    for args in ((7, 0, 1000, 1), (7, 3, 0, 5), (7, 17, 100000, 10), (11, 1, 10000, 10000)):
+    for args in ((7, 0, 1000, 1), (7, 3, 0, 5), (7, 17, 7, 10), (11, 1, 10000, 10000), (7, 16, 256, 5)):
         assert ask(*args, n) == _lib.YTM_OK and n.value == 0
-    assert ask(7, 16, 20000, 10, n) == _lib.YTM_OK and n.value > 0
+    for args in ((7, 16, 20000, 10), (11, 17, 8, 1)):
+        assert ask(*args, n) == _lib.YTM_OK and n.value > 0

@@ -43,6 +43,9 @@ constexpr int64_t kMaxScores = 1 << 23;
 // Clauses of a readout: fewer than 65536 steps of 32.
 constexpr int64_t kMaxClauses = 65535 * 32;
 
+// Bytes from a row to the next of a readout's operands: a block's rows, 192 at most, lie within 2^31.
+constexpr int64_t kMaxApart = 8 << 20;
+
 inline bool decode_float(int dtype) {
   return dtype == YTM_DTYPE_F32 || dtype == YTM_DTYPE_F16 || dtype == YTM_DTYPE_BF16;
 }

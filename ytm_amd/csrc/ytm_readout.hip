@@ -49,10 +49,13 @@ struct ReadoutArgs {
   int out_dtype;
   int64_t out_stride;
   int chunks, part_chunks, out_tiles, row_tiles;
-  float* parts;
+  float* parts;  // the workspace, of few rows' sums or many rows' operands
+  v4u* frag;
 };
 
 // What x is: its element, the number of 16-bit operands it is the sum of, whether these are float16.
+template <int X>
+constexpr int kSize = X == YTM_DTYPE_BITS || X == YTM_DTYPE_F32 ? 4 : 2;  // bytes of what x_stride counts
 template <int X>
 struct Kind;
 template <>
@@ -80,41 +83,67 @@ struct Kind<YTM_DTYPE_F32> {
 // Eight clauses of a row as they are in memory, and as 16-bit operands: bits as 0 and 1, float32
 // as the sum of three bfloat16, each cut (not rounded) to one, so that nothing overflows; where
 // the first is infinite or NaN the others are zero.
+//
+// The load has no branch (rows have eight clauses or more), so that others can follow it before
+// it is there: a piece that would pass the row's end is taken from its last eight clauses, and moved
+// to its place, with zeros after it, when it becomes operands.
 template <int X>
 struct Piece {
-  v4u raw[X == YTM_DTYPE_F32 ? 2 : 1];
+  static constexpr int kWords = X == YTM_DTYPE_F32 ? 8 : X == YTM_DTYPE_BITS ? 1 : 4;
+  uint32_t raw[kWords];
 
-  // clauses c .. c + 7 of row n; zero from clause C on
-  __device__ __forceinline__ void load(const ReadoutArgs& a, int n, int c) {
+  // of the row `off` bytes from x's uniform address `x`, clauses c .. c + 7
+  __device__ __forceinline__ void load(const ReadoutArgs& a, const char* x, uint32_t off, int c) {
     if (X == YTM_DTYPE_BITS) {
-      const uint32_t* words = (const uint32_t*)a.x + n * a.x_stride;
-      const uint32_t bits = c < a.C ? words[c / 32] >> (c % 32) & 255u : 0u;
-      raw[0][0] = a.C - c >= 8 ? bits : bits & ((1u << (a.C > c ? a.C - c : 0)) - 1u);
+      const int at = c < a.C ? c : a.C - 1;
+      raw[0] = *(const uint32_t*)(x + (off + at / 32 * 4));
       return;
     }
-    typedef typename std::conditional<X == YTM_DTYPE_F32, uint32_t, uint16_t>::type Bits;
-    const Bits* from = (const Bits*)a.x + n * a.x_stride + c;
-    if (c + 8 <= a.C) {
-      __builtin_memcpy(raw, from, sizeof raw);
-      return;
-    }
-    Bits e[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) e[j] = c + j < a.C ? from[j] : (Bits)0;
-    __builtin_memcpy(raw, e, sizeof raw);
+    const int at = c < a.C - 8 ? c : a.C - 8;
+    __builtin_memcpy(raw, x + (off + at * (X == YTM_DTYPE_F32 ? 4 : 2)), sizeof raw);
   }
 
-  __device__ __forceinline__ void operands(v4u (&plane)[Kind<X>::kPlanes]) const {
+  // the operands of clauses c .. c + 7, which load() was asked for
+  __device__ __forceinline__ void operands(const ReadoutArgs& a, int c, v4u (&plane)[Kind<X>::kPlanes]) const {
+    const int over = c + 8 - a.C;  // of the eight, past the last clause
     if (X == YTM_DTYPE_BITS) {
+      uint32_t bits = raw[0] >> (c % 32);
+      if (over > 0) bits = over < 8 ? bits & (255u >> over) : 0u;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const uint32_t two = raw[0][0] >> (2 * q);
+        const uint32_t two = bits >> (2 * q);
         plane[0][q] = ((two & 1u) | (two & 2u) << 15) * 0x3F80u;  // 1.0 at either half
       }
       return;
     }
+    uint32_t r[kWords];
+#pragma unroll
+    for (int q = 0; q < kWords; ++q) r[q] = raw[q];
+    if (over > 0) {  // what is in place `over` moves to place 0
+      if (X == YTM_DTYPE_F32) {
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1)
+#pragma unroll
+          for (int q = 0; q < kWords; ++q) r[q] = over & d ? (q + d < kWords ? r[(q + d) % kWords] : 0u) : r[q];
+      } else {
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) {
+          const uint32_t next = q + 1 < kWords ? r[(q + 1) % kWords] : 0u;
+          r[q] = over & 1 ? r[q] >> 16 | next << 16 : r[q];
+        }
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1)
+#pragma unroll
+          for (int q = 0; q < kWords; ++q) r[q] = over & 2 * d ? (q + d < kWords ? r[(q + d) % kWords] : 0u) : r[q];
+      }
+      if (over >= 8) {
+#pragma unroll
+        for (int q = 0; q < kWords; ++q) r[q] = 0u;
+      }
+    }
     if (X != YTM_DTYPE_F32) {
-      plane[0] = raw[0];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) plane[0][q] = r[q % kWords];
       return;
     }
 #pragma unroll
@@ -122,16 +151,12 @@ struct Piece {
       uint32_t part[3][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int j = 2 * q + h;
-        const uint32_t u = raw[j / 4 % (X == YTM_DTYPE_F32 ? 2 : 1)][j % 4];
-        const float v = __uint_as_float(u);
-        const uint32_t hi = u & 0xFFFF0000u;
+        const uint32_t u = r[(2 * q + h) % kWords];
         const bool finite = (u & 0x7F800000u) != 0x7F800000u;
-        const float rest = finite ? v - __uint_as_float(hi) : 0.0f;
-        const uint32_t mid = __float_as_uint(rest) & 0xFFFF0000u;
+        const float rest = finite ? __uint_as_float(u) - __uint_as_float(u & 0xFFFF0000u) : 0.0f;
         part[0][h] = (u & 0x7FFFFFFFu) > 0x7F800000u ? u | 0x00400000u : u;  // a NaN stays one
-        part[1][h] = mid;
-        part[2][h] = __float_as_uint(rest - __uint_as_float(mid));
+        part[1][h] = __float_as_uint(rest);
+        part[2][h] = __float_as_uint(rest - __uint_as_float(part[1][h] & 0xFFFF0000u));
       }
 #pragma unroll
       for (int p = 0; p < Kind<X>::kPlanes; ++p)
@@ -190,30 +215,26 @@ __device__ __forceinline__ int place_of(int i) {
 template <int GRAIN>
 struct Codes {
   v4u w;
-  uint32_t scale;
+  uint16_t low, high;  // of the scale; the same twice where it has 16 bits, so that no load needs a branch
 
-  // Chunks past the last take what the first holds: their rows are zero.
-  __device__ __forceinline__ void load(const ReadoutArgs& a, const uint8_t* codes, const char* scales, int chunk) {
-    const int g = threadIdx.x % kWave / 16;
-    const int at = chunk * (kChunk / 2) + g * 16;
-    const bool in = at < (a.C + 31) / 32 * 16;
-    w = *(const v4u*)(codes + (in ? at : 0));
-    const uint32_t step = (uint32_t)chunk * 4 + (GRAIN == kChunk ? 0 : g);
-    const uint32_t q = in || GRAIN == kChunk && chunk < a.chunks ? __umulhi(step + 1, a.inverse) : 0u;
-    if (a.scale_dtype == YTM_DTYPE_F32)
-      scale = ((const uint32_t*)scales)[q];
-    else
-      scale = ((const uint16_t*)scales)[q];
+  // of the output whose codes are `code` bytes from the uniform address `codes` and whose scales are
+  // `scale` bytes from `scales`.  Past the last clause the last codes are taken: the rows are zero there.
+  __device__ __forceinline__ void load(const ReadoutArgs& a, const uint8_t* codes, uint32_t code, const char* scales,
+                                       uint32_t scale, int chunk) {
+    const uint32_t steps = (a.C + kStep - 1) / kStep;
+    const uint32_t mine = chunk * 4 + threadIdx.x % kWave / 16;
+    w = *(const v4u*)(codes + (code + 16 * (mine < steps ? mine : steps - 1)));
+    const uint32_t step = GRAIN == kChunk ? chunk * 4 : mine;
+    const uint32_t size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
+    scale += __umulhi(step < steps ? step + 1 : steps, a.inverse) * size;
+    low = *(const uint16_t*)(scales + scale);
+    high = *(const uint16_t*)(scales + (scale + size - 2));
   }
   // scales of the four products
   __device__ __forceinline__ void scaled(const ReadoutArgs& a, float (&f)[4]) const {
-    float v;
-    if (a.scale_dtype == YTM_DTYPE_F32)
-      v = __uint_as_float(scale);
-    else if (a.scale_dtype == YTM_DTYPE_BF16)
-      v = __uint_as_float(scale << 16);
-    else
-      v = (float)__builtin_bit_cast(_Float16, (uint16_t)scale);
+    const float half = (float)__builtin_bit_cast(_Float16, high);
+    const float full = __uint_as_float((uint32_t)high << 16 | (a.scale_dtype == YTM_DTYPE_F32 ? low : 0u));
+    const float v = a.scale_dtype == YTM_DTYPE_F16 ? half : full;
     const uint32_t u = __float_as_uint(v);
     const v4u t = turn<GRAIN>(v4u{u, u, u, u});
 #pragma unroll
@@ -270,11 +291,32 @@ __device__ __forceinline__ void add_chunk(const ReadoutArgs& a, const Codes<GRAI
 #pragma unroll
           for (int r = 0; r < 4; ++r) total[n][b][r] = __builtin_fmaf(scale[b][s], sum[n][b][r], total[n][b][r]);
     }
+    // or the compiler reads the operands of all four products first, and runs out of registers
+    if (NT * OB > 4) __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// Many rows: a block takes 16 NT RW rows and 16 OB WO outputs; its waves are WK groups, each with
-// chunks of clauses of its own, of WO x RW waves, each with NT tiles of rows and OB of outputs.  Lane l takes
+// Many rows: their operands in the order in which products take them, frag[chunk][plane][step][row
+// tile][lane], zero past the last clause, the last row's past the last row.  A block makes a chunk
+// (the grid's first axis) of a row tile, a thread a piece; 16 of them read 256 or 512 bytes in a row.
+template <int X, int GRAIN>
+__global__ __launch_bounds__(kPieces* kTile) void rows_kernel(ReadoutArgs a) {
+  constexpr int kPlanes = Kind<X>::kPlanes;
+  const int chunk = blockIdx.x, tile = blockIdx.y, row = threadIdx.x / kPieces, i = threadIdx.x % kPieces;
+  const int place = place_of<GRAIN>(i), c = chunk * kChunk + i * 8;
+  const int n = tile * kTile + row < a.N ? tile * kTile + row : a.N - 1;
+  Piece<X> piece;
+  v4u plane[kPlanes];
+  piece.load(a, (const char*)a.x + n * a.x_stride * kSize<X>, 0, c);
+  piece.operands(a, c, plane);
+#pragma unroll
+  for (int p = 0; p < kPlanes; ++p)
+    a.frag[(((int64_t)(chunk * kPlanes + p) * 4 + place / 4) * a.row_tiles + tile) * kWave + place % 4 * 16 + row] =
+        plane[p];
+}
+
+// A block takes 16 NT RW rows and 16 OB WO outputs; its waves are WK groups, each with chunks of
+// clauses of its own, of WO x RW waves, each with NT tiles of rows and OB of outputs.  Lane l takes
 // the codes of output l % 16 as a product's second operand and gets sums of rows 4 (l / 16) .. + 3
 // of that output.  A group keeps a chunk of its rows' operands in LDS; the next chunk is in
 // registers or on its way, and the one after it is asked for before the products of this one, as
@@ -282,59 +324,58 @@ __device__ __forceinline__ void add_chunk(const ReadoutArgs& a, const Codes<GRAI
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) {
   constexpr int kPlanes = Kind<X>::kPlanes;
-  constexpr int kGroupThreads = kWave * RW * WO;
+  constexpr int kGroupWaves = RW * WO;
   constexpr int kTiles = NT * RW;               // of rows
-  constexpr int kFrags = kPlanes * 4 * kTiles;  // operands of a buffer
-  constexpr int kEach = kPieces * kTile * kTiles / kGroupThreads;  // pieces a thread loads
-  static_assert(kPieces * kTile * kTiles % kGroupThreads == 0, "");
-  constexpr int kJoin = (WK - 1) * RW * WO * NT * OB;
+  constexpr int kFrags = kPlanes * 4 * kTiles;  // operands of a chunk
+  constexpr int kEach = kFrags / kGroupWaves;   // that a wave loads
+  static_assert(kFrags % kGroupWaves == 0, "");
+  constexpr int kJoin = (WK - 1) * kGroupWaves * NT * OB;
   __shared__ v4u lds[(2 * WK * kFrags > kJoin ? 2 * WK * kFrags : kJoin) * kWave];
 
   // blocks of the same outputs one after the other on the same XCD, whose L2 then has the codes
+  const int row_blocks = (a.row_tiles + kTiles - 1) / kTiles;
   const int slot = blockIdx.x / 8;
-  const int out_tile = slot / a.row_tiles * 8 + blockIdx.x % 8, row_tile = slot % a.row_tiles;
+  const int out_tile = slot / row_blocks * 8 + blockIdx.x % 8, row_block = slot % row_blocks;
   if (out_tile >= a.out_tiles) return;
-  const int l = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int group = wave / (RW * WO), wo = wave % (RW * WO) / RW, rw = wave % RW;
-  const int t = threadIdx.x % kGroupThreads;
-  const int first_row = row_tile * kTile * kTiles;
+  const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int group = wave / kGroupWaves, mine = wave % kGroupWaves, wo = mine / RW, rw = mine % RW;
   const int first_out = (out_tile * WO + wo) * OB * kTile + l % 16;
 
-  const uint8_t* codes[OB];
-  const char* scales[OB];
+  // uniform addresses and 32-bit distances from them take fewer registers than addresses
+  const int block_out = out_tile * WO * OB * kTile;
+  const int size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  const uint8_t* codes = a.codes + block_out * a.code_stride;
+  const char* scales = (const char*)a.scales + block_out * a.scale_stride * size;
+  uint32_t code_off[OB], scale_off[OB];
 #pragma unroll
   for (int b = 0; b < OB; ++b) {  // outputs past the last take its codes and are not stored
-    const int o = first_out + b * kTile < a.K ? first_out + b * kTile : a.K - 1;
-    codes[b] = a.codes + o * a.code_stride;
-    scales[b] = (const char*)a.scales + o * a.scale_stride * (a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2);
+    const uint32_t o = (first_out + b * kTile < a.K ? first_out + b * kTile : a.K - 1) - block_out;
+    code_off[b] = o * (uint32_t)a.code_stride;
+    scale_off[b] = o * (uint32_t)a.scale_stride * size;
   }
   struct Round {
-    Piece<X> piece[kEach];
+    v4u x[kEach];
     Codes<GRAIN> code[OB];
   };
+  // Rounds past the last are loaded too (what the last holds): whether to load would be a branch,
+  // after which every load has to be waited for.
+  const int rounds = (a.chunks + WK - 1) / WK;
   const auto load = [&](int i, Round& to) {  // round i of this group
-    const int chunk = i * WK + group;
+    const int chunk = (i < rounds ? i : rounds - 1) * WK + group;
 #pragma unroll
-    for (int b = 0; b < OB; ++b) to.code[b].load(a, codes[b], scales[b], chunk);
+    for (int b = 0; b < OB; ++b) to.code[b].load(a, codes, code_off[b], scales, scale_off[b], chunk);
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {  // rows past the last take its clauses and are not stored
-      const int j = e * kGroupThreads + t;
-      const int n = first_row + j / kPieces;
-      to.piece[e].load(a, n < a.N ? n : a.N - 1, chunk * kChunk + j % kPieces * 8);
+    for (int e = 0; e < kEach; ++e) {  // row tiles past the last take its rows and are not stored
+      const int f = e * kGroupWaves + mine, tile = row_block * kTiles + f % kTiles;
+      const v4u* from = a.frag + (((int64_t)chunk * kPlanes * 4 + f / kTiles) * a.row_tiles +
+                                  (tile < a.row_tiles ? tile : a.row_tiles - 1)) * kWave;
+      to.x[e] = from[l];
     }
   };
-  const auto keep = [&](const Round& of, int buffer) {
-    v4u* to = lds + (buffer * WK + group) * kFrags * kWave;
+  const auto keep = [&](const Round& of, int i) {  // of round i
+    v4u* to = lds + (i % 2 * WK + group) * kFrags * kWave;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int j = e * kGroupThreads + t;
-      const int row = j / kPieces, place = place_of<GRAIN>(j % kPieces);
-      v4u plane[kPlanes];
-      of.piece[e].operands(plane);
-#pragma unroll
-      for (int p = 0; p < kPlanes; ++p)
-        to[((p * 4 + place / 4) * kTiles + row / kTile) * kWave + place % 4 * 16 + row % kTile] = plane[p];
-    }
+    for (int e = 0; e < kEach; ++e) to[(e * kGroupWaves + mine) * kWave + l] = of.x[e];
   };
 
   v4f total[NT][OB];
@@ -346,26 +387,25 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
     add_chunk<X, GRAIN, NT, OB>(a, code, lds + ((buffer * WK + group) * kFrags + rw * NT) * kWave + l,
                                 4 * kTiles * kWave, kTiles * kWave, kWave, total);
   };
-  const int rounds = (a.chunks + WK - 1) / WK;
   Round even, odd;
   load(0, even);
-  if (rounds > 1) load(1, odd);
+  load(1, odd);
   keep(even, 0);
   for (int i = 0; i < rounds; i += 2) {
     __syncthreads();
     Codes<GRAIN> now[OB];
 #pragma unroll
     for (int b = 0; b < OB; ++b) now[b] = even.code[b];
-    if (i + 2 < rounds) load(i + 2, even);
+    load(i + 2, even);
     add(now, 0);
     if (i + 1 >= rounds) break;
-    keep(odd, 1);
+    keep(odd, i + 1);
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < OB; ++b) now[b] = odd.code[b];
-    if (i + 3 < rounds) load(i + 3, odd);
+    load(i + 3, odd);
     add(now, 1);
-    if (i + 2 < rounds) keep(even, 0);
+    keep(even, i + 2);
   }
   v4f* join = (v4f*)lds;
   if (WK > 1) {
@@ -375,7 +415,7 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int b = 0; b < OB; ++b)
-          join[(((group - 1) * RW * WO + wave % (RW * WO)) * NT * OB + n * OB + b) * kWave + l] = total[n][b];
+          join[(((group - 1) * kGroupWaves + mine) * NT * OB + n * OB + b) * kWave + l] = total[n][b];
     }
     __syncthreads();
     if (group > 0) return;
@@ -385,21 +425,29 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
 #pragma unroll
     for (int b = 0; b < OB; ++b) {
       v4f v = total[n][b];
-      for (int g = 0; g < WK - 1; ++g) v += join[((g * RW * WO + wave) * NT * OB + n * OB + b) * kWave + l];
+      for (int g = 0; g < WK - 1; ++g) v += join[((g * kGroupWaves + mine) * NT * OB + n * OB + b) * kWave + l];
       const int o = first_out + b * kTile;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = first_row + (rw * NT + n) * kTile + l / 16 * 4 + r;
+        const int row = (row_block * kTiles + rw * NT + n) * kTile + l / 16 * 4 + r;
         if (o < a.K && row < a.N) store_out(a, row, o, v[r]);
       }
     }
 }
 
+// Chunks of the rows' operands: a whole number for each of up to kGroups groups of waves.
+constexpr int kGroups = 2;
+int padded_of(int chunks) { return (chunks + kGroups - 1) / kGroups * kGroups; }
+
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 hipError_t launch_tile(ReadoutArgs a, hipStream_t s) {
-  a.row_tiles = (a.N + kTile * NT * RW - 1) / (kTile * NT * RW);
+  static_assert(WK <= kGroups && kGroups % WK == 0, "");
+  a.row_tiles = (a.N + kTile - 1) / kTile;
   a.out_tiles = (a.K + kTile * OB * WO - 1) / (kTile * OB * WO);
-  const unsigned grid = (unsigned)((a.out_tiles + 7) / 8 * 8 * a.row_tiles);
+  rows_kernel<X, GRAIN><<<dim3(padded_of(a.chunks), a.row_tiles), kPieces * kTile, 0, s>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const unsigned grid = (unsigned)((a.out_tiles + 7) / 8 * 8 * ((a.row_tiles + NT * RW - 1) / (NT * RW)));
   tile_kernel<X, GRAIN, NT, RW, OB, WO, WK><<<grid, kWave * RW * WO * WK, 0, s>>>(a);
   return hipGetLastError();
 }
@@ -422,33 +470,49 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
   const int begin = blockIdx.y * a.part_chunks;
   const int end = begin + a.part_chunks < a.chunks ? begin + a.part_chunks : a.chunks;
   const int first_out = (blockIdx.x * WO + wo) * OB * kTile + l % 16;
-  const uint8_t* codes[OB];
-  const char* scales[OB];
+  const int block_out = blockIdx.x * WO * OB * kTile;
+  const int size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  const uint8_t* codes = a.codes + block_out * a.code_stride;
+  const char* scales = (const char*)a.scales + block_out * a.scale_stride * size;
+  uint32_t code_off[OB], scale_off[OB];
 #pragma unroll
   for (int b = 0; b < OB; ++b) {
-    const int o = first_out + b * kTile < a.K ? first_out + b * kTile : a.K - 1;
-    codes[b] = a.codes + o * a.code_stride;
-    scales[b] = (const char*)a.scales + o * a.scale_stride * (a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2);
+    const uint32_t o = (first_out + b * kTile < a.K ? first_out + b * kTile : a.K - 1) - block_out;
+    code_off[b] = o * (uint32_t)a.code_stride;
+    scale_off[b] = o * (uint32_t)a.scale_stride * size;
   }
   Codes<GRAIN> code[kDeep][OB];
   const auto load = [&](int chunk) {
 #pragma unroll
     for (int u = 0; u < kDeep; ++u)
 #pragma unroll
-      for (int b = 0; b < OB; ++b) code[u][b].load(a, codes[b], scales[b], chunk + u * WK);
+      for (int b = 0; b < OB; ++b)
+        code[u][b].load(a, codes, code_off[b], scales, scale_off[b], chunk + u * WK);
   };
-  if (begin < end) load(begin + wk);  // without clauses there are no codes either
+  load(begin + wk);
   const int count = (end - begin) * kPieces;
-  for (int n = 0; n < a.N; ++n)
-    for (int i = threadIdx.x; i < count; i += kWave * WO * WK) {
-      Piece<X> piece;
-      piece.load(a, n, begin * kChunk + 8 * i);
+  constexpr int kAtOnce = kPlanes == 1 ? 4 : 2;
+  for (int first = threadIdx.x; first < a.N * count; first += kAtOnce * kWave * WO * WK) {
+    Piece<X> piece[kAtOnce];
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) {
+      const int j = first + e * kWave * WO * WK;
+      const int n = j < a.N * count ? j / count : 0;
+      piece[e].load(a, (const char*)a.x, n * (uint32_t)a.x_stride * kSize<X>,
+                    begin * kChunk + 8 * (j < a.N * count ? j - n * count : 0));
+    }
+#pragma unroll
+    for (int e = 0; e < kAtOnce; ++e) {
+      const int j = first + e * kWave * WO * WK;
+      if (j >= a.N * count) break;
+      const int n = j / count, i = j - n * count;
       v4u plane[kPlanes];
-      piece.operands(plane);
+      piece[e].operands(a, begin * kChunk + 8 * i, plane);
       const int place = i / kPieces * kPieces + place_of<GRAIN>(i % kPieces);
 #pragma unroll
       for (int p = 0; p < kPlanes; ++p) held[(p * count + place) * a.N + n] = plane[p];
     }
+  }
   __syncthreads();
   const v4u* from = held + l / 16 * a.N + (l % 16 < a.N ? l % 16 : 0);
   v4f total[1][OB];
@@ -504,20 +568,20 @@ __global__ __launch_bounds__(256) void parts_kernel(ReadoutArgs a, int parts) {
 constexpr int64_t kHeldLimit = 64 * 1024;
 int part_chunks_of(int planes, int N, int chunks) {
   const int64_t most = kHeldLimit / ((int64_t)planes * N * kPieces * 16);
-  if (most >= chunks) return chunks > 0 ? chunks : 1;
+  if (most >= chunks) return chunks;
   const int64_t parts = (chunks + most - 1) / most;
   return (int)((chunks + parts - 1) / parts);
 }
 int parts_of(int planes, int N, int chunks) {
   const int each = part_chunks_of(planes, N, chunks);
-  return chunks > 0 ? (chunks + each - 1) / each : 1;
+  return (chunks + each - 1) / each;
 }
 
 template <int X, int GRAIN, int OB, int WO, int WK>
 hipError_t launch_held(ReadoutArgs a, hipStream_t s) {
   const int parts = parts_of(Kind<X>::kPlanes, a.N, a.chunks);
   a.part_chunks = part_chunks_of(Kind<X>::kPlanes, a.N, a.chunks);
-  const size_t lds = (size_t)a.N * Kind<X>::kPlanes * (a.part_chunks < a.chunks ? a.part_chunks : a.chunks) * kPieces * 16;
+  const size_t lds = (size_t)a.N * Kind<X>::kPlanes * a.part_chunks * kPieces * 16;
   const dim3 grid((unsigned)((a.K + kTile * OB * WO - 1) / (kTile * OB * WO)), (unsigned)parts);
   held_kernel<X, GRAIN, OB, WO, WK><<<grid, kWave * WO * WK, lds, s>>>(a);
   hipError_t e = hipGetLastError();
@@ -529,10 +593,38 @@ hipError_t launch_held(ReadoutArgs a, hipStream_t s) {
 
 constexpr int kFewRows = 16;
 
+// Fewer than eight clauses, which no load of a piece fits: a thread an output.
+template <int X>
+__global__ __launch_bounds__(256) void short_kernel(ReadoutArgs a) {
+  const int64_t each = (int64_t)a.N * a.K;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < each; i += (int64_t)gridDim.x * blockDim.x) {
+    const int n = (int)(i / a.K), o = (int)(i % a.K);
+    float sum = 0.0f;
+    for (int c = 0; c < a.C; ++c) {
+      const int64_t at = n * a.x_stride + c;
+      const float x = X == YTM_DTYPE_BITS   ? (float)(((const uint32_t*)a.x)[n * a.x_stride] >> c & 1u)
+                      : X == YTM_DTYPE_F16  ? to_float(((const f16*)a.x)[at])
+                      : X == YTM_DTYPE_BF16 ? to_float(((const bf16*)a.x)[at])
+                                            : ((const float*)a.x)[at];
+      const uint32_t code = a.codes[o * a.code_stride + c / 2] >> (c % 2 * 4) & 15u;
+      const uint32_t m = code & 7u;  // 0 and 0.5, then two to each power of two
+      const float v = m < 2 ? 0.5f * m : __uint_as_float((126u + (m >> 1)) << 23 | (m & 1u) << 22);
+      sum = __builtin_fmaf(x, code & 8u ? -v : v, sum);
+    }
+    if (a.C > 0) {
+      const int64_t at = o * a.scale_stride;
+      sum *= a.scale_dtype == YTM_DTYPE_F32   ? ((const float*)a.scales)[at]
+             : a.scale_dtype == YTM_DTYPE_F16 ? to_float(((const f16*)a.scales)[at])
+                                              : to_float(((const bf16*)a.scales)[at]);
+    }
+    store_out(a, n, o, sum);
+  }
+}
+
 template <int X, int GRAIN>
 hipError_t launch_rows(const ReadoutArgs& a, hipStream_t s) {
   constexpr bool kOne = Kind<X>::kPlanes == 1;
-  if (a.chunks == 0 || a.N <= kFewRows) {
+  if (a.N <= kFewRows) {
     if (parts_of(Kind<X>::kPlanes, a.N, a.chunks) > 1) return launch_held<X, GRAIN, 2, 4, 2>(a, s);
     return a.K <= 4096 ? launch_held<X, GRAIN, 1, 1, 16>(a, s) : launch_held<X, GRAIN, 1, 1, 4>(a, s);
   }
@@ -547,6 +639,11 @@ hipError_t launch_rows(const ReadoutArgs& a, hipStream_t s) {
 
 template <int X>
 hipError_t launch_readout(const ReadoutArgs& a, int64_t group, hipStream_t s) {
+  if (a.C < 8) {
+    const int64_t blocks = ((int64_t)a.N * a.K + 255) / 256;
+    short_kernel<X><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(a);
+    return hipGetLastError();
+  }
   return group % kChunk == 0 ? launch_rows<X, kChunk>(a, s) : launch_rows<X, kStep>(a, s);
 }
 
@@ -563,9 +660,14 @@ int ytm_readout_workspace(int x_dtype, int64_t N, int64_t C, int64_t K, int64_t*
       N > ytm::kDecodeRows || C > ytm::kMaxClauses || K > ytm::kMaxScores)
     return fail(YTM_EINVAL, "bad readout_workspace arguments");
   *bytes = 0;
-  if (N == 0 || K == 0 || C == 0 || N > ytm::kFewRows) return YTM_OK;
-  const int parts = ytm::parts_of(x_dtype == YTM_DTYPE_F32 ? 3 : 1, (int)N, (int)((C + 127) / 128));
-  if (parts > 1) *bytes = parts * N * K * 4;
+  if (N == 0 || K == 0 || C < 8) return YTM_OK;
+  const int planes = x_dtype == YTM_DTYPE_F32 ? 3 : 1, chunks = (int)((C + 127) / 128);
+  if (N > ytm::kFewRows) {
+    *bytes = (N + 15) / 16 * ytm::padded_of(chunks) * planes * 4096;
+  } else {
+    const int parts = ytm::parts_of(planes, (int)N, chunks);
+    if (parts > 1) *bytes = parts * N * K * 4;
+  }
   return YTM_OK;
 }
 
@@ -588,15 +690,22 @@ int ytm_readout(const void* x, int x_dtype, int64_t x_stride, int64_t N, int64_t
   if ((K > 1 && (code_stride < (C + 31) / 32 * 16 || scale_stride < (C + group - 1) / group)) ||
       (N > 1 && (x_stride < width || out_stride < K)))
     return fail(YTM_EINVAL, "readout: rows overlap");
+  const int64_t x_size = x_dtype == YTM_DTYPE_BITS || x_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  const int64_t scale_size = scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  if (N == 1) x_stride = 0;
+  if (K == 1) code_stride = scale_stride = 0;
+  if (x_stride * x_size > ytm::kMaxApart || code_stride > ytm::kMaxApart || scale_stride * scale_size > ytm::kMaxApart)
+    return fail(YTM_EINVAL, "readout rows, codes and scales are at most 8 MiB apart");
   int64_t need = 0;
   if (int rc = ytm_readout_workspace(x_dtype, N, C, K, &need)) return rc;
-  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4))
-    return fail(YTM_EINVAL, "readout: the workspace is too small or not at a multiple of 4 bytes");
+  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return fail(YTM_EINVAL, "readout: the workspace is too small or not at a multiple of 16 bytes");
   const int64_t steps = (C + 31) / 32, units = group / 32;
   // (step + 1) * floor((2^32 - 1) / units) >> 32 is step / units while (step + 1) * units < 2^32
   const uint32_t inverse = units >= steps ? 0u : (uint32_t)(0xFFFFFFFFu / units);
   const ytm::ReadoutArgs a{x, x_stride, (int)N, (int)C, codes, code_stride, scales, scale_dtype, scale_stride, inverse,
-                           (int)K, out, out_dtype, out_stride, (int)((C + 127) / 128), 0, 0, 0, (float*)workspace};
+                           (int)K, out, out_dtype, out_stride, (int)((C + 127) / 128), 0, 0, 0, (float*)workspace,
+                           (ytm::v4u*)workspace};
   hipStream_t s = (hipStream_t)stream;
   hipError_t e;
   switch (x_dtype) {

@@ -201,7 +201,7 @@ def readout(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: i
         _refuse(scales, "scales", (2,), _FLOATS, "" if fits else f"({K}, {groups})", device)
     out, out_type = _result(out, (N, K), device)
     need, workspace = 0, None
-    if N <= 16 and C * N > 4096:  # more rows, or rows that one block holds, need none
+    if N > 16 or C * N > 4096:  # fewer are held in one block's LDS
         need = ctypes.c_int64()
         rc = lib.ytm_readout_workspace(x_type, N, C, K, need)
         if rc:
