@@ -251,48 +251,47 @@ __device__ __forceinline__ void store_out(const ReadoutArgs& a, int n, int o, fl
   }
 }
 
-// A chunk's products of NT row tiles, whose operands lie at from[((plane * steps + step) * stride + tile) *
-// kWave], and OB output tiles, added to the sums so far.
-template <int X, int GRAIN, int NT, int OB>
+// A chunk's products of NT row tiles, whose operands lie at from[plane * .. + step * .. + tile * ..], and OB
+// output tiles, added to the sums so far.  One output tile after the other, so that the scaling
+// of one can go beside the products of the next; next(b) is called once tile b's codes are not
+// needed any more.
+template <int X, int GRAIN, int NT, int OB, typename Next>
 __device__ __forceinline__ void add_chunk(const ReadoutArgs& a, const Codes<GRAIN> (&code)[OB], const v4u* from,
-                                          int plane, int step, int tile, v4f (&total)[NT][OB]) {
+                                          int plane, int step, int tile, v4f (&total)[NT][OB], Next next) {
   constexpr int kPlanes = Kind<X>::kPlanes;
   constexpr bool kHalf = Kind<X>::kHalf;
-  v4u w[OB];
-  float scale[OB][4];
-  v4f sum[NT][OB];
+  v4u x[4][kPlanes][NT];
 #pragma unroll
-  for (int b = 0; b < OB; ++b) {
-    w[b] = turn<GRAIN>(code[b].w);
-    code[b].scaled(a, scale[b]);
-  }
-#pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    v4u x[kPlanes][NT];
+  for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) x[p][n] = from[p * plane + s * step + n * tile];
+      for (int n = 0; n < NT; ++n) x[s][p][n] = from[p * plane + s * step + n * tile];
 #pragma unroll
-    for (int b = 0; b < OB; ++b) {
-      const v4u y = codes_to_16<kHalf>(w[b][s]);
+  for (int b = 0; b < OB; ++b) {
+    const v4u w = turn<GRAIN>(code[b].w);
+    float scale[4];
+    code[b].scaled(a, scale);
+    v4u y[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) y[s] = codes_to_16<kHalf>(w[s]);
+    next(b);
+    v4f sum[NT];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        if (s * kStep % GRAIN == 0) sum[n][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (s * kStep % GRAIN == 0) sum[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int p = kPlanes - 1; p >= 0; --p) sum[n][b] = product<kHalf>(x[p][n], y, sum[n][b]);
+        for (int p = kPlanes - 1; p >= 0; --p) sum[n] = product<kHalf>(x[s][p][n], y[s], sum[n]);
       }
-    }
-    if ((s + 1) * kStep % GRAIN == 0) {
-#pragma unroll
-      for (int b = 0; b < OB; ++b)
+      if ((s + 1) * kStep % GRAIN == 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) total[n][b][r] = __builtin_fmaf(scale[b][s], sum[n][b][r], total[n][b][r]);
+          for (int r = 0; r < 4; ++r) total[n][b][r] = __builtin_fmaf(scale[s], sum[n][r], total[n][b][r]);
+      }
     }
-    // or the compiler reads the operands of all four products first, and runs out of registers
-    if (NT * OB > 4) __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -360,14 +359,15 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   // Rounds past the last are loaded too (what the last holds): whether to load would be a branch,
   // after which every load has to be waited for.
   const int rounds = (a.chunks + WK - 1) / WK;
-  const auto load = [&](int i, Round& to) {  // round i of this group
-    const int chunk = (i < rounds ? i : rounds - 1) * WK + group;
-#pragma unroll
-    for (int b = 0; b < OB; ++b) to.code[b].load(a, codes, code_off[b], scales, scale_off[b], chunk);
+  const auto chunk_of = [&](int i) { return (i < rounds ? i : rounds - 1) * WK + group; };
+  const auto load_code = [&](int i, Round& to, int b) {
+    to.code[b].load(a, codes, code_off[b], scales, scale_off[b], chunk_of(i));
+  };
+  const auto load_rows = [&](int i, Round& to) {  // of round i of this group
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {  // row tiles past the last take its rows and are not stored
       const int f = e * kGroupWaves + mine, tile = row_block * kTiles + f % kTiles;
-      const v4u* from = a.frag + (((int64_t)chunk * kPlanes * 4 + f / kTiles) * a.row_tiles +
+      const v4u* from = a.frag + (((int64_t)chunk_of(i) * kPlanes * 4 + f / kTiles) * a.row_tiles +
                                   (tile < a.row_tiles ? tile : a.row_tiles - 1)) * kWave;
       to.x[e] = from[l];
     }
@@ -383,29 +383,27 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int b = 0; b < OB; ++b) total[n][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  const auto add = [&](const Codes<GRAIN>(&code)[OB], int buffer) {
-    add_chunk<X, GRAIN, NT, OB>(a, code, lds + ((buffer * WK + group) * kFrags + rw * NT) * kWave + l,
-                                4 * kTiles * kWave, kTiles * kWave, kWave, total);
+  // Round i: the rows of the round after the next are asked for, the products made, the codes of the
+  // round after the next asked for as soon as those here are used, the next round's rows put into LDS.
+  const auto round = [&](int i, Round& now, const Round& next) {
+    __syncthreads();
+    load_rows(i + 2, now);
+    add_chunk<X, GRAIN, NT, OB>(a, now.code, lds + ((i % 2 * WK + group) * kFrags + rw * NT) * kWave + l,
+                                4 * kTiles * kWave, kTiles * kWave, kWave, total,
+                                [&](int b) { load_code(i + 2, now, b); });
+    keep(next, i + 1);
   };
   Round even, odd;
-  load(0, even);
-  load(1, odd);
+#pragma unroll
+  for (int b = 0; b < OB; ++b) load_code(0, even, b);
+  load_rows(0, even);
+#pragma unroll
+  for (int b = 0; b < OB; ++b) load_code(1, odd, b);
+  load_rows(1, odd);
   keep(even, 0);
   for (int i = 0; i < rounds; i += 2) {
-    __syncthreads();
-    Codes<GRAIN> now[OB];
-#pragma unroll
-    for (int b = 0; b < OB; ++b) now[b] = even.code[b];
-    load(i + 2, even);
-    add(now, 0);
-    if (i + 1 >= rounds) break;
-    keep(odd, i + 1);
-    __syncthreads();
-#pragma unroll
-    for (int b = 0; b < OB; ++b) now[b] = odd.code[b];
-    load(i + 3, odd);
-    add(now, 1);
-    keep(even, i + 2);
+    round(i, even, odd);
+    if (i + 1 < rounds) round(i + 1, odd, even);
   }
   v4f* join = (v4f*)lds;
   if (WK > 1) {
@@ -529,7 +527,8 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
     for (int u = 0; u < kDeep; ++u) {
       const int chunk = first + u * WK;
       if (chunk >= end) break;
-      add_chunk<X, GRAIN, 1, OB>(a, now[u], from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total);
+      add_chunk<X, GRAIN, 1, OB>(a, now[u], from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total,
+                                 [](int) {});
     }
   }
 #pragma unroll
