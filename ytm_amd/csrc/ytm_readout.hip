@@ -210,6 +210,13 @@ __device__ __forceinline__ int place_of(int i) {
   return GRAIN == kChunk ? 4 * (i % 4) + i / 4 : i;
 }
 
+// A scale from its two halves, or the same 16 bits twice.
+__device__ __forceinline__ float scale_value(const ReadoutArgs& a, uint16_t low, uint16_t high) {
+  const float half = (float)__builtin_bit_cast(_Float16, high);
+  const float full = __uint_as_float((uint32_t)high << 16 | (a.scale_dtype == YTM_DTYPE_F32 ? low : 0u));
+  return a.scale_dtype == YTM_DTYPE_F16 ? half : full;
+}
+
 // A chunk's codes of one output a lane, and a scale: that of the whole chunk (GRAIN 128), or of the
 // 32 clauses whose codes the lane holds, which turn() then hands to all.
 template <int GRAIN>
@@ -232,10 +239,7 @@ struct Codes {
   }
   // scales of the four products
   __device__ __forceinline__ void scaled(const ReadoutArgs& a, float (&f)[4]) const {
-    const float half = (float)__builtin_bit_cast(_Float16, high);
-    const float full = __uint_as_float((uint32_t)high << 16 | (a.scale_dtype == YTM_DTYPE_F32 ? low : 0u));
-    const float v = a.scale_dtype == YTM_DTYPE_F16 ? half : full;
-    const uint32_t u = __float_as_uint(v);
+    const uint32_t u = __float_as_uint(scale_value(a, low, high));
     const v4u t = turn<GRAIN>(v4u{u, u, u, u});
 #pragma unroll
     for (int s = 0; s < 4; ++s) f[s] = __uint_as_float(t[s]);
@@ -253,11 +257,11 @@ __device__ __forceinline__ void store_out(const ReadoutArgs& a, int n, int o, fl
 
 // A chunk's products of NT row tiles, whose operands lie at from[plane * .. + step * .. + tile * ..], and OB
 // output tiles, added to the sums so far.  One output tile after the other, so that the scaling
-// of one can go beside the products of the next; next(b) is called once tile b's codes are not
-// needed any more.
-template <int X, int GRAIN, int NT, int OB, typename Next>
-__device__ __forceinline__ void add_chunk(const ReadoutArgs& a, const Codes<GRAIN> (&code)[OB], const v4u* from,
-                                          int plane, int step, int tile, v4f (&total)[NT][OB], Next next) {
+// of one can go beside the products of the next; code(b, w, scale) gives tile b's codes and the
+// scales of its four products.
+template <int X, int GRAIN, int NT, int OB, typename Code>
+__device__ __forceinline__ void add_chunk(const v4u* from, int plane, int step, int tile, v4f (&total)[NT][OB],
+                                          Code code) {
   constexpr int kPlanes = Kind<X>::kPlanes;
   constexpr bool kHalf = Kind<X>::kHalf;
   v4u x[4][kPlanes][NT];
@@ -269,21 +273,19 @@ __device__ __forceinline__ void add_chunk(const ReadoutArgs& a, const Codes<GRAI
       for (int n = 0; n < NT; ++n) x[s][p][n] = from[p * plane + s * step + n * tile];
 #pragma unroll
   for (int b = 0; b < OB; ++b) {
-    const v4u w = turn<GRAIN>(code[b].w);
+    v4u w;
     float scale[4];
-    code[b].scaled(a, scale);
-    v4u y[4];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) y[s] = codes_to_16<kHalf>(w[s]);
-    next(b);
+    code(b, w, scale);
+    w = turn<GRAIN>(w);
     v4f sum[NT];
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
+      const v4u y = codes_to_16<kHalf>(w[s]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (s * kStep % GRAIN == 0) sum[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int p = kPlanes - 1; p >= 0; --p) sum[n] = product<kHalf>(x[s][p][n], y[s], sum[n]);
+        for (int p = kPlanes - 1; p >= 0; --p) sum[n] = product<kHalf>(x[s][p][n], y, sum[n]);
       }
       if ((s + 1) * kStep % GRAIN == 0) {
 #pragma unroll
@@ -317,19 +319,31 @@ __global__ __launch_bounds__(kPieces* kTile) void rows_kernel(ReadoutArgs a) {
 // A block takes 16 NT RW rows and 16 OB WO outputs; its waves are WK groups, each with chunks of
 // clauses of its own, of WO x RW waves, each with NT tiles of rows and OB of outputs.  Lane l takes
 // the codes of output l % 16 as a product's second operand and gets sums of rows 4 (l / 16) .. + 3
-// of that output.  A group keeps a chunk of its rows' operands in LDS; the next chunk is in
-// registers or on its way, and the one after it is asked for before the products of this one, as
-// are the codes.  The groups' sums are joined in LDS in their order.
+// of that output.
+//
+// A group keeps a chunk of its rows' operands in LDS, and two chunks of its outputs' codes and
+// scales: 128 bytes of codes in a row, which a wave that loaded its own 16 outputs' chunk would take
+// in halves, and twice where two waves have the same outputs.  (With each wave loading its own,
+// 512 rows x 20000 clauses x 10000 outputs took 340 us, of which 150 went without these loads.)
+// What comes next is on its way meanwhile: rows are asked for a chunk ahead, codes two.  The groups' sums are joined in LDS in their order.
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) {
   constexpr int kPlanes = Kind<X>::kPlanes;
-  constexpr int kGroupWaves = RW * WO;
+  constexpr int kGroupWaves = RW * WO, kGroupThreads = kWave * kGroupWaves;
   constexpr int kTiles = NT * RW;               // of rows
   constexpr int kFrags = kPlanes * 4 * kTiles;  // operands of a chunk
   constexpr int kEach = kFrags / kGroupWaves;   // that a wave loads
   static_assert(kFrags % kGroupWaves == 0, "");
+  constexpr int kOuts = kTile * OB * WO;
+  constexpr int kGrains = kChunk / GRAIN;                      // scales of a chunk
+  constexpr int kCodes = 2 * 4 * kOuts / kGroupThreads;        // 16-byte pieces of codes a thread loads
+  constexpr int kScales = (2 * kGrains * kOuts + kGroupThreads - 1) / kGroupThreads;
+  static_assert(2 * 4 * kOuts % kGroupThreads == 0, "");
   constexpr int kJoin = (WK - 1) * kGroupWaves * NT * OB;
-  __shared__ v4u lds[(2 * WK * kFrags > kJoin ? 2 * WK * kFrags : kJoin) * kWave];
+  constexpr int kRowSpace = 2 * WK * kFrags;
+  __shared__ v4u lds[(kRowSpace > kJoin ? kRowSpace : kJoin) * kWave];
+  __shared__ v4u held_codes[2][WK][2][kOuts * 4];
+  __shared__ float held_scales[2][WK][2][kGrains][kOuts];
 
   // blocks of the same outputs one after the other on the same XCD, whose L2 then has the codes
   const int row_blocks = (a.row_tiles + kTiles - 1) / kTiles;
@@ -338,41 +352,72 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   if (out_tile >= a.out_tiles) return;
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int group = wave / kGroupWaves, mine = wave % kGroupWaves, wo = mine / RW, rw = mine % RW;
-  const int first_out = (out_tile * WO + wo) * OB * kTile + l % 16;
+  const int t = threadIdx.x % kGroupThreads;
+  const int block_out = out_tile * kOuts;
 
   // uniform addresses and 32-bit distances from them take fewer registers than addresses
-  const int block_out = out_tile * WO * OB * kTile;
-  const int size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  const uint32_t size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
   const uint8_t* codes = a.codes + block_out * a.code_stride;
   const char* scales = (const char*)a.scales + block_out * a.scale_stride * size;
-  uint32_t code_off[OB], scale_off[OB];
+  // outputs past the last take its codes and are not stored
+  const auto output = [&](int o) { return (uint32_t)((block_out + o < a.K ? block_out + o : a.K - 1) - block_out); };
+  uint32_t code_off[kCodes], scale_off[kScales];
 #pragma unroll
-  for (int b = 0; b < OB; ++b) {  // outputs past the last take its codes and are not stored
-    const uint32_t o = (first_out + b * kTile < a.K ? first_out + b * kTile : a.K - 1) - block_out;
-    code_off[b] = o * (uint32_t)a.code_stride;
-    scale_off[b] = o * (uint32_t)a.scale_stride * size;
+  for (int e = 0; e < kCodes; ++e) code_off[e] = output((e * kGroupThreads + t) / 8) * (uint32_t)a.code_stride;
+#pragma unroll
+  for (int e = 0; e < kScales; ++e) {
+    const int j = (e * kGroupThreads + t) / (2 * kGrains);
+    scale_off[e] = output(j < kOuts ? j : 0) * (uint32_t)a.scale_stride * size;
   }
-  struct Round {
+  // Chunks past the last are loaded too: whether to load would be a branch, after which every load
+  // has to be waited for.  Their rows are zero up to the last pair's end, and what is loaded past it is
+  // not used.
+  const int pairs = (a.chunks + 2 * WK - 1) / (2 * WK);
+  const uint32_t steps = (a.C + kStep - 1) / kStep;
+  v4u code[kCodes];
+  uint16_t low[kScales], high[kScales];
+  const auto load_codes = [&](int pair) {
+    const uint32_t first = (uint32_t)(pair * WK + group) * 2 * 4;  // step
+#pragma unroll
+    for (int e = 0; e < kCodes; ++e) {
+      const uint32_t step = first + (e * kGroupThreads + t) % 8;
+      code[e] = *(const v4u*)(codes + (code_off[e] + 16 * (step < steps ? step : steps - 1)));
+    }
+#pragma unroll
+    for (int e = 0; e < kScales; ++e) {
+      const uint32_t step = first + (e * kGroupThreads + t) % (2 * kGrains) * (4 / kGrains);
+      const uint32_t at = scale_off[e] + __umulhi(step < steps ? step + 1 : steps, a.inverse) * size;
+      low[e] = *(const uint16_t*)(scales + at);
+      high[e] = *(const uint16_t*)(scales + (at + size - 2));
+    }
+  };
+  const auto keep_codes = [&](int pair) {
+#pragma unroll
+    for (int e = 0; e < kCodes; ++e) {
+      const int j = e * kGroupThreads + t;
+      held_codes[pair % 2][group][j % 8 / 4][j / 8 * 4 + j % 4] = code[e];
+    }
+#pragma unroll
+    for (int e = 0; e < kScales; ++e) {
+      const int j = e * kGroupThreads + t, o = j / (2 * kGrains), i = j % (2 * kGrains);
+      if (o < kOuts) held_scales[pair % 2][group][i / kGrains][i % kGrains][o] = scale_value(a, low[e], high[e]);
+    }
+  };
+  const int padded = pairs * 2 * WK;
+  struct Rows {
     v4u x[kEach];
-    Codes<GRAIN> code[OB];
   };
-  // Rounds past the last are loaded too (what the last holds): whether to load would be a branch,
-  // after which every load has to be waited for.
-  const int rounds = (a.chunks + WK - 1) / WK;
-  const auto chunk_of = [&](int i) { return (i < rounds ? i : rounds - 1) * WK + group; };
-  const auto load_code = [&](int i, Round& to, int b) {
-    to.code[b].load(a, codes, code_off[b], scales, scale_off[b], chunk_of(i));
-  };
-  const auto load_rows = [&](int i, Round& to) {  // of round i of this group
+  const auto load_rows = [&](int i, Rows& to) {  // of chunk i of this group's
+    const int own = (i / 2 * WK + group) * 2 + i % 2, chunk = own < padded ? own : padded - 1;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {  // row tiles past the last take its rows and are not stored
       const int f = e * kGroupWaves + mine, tile = row_block * kTiles + f % kTiles;
-      const v4u* from = a.frag + (((int64_t)chunk_of(i) * kPlanes * 4 + f / kTiles) * a.row_tiles +
+      const v4u* from = a.frag + (((int64_t)chunk * kPlanes * 4 + f / kTiles) * a.row_tiles +
                                   (tile < a.row_tiles ? tile : a.row_tiles - 1)) * kWave;
       to.x[e] = from[l];
     }
   };
-  const auto keep = [&](const Round& of, int i) {  // of round i
+  const auto keep_rows = [&](const Rows& of, int i) {
     v4u* to = lds + (i % 2 * WK + group) * kFrags * kWave;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) to[(e * kGroupWaves + mine) * kWave + l] = of.x[e];
@@ -383,27 +428,35 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int b = 0; b < OB; ++b) total[n][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  // Round i: the rows of the round after the next are asked for, the products made, the codes of the
-  // round after the next asked for as soon as those here are used, the next round's rows put into LDS.
-  const auto round = [&](int i, Round& now, const Round& next) {
-    __syncthreads();
-    load_rows(i + 2, now);
-    add_chunk<X, GRAIN, NT, OB>(a, now.code, lds + ((i % 2 * WK + group) * kFrags + rw * NT) * kWave + l,
-                                4 * kTiles * kWave, kTiles * kWave, kWave, total,
-                                [&](int b) { load_code(i + 2, now, b); });
-    keep(next, i + 1);
+  const auto add = [&](int pair, int half) {
+    const int o = wo * OB * kTile;
+    const v4u* w_from = held_codes[pair % 2][group][half] + (o + l % 16) * 4 + l / 16;
+    const float* s_from = held_scales[pair % 2][group][half][0] + o + l % 16;
+    add_chunk<X, GRAIN, NT, OB>(lds + ((half * WK + group) * kFrags + rw * NT) * kWave + l, 4 * kTiles * kWave,
+                                kTiles * kWave, kWave, total, [&](int b, v4u& w, float(&scale)[4]) {
+                                  w = w_from[b * kTile * 4];
+#pragma unroll
+                                  for (int s = 0; s < 4; ++s) scale[s] = s_from[s * kGrains / 4 * kOuts + b * kTile];
+                                });
   };
-  Round even, odd;
-#pragma unroll
-  for (int b = 0; b < OB; ++b) load_code(0, even, b);
-  load_rows(0, even);
-#pragma unroll
-  for (int b = 0; b < OB; ++b) load_code(1, odd, b);
-  load_rows(1, odd);
-  keep(even, 0);
-  for (int i = 0; i < rounds; i += 2) {
-    round(i, even, odd);
-    if (i + 1 < rounds) round(i + 1, odd, even);
+  Rows next;
+  load_codes(0);
+  load_rows(0, next);
+  keep_codes(0);
+  keep_rows(next, 0);
+  for (int i = 0; i < pairs; ++i) {
+    __syncthreads();
+    load_codes(i + 1);
+    load_rows(2 * i + 1, next);
+    __builtin_amdgcn_sched_barrier(0);  // or the loads sink to where they are needed
+    add(i, 0);
+    keep_rows(next, 1);
+    __syncthreads();
+    load_rows(2 * i + 2, next);
+    __builtin_amdgcn_sched_barrier(0);
+    add(i, 1);
+    keep_rows(next, 0);
+    keep_codes(i + 1);
   }
   v4f* join = (v4f*)lds;
   if (WK > 1) {
@@ -424,7 +477,7 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
     for (int b = 0; b < OB; ++b) {
       v4f v = total[n][b];
       for (int g = 0; g < WK - 1; ++g) v += join[((g * kGroupWaves + mine) * NT * OB + n * OB + b) * kWave + l];
-      const int o = first_out + b * kTile;
+      const int o = block_out + (wo * OB + b) * kTile + l % 16;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = (row_block * kTiles + rw * NT + n) * kTile + l / 16 * 4 + r;
@@ -433,9 +486,9 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
     }
 }
 
-// Chunks of the rows' operands: a whole number for each of up to kGroups groups of waves.
+// Chunks of the rows' operands: whole pairs for each of up to kGroups groups of waves.
 constexpr int kGroups = 2;
-int padded_of(int chunks) { return (chunks + kGroups - 1) / kGroups * kGroups; }
+int padded_of(int chunks) { return (chunks + 2 * kGroups - 1) / (2 * kGroups) * (2 * kGroups); }
 
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 hipError_t launch_tile(ReadoutArgs a, hipStream_t s) {
@@ -527,8 +580,11 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
     for (int u = 0; u < kDeep; ++u) {
       const int chunk = first + u * WK;
       if (chunk >= end) break;
-      add_chunk<X, GRAIN, 1, OB>(a, now[u], from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total,
-                                 [](int) {});
+      add_chunk<X, GRAIN, 1, OB>(from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total,
+                                 [&](int b, v4u& w, float(&scale)[4]) {
+                                   w = now[u][b].w;
+                                   now[u][b].scaled(a, scale);
+                                 });
     }
   }
 #pragma unroll
