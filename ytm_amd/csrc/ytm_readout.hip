@@ -218,28 +218,30 @@ __device__ __forceinline__ float scale_value(const ReadoutArgs& a, uint16_t low,
 }
 
 // A chunk's codes of one output a lane, and a scale: that of the whole chunk (GRAIN 128), or of the
-// 32 clauses whose codes the lane holds, which turn() then hands to all.
-template <int GRAIN>
+// 32 clauses whose codes the lane holds, which turn() then hands to all.  WIDE: scales are float32.
+template <int GRAIN, bool WIDE>
 struct Codes {
   v4u w;
-  uint16_t low, high;  // of the scale; the same twice where it has 16 bits, so that no load needs a branch
+  typename std::conditional<WIDE, float, uint16_t>::type scale;
 
   // of the output whose codes are `code` bytes from the uniform address `codes` and whose scales are
-  // `scale` bytes from `scales`.  Past the last clause the last codes are taken: the rows are zero there.
+  // `at` bytes from `scales`.  Past the last clause the last codes are taken: the rows are zero there.
   __device__ __forceinline__ void load(const ReadoutArgs& a, const uint8_t* codes, uint32_t code, const char* scales,
-                                       uint32_t scale, int chunk) {
+                                       uint32_t at, int chunk) {
     const uint32_t steps = (a.C + kStep - 1) / kStep;
     const uint32_t mine = chunk * 4 + threadIdx.x % kWave / 16;
     w = *(const v4u*)(codes + (code + 16 * (mine < steps ? mine : steps - 1)));
     const uint32_t step = GRAIN == kChunk ? chunk * 4 : mine;
-    const uint32_t size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
-    scale += __umulhi(step < steps ? step + 1 : steps, a.inverse) * size;
-    low = *(const uint16_t*)(scales + scale);
-    high = *(const uint16_t*)(scales + (scale + size - 2));
+    const uint32_t q = __umulhi(step < steps ? step + 1 : steps, a.inverse);
+    scale = *(const decltype(scale)*)(scales + (at + q * (uint32_t)sizeof scale));
   }
   // scales of the four products
   __device__ __forceinline__ void scaled(const ReadoutArgs& a, float (&f)[4]) const {
-    const uint32_t u = __float_as_uint(scale_value(a, low, high));
+    uint32_t u;
+    if constexpr (WIDE)
+      u = __float_as_uint(scale);
+    else
+      u = __float_as_uint(scale_value(a, scale, scale));
     const v4u t = turn<GRAIN>(v4u{u, u, u, u});
 #pragma unroll
     for (int s = 0; s < 4; ++s) f[s] = __uint_as_float(t[s]);
@@ -336,9 +338,9 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   static_assert(kFrags % kGroupWaves == 0, "");
   constexpr int kOuts = kTile * OB * WO;
   constexpr int kGrains = kChunk / GRAIN;                      // scales of a chunk
-  constexpr int kCodes = 2 * 4 * kOuts / kGroupThreads;        // 16-byte pieces of codes a thread loads
+  // 16-byte pieces of codes and scales a thread loads, the last of them twice where they do not come out even
+  constexpr int kCodes = (2 * 4 * kOuts + kGroupThreads - 1) / kGroupThreads;
   constexpr int kScales = (2 * kGrains * kOuts + kGroupThreads - 1) / kGroupThreads;
-  static_assert(2 * 4 * kOuts % kGroupThreads == 0, "");
   constexpr int kJoin = (WK - 1) * kGroupWaves * NT * OB;
   constexpr int kRowSpace = 2 * WK * kFrags;
   __shared__ v4u lds[(kRowSpace > kJoin ? kRowSpace : kJoin) * kWave];
@@ -363,7 +365,10 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   const auto output = [&](int o) { return (uint32_t)((block_out + o < a.K ? block_out + o : a.K - 1) - block_out); };
   uint32_t code_off[kCodes], scale_off[kScales];
 #pragma unroll
-  for (int e = 0; e < kCodes; ++e) code_off[e] = output((e * kGroupThreads + t) / 8) * (uint32_t)a.code_stride;
+  for (int e = 0; e < kCodes; ++e) {
+    const int j = (e * kGroupThreads + t) / 8;
+    code_off[e] = output(j < kOuts ? j : 0) * (uint32_t)a.code_stride;
+  }
 #pragma unroll
   for (int e = 0; e < kScales; ++e) {
     const int j = (e * kGroupThreads + t) / (2 * kGrains);
@@ -395,7 +400,7 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
 #pragma unroll
     for (int e = 0; e < kCodes; ++e) {
       const int j = e * kGroupThreads + t;
-      held_codes[pair % 2][group][j % 8 / 4][j / 8 * 4 + j % 4] = code[e];
+      if (j < 8 * kOuts) held_codes[pair % 2][group][j % 8 / 4][j / 8 * 4 + j % 4] = code[e];
     }
 #pragma unroll
     for (int e = 0; e < kScales; ++e) {
@@ -506,11 +511,11 @@ hipError_t launch_tile(ReadoutArgs a, hipStream_t s) {
 // Few rows (up to 16): a block has 16 OB WO outputs and the clauses of one of the parts that the
 // grid's second axis counts, whose row operands lie in LDS from the start (without those of rows
 // that are not there), so that nothing waits between its first and last chunk.  WK waves share
-// an output tile's chunks; each loads kAhead of them before the first is looked at.  With more
+// an output tile's chunks, two at a time (128 bytes of codes); each loads kAhead of them before the first is looked at.  With more
 // than one part the sums go to the workspace, [part][row][output].
 template <int OB>
 constexpr int kAhead = OB == 1 ? 4 : 2;
-template <int X, int GRAIN, int OB, int WO, int WK>
+template <int X, int GRAIN, int OB, int WO, int WK, bool WIDE>
 __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
   constexpr int kPlanes = Kind<X>::kPlanes;
   constexpr int kDeep = kAhead<OB>;
@@ -522,7 +527,7 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
   const int end = begin + a.part_chunks < a.chunks ? begin + a.part_chunks : a.chunks;
   const int first_out = (blockIdx.x * WO + wo) * OB * kTile + l % 16;
   const int block_out = blockIdx.x * WO * OB * kTile;
-  const int size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  constexpr int size = WIDE ? 4 : 2;
   const uint8_t* codes = a.codes + block_out * a.code_stride;
   const char* scales = (const char*)a.scales + block_out * a.scale_stride * size;
   uint32_t code_off[OB], scale_off[OB];
@@ -532,15 +537,17 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
     code_off[b] = o * (uint32_t)a.code_stride;
     scale_off[b] = o * (uint32_t)a.scale_stride * size;
   }
-  Codes<GRAIN> code[kDeep][OB];
-  const auto load = [&](int chunk) {
+  Codes<GRAIN, WIDE> code[kDeep][OB];
+  // this wave's u-th chunk from `first` on
+  const auto chunk_at = [&](int first, int u) { return first + u / 2 * (2 * WK) + u % 2; };
+  const auto load = [&](int first) {
 #pragma unroll
     for (int u = 0; u < kDeep; ++u)
 #pragma unroll
       for (int b = 0; b < OB; ++b)
-        code[u][b].load(a, codes, code_off[b], scales, scale_off[b], chunk + u * WK);
+        code[u][b].load(a, codes, code_off[b], scales, scale_off[b], chunk_at(first, u));
   };
-  load(begin + wk);
+  load(begin + 2 * wk);
   const int count = (end - begin) * kPieces;
   constexpr int kAtOnce = kPlanes == 1 ? 4 : 2;
   for (int first = threadIdx.x; first < a.N * count; first += kAtOnce * kWave * WO * WK) {
@@ -569,8 +576,8 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
   v4f total[1][OB];
 #pragma unroll
   for (int b = 0; b < OB; ++b) total[0][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int first = begin + wk; first < end; first += kDeep * WK) {
-    Codes<GRAIN> now[kDeep][OB];
+  for (int first = begin + 2 * wk; first < end; first += kDeep * WK) {
+    Codes<GRAIN, WIDE> now[kDeep][OB];
 #pragma unroll
     for (int u = 0; u < kDeep; ++u)
 #pragma unroll
@@ -578,7 +585,7 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
     if (first + kDeep * WK < end) load(first + kDeep * WK);
 #pragma unroll
     for (int u = 0; u < kDeep; ++u) {
-      const int chunk = first + u * WK;
+      const int chunk = chunk_at(first, u);
       if (chunk >= end) break;
       add_chunk<X, GRAIN, 1, OB>(from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total,
                                  [&](int b, v4u& w, float(&scale)[4]) {
@@ -638,7 +645,10 @@ hipError_t launch_held(ReadoutArgs a, hipStream_t s) {
   a.part_chunks = part_chunks_of(Kind<X>::kPlanes, a.N, a.chunks);
   const size_t lds = (size_t)a.N * Kind<X>::kPlanes * a.part_chunks * kPieces * 16;
   const dim3 grid((unsigned)((a.K + kTile * OB * WO - 1) / (kTile * OB * WO)), (unsigned)parts);
-  held_kernel<X, GRAIN, OB, WO, WK><<<grid, kWave * WO * WK, lds, s>>>(a);
+  if (a.scale_dtype == YTM_DTYPE_F32)
+    held_kernel<X, GRAIN, OB, WO, WK, true><<<grid, kWave * WO * WK, lds, s>>>(a);
+  else
+    held_kernel<X, GRAIN, OB, WO, WK, false><<<grid, kWave * WO * WK, lds, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || parts == 1) return e;
   const int64_t blocks = ((int64_t)a.N * a.K + 255) / 256;
@@ -680,7 +690,7 @@ template <int X, int GRAIN>
 hipError_t launch_rows(const ReadoutArgs& a, hipStream_t s) {
   constexpr bool kOne = Kind<X>::kPlanes == 1;
   if (a.N <= kFewRows) {
-    if (parts_of(Kind<X>::kPlanes, a.N, a.chunks) > 1) return launch_held<X, GRAIN, 2, 4, 2>(a, s);
+    if (parts_of(Kind<X>::kPlanes, a.N, a.chunks) > 1) return launch_held<X, GRAIN, 2, 8, 1>(a, s);
     return a.K <= 4096 ? launch_held<X, GRAIN, 1, 1, 16>(a, s) : launch_held<X, GRAIN, 1, 1, 4>(a, s);
   }
   if (a.N <= 32) return launch_tile<X, GRAIN, 2, 1, 2, 4, kOne ? 2 : 1>(a, s);
@@ -688,7 +698,7 @@ hipError_t launch_rows(const ReadoutArgs& a, hipStream_t s) {
   if constexpr (kOne) {
     const bool narrow = (a.N + 95) / 96 * 96 < (a.N + 127) / 128 * 128;
     if (narrow) return launch_tile<X, GRAIN, 3, 2, 2, 4, 1>(a, s);
-    return launch_tile<X, GRAIN, 4, 2, GRAIN == kChunk ? 3 : 2, 4, 1>(a, s);
+    return launch_tile<X, GRAIN, 2, 4, 5, 2, 1>(a, s);
   }
 }
 
