@@ -36,59 +36,123 @@ struct AdjustArgs {
   int64_t out_stride;
 };
 
+// A block takes kPacks packs of 16 bytes of scores for each of its threads, and counts its answers'
+// occurrences in LDS from the whole of the row's history: integers, so their order does not matter.
+// What it reads of scores, bias and grammar is on its way before the history is looked at.
 constexpr int kAdjustThreads = 256;
-constexpr int kChunk = 4096;            // answers of a block
-constexpr uint32_t kTold = 0x80000000u; // the answer stands in the prompt
+constexpr uint32_t kTold = 0x80000000u;  // the answer stands in the prompt
 
-template <typename In, typename Out>
+template <typename In, typename Out, int kPacks>
 __global__ __launch_bounds__(kAdjustThreads) void adjust_kernel(AdjustArgs a) {
+  constexpr int n_ = 16 / sizeof(In);  // scores of a pack
+  constexpr int kChunk = kPacks * n_ * kAdjustThreads;
   __shared__ uint32_t counts[kChunk];
   const int64_t n = blockIdx.y;
   const int64_t first = blockIdx.x * (int64_t)kChunk;
   const int here = (int)(a.V - first < kChunk ? a.V - first : kChunk);
-  if (a.tokens) {
-    for (int i = threadIdx.x; i < kChunk; i += kAdjustThreads) counts[i] = 0u;
-    __syncthreads();
-    const int64_t length = a.lengths ? (a.lengths[n] < a.T ? a.lengths[n] : a.T) : a.T;
-    const int64_t prompt = a.prompt ? a.prompt[n] : 0;
-    const int32_t* tokens = a.tokens + n * a.token_stride;
-    for (int64_t i = threadIdx.x; i < length; i += kAdjustThreads) {
-      const int64_t at = tokens[i] - first;
-      if (at >= 0 && at < here) {
-        if (i >= prompt)
-          atomicAdd(&counts[at], 1u);
-        else
-          atomicOr(&counts[at], kTold);
-      }
-    }
-    __syncthreads();
-  }
-  const float repetition = a.repetition ? a.repetition[n] : 1.0f;
-  const float frequency = a.frequency ? a.frequency[n] : 0.0f, presence = a.presence ? a.presence[n] : 0.0f;
   const In* in = (const In*)a.scores + n * a.stride + first;
   Out* out = (Out*)a.out + n * a.out_stride + first;
   const float* bias = a.bias ? a.bias + n * a.bias_stride + first : nullptr;
   const uint32_t* allowed = a.allowed ? a.allowed + n * a.allowed_stride + first / 32 : nullptr;
-  for (int i = threadIdx.x; i < here; i += kAdjustThreads) {
-    float s = to_float(in[i]);
-    const uint32_t c = a.tokens ? counts[i] : 0u;
-    if (c) {
-      s = s > 0.0f ? s / repetition : s * repetition;
-      if (c & ~kTold) {
-        s -= frequency * (float)(c & ~kTold);
-        s -= presence;
+  In score[kPacks][n_];
+  float more[kPacks][n_];
+  uint32_t may[kPacks];
+#pragma unroll
+  for (int p = 0; p < kPacks; ++p) {
+    const int i = (p * kAdjustThreads + threadIdx.x) * n_;
+    if (i + n_ <= here) {
+      __builtin_memcpy(score[p], in + i, sizeof score[p]);
+      if (bias) __builtin_memcpy(more[p], bias + i, sizeof more[p]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < n_; ++j) {
+        score[p][j] = i + j < here ? in[i + j] : In{};
+        if (bias) more[p][j] = i + j < here ? bias[i + j] : 0.0f;
       }
     }
-    if (bias) s += bias[i];
-    if (allowed && !(allowed[i / 32] >> (i % 32) & 1u)) s = -INFINITY;
-    out[i] = from_float<Out>(s);
+    may[p] = allowed && i < here ? allowed[i / 32] : 0xFFFFFFFFu;
+  }
+  bool said = false;
+  float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
+  if (a.tokens) {
+    const int64_t length = a.lengths ? (a.lengths[n] < a.T ? a.lengths[n] : a.T) : a.T;
+    const int64_t prompt = a.prompt ? a.prompt[n] : 0;
+    const int32_t* tokens = a.tokens + n * a.token_stride;
+    if (a.repetition) repetition = a.repetition[n];
+    if (a.frequency) frequency = a.frequency[n];
+    if (a.presence) presence = a.presence[n];
+    for (int i = threadIdx.x; i < kChunk / 4; i += kAdjustThreads) ((uint4*)counts)[i] = uint4{0u, 0u, 0u, 0u};
+    __syncthreads();
+    for (int64_t at = threadIdx.x; at < length; at += 8 * kAdjustThreads) {
+      int32_t t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // past the end the last entry, which is not counted again
+        const int64_t k = at + j * kAdjustThreads;
+        t[j] = tokens[k < length ? k : length - 1];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t k = at + j * kAdjustThreads, v = t[j] - first;
+        if (k < length && v >= 0 && v < here) {
+          said = true;
+          if (k >= prompt)
+            atomicAdd(&counts[v], 1u);
+          else
+            atomicOr(&counts[v], kTold);
+        }
+      }
+    }
+    said = __syncthreads_or(said);
+  }
+#pragma unroll
+  for (int p = 0; p < kPacks; ++p) {
+    const int i = (p * kAdjustThreads + threadIdx.x) * n_;
+    if (i >= here) break;
+    float s[n_];
+#pragma unroll
+    for (int j = 0; j < n_; ++j) s[j] = to_float(score[p][j]);
+    if (said) {
+      uint32_t c[n_];
+#pragma unroll
+      for (int j = 0; j < n_; j += 4) *(uint4*)(c + j) = *(const uint4*)(counts + i + j);
+#pragma unroll
+      for (int j = 0; j < n_; ++j)
+        if (c[j]) {
+          s[j] = s[j] > 0.0f ? s[j] / repetition : s[j] * repetition;
+          if (c[j] & ~kTold) {
+            s[j] -= frequency * (float)(c[j] & ~kTold);
+            s[j] -= presence;
+          }
+        }
+    }
+    Out r[n_];
+#pragma unroll
+    for (int j = 0; j < n_; ++j) {
+      if (bias) s[j] += more[p][j];
+      r[j] = from_float<Out>(may[p] >> ((i + j) % 32) & 1u ? s[j] : -INFINITY);
+    }
+    if (i + n_ <= here) {
+      __builtin_memcpy(out + i, r, sizeof r);
+    } else {
+#pragma unroll
+      for (int j = 0; j < n_; ++j)
+        if (i + j < here) out[i + j] = r[j];
+    }
   }
 }
 
+// Blocks of 4096 answers count a row's history 4096 / 1024 times less often than blocks of 1024,
+// which a few short rows take so that more than a few CUs work.
 template <typename In, typename Out>
 hipError_t launch_adjust(const AdjustArgs& a, int64_t N, hipStream_t s) {
-  const dim3 grid((unsigned)((a.V + kChunk - 1) / kChunk), (unsigned)N);
-  adjust_kernel<In, Out><<<grid, kAdjustThreads, 0, s>>>(a);
+  constexpr int kMany = 16 / (16 / sizeof(In));
+  const auto blocks = [&](int answers) { return (a.V + answers - 1) / answers; };
+  if (N * blocks(4096) >= 256)
+    adjust_kernel<In, Out, kMany><<<dim3((unsigned)blocks(4096), (unsigned)N), kAdjustThreads, 0, s>>>(a);
+  else if (sizeof(In) == 4)
+    adjust_kernel<In, Out, 1><<<dim3((unsigned)blocks(1024), (unsigned)N), kAdjustThreads, 0, s>>>(a);
+  else
+    adjust_kernel<In, Out, 1><<<dim3((unsigned)blocks(2048), (unsigned)N), kAdjustThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
