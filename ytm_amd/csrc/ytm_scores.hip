@@ -202,10 +202,13 @@ constexpr int kChooseThreads = 1024;
 constexpr int kChooseWaves = kChooseThreads / kWave;
 constexpr int kDigits = 256;
 constexpr float kMass = 1099511627776.0f;  // 2^40
-constexpr int kPack = 8;                   // scores a thread takes at once
-constexpr int kRound = kPack * kChooseThreads;
+template <typename In>
+constexpr int kPack = 16 / sizeof(In);  // scores of a 16-byte load
+template <typename In>
+constexpr int kRound = kPack<In> * kChooseThreads;
 constexpr int kList = 4096;
-constexpr int kMaxSeek = 256;  // a quarter of the threads, so that few maxima share a thread
+constexpr int kSmall = 256;    // entries that one wave sorts in registers
+constexpr int kMaxSeek = 256;  // a quarter of the threads, so that few of the largest share a thread
 constexpr int kBins = 2048;
 constexpr float kBinsPerUnit = 64.0f;
 
@@ -239,29 +242,29 @@ __device__ __forceinline__ u64 drawn_of(float z, int i, const float* noise) {
   return (u64)key_of(y) << 32 | (uint32_t)~i;
 }
 
-// kPack elements of a row from element i on, as they are in memory: loads that need no alignment
+// P elements of a row from element i on, as they are in memory: loads that need no alignment
 // and no branch, so that several are on their way at once.  A pack that would pass the row's end
-// V is taken from V - kPack, and the elements before i are not its own.
-template <typename In>
+// V is taken from V - P, and the elements before i are not its own.
+template <typename In, int P>
 struct Pack {
-  In raw[kPack];
+  In raw[P];
   __device__ __forceinline__ int load(const In* in, int i, int V) {
-    const int at = i + kPack <= V ? i : V - kPack;
-    if (V >= kPack) {
+    const int at = i + P <= V ? i : V - P;
+    if (V >= P) {
       __builtin_memcpy(raw, in + at, sizeof raw);
     } else {
 #pragma unroll
-      for (int j = 0; j < kPack; ++j) raw[j] = at + j >= 0 ? in[at + j] : In{};
+      for (int j = 0; j < P; ++j) raw[j] = at + j >= 0 ? in[at + j] : In{};
     }
     return at;
   }
   // the elements as floats, `past` for those not the pack's own
-  __device__ __forceinline__ void values(int i, int at, float past, float (&v)[kPack]) const {
+  __device__ __forceinline__ void values(int i, int at, float past, float (&v)[P]) const {
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) v[j] = to_float(raw[j]);
+    for (int j = 0; j < P; ++j) v[j] = to_float(raw[j]);
     if (at != i) {
 #pragma unroll
-      for (int j = 0; j < kPack; ++j) v[j] = at + j >= i && at + j >= 0 ? v[j] : past;
+      for (int j = 0; j < P; ++j) v[j] = at + j >= i && at + j >= 0 ? v[j] : past;
     }
   }
 };
@@ -271,25 +274,81 @@ struct Pack {
 // looked at.
 template <int U, typename In, typename F>
 __device__ __forceinline__ void each_pack(const In* in, int V, int end, F f) {
-  for (int first = kPack * threadIdx.x; first < end; first += U * kRound) {
-    Pack<In> pack[U];
+  constexpr int P = kPack<In>;
+  for (int first = P * threadIdx.x; first < end; first += U * kRound<In>) {
+    Pack<In, P> pack[U];
     int at[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) at[u] = pack[u].load(in, first + u * kRound, V);
+    for (int u = 0; u < U; ++u) at[u] = pack[u].load(in, first + u * kRound<In>, V);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float v[kPack];
-      pack[u].values(first + u * kRound, at[u], -INFINITY, v);
+      float v[P];
+      pack[u].values(first + u * kRound<In>, at[u], -INFINITY, v);
       f(at[u], v);
     }
   }
 }
 
-__device__ __forceinline__ float most(const float (&v)[kPack]) {  // NaN only where all are
+template <int P>
+__device__ __forceinline__ float most(const float (&v)[P]) {  // NaN only where all are
   float m = v[0];
 #pragma unroll
-  for (int j = 1; j < kPack; ++j) m = fmaxf(m, v[j]);
+  for (int j = 1; j < P; ++j) m = fmaxf(m, v[j]);
   return m;
+}
+
+// ---- sums, maxima and exchanges of a wave in registers (data-parallel moves between lanes)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved(u64 v) {  // 0 where no lane's value moves to
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, true);
+  return (u64)hi << 32 | lo;
+}
+// Inclusive scans: 1, 2, 4 and 8 lanes up within rows of 16, then the last of a row to the next
+// row and the last of the lower half to the upper.
+template <typename Op>
+__device__ __forceinline__ u64 wave_scan(u64 v, Op op) {
+  v = op(v, moved<0x111, 0xF>(v));
+  v = op(v, moved<0x112, 0xF>(v));
+  v = op(v, moved<0x114, 0xF>(v));
+  v = op(v, moved<0x118, 0xF>(v));
+  v = op(v, moved<0x142, 0xA>(v));
+  v = op(v, moved<0x143, 0xC>(v));
+  return v;
+}
+struct Add {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a > b ? a : b; }
+};
+__device__ __forceinline__ u64 lane_value(u64 v, int lane) {  // uniform lane
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+  return (u64)hi << 32 | lo;
+}
+template <typename Op>
+__device__ __forceinline__ u64 wave_all(u64 v, Op op) {
+  return lane_value(wave_scan(v, op), kWave - 1);
+}
+// The value of lane l ^ M.
+template <int M>
+__device__ __forceinline__ uint32_t across(uint32_t v) {
+  if constexpr (M == 1) return __builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);
+  if constexpr (M == 2) return __builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);
+  if constexpr (M == 4)  // mirrored in eight, then in four
+    return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true), 0x1B, 0xF, 0xF, true);
+  if constexpr (M == 8) return __builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, true);
+  if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return threadIdx.x & 32 ? r[0] : r[1];
+}
+template <int M>
+__device__ __forceinline__ u64 across64(u64 v) {
+  return (u64)across<M>((uint32_t)(v >> 32)) << 32 | across<M>((uint32_t)v);
 }
 
 // The last answer kept: all of a larger key are, and of its own key those up to its index.
@@ -305,46 +364,44 @@ struct ChooseShared {
   uint32_t count[kBins];
   u64 part[kChooseWaves];
   double sums[kChooseWaves];
-  float tops[kChooseWaves];
+  uint32_t tops[kChooseWaves];
   u64 above, in;
   uint32_t listed;
   int digit;
   int found;
 };
 
-__device__ __forceinline__ u64 block_max(u64 v, ChooseShared& sh) {
-  for (int d = 32; d; d >>= 1) {
-    const u64 o = __shfl_xor(v, d);
-    v = o > v ? o : v;
-  }
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) sh.part[threadIdx.x / kWave] = v;
-  __syncthreads();
-  for (int w = 0; w < kChooseWaves; ++w) v = sh.part[w] > v ? sh.part[w] : v;
-  return v;
+// Of the waves' values in sh.part, those of the first `waves` (uniform).
+template <typename Op>
+__device__ __forceinline__ u64 parts_all(int waves, ChooseShared& sh, Op op) {
+  const int l = threadIdx.x % kWave;
+  static_assert(kChooseWaves == 16, "a row of lanes");
+  u64 v = l < waves ? sh.part[l % kChooseWaves] : 0;
+  v = op(v, moved<0x111, 0xF>(v));
+  v = op(v, moved<0x112, 0xF>(v));
+  v = op(v, moved<0x114, 0xF>(v));
+  v = op(v, moved<0x118, 0xF>(v));
+  return lane_value(v, kChooseWaves - 1);
 }
 
-__device__ __forceinline__ u64 block_sum(u64 v, ChooseShared& sh) {
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) sh.part[threadIdx.x / kWave] = v;
-  __syncthreads();
-  v = 0;
-  for (int w = 0; w < kChooseWaves; ++w) v += sh.part[w];
-  return v;
-}
-
-// Sum of the v of this thread and those before it.
-__device__ __forceinline__ u64 block_upto(u64 v, ChooseShared& sh) {
-  for (int d = 1; d < kWave; d <<= 1) {
-    const u64 o = __shfl_up(v, d);
-    if ((int)(threadIdx.x % kWave) >= d) v += o;
-  }
+template <typename Op>
+__device__ __forceinline__ u64 block_all(u64 v, ChooseShared& sh, Op op) {
+  v = wave_scan(v, op);
   __syncthreads();
   if (threadIdx.x % kWave == kWave - 1) sh.part[threadIdx.x / kWave] = v;
   __syncthreads();
-  for (int w = 0; w < (int)threadIdx.x / kWave; ++w) v += sh.part[w];
-  return v;
+  return parts_all(kChooseWaves, sh, op);
+}
+__device__ __forceinline__ u64 block_max(u64 v, ChooseShared& sh) { return block_all(v, sh, Max()); }
+__device__ __forceinline__ u64 block_sum(u64 v, ChooseShared& sh) { return block_all(v, sh, Add()); }
+
+// Sum of the v of this thread and those before it.
+__device__ __forceinline__ u64 block_upto(u64 v, ChooseShared& sh) {
+  v = wave_scan(v, Add());
+  __syncthreads();
+  if (threadIdx.x % kWave == kWave - 1) sh.part[threadIdx.x / kWave] = v;
+  __syncthreads();
+  return v + parts_all(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave), sh, Add());
 }
 
 // The first wave finds the highest bin at which the bins from the top on (bin 0 first where
@@ -359,11 +416,7 @@ __device__ __forceinline__ void find_bin(const T* bins, u64 before, u64 target, 
     u64 own = 0;
 #pragma unroll 4
     for (int j = 0; j < kEach; ++j) own += at(kEach * threadIdx.x + j);
-    u64 upto = own;
-    for (int d = 1; d < kWave; d <<= 1) {
-      const u64 o = __shfl_up(upto, d);
-      if ((int)threadIdx.x >= d) upto += o;
-    }
+    const u64 upto = wave_scan(own, Add());
     const u64 reached = __ballot(before + upto >= target);
     if (threadIdx.x == 0) sh.digit = -1;
     if (reached && (int)threadIdx.x == __ffsll(reached) - 1) {
@@ -541,9 +594,9 @@ __device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, int co
   const int at = (int)~(uint32_t)drawn;
   // z of the answer drawn: its noise taken off again would not be exact
   for (int i = threadIdx.x; i < count; i += kChooseThreads)
-    if ((uint32_t)~sh.list[i] == (uint32_t)at) sh.tops[0] = value_of((uint32_t)(sh.list[i] >> 32));
+    if ((uint32_t)~sh.list[i] == (uint32_t)at) sh.tops[0] = (uint32_t)(sh.list[i] >> 32);
   __syncthreads();
-  answer(a, n, drawn, sh.tops[0], best, sum);
+  answer(a, n, drawn, value_of(sh.tops[0]), best, sum);
 }
 
 // Every answer may be drawn.  Sums are kept in double: a float's would lose what many small terms
@@ -554,26 +607,24 @@ __device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const R
   float top = -INFINITY;
   double sum = 0.0;
   u64 drawn = 0;
-  for (int first = kPack * threadIdx.x; first < a.V; first += 2 * kRound) {
-    Pack<In> score[2];
-    Pack<float> more[2];
+  constexpr int P = kPack<In>;
+  for (int first = P * threadIdx.x; first < a.V; first += 2 * kRound<In>) {
+    Pack<In, P> score[2];
+    Pack<float, P> more[2];
     int at[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      at[u] = score[u].load(row.in, first + u * kRound, a.V);
-      if (noise) more[u].load(noise, first + u * kRound, a.V);
+      at[u] = score[u].load(row.in, first + u * kRound<In>, a.V);
+      if (noise) more[u].load(noise, first + u * kRound<In>, a.V);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      float z[kPack], g[kPack];
-      score[u].values(first + u * kRound, at[u], -INFINITY, z);
-      if (noise) more[u].values(first + u * kRound, at[u], 0.0f, g);
-      float here = -INFINITY;
+      float z[P], g[P];
+      score[u].values(first + u * kRound<In>, at[u], -INFINITY, z);
+      if (noise) more[u].values(first + u * kRound<In>, at[u], 0.0f, g);
 #pragma unroll
-      for (int j = 0; j < kPack; ++j) {
-        z[j] = scaled(z[j], row.t);
-        here = fmaxf(here, z[j]);
-      }
+      for (int j = 0; j < P; ++j) z[j] = scaled(z[j], row.t);
+      const float here = most(z);
       if (here > top) {
         sum *= (double)expf(top - here);  // 0 the first time
         top = here;
@@ -581,7 +632,7 @@ __device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const R
       if (top == -INFINITY) continue;
       float part = 0.0f;
 #pragma unroll
-      for (int j = 0; j < kPack; ++j) {
+      for (int j = 0; j < P; ++j) {
         part += expf(z[j] - top);
         float y = noise ? z[j] + g[j] : z[j];
         y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
@@ -591,24 +642,25 @@ __device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const R
       sum += (double)part;
     }
   }
-  for (int d = 32; d; d >>= 1) {
-    const float o = __shfl_xor(top, d);
-    const double s = __shfl_xor(sum, d);
-    const float m = fmaxf(top, o);
-    if (m > -INFINITY) sum = sum * (double)expf(top - m) + s * (double)expf(o - m);
-    top = m;
+  // the largest z of all and the largest z + noise, then the sums against it, in lanes' and waves' order
+  drawn = wave_scan(drawn, Max());
+  const u64 high = wave_scan(key_of(top), Max());
+  if (threadIdx.x % kWave == kWave - 1) {
+    sh.part[threadIdx.x / kWave] = drawn;
+    sh.tops[threadIdx.x / kWave] = (uint32_t)high;
   }
-  if (threadIdx.x % kWave == 0) {
-    sh.tops[threadIdx.x / kWave] = top;
-    sh.sums[threadIdx.x / kWave] = sum;
-  }
-  drawn = block_max(drawn, sh);  // waits for the others' too
+  __syncthreads();
+  drawn = parts_all(kChooseWaves, sh, Max());
   if (drawn == 0) return no_answer(a, n);
-  float best = -INFINITY;
-  for (int w = 0; w < kChooseWaves; ++w) best = fmaxf(best, sh.tops[w]);
-  sum = 0.0;
-  for (int w = 0; w < kChooseWaves; ++w) sum += sh.sums[w] * (double)expf(sh.tops[w] - best);
+  const int l = threadIdx.x % kWave;
+  const float best = value_of((uint32_t)wave_all(sh.tops[l % kChooseWaves], Max()));
+  sum *= (double)expf(top - best);
+  for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
+  if (l == 0) sh.sums[threadIdx.x / kWave] = sum;
+  __syncthreads();
   if (threadIdx.x == 0) {
+    sum = 0.0;
+    for (int w = 0; w < kChooseWaves; ++w) sum += sh.sums[w];
     const int i = (int)~(uint32_t)drawn;
     a.tokens[n] = i;
     a.logprobs[n] = (row(i) - best) - logf((float)sum);
@@ -625,9 +677,9 @@ __device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const 
     sh.count[i] = 0;
   }
   __syncthreads();
-  each_pack<2>(row.in, a.V, a.V, [&](int, float(&v)[kPack]) {
+  each_pack<2>(row.in, a.V, a.V, [&](int, auto& v) {
 #pragma unroll
-    for (int j = 0; j < kPack; ++j) {
+    for (int j = 0; j < kPack<In>; ++j) {
       const float z = scaled(v[j], row.t);
       if (key_of(z) < cut.key) continue;
       const int b = bin_of(z);
@@ -646,9 +698,9 @@ __device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const 
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     drawn = 0;
-    each_pack<2>(row.in, a.V, a.V, [&](int i, float(&v)[kPack]) {
+    each_pack<2>(row.in, a.V, a.V, [&](int i, auto& v) {
 #pragma unroll
-      for (int j = 0; j < kPack; ++j) {
+      for (int j = 0; j < kPack<In>; ++j) {
         const float z = scaled(v[j], row.t);
         if (key_of(z) < cut.key) continue;
         const int at = bin_of(z);
@@ -769,27 +821,27 @@ __device__ __forceinline__ float with_equals(float score, float t) {
 // it knows its place in the list: few reach `least`.
 template <typename In>
 __device__ __forceinline__ bool list_from(const In* in, int V, float least, ChooseShared& sh) {
-  constexpr int kWords = 4, kPacks = 4;  // packs to a word of marks
+  constexpr int P = kPack<In>, kWords = 4, kPacks = 32 / P;  // packs to a word of marks
   uint32_t listed = 0;
   least = fmaxf(least, -FLT_MAX);  // nothing where it is NaN: the largest is what is left of both
-  for (int start = 0; start < V; start += kWords * kPacks * kRound) {
+  for (int start = 0; start < V; start += kWords * kPacks * kRound<In>) {
     uint32_t marks[kWords];
     uint32_t own = 0;
 #pragma unroll
     for (int w = 0; w < kWords; ++w) {
-      const int first = start + w * kPacks * kRound + kPack * (int)threadIdx.x;
+      const int first = start + w * kPacks * kRound<In>;
       uint32_t m = 0;
-      if (first - kPack * (int)threadIdx.x < V) {
-        Pack<In> pack[kPacks];
+      if (first < V) {
+        Pack<In, P> pack[kPacks];
         int at[kPacks];
 #pragma unroll
-        for (int u = 0; u < kPacks; ++u) at[u] = pack[u].load(in, first + u * kRound, V);
+        for (int u = 0; u < kPacks; ++u) at[u] = pack[u].load(in, first + u * kRound<In> + P * (int)threadIdx.x, V);
 #pragma unroll
         for (int u = 0; u < kPacks; ++u) {
-          float v[kPack];
-          pack[u].values(first + u * kRound, at[u], -INFINITY, v);
+          float v[P];
+          pack[u].values(first + u * kRound<In> + P * (int)threadIdx.x, at[u], -INFINITY, v);
 #pragma unroll
-          for (int j = 0; j < kPack; ++j) m = m * 2 + (v[j] >= least ? 1u : 0u);
+          for (int j = 0; j < P; ++j) m = m * 2 + (v[j] >= least ? 1u : 0u);
         }
       }
       marks[w] = m;
@@ -805,10 +857,10 @@ __device__ __forceinline__ bool list_from(const In* in, int V, float least, Choo
 #pragma unroll
     for (int w = 0; w < kWords; ++w)
       for (uint32_t m = marks[w]; m;) {
-        const int b = __clz(m);  // pack b / kPack of the word, its element b % kPack
+        const int b = __clz(m);  // pack b / P of the word, its element b % P
         m &= ~(0x80000000u >> b);
-        const int i = start + (w * kPacks + b / kPack) * kRound + kPack * (int)threadIdx.x;
-        const int e = (i + kPack <= V ? i : V - kPack) + b % kPack;
+        const int i = start + (w * kPacks + b / P) * kRound<In> + P * (int)threadIdx.x;
+        const int e = (i + P <= V ? i : V - P) + b % P;
         sh.list[place++] = (u64)key_of(to_float(in[e]) + 0.0f) << 32 | (uint32_t)~e;
       }
   }
@@ -822,9 +874,140 @@ __device__ __forceinline__ bool list_from(const In* in, int V, float least, Choo
 template <typename In>
 __device__ __forceinline__ float own_most(const In* in, int V, int rounds) {
   float top = -INFINITY;
-  each_pack<4>(in, V, V < (int64_t)rounds * kRound ? V : rounds * kRound,
-               [&](int, float(&v)[kPack]) { top = fmaxf(top, most(v)); });
+  each_pack<32 / kPack<In>>(in, V, V < (int64_t)rounds * kRound<In> ? V : rounds * kRound<In>,
+                            [&](int, auto& v) { top = fmaxf(top, most(v)); });
   return top;
+}
+
+// A key no larger than the k-th largest of the threads' keys: its upper 16 bits.
+__device__ __forceinline__ uint32_t kth_of(uint32_t own, int k, ChooseShared& sh) {
+  uint32_t prefix = 0u;
+  u64 above = 0;
+  for (int shift = 24; shift >= 16; shift -= 8) {
+    for (int i = threadIdx.x; i < kDigits; i += kChooseThreads) sh.count[i] = 0;
+    __syncthreads();
+    if (shift == 24 || own >> 24 == prefix >> 24) atomicAdd(&sh.count[own >> shift & 255u], 1u);
+    find_bin<kDigits, false>(sh.count, above, (u64)k, sh);
+    prefix |= (uint32_t)sh.digit << shift;
+    above = sh.above;
+    __syncthreads();
+  }
+  return prefix;
+}
+
+// Leaves out of a list what the same bound over the list itself leaves out; the new length.
+__device__ __forceinline__ int shorten_list(int count, float t, int k, ChooseShared& sh) {
+  constexpr int kEach = kList / kChooseThreads;
+  u64 own[kEach];
+  u64 most_ = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = j * kChooseThreads + threadIdx.x;
+    own[j] = i < count ? sh.list[i] : 0;
+    most_ = own[j] > most_ ? own[j] : most_;
+  }
+  const uint32_t bound = kth_of((uint32_t)(most_ >> 32), k, sh);
+  const uint32_t least = bound > kNone ? key_of(with_equals(value_of(bound), t) + 0.0f) : 0u;
+  uint32_t keep = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) keep += own[j] && (uint32_t)(own[j] >> 32) >= least;
+  const uint32_t upto = (uint32_t)block_upto(keep, sh);  // the list has been read by then
+  uint32_t place = upto - keep;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (own[j] && (uint32_t)(own[j] >> 32) >= least) sh.list[place++] = own[j];
+  if (threadIdx.x == kChooseThreads - 1) sh.listed = upto;
+  __syncthreads();
+  return (int)sh.listed;
+}
+
+// One step of a bitonic sort (descending) of 4 x 64 values, value 4 l + r being register r of lane l:
+// pairs at distance J within runs of K that go down and up in turn.
+template <int K, int J>
+__device__ __forceinline__ void sort_step(u64 (&v)[4], int l) {
+  if constexpr (J >= 4) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const u64 o = across64<J / 4>(v[r]);
+      const bool larger = ((4 * l & J) == 0) == ((4 * l & K) == 0);  // this place takes the larger
+      v[r] = (o > v[r]) == larger ? o : v[r];
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if ((r & J) == 0) {
+        const bool down = ((4 * l + r) & K) == 0;
+        const u64 x = v[r], y = v[r | J];
+        const bool swap = (x < y) == down;
+        v[r] = swap ? y : x;
+        v[r | J] = swap ? x : y;
+      }
+  }
+  if constexpr (J > 1) sort_step<K, J / 2>(v, l);
+}
+template <int K>
+__device__ __forceinline__ void sort_runs(u64 (&v)[4], int l) {
+  if constexpr (K > 2) sort_runs<K / 2>(v, l);
+  sort_step<K, K / 2>(v, l);
+}
+
+// from_list for up to kSmall entries: one wave, in registers, without a barrier.
+__device__ __forceinline__ void from_small(const ChooseArgs& a, int64_t n, int count, float t, int k,
+                                           ChooseShared& sh) {
+  if (threadIdx.x >= kWave) return;
+  const int l = threadIdx.x;
+  u64 v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = r * kWave + l;
+    v[r] = i < count ? sh.list[i] : 0;
+    if (v[r]) v[r] = (u64)key_of(scaled(value_of((uint32_t)(v[r] >> 32)), t)) << 32 | (uint32_t)v[r];
+  }
+  sort_runs<kSmall>(v, l);
+  const uint32_t top = (uint32_t)(lane_value(v[0], 0) >> 32);
+  if (top <= kNone) return no_answer(a, n);
+  const float best = value_of(top);
+  uint32_t least = kNone + 1u;
+  if (a.min_p && a.min_p[n] > 0.0f) {
+    const float z = best + logf(a.min_p[n]);
+    const uint32_t key = key_of((z <= best ? z : best) + 0.0f);
+    if (key > least) least = key;
+  }
+  const float p = a.top_p ? a.top_p[n] : 1.0f;
+  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
+  u64 mass[4], own = 0;
+  bool in[4];
+  float z[4], g[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    in[r] = (uint32_t)(v[r] >> 32) >= least && (k <= 0 || 4 * l + r < k);
+    z[r] = value_of((uint32_t)(v[r] >> 32));
+    g[r] = noise && in[r] ? noise[(int)~(uint32_t)v[r]] : 0.0f;
+    mass[r] = in[r] ? mass_of(z[r], best) : 0;
+    own += mass[r];
+  }
+  const u64 upto = wave_scan(own, Add());
+  const u64 target = p >= 1.0f ? ~0ull : share_of(p, lane_value(upto, kWave - 1));
+  u64 before = upto - own, sum = 0, drawn = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    if (in[r] && (before < target || (l == 0 && r == 0))) {
+      sum += mass[r];
+      float y = noise ? z[r] + g[r] : z[r];
+      y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
+      const u64 d = (u64)key_of(y) << 32 | (uint32_t)v[r];
+      drawn = d > drawn ? d : drawn;
+    }
+    before += mass[r];
+  }
+  sum = wave_all(sum, Add());
+  drawn = wave_all(drawn, Max());
+#pragma unroll
+  for (int r = 0; r < 4; ++r)  // the lane whose answer it is
+    if (in[r] && (uint32_t)v[r] == (uint32_t)drawn) {
+      a.tokens[n] = (int)~(uint32_t)drawn;
+      a.logprobs[n] = (z[r] - best) - logf((float)sum * (1.0f / kMass));
+    }
 }
 
 template <typename In>
@@ -845,24 +1028,15 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   const Row<In> row{(const In*)a.scores + n * a.stride, t};
   if (k <= 0 && p >= 1.0f && !bounded) return from_all(a, n, row, sh);
   if (k > 0 && k <= kMaxSeek) {
-    const int rounds = (V + kRound - 1) / kRound;
-    const uint32_t own = key_of(own_most(row.in, V, (rounds + 3) / 4) + 0.0f);
-    // the upper 16 bits of the k-th largest
-    uint32_t prefix = 0u;
-    u64 above = 0;
-    for (int shift = 24; shift >= 16; shift -= 8) {
-      for (int i = threadIdx.x; i < kDigits; i += kChooseThreads) sh.count[i] = 0;
-      __syncthreads();
-      if (shift == 24 || own >> 24 == prefix >> 24) atomicAdd(&sh.count[own >> shift & 255u], 1u);
-      find_bin<kDigits, false>(sh.count, above, (u64)k, sh);
-      prefix |= (uint32_t)sh.digit << shift;
-      above = sh.above;
-      __syncthreads();
+    const int rounds = (V + kRound<In> - 1) / kRound<In>;
+    const uint32_t bound = kth_of(key_of(own_most(row.in, V, (rounds + 3) / 4) + 0.0f), k, sh);
+    if (list_from(row.in, V, bound > kNone ? with_equals(value_of(bound), t) : -INFINITY, sh)) {
+      int count = (int)sh.listed;
+      if (count > kSmall) count = shorten_list(count, t, k, sh);
+      return count <= kSmall ? from_small(a, n, count, t, k, sh) : from_list(a, n, count, t, k, sh);
     }
-    if (list_from(row.in, V, prefix > kNone ? with_equals(value_of(prefix), t) : -INFINITY, sh))
-      return from_list(a, n, (int)sh.listed, t, k, sh);
   }
-  const float own = own_most(row.in, V, (V + kRound - 1) / kRound);
+  const float own = own_most(row.in, V, (V + kRound<In> - 1) / kRound<In>);
   const float best = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), t);
   if (best == -INFINITY) return no_answer(a, n);
   Cut cut{kNone + 1u, V - 1};
@@ -871,7 +1045,8 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
     const uint32_t key = key_of((least <= best ? least : best) + 0.0f);
     if (key > cut.key) cut.key = key;
     if (k <= 0 && list_from(row.in, V, with_equals(least * t, t), sh))
-      return from_list(a, n, (int)sh.listed, t, k, sh);
+      return (int)sh.listed <= kSmall ? from_small(a, n, (int)sh.listed, t, k, sh)
+                                      : from_list(a, n, (int)sh.listed, t, k, sh);
   }
   if ((k > 0 || p < 1.0f) && from_bins(a, n, row, best, k, p, cut, sh)) return;
   __syncthreads();
