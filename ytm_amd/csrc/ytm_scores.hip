@@ -207,6 +207,7 @@ constexpr int kPack = 16 / sizeof(In);  // scores of a 16-byte load
 template <typename In>
 constexpr int kRound = kPack<In> * kChooseThreads;
 constexpr int kList = 4096;
+constexpr int kSub = 1024;  // answers of a slice of the histogram
 constexpr int kSmall = 256;    // entries that one wave sorts in registers
 constexpr int kMaxSeek = 256;  // a quarter of the threads, so that few of the largest share a thread
 constexpr int kBins = 2048;
@@ -360,6 +361,7 @@ struct Cut {
 
 struct ChooseShared {
   u64 list[kList];
+  u64 sub[kSub];
   u64 mass[kBins];
   uint32_t count[kBins];
   u64 part[kChooseWaves];
@@ -530,73 +532,43 @@ __device__ __forceinline__ void sort_list(u64* list, int size) {
   __syncthreads();
 }
 
-// Sorts the list's `count` entries (descending; zeros follow them).
-__device__ __forceinline__ void order_list(int count, ChooseShared& sh) {
+// Sorts a list's `count` entries (descending; zeros follow them).
+__device__ __forceinline__ void order_list(u64* list, int count) {
   int size = 2 * kWave;
   while (size < count) size <<= 1;
   __syncthreads();
-  for (int i = count + threadIdx.x; i < size; i += kChooseThreads) sh.list[i] = 0;
-  sort_list(sh.list, size);
+  for (int i = count + threadIdx.x; i < size; i += kChooseThreads) list[i] = 0;
+  sort_list(list, size);
 }
 
-__device__ __forceinline__ void put(u64 entry, ChooseShared& sh) {
-  const uint32_t at = atomicAdd(&sh.listed, 1u);
-  if (at < kList) sh.list[at] = entry;
+// One step of a bitonic sort (descending) of 4 x 64 values, value 4 l + r being register r of lane l:
+// pairs at distance J within runs of K that go down and up in turn.
+template <int K, int J>
+__device__ __forceinline__ void sort_step(u64 (&v)[4], int l) {
+  if constexpr (J >= 4) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const u64 o = across64<J / 4>(v[r]);
+      const bool larger = ((4 * l & J) == 0) == ((4 * l & K) == 0);  // this place takes the larger
+      v[r] = (o > v[r]) == larger ? o : v[r];
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if ((r & J) == 0) {
+        const bool down = ((4 * l + r) & K) == 0;
+        const u64 x = v[r], y = v[r | J];
+        const bool swap = (x < y) == down;
+        v[r] = swap ? y : x;
+        v[r | J] = swap ? x : y;
+      }
+  }
+  if constexpr (J > 1) sort_step<K, J / 2>(v, l);
 }
-
-// The answer from a list (of key of score, ~index) that holds every answer the filters may keep.
-__device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, int count, float t, int k, ChooseShared& sh) {
-  for (int i = threadIdx.x; i < count; i += kChooseThreads) {
-    const u64 e = sh.list[i];
-    sh.list[i] = (u64)key_of(scaled(value_of((uint32_t)(e >> 32)), t)) << 32 | (uint32_t)e;
-  }
-  order_list(count, sh);
-  const uint32_t top = (uint32_t)(sh.list[0] >> 32);
-  if (count == 0 || top <= kNone) return no_answer(a, n);
-  const float best = value_of(top);
-  uint32_t least = kNone + 1u;
-  if (a.min_p && a.min_p[n] > 0.0f) {
-    const float z = best + logf(a.min_p[n]);
-    const uint32_t key = key_of((z <= best ? z : best) + 0.0f);
-    if (key > least) least = key;
-  }
-  if (k > 0 && k < count) count = k;
-  const float p = a.top_p ? a.top_p[n] : 1.0f;
-  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
-  u64 total = 0, drawn = 0, sum = 0;
-  for (int i = threadIdx.x; i < count; i += kChooseThreads) {
-    const uint32_t key = (uint32_t)(sh.list[i] >> 32);
-    if (key >= least) total += mass_of(value_of(key), best);
-  }
-  total = block_sum(total, sh);
-  const u64 target = p >= 1.0f ? ~0ull : share_of(p, total);
-  u64 before = 0;
-  for (int first = 0; first < count; first += kChooseThreads) {
-    const int i = first + threadIdx.x;
-    const u64 e = i < count ? sh.list[i] : 0;
-    const uint32_t key = (uint32_t)(e >> 32);
-    const u64 mass = key >= least ? mass_of(value_of(key), best) : 0;
-    const u64 upto = before + block_upto(mass, sh);
-    if (key >= least && (upto - mass < target || i == 0)) {
-      sum += mass;
-      const u64 d = drawn_of(value_of(key), (int)~(uint32_t)e, noise);
-      drawn = d > drawn ? d : drawn;
-    }
-    if (first + kChooseThreads < count) {  // what this round holds
-      __syncthreads();
-      if (threadIdx.x == kChooseThreads - 1) sh.above = upto;
-      __syncthreads();
-      before = sh.above;
-    }
-  }
-  sum = block_sum(sum, sh);
-  drawn = block_max(drawn, sh);
-  const int at = (int)~(uint32_t)drawn;
-  // z of the answer drawn: its noise taken off again would not be exact
-  for (int i = threadIdx.x; i < count; i += kChooseThreads)
-    if ((uint32_t)~sh.list[i] == (uint32_t)at) sh.tops[0] = (uint32_t)(sh.list[i] >> 32);
-  __syncthreads();
-  answer(a, n, drawn, value_of(sh.tops[0]), best, sum);
+template <int K>
+__device__ __forceinline__ void sort_runs(u64 (&v)[4], int l) {
+  if constexpr (K > 2) sort_runs<K / 2>(v, l);
+  sort_step<K, K / 2>(v, l);
 }
 
 // Every answer may be drawn.  Sums are kept in double: a float's would lose what many small terms
@@ -667,80 +639,96 @@ __device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const R
   }
 }
 
-// The cut from histograms over max - z; false where a slice holds more than the list.
-template <typename In>
-__device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, float best, int k, float p, Cut cut,
-                          ChooseShared& sh) {
+// The answer from a histogram over max - z: the slice in which a cut lies, and that slice's answers,
+// sorted, the cut.  each(least, f) calls f(z, index) for this thread's answers, those of a z below
+// `least` not for certain.  False, with nothing written, where a slice holds more than kSub.
+template <typename In, typename Each>
+__device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, Each each, float best,
+                                          int k, float p, Cut cut, ChooseShared& sh) {
   const auto bin_of = [&](float z) { return (int)fminf((best - z) * kBinsPerUnit, (float)(kBins - 1)); };
   for (int i = threadIdx.x; i < kBins; i += kChooseThreads) {
     sh.mass[i] = 0;
     sh.count[i] = 0;
   }
   __syncthreads();
-  each_pack<2>(row.in, a.V, a.V, [&](int, auto& v) {
-#pragma unroll
-    for (int j = 0; j < kPack<In>; ++j) {
-      const float z = scaled(v[j], row.t);
-      if (key_of(z) < cut.key) continue;
-      const int b = bin_of(z);
-      atomicAdd(&sh.mass[b], mass_of(z, best));
-      atomicAdd(&sh.count[b], 1u);
+  const bool counted = k > 0;
+  const float lightest = best - 28.0f;  // from here on masses are below 2^-40, none
+  uint32_t rest = 0;                    // answers of the last slice, which may be nearly all
+  each(counted ? -INFINITY : lightest, [&](float z, int) {
+    if (key_of(z) < cut.key) return;
+    const int b = bin_of(z);
+    const u64 m = mass_of(z, best);
+    if (m) atomicAdd(&sh.mass[b], m);
+    if (counted) {
+      if (b == kBins - 1)
+        ++rest;
+      else
+        atomicAdd(&sh.count[b], 1u);
     }
   });
+  if (counted && rest) atomicAdd(&sh.count[kBins - 1], rest);
   const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
   u64 total = 0;  // of what top_k leaves
   u64 drawn = 0, sum = 0;
   int listed = -1, count = 0;  // the slice in the list
-  // puts the answers of slice b into the list in their order, and the largest z + noise of those before it
-  // into `drawn`
+  // puts the answers of slice b into sh.sub in their order, and the largest z + noise of those before it
+  // into `drawn`; whether they fit
   const auto gather = [&](int b) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     drawn = 0;
-    each_pack<2>(row.in, a.V, a.V, [&](int i, auto& v) {
-#pragma unroll
-      for (int j = 0; j < kPack<In>; ++j) {
-        const float z = scaled(v[j], row.t);
-        if (key_of(z) < cut.key) continue;
-        const int at = bin_of(z);
-        if (at == b) put((u64)key_of(z) << 32 | (uint32_t)~(i + j), sh);
-        if (at < b) {
-          const u64 d = drawn_of(z, i + j, noise);
-          drawn = d > drawn ? d : drawn;
-        }
+    each(b < kBins - 1 ? best - (float)(b + 2) / kBinsPerUnit : -INFINITY, [&](float z, int i) {
+      if (key_of(z) < cut.key) return;
+      const int at = bin_of(z);
+      if (at == b) {
+        const uint32_t place = atomicAdd(&sh.listed, 1u);
+        if (place < kSub) sh.sub[place] = (u64)key_of(z) << 32 | (uint32_t)~i;
+      }
+      if (at < b) {
+        const u64 d = drawn_of(z, i, noise);
+        drawn = d > drawn ? d : drawn;
       }
     });
     __syncthreads();
     listed = b;
     count = (int)sh.listed;
-    order_list(count, sh);
-  };
-  // the number of the list's first answers whose masses reach `target` (all where they never do), and their sum
-  const auto upto = [&](int most_, u64 target) {
-    u64 before = 0;
-    int kept = 0;
-    sum = 0;
-    for (int first = 0; first < most_; first += kChooseThreads) {
-      const int i = first + threadIdx.x;
-      const u64 mass = i < most_ ? mass_of(value_of((uint32_t)(sh.list[i] >> 32)), best) : 0;
-      const u64 up = before + block_upto(mass, sh);
-      const bool keep = i < most_ && (up - mass < target || i == 0);
-      kept += (int)block_sum(keep ? 1 : 0, sh);
-      sum += block_sum(keep ? mass : 0, sh);
-      before += block_sum(mass, sh);
+    if (count > kSub) return false;
+    if (count <= kSmall) {  // one wave, in registers
+      if (threadIdx.x < kWave) {
+        u64 v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = r * kWave + (int)threadIdx.x < count ? sh.sub[r * kWave + threadIdx.x] : 0;
+        sort_runs<kSmall>(v, threadIdx.x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sh.sub[4 * threadIdx.x + r] = v[r];
+      }
+      __syncthreads();
+    } else {
+      order_list(sh.sub, count);
     }
-    return kept;
+    return true;
+  };
+  // the number of the first `among` of them whose masses reach `target` (all where they never do), and their sum
+  const auto upto = [&](int among, u64 target) {
+    const int i = threadIdx.x;
+    static_assert(kSub <= kChooseThreads, "");
+    const u64 mass = i < among ? mass_of(value_of((uint32_t)(sh.sub[i] >> 32)), best) : 0;
+    const u64 up = block_upto(mass, sh);
+    const bool keep = i < among && up - mass < target;
+    sum = block_sum(keep ? mass : 0, sh);
+    return (int)block_sum(keep ? 1 : 0, sh);
   };
   int kept = 0;  // of the list
   u64 above = 0;
   int end = kBins;  // slices from here on are left out
-  find_bin<kBins, true>(sh.count, 0, k > 0 ? (u64)k : ~0ull, sh);
+  sh.digit = -1;
+  if (counted) find_bin<kBins, true>(sh.count, 0, (u64)k, sh);
+  __syncthreads();
   if (sh.digit >= 0) {
     end = sh.digit;
-    if (sh.in > kList) return false;
     const int r = k - (int)sh.above;
-    gather(end);
+    if (!gather(end)) return false;
     u64 m = 0;
     for (int i = threadIdx.x; i < end; i += kChooseThreads) m += sh.mass[i];
     above = block_sum(m, sh);
@@ -757,8 +745,7 @@ __device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const 
     const int b = sh.digit;
     if (b >= 0 && b < end) {  // in a slice that top_k leaves whole
       above = sh.above;
-      if (sh.count[b] > kList) return false;
-      gather(b);
+      if (!gather(b)) return false;
       kept = upto(count, target - above);
     } else if (listed >= 0) {
       kept = upto(kept, target - above);
@@ -769,14 +756,80 @@ __device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const 
     above = total;
     sum = 0;
   }
-  for (int i = threadIdx.x; i < kept; i += kChooseThreads) {
-    const u64 e = sh.list[i];
+  if ((int)threadIdx.x < kept) {
+    const u64 e = sh.sub[threadIdx.x];
     const u64 d = drawn_of(value_of((uint32_t)(e >> 32)), (int)~(uint32_t)e, noise);
     drawn = d > drawn ? d : drawn;
   }
   drawn = block_max(drawn, sh);
   answer(a, n, drawn, row((int)~(uint32_t)drawn), best, above + sum);
   return true;
+}
+
+// The answer from a list (of key of score, ~index) that holds every answer the filters may keep:
+// from a histogram over it, or from the whole list sorted where a slice holds too many.
+template <typename In>
+__device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, const Row<In>& row, int count, int k,
+                                          ChooseShared& sh) {
+  u64 first = 0;
+  for (int i = threadIdx.x; i < count; i += kChooseThreads) {
+    const u64 e = sh.list[i];
+    const u64 z = (u64)key_of(scaled(value_of((uint32_t)(e >> 32)), row.t)) << 32 | (uint32_t)e;
+    sh.list[i] = z;
+    first = z > first ? z : first;
+  }
+  const uint32_t top = (uint32_t)(block_max(first, sh) >> 32);
+  if (top <= kNone) return no_answer(a, n);
+  const float best = value_of(top);
+  uint32_t least = kNone + 1u;
+  if (a.min_p && a.min_p[n] > 0.0f) {
+    const float z = best + logf(a.min_p[n]);
+    const uint32_t key = key_of((z <= best ? z : best) + 0.0f);
+    if (key > least) least = key;
+  }
+  const float p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
+  const auto each = [&](float, auto f) {
+    for (int i = threadIdx.x; i < count; i += kChooseThreads)
+      f(value_of((uint32_t)(sh.list[i] >> 32)), (int)~(uint32_t)sh.list[i]);
+  };
+  if (from_bins(a, n, row, each, best, k, p, Cut{least, a.V - 1}, sh)) return;
+  order_list(sh.list, count);
+  if (k > 0 && k < count) count = k;
+  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
+  u64 total = 0, drawn = 0, sum = 0;
+  for (int i = threadIdx.x; i < count; i += kChooseThreads) {
+    const uint32_t key = (uint32_t)(sh.list[i] >> 32);
+    if (key >= least) total += mass_of(value_of(key), best);
+  }
+  total = block_sum(total, sh);
+  const u64 target = p >= 1.0f ? ~0ull : share_of(p, total);
+  u64 before = 0;
+  for (int first = 0; first < count; first += kChooseThreads) {
+    const int i = first + threadIdx.x;
+    const u64 e = i < count ? sh.list[i] : 0;
+    const uint32_t key = (uint32_t)(e >> 32);
+    const u64 mass = key >= least ? mass_of(value_of(key), best) : 0;
+    const u64 upto = before + block_upto(mass, sh);
+    if (key >= least && (upto - mass < target || i == 0)) {
+      sum += mass;
+      const u64 d = drawn_of(value_of(key), (int)~(uint32_t)e, noise);
+      drawn = d > drawn ? d : drawn;
+    }
+    if (first + kChooseThreads < count) {  // what this round holds
+      __syncthreads();
+      if (threadIdx.x == kChooseThreads - 1) sh.above = upto;
+      __syncthreads();
+      before = sh.above;
+    }
+  }
+  sum = block_sum(sum, sh);
+  drawn = block_max(drawn, sh);
+  const int at = (int)~(uint32_t)drawn;
+  // z of the answer drawn: its noise taken off again would not be exact
+  for (int i = threadIdx.x; i < count; i += kChooseThreads)
+    if ((uint32_t)~sh.list[i] == (uint32_t)at) sh.tops[0] = (uint32_t)(sh.list[i] >> 32);
+  __syncthreads();
+  answer(a, n, drawn, value_of(sh.tops[0]), best, sum);
 }
 
 // Passes over the whole row for each step: right for every row, and what is left for lists
@@ -817,12 +870,13 @@ __device__ __forceinline__ float with_equals(float score, float t) {
 }
 
 // Lists the row's scores from `least` on (those above -inf) in an order of threads; whether they
-// fit.  A thread marks those of 16 packs in 128 bits, without a branch, and reads them again once
+// fit.  `top` is raised to the largest score this thread has seen.  A thread marks those of 16 packs in 128 bits, without a branch, and reads them again once
 // it knows its place in the list: few reach `least`.
 template <typename In>
-__device__ __forceinline__ bool list_from(const In* in, int V, float least, ChooseShared& sh) {
+__device__ __forceinline__ bool list_from(const In* in, int V, float least, float& top, ChooseShared& sh) {
   constexpr int P = kPack<In>, kWords = 4, kPacks = 32 / P;  // packs to a word of marks
   uint32_t listed = 0;
+  bool fits = true;
   least = fmaxf(least, -FLT_MAX);  // nothing where it is NaN: the largest is what is left of both
   for (int start = 0; start < V; start += kWords * kPacks * kRound<In>) {
     uint32_t marks[kWords];
@@ -842,6 +896,7 @@ __device__ __forceinline__ bool list_from(const In* in, int V, float least, Choo
           pack[u].values(first + u * kRound<In> + P * (int)threadIdx.x, at[u], -INFINITY, v);
 #pragma unroll
           for (int j = 0; j < P; ++j) m = m * 2 + (v[j] >= least ? 1u : 0u);
+          top = fmaxf(top, most(v));
         }
       }
       marks[w] = m;
@@ -853,7 +908,10 @@ __device__ __forceinline__ bool list_from(const In* in, int V, float least, Choo
     if (threadIdx.x == kChooseThreads - 1) sh.listed = upto;
     __syncthreads();
     listed += sh.listed;
-    if (listed > kList) return false;
+    if (listed > kList) {  // what is left is looked at for its largest score alone
+      fits = false;
+      continue;
+    }
 #pragma unroll
     for (int w = 0; w < kWords; ++w)
       for (uint32_t m = marks[w]; m;) {
@@ -867,7 +925,7 @@ __device__ __forceinline__ bool list_from(const In* in, int V, float least, Choo
   __syncthreads();
   if (threadIdx.x == 0) sh.listed = listed;
   __syncthreads();
-  return true;
+  return fits;
 }
 
 // The largest of this thread's packs over the row's first `rounds` rounds.
@@ -919,36 +977,6 @@ __device__ __forceinline__ int shorten_list(int count, float t, int k, ChooseSha
   if (threadIdx.x == kChooseThreads - 1) sh.listed = upto;
   __syncthreads();
   return (int)sh.listed;
-}
-
-// One step of a bitonic sort (descending) of 4 x 64 values, value 4 l + r being register r of lane l:
-// pairs at distance J within runs of K that go down and up in turn.
-template <int K, int J>
-__device__ __forceinline__ void sort_step(u64 (&v)[4], int l) {
-  if constexpr (J >= 4) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const u64 o = across64<J / 4>(v[r]);
-      const bool larger = ((4 * l & J) == 0) == ((4 * l & K) == 0);  // this place takes the larger
-      v[r] = (o > v[r]) == larger ? o : v[r];
-    }
-  } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if ((r & J) == 0) {
-        const bool down = ((4 * l + r) & K) == 0;
-        const u64 x = v[r], y = v[r | J];
-        const bool swap = (x < y) == down;
-        v[r] = swap ? y : x;
-        v[r | J] = swap ? x : y;
-      }
-  }
-  if constexpr (J > 1) sort_step<K, J / 2>(v, l);
-}
-template <int K>
-__device__ __forceinline__ void sort_runs(u64 (&v)[4], int l) {
-  if constexpr (K > 2) sort_runs<K / 2>(v, l);
-  sort_step<K, K / 2>(v, l);
 }
 
 // from_list for up to kSmall entries: one wave, in registers, without a barrier.
@@ -1027,28 +1055,46 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   const bool bounded = a.min_p && a.min_p[n] > 0.0f;
   const Row<In> row{(const In*)a.scores + n * a.stride, t};
   if (k <= 0 && p >= 1.0f && !bounded) return from_all(a, n, row, sh);
-  if (k > 0 && k <= kMaxSeek) {
-    const int rounds = (V + kRound<In> - 1) / kRound<In>;
-    const uint32_t bound = kth_of(key_of(own_most(row.in, V, (rounds + 3) / 4) + 0.0f), k, sh);
-    if (list_from(row.in, V, bound > kNone ? with_equals(value_of(bound), t) : -INFINITY, sh)) {
-      int count = (int)sh.listed;
-      if (count > kSmall) count = shorten_list(count, t, k, sh);
-      return count <= kSmall ? from_small(a, n, count, t, k, sh) : from_list(a, n, count, t, k, sh);
+  const int rounds = (V + kRound<In> - 1) / kRound<In>;
+  float own = -INFINITY;
+  const bool seek = k > 0 && k <= kMaxSeek;
+  if (seek || bounded) {  // a bound from a quarter of the row, and the list of what reaches it
+    own = own_most(row.in, V, (rounds + 3) / 4);
+    float least;
+    if (seek) {
+      const uint32_t bound = kth_of(key_of(own + 0.0f), k, sh);
+      least = bound > kNone ? with_equals(value_of(bound), t) : -INFINITY;
+    } else {  // no larger than that of the row's largest
+      const float z = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), t);
+      const float low = z + logf(a.min_p[n]);
+      least = with_equals((low <= z ? low : z) * t, t);
     }
+    if (list_from(row.in, V, least, own, sh)) {
+      int count = (int)sh.listed;
+      if (seek && count > kSmall) count = shorten_list(count, t, k, sh);
+      return count <= kSmall ? from_small(a, n, count, t, k, sh) : from_list(a, n, row, count, k, sh);
+    }
+  } else {
+    own = own_most(row.in, V, rounds);
   }
-  const float own = own_most(row.in, V, (V + kRound<In> - 1) / kRound<In>);
   const float best = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), t);
   if (best == -INFINITY) return no_answer(a, n);
   Cut cut{kNone + 1u, V - 1};
   if (bounded) {
-    const float least = best + logf(a.min_p[n]);
-    const uint32_t key = key_of((least <= best ? least : best) + 0.0f);
+    const float low = best + logf(a.min_p[n]);
+    const uint32_t key = key_of((low <= best ? low : best) + 0.0f);
     if (key > cut.key) cut.key = key;
-    if (k <= 0 && list_from(row.in, V, with_equals(least * t, t), sh))
-      return (int)sh.listed <= kSmall ? from_small(a, n, (int)sh.listed, t, k, sh)
-                                      : from_list(a, n, (int)sh.listed, t, k, sh);
   }
-  if ((k > 0 || p < 1.0f) && from_bins(a, n, row, best, k, p, cut, sh)) return;
+  const auto each = [&](float least, auto f) {
+    const float from = least > -INFINITY ? with_equals(least * t, t) : -FLT_MAX;
+    each_pack<16 / kPack<In>>(row.in, V, V, [&](int i, auto& v) {
+      if (!(most(v) >= from)) return;
+#pragma unroll
+      for (int j = 0; j < kPack<In>; ++j)
+        if (v[j] >= from) f(scaled(v[j], t), i + j);
+    });
+  };
+  if ((k > 0 || p < 1.0f) && from_bins(a, n, row, each, best, k, p, cut, sh)) return;
   __syncthreads();
   from_row(a, n, row, best, k, p, cut, sh);
 }
