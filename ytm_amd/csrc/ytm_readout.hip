@@ -377,12 +377,14 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   // Chunks past the last are loaded too: whether to load would be a branch, after which every load
   // has to be waited for.  Their rows are zero up to the last pair's end, and what is loaded past it is
   // not used.
-  const int pairs = (a.chunks + 2 * WK - 1) / (2 * WK);
+  const int all_pairs = (a.chunks + 2 * WK - 1) / (2 * WK);
+  const int first_pair = blockIdx.y * a.part_chunks;  // of this part; part_chunks counts pairs here
+  const int pairs = all_pairs - first_pair < a.part_chunks ? all_pairs - first_pair : a.part_chunks;
   const uint32_t steps = (a.C + kStep - 1) / kStep;
   v4u code[kCodes];
   uint16_t low[kScales], high[kScales];
   const auto load_codes = [&](int pair) {
-    const uint32_t first = (uint32_t)(pair * WK + group) * 2 * 4;  // step
+    const uint32_t first = (uint32_t)((first_pair + pair) * WK + group) * 2 * 4;  // step
 #pragma unroll
     for (int e = 0; e < kCodes; ++e) {
       const uint32_t step = first + (e * kGroupThreads + t) % 8;
@@ -408,12 +410,12 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
       if (o < kOuts) held_scales[pair % 2][group][i / kGrains][i % kGrains][o] = scale_value(a, low[e], high[e]);
     }
   };
-  const int padded = pairs * 2 * WK;
+  const int padded = all_pairs * 2 * WK;
   struct Rows {
     v4u x[kEach];
   };
   const auto load_rows = [&](int i, Rows& to) {  // of chunk i of this group's
-    const int own = (i / 2 * WK + group) * 2 + i % 2, chunk = own < padded ? own : padded - 1;
+    const int own = ((first_pair + i / 2) * WK + group) * 2 + i % 2, chunk = own < padded ? own : padded - 1;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {  // row tiles past the last take its rows and are not stored
       const int f = e * kGroupWaves + mine, tile = row_block * kTiles + f % kTiles;
@@ -486,26 +488,96 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = (row_block * kTiles + rw * NT + n) * kTile + l / 16 * 4 + r;
-        if (o < a.K && row < a.N) store_out(a, row, o, v[r]);
+        if (o >= a.K || row >= a.N) continue;
+        if (gridDim.y > 1)
+          a.parts[((int64_t)blockIdx.y * a.N + row) * a.K + o] = v[r];
+        else
+          store_out(a, row, o, v[r]);
       }
     }
 }
 
-// Chunks of the rows' operands: whole pairs for each of up to kGroups groups of waves.
-constexpr int kGroups = 2;
-int padded_of(int chunks) { return (chunks + 2 * kGroups - 1) / (2 * kGroups) * (2 * kGroups); }
+// The parts' sums added in their order.
+__global__ __launch_bounds__(256) void parts_kernel(ReadoutArgs a, int parts) {
+  const int64_t each = (int64_t)a.N * a.K;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < each; i += (int64_t)gridDim.x * blockDim.x) {
+    float v = a.parts[i];
+    for (int p = 1; p < parts; ++p) v += a.parts[p * each + i];
+    store_out(a, (int)(i / a.K), (int)(i % a.K), v);
+  }
+}
+hipError_t launch_parts(const ReadoutArgs& a, int parts, hipStream_t s) {
+  const int64_t blocks = ((int64_t)a.N * a.K + 255) / 256;
+  parts_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(a, parts);
+  return hipGetLastError();
+}
+
+// What a block of tile_kernel takes, by the number of rows: 32, 64, or 96 and 128, whichever leaves
+// fewer rows that are not there; float32, whose operands take three times the LDS, up to 64.  With
+// four scales a chunk (grain 32) 160 outputs do not fit the registers.
+struct Tile {
+  int rows, outs, groups;
+};
+constexpr Tile kTile32{32, 128, 2}, kTile64{64, 128, 2}, kTile96{96, 128, 1};
+constexpr Tile kWide32{32, 128, 1}, kWide64{64, 128, 1};
+Tile tile_of(int planes, int grain, int N) {
+  if (planes > 1) return N <= 32 ? kWide32 : kWide64;
+  if (N <= 64) return N <= 32 ? kTile32 : kTile64;
+  return (N + 95) / 96 * 96 < (N + 127) / 128 * 128 ? kTile96 : Tile{128, grain == kChunk ? 160 : 128, 1};
+}
+// Pairs of chunks in a part of the clauses: all, or where that leaves half of the 256 CUs without
+// a block, as many as give each CU one (103 rows x 10012 clauses x 22 outputs, one block: 909 us;
+// two pairs a part: 25).
+int part_pairs_of(int planes, int grain, int N, int chunks, int K) {
+  const Tile t = tile_of(planes, grain, N);
+  const int64_t blocks = (int64_t)((N + t.rows - 1) / t.rows) * ((K + t.outs - 1) / t.outs);
+  const int pairs = (chunks + 2 * t.groups - 1) / (2 * t.groups);
+  if (blocks > 128 || pairs < 4) return pairs;
+  const int parts = (int)(256 / blocks) < pairs / 2 ? (int)(256 / blocks) : pairs / 2;
+  return (pairs + parts - 1) / parts;
+}
+int tile_parts_of(int planes, int grain, int N, int chunks, int K) {
+  const Tile t = tile_of(planes, grain, N);
+  const int each = part_pairs_of(planes, grain, N, chunks, K);
+  return ((chunks + 2 * t.groups - 1) / (2 * t.groups) + each - 1) / each;
+}
+// Chunks of the rows' operands: whole pairs for each group of waves, of which a block has up to two.
+int padded_of(int chunks) { return (chunks + 3) / 4 * 4; }
+int64_t frag_bytes(int planes, int N, int chunks) {
+  return (int64_t)(N + kTile - 1) / kTile * padded_of(chunks) * planes * 4 * kWave * 16;
+}
 
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 hipError_t launch_tile(ReadoutArgs a, hipStream_t s) {
-  static_assert(WK <= kGroups && kGroups % WK == 0, "");
+  constexpr int kPlanes = Kind<X>::kPlanes;
   a.row_tiles = (a.N + kTile - 1) / kTile;
   a.out_tiles = (a.K + kTile * OB * WO - 1) / (kTile * OB * WO);
+  a.part_chunks = part_pairs_of(kPlanes, GRAIN, a.N, a.chunks, a.K);
+  a.parts = (float*)((char*)a.frag + frag_bytes(kPlanes, a.N, a.chunks));
+  const int parts = tile_parts_of(kPlanes, GRAIN, a.N, a.chunks, a.K);
   rows_kernel<X, GRAIN><<<dim3(padded_of(a.chunks), a.row_tiles), kPieces * kTile, 0, s>>>(a);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const unsigned grid = (unsigned)((a.out_tiles + 7) / 8 * 8 * ((a.row_tiles + NT * RW - 1) / (NT * RW)));
-  tile_kernel<X, GRAIN, NT, RW, OB, WO, WK><<<grid, kWave * RW * WO * WK, 0, s>>>(a);
-  return hipGetLastError();
+  tile_kernel<X, GRAIN, NT, RW, OB, WO, WK><<<dim3(grid, parts), kWave * RW * WO * WK, 0, s>>>(a);
+  e = hipGetLastError();
+  return e != hipSuccess || parts == 1 ? e : launch_parts(a, parts, s);
+}
+template <int X, int GRAIN>
+hipError_t launch_tiles(const ReadoutArgs& a, hipStream_t s) {
+  const int rows = tile_of(Kind<X>::kPlanes, GRAIN, a.N).rows;
+  if constexpr (Kind<X>::kPlanes > 1) {
+    return rows == 32 ? launch_tile<X, GRAIN, 2, 1, 2, 4, 1>(a, s) : launch_tile<X, GRAIN, 2, 2, 2, 4, 1>(a, s);
+  } else {
+    switch (rows) {
+      case 32: return launch_tile<X, GRAIN, 2, 1, 2, 4, 2>(a, s);
+      case 64: return launch_tile<X, GRAIN, 4, 1, 2, 4, 2>(a, s);
+      case 96: return launch_tile<X, GRAIN, 3, 2, 2, 4, 1>(a, s);
+      default:
+        if constexpr (GRAIN == kChunk) return launch_tile<X, GRAIN, 2, 4, 5, 2, 1>(a, s);
+        else return launch_tile<X, GRAIN, 4, 2, 2, 4, 1>(a, s);
+    }
+  }
 }
 
 // Few rows (up to 16): a block has 16 OB WO outputs and the clauses of one of the parts that the
@@ -615,16 +687,6 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
   }
 }
 
-// The parts' sums added in their order.
-__global__ __launch_bounds__(256) void parts_kernel(ReadoutArgs a, int parts) {
-  const int64_t each = (int64_t)a.N * a.K;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < each; i += (int64_t)gridDim.x * blockDim.x) {
-    float v = a.parts[i];
-    for (int p = 1; p < parts; ++p) v += a.parts[p * each + i];
-    store_out(a, (int)(i / a.K), (int)(i % a.K), v);
-  }
-}
-
 // A chunk's row operands take rows * kPlanes * 256 bytes of LDS; a part has as many chunks as
 // kHeldLimit takes, which leaves room for two blocks on a CU.
 constexpr int64_t kHeldLimit = 64 * 1024;
@@ -649,11 +711,8 @@ hipError_t launch_held(ReadoutArgs a, hipStream_t s) {
     held_kernel<X, GRAIN, OB, WO, WK, true><<<grid, kWave * WO * WK, lds, s>>>(a);
   else
     held_kernel<X, GRAIN, OB, WO, WK, false><<<grid, kWave * WO * WK, lds, s>>>(a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || parts == 1) return e;
-  const int64_t blocks = ((int64_t)a.N * a.K + 255) / 256;
-  parts_kernel<<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(a, parts);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || parts == 1 ? e : launch_parts(a, parts, s);
 }
 
 constexpr int kFewRows = 16;
@@ -688,18 +747,9 @@ __global__ __launch_bounds__(256) void short_kernel(ReadoutArgs a) {
 
 template <int X, int GRAIN>
 hipError_t launch_rows(const ReadoutArgs& a, hipStream_t s) {
-  constexpr bool kOne = Kind<X>::kPlanes == 1;
-  if (a.N <= kFewRows) {
-    if (parts_of(Kind<X>::kPlanes, a.N, a.chunks) > 1) return launch_held<X, GRAIN, 2, 8, 1>(a, s);
-    return a.K <= 4096 ? launch_held<X, GRAIN, 1, 1, 16>(a, s) : launch_held<X, GRAIN, 1, 1, 4>(a, s);
-  }
-  if (a.N <= 32) return launch_tile<X, GRAIN, 2, 1, 2, 4, kOne ? 2 : 1>(a, s);
-  if (a.N <= 64 || !kOne) return launch_tile<X, GRAIN, kOne ? 4 : 2, kOne ? 1 : 2, 2, 4, kOne ? 2 : 1>(a, s);
-  if constexpr (kOne) {
-    const bool narrow = (a.N + 95) / 96 * 96 < (a.N + 127) / 128 * 128;
-    if (narrow) return launch_tile<X, GRAIN, 3, 2, 2, 4, 1>(a, s);
-    return launch_tile<X, GRAIN, 2, 4, 5, 2, 1>(a, s);
-  }
+  if (a.N > kFewRows) return launch_tiles<X, GRAIN>(a, s);
+  if (a.K > 1024 && parts_of(Kind<X>::kPlanes, a.N, a.chunks) > 1) return launch_held<X, GRAIN, 2, 8, 1>(a, s);
+  return a.K <= 4096 ? launch_held<X, GRAIN, 1, 1, 16>(a, s) : launch_held<X, GRAIN, 1, 1, 4>(a, s);
 }
 
 template <int X>
@@ -728,7 +778,10 @@ int ytm_readout_workspace(int x_dtype, int64_t N, int64_t C, int64_t K, int64_t*
   if (N == 0 || K == 0 || C < 8) return YTM_OK;
   const int planes = x_dtype == YTM_DTYPE_F32 ? 3 : 1, chunks = (int)((C + 127) / 128);
   if (N > ytm::kFewRows) {
-    *bytes = (N + 15) / 16 * ytm::padded_of(chunks) * planes * 4096;
+    *bytes = ytm::frag_bytes(planes, (int)N, chunks);
+    const int whole = ytm::tile_parts_of(planes, ytm::kChunk, (int)N, chunks, (int)K);
+    const int four = ytm::tile_parts_of(planes, ytm::kStep, (int)N, chunks, (int)K);
+    if (whole > 1 || four > 1) *bytes += (whole > four ? whole : four) * N * K * 4;
   } else {
     const int parts = ytm::parts_of(planes, (int)N, chunks);
     if (parts > 1) *bytes = parts * N * K * 4;
