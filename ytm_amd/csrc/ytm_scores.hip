@@ -248,21 +248,29 @@ __device__ __forceinline__ u64 drawn_of(float z, int i, const float* noise) {
 // V is taken from V - P, and the elements before i are not its own.
 template <typename In, int P>
 struct Pack {
-  In raw[P];
+  uint32_t raw[P * sizeof(In) / 4];  // not In[P]: 16-bit elements would take a register each
   __device__ __forceinline__ int load(const In* in, int i, int V) {
     const int at = i + P <= V ? i : V - P;
     if (V >= P) {
       __builtin_memcpy(raw, in + at, sizeof raw);
     } else {
+      In e[P];
 #pragma unroll
-      for (int j = 0; j < P; ++j) raw[j] = at + j >= 0 ? in[at + j] : In{};
+      for (int j = 0; j < P; ++j) e[j] = at + j >= 0 ? in[at + j] : In{};
+      __builtin_memcpy(raw, e, sizeof raw);
     }
     return at;
+  }
+  __device__ __forceinline__ float value(int j) const {
+    if constexpr (sizeof(In) == 4)
+      return __uint_as_float(raw[j]);
+    else
+      return to_float(__builtin_bit_cast(In, (uint16_t)(raw[j / 2] >> (16 * (j % 2)))));
   }
   // the elements as floats, `past` for those not the pack's own
   __device__ __forceinline__ void values(int i, int at, float past, float (&v)[P]) const {
 #pragma unroll
-    for (int j = 0; j < P; ++j) v[j] = to_float(raw[j]);
+    for (int j = 0; j < P; ++j) v[j] = value(j);
     if (at != i) {
 #pragma unroll
       for (int j = 0; j < P; ++j) v[j] = at + j >= i && at + j >= 0 ? v[j] : past;
@@ -640,8 +648,8 @@ __device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const R
 }
 
 // The answer from a histogram over max - z: the slice in which a cut lies, and that slice's answers,
-// sorted, the cut.  each(least, f) calls f(z, index) for this thread's answers, those of a z below
-// `least` not for certain.  False, with nothing written, where a slice holds more than kSub.
+// sorted, the cut.  each(least, few, f) calls f(z, index) for this thread's answers, those of a z below
+// `least` not for certain; `few`: not many are above it.  False, with nothing written, where a slice holds more than kSub.
 template <typename In, typename Each>
 __device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const Row<In>& row, Each each, float best,
                                           int k, float p, Cut cut, ChooseShared& sh) {
@@ -654,7 +662,9 @@ __device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const 
   const bool counted = k > 0;
   const float lightest = best - 28.0f;  // from here on masses are below 2^-40, none
   uint32_t rest = 0;                    // answers of the last slice, which may be nearly all
-  each(counted ? -INFINITY : lightest, [&](float z, int) {
+  const float floor = value_of(cut.key);
+  const bool bounded = cut.key > kNone + 1u;
+  each(counted ? floor : fmaxf(floor, lightest), bounded, [&](float z, int) {
     if (key_of(z) < cut.key) return;
     const int b = bin_of(z);
     const u64 m = mass_of(z, best);
@@ -678,7 +688,8 @@ __device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const 
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     drawn = 0;
-    each(b < kBins - 1 ? best - (float)(b + 2) / kBinsPerUnit : -INFINITY, [&](float z, int i) {
+    each(b < kBins - 1 ? fmaxf(floor, best - (float)(b + 2) / kBinsPerUnit) : floor, b < kBins - 1 || bounded,
+         [&](float z, int i) {
       if (key_of(z) < cut.key) return;
       const int at = bin_of(z);
       if (at == b) {
@@ -788,7 +799,7 @@ __device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, const 
     if (key > least) least = key;
   }
   const float p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
-  const auto each = [&](float, auto f) {
+  const auto each = [&](float, bool, auto f) {
     for (int i = threadIdx.x; i < count; i += kChooseThreads)
       f(value_of((uint32_t)(sh.list[i] >> 32)), (int)~(uint32_t)sh.list[i]);
   };
@@ -869,39 +880,75 @@ __device__ __forceinline__ float with_equals(float score, float t) {
   return t < 1.0f ? fminf(lower, FLT_MAX * t * (1.0f - 0x1p-20f)) : lower;
 }
 
-// Lists the row's scores from `least` on (those above -inf) in an order of threads; whether they
-// fit.  `top` is raised to the largest score this thread has seen.  A thread marks those of 16 packs in 128 bits, without a branch, and reads them again once
-// it knows its place in the list: few reach `least`.
+// Marks, a bit an element, of this thread's packs of kWords x kPacks rounds from `start` on: those of
+// `least` or more.  No branch on what they are; the next four packs are on their way while four are
+// looked at.
 template <typename In>
-__device__ __forceinline__ bool list_from(const In* in, int V, float least, float& top, ChooseShared& sh) {
-  constexpr int P = kPack<In>, kWords = 4, kPacks = 32 / P;  // packs to a word of marks
-  uint32_t listed = 0;
-  bool fits = true;
-  least = fmaxf(least, -FLT_MAX);  // nothing where it is NaN: the largest is what is left of both
-  for (int start = 0; start < V; start += kWords * kPacks * kRound<In>) {
-    uint32_t marks[kWords];
-    uint32_t own = 0;
+struct Marks {
+  static constexpr int P = kPack<In>, kWords = 4, kPacks = 32 / P;  // packs to a word of marks
+  static constexpr int kSpan = kWords * kPacks * kRound<In>;
+  uint32_t word[kWords];
+
+  __device__ __forceinline__ void make(const In* in, int V, int start, float least, float& top) {
+    constexpr int kAtOnce = 4, kSteps = kWords * kPacks / kAtOnce;
+    Pack<In, P> pack[2][kAtOnce];
+    int at[2][kAtOnce];
+    const auto load = [&](int step) {
 #pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-      const int first = start + w * kPacks * kRound<In>;
-      uint32_t m = 0;
-      if (first < V) {
-        Pack<In, P> pack[kPacks];
-        int at[kPacks];
+      for (int u = 0; u < kAtOnce; ++u)
+        at[step % 2][u] = pack[step % 2][u].load(in, index(start, step * kAtOnce + u), V);
+    };
+    load(0);
 #pragma unroll
-        for (int u = 0; u < kPacks; ++u) at[u] = pack[u].load(in, first + u * kRound<In> + P * (int)threadIdx.x, V);
+    for (int w = 0; w < kWords; ++w) word[w] = 0;
 #pragma unroll
-        for (int u = 0; u < kPacks; ++u) {
+    for (int step = 0; step < kSteps; ++step) {
+      if (start + step * kAtOnce * kRound<In> < V) {
+        if (step + 1 < kSteps) load(step + 1);
+        uint32_t m = 0;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
           float v[P];
-          pack[u].values(first + u * kRound<In> + P * (int)threadIdx.x, at[u], -INFINITY, v);
+          pack[step % 2][u].values(index(start, step * kAtOnce + u), at[step % 2][u], -INFINITY, v);
 #pragma unroll
           for (int j = 0; j < P; ++j) m = m * 2 + (v[j] >= least ? 1u : 0u);
           top = fmaxf(top, most(v));
         }
+        word[step * kAtOnce / kPacks] |= m << (32 - P * kAtOnce * (step % (kPacks / kAtOnce) + 1));
       }
-      marks[w] = m;
-      own += __popc(m);
     }
+  }
+  __device__ __forceinline__ static int index(int start, int pack) {
+    return start + pack * kRound<In> + P * (int)threadIdx.x;
+  }
+  // f(index) of the marked elements
+  template <typename F>
+  __device__ __forceinline__ void each(int V, int start, F f) const {
+#pragma unroll
+    for (int w = 0; w < kWords; ++w)
+      for (uint32_t m = word[w]; m;) {
+        const int b = __clz(m);  // pack b / P of the word, its element b % P
+        m &= ~(0x80000000u >> b);
+        const int i = index(start, w * kPacks + b / P);
+        f((i + P <= V ? i : V - P) + b % P);
+      }
+  }
+};
+
+// Lists the row's scores from `least` on (those above -inf) in an order of threads; whether they
+// fit.  They are marked first and read again once each thread knows its place in the list: few reach
+// `least`.  `top` is raised to the largest score this thread has seen.
+template <typename In>
+__device__ __forceinline__ bool list_from(const In* in, int V, float least, float& top, ChooseShared& sh) {
+  uint32_t listed = 0;
+  bool fits = true;
+  least = fmaxf(least, -FLT_MAX);  // nothing where it is NaN: the largest is what is left of both
+  for (int start = 0; start < V; start += Marks<In>::kSpan) {
+    Marks<In> marks;
+    marks.make(in, V, start, least, top);
+    uint32_t own = 0;
+#pragma unroll
+    for (int w = 0; w < Marks<In>::kWords; ++w) own += __popc(marks.word[w]);
     const uint32_t upto = (uint32_t)block_upto(own, sh);
     uint32_t place = listed + upto - own;
     __syncthreads();
@@ -912,15 +959,9 @@ __device__ __forceinline__ bool list_from(const In* in, int V, float least, floa
       fits = false;
       continue;
     }
-#pragma unroll
-    for (int w = 0; w < kWords; ++w)
-      for (uint32_t m = marks[w]; m;) {
-        const int b = __clz(m);  // pack b / P of the word, its element b % P
-        m &= ~(0x80000000u >> b);
-        const int i = start + (w * kPacks + b / P) * kRound<In> + P * (int)threadIdx.x;
-        const int e = (i + P <= V ? i : V - P) + b % P;
-        sh.list[place++] = (u64)key_of(to_float(in[e]) + 0.0f) << 32 | (uint32_t)~e;
-      }
+    marks.each(V, start, [&](int e) {
+      sh.list[place++] = (u64)key_of(to_float(in[e]) + 0.0f) << 32 | (uint32_t)~e;
+    });
   }
   __syncthreads();
   if (threadIdx.x == 0) sh.listed = listed;
@@ -1085,10 +1126,20 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
     const uint32_t key = key_of((low <= best ? low : best) + 0.0f);
     if (key > cut.key) cut.key = key;
   }
-  const auto each = [&](float least, auto f) {
+  // Where a bound leaves few scores, the threads mark them and go through their marks: every lane
+  // of a wave would wait for those few otherwise.
+  const auto each = [&](float least, bool few, auto f) {
     const float from = least > -INFINITY ? with_equals(least * t, t) : -FLT_MAX;
+    if (few) {
+      for (int start = 0; start < V; start += Marks<In>::kSpan) {
+        Marks<In> marks;
+        float unused = -INFINITY;
+        marks.make(row.in, V, start, fmaxf(from, -FLT_MAX), unused);
+        marks.each(V, start, [&](int e) { f(row(e), e); });
+      }
+      return;
+    }
     each_pack<16 / kPack<In>>(row.in, V, V, [&](int i, auto& v) {
-      if (!(most(v) >= from)) return;
 #pragma unroll
       for (int j = 0; j < kPack<In>; ++j)
         if (v[j] >= from) f(scaled(v[j], t), i + j);
