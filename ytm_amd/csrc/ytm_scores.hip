@@ -890,7 +890,7 @@ struct Marks {
   uint32_t word[kWords];
 
   __device__ __forceinline__ void make(const In* in, int V, int start, float least, float& top) {
-    constexpr int kAtOnce = 4, kSteps = kWords * kPacks / kAtOnce;
+    constexpr int kAtOnce = sizeof(In) == 4 ? 4 : 2, kSteps = kWords * kPacks / kAtOnce;
     Pack<In, P> pack[2][kAtOnce];
     int at[2][kAtOnce];
     const auto load = [&](int step) {
