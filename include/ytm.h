@@ -318,10 +318,13 @@ int ytm_adjust_scores(const void *scores, int dtype, int64_t stride, int64_t N, 
  * tokens[n] = the index of the largest z + noise[n][v] (NULL: of z) of the kept answers, the
  * lowest of equal ones, and logprobs[n] = z of it - log of the kept answers' sum of exp(z).
  * With standard Gumbel noise -log(-log(u)) that is a draw from softmax(z) over the kept
- * answers.  Noise is finite.  -1 and -inf where no score is above -inf. */
+ * answers.  Noise is finite.  -1 and -inf where no score is above -inf.  workspace: device memory
+ * of ytm_choose_workspace's bytes at a multiple of 16 bytes, for the time of the call's work (NULL
+ * where that is 0: rows that are short or many). */
+int ytm_choose_workspace(int dtype, int64_t N, int64_t V, int64_t *bytes);
 int ytm_choose(const void *scores, int dtype, int64_t stride, int64_t N, int64_t V, const float *temperature,
                const int32_t *top_k, const float *top_p, const float *min_p, const float *noise, int64_t noise_stride,
-               int32_t *tokens, float *logprobs, void *stream);
+               int32_t *tokens, float *logprobs, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -85,7 +85,7 @@ ADJUST = dict(scores=P, dtype=7, stride=8, N=2, V=8, tokens=P, token_stride=4, T
               repetition=None, frequency=None, presence=None, bias=P, bias_stride=8, allowed=P, allowed_stride=1,
               out=P, out_dtype=7, out_stride=8, stream=None)
 CHOOSE = dict(scores=P, dtype=7, stride=8, N=2, V=8, temperature=None, top_k=None, top_p=None, min_p=None, noise=P,
-              noise_stride=8, tokens=P, logprobs=P, stream=None)
+              noise_stride=8, tokens=P, logprobs=P, workspace=None, workspace_bytes=0, stream=None)
 
 
 @pytest.mark.parametrize("function,base,wrong", [
@@ -107,7 +107,9 @@ CHOOSE = dict(scores=P, dtype=7, stride=8, N=2, V=8, temperature=None, top_k=Non
 ] + [
     ("ytm_choose", CHOOSE, w) for w in (
         dict(dtype=8), dict(N=-1), dict(V=-1), dict(V=(1 << 23) + 1), dict(scores=None), dict(tokens=None),
-        dict(logprobs=None), dict(stride=7), dict(noise_stride=7))
+        dict(logprobs=None), dict(stride=7), dict(noise_stride=7),
+        *(dict(V=100000, stride=100000, noise_stride=100000, **w) for w in (
+            {}, dict(workspace=P, workspace_bytes=100), dict(workspace=P + 8, workspace_bytes=1 << 30))))
 ])
 def test_boundary_refusals(function, base, wrong):
     assert getattr(_lib.lib, function)(*{**base, **wrong}.values()) == _lib.YTM_EINVAL
@@ -129,4 +131,15 @@ def test_workspace():
     for args in ((7, 0, 1000, 1), (7, 3, 0, 5), (7, 17, 7, 10), (11, 1, 10000, 10000), (7, 16, 256, 5)):
         assert ask(*args, n) == _lib.YTM_OK and n.value == 0
     for args in ((7, 16, 20000, 10), (11, 17, 8, 1)):
+        assert ask(*args, n) == _lib.YTM_OK and n.value > 0
+
+
+def test_choose_workspace():
+    n = ctypes.c_int64(-1)
+    ask = _lib.lib.ytm_choose_workspace
+    for wrong in ((8, 1, 1, n), (7, -1, 1, n), (7, 1, -1, n), (7, 1, (1 << 23) + 1, n), (7, 1, 1, None)):
+        assert ask(*wrong) == _lib.YTM_EINVAL
+    for args in ((7, 0, 100000), (7, 3, 32767), (10, 1, 65535), (7, 65, 100000)):
+        assert ask(*args, n) == _lib.YTM_OK and n.value == 0
+    for args in ((7, 1, 32768), (9, 64, 65536)):
         assert ask(*args, n) == _lib.YTM_OK and n.value > 0

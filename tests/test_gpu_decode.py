@@ -452,6 +452,22 @@ def test_choose_many_rows():
     choose_case(300, 700, "normal", "kmp", 2)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["normal", "flat", "odd"])
+@pytest.mark.parametrize("filters", ["", "k", "m", "p", "kmp"])
+def test_choose_many_long_rows(kind, filters, dtype):
+    """Rows long enough to be sliced where they are few, and too many for that."""
+    choose_case(66, 66000, kind, filters, 4, dtype)
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 32767), ("f32", 32768), ("f16", 65535), ("bf16", 65536), ("f32", 300001)])
+@pytest.mark.parametrize("filters", ["", "k", "m", "kmp"])
+def test_choose_sliced_rows(dtype, V, filters):
+    """Around the length from which few rows are sliced, and slices of the largest size."""
+    for kind in ("normal", "masked", "odd"):
+        choose_case(3, V, kind, filters, 6, dtype)
+
+
 def test_choose_filter_ends():
     """Bounds that keep the first answer alone, or all of them."""
     x = torch.tensor([[0.0, 2.0, 1.0, 2.0]], device="cuda").repeat(6, 1)

@@ -103,7 +103,8 @@ SIGNATURES = {
                                    ctypes.c_int, _I64, _P, _I64, _P]),
     "ytm_adjust_scores": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P,
                                          _I64, _P, _I64, _P, ctypes.c_int, _I64, _P]),
-    "ytm_choose": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P]),
+    "ytm_choose_workspace": (ctypes.c_int, [ctypes.c_int, _I64, _I64, ctypes.POINTER(_I64)]),
+    "ytm_choose": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _P]),
 }
 
 # Element types of the answering operators (YTM_DTYPE_* of include/ytm.h).

@@ -194,6 +194,8 @@ struct ChooseArgs {
   int64_t noise_stride;
   int32_t* tokens;
   float* logprobs;
+  int slices, each;  // of a row, and scores in one (0: rows are not sliced)
+  struct Slice* found;
 };
 
 typedef unsigned long long u64;
@@ -579,23 +581,34 @@ __device__ __forceinline__ void sort_runs(u64 (&v)[4], int l) {
   sort_step<K, K / 2>(v, l);
 }
 
-// Every answer may be drawn.  Sums are kept in double: a float's would lose what many small terms
-// add up to.
+// The largest z of a part of a row, the sum of exp(z - it), the largest z + noise with its index
+// (0: no z above -inf).
+struct All {
+  float best;
+  double sum;
+  u64 drawn;
+};
+
+// Every answer may be drawn: what a block finds of answers begin .. end - 1, sum in thread 0 alone.
+// Sums are kept in double: a float's would lose what many small terms add up to.
 template <typename In>
-__device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const Row<In>& row, ChooseShared& sh) {
-  const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
+__device__ __forceinline__ All all_of(const ChooseArgs& a, int64_t n, const Row<In>& row, int begin, int end,
+                                      ChooseShared& sh) {
+  const float* noise = a.noise ? a.noise + n * a.noise_stride + begin : nullptr;
+  const In* in = row.in + begin;
+  const int V = end - begin;
   float top = -INFINITY;
   double sum = 0.0;
   u64 drawn = 0;
   constexpr int P = kPack<In>;
-  for (int first = P * threadIdx.x; first < a.V; first += 2 * kRound<In>) {
+  for (int first = P * threadIdx.x; first < V; first += 2 * kRound<In>) {
     Pack<In, P> score[2];
     Pack<float, P> more[2];
     int at[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      at[u] = score[u].load(row.in, first + u * kRound<In>, a.V);
-      if (noise) more[u].load(noise, first + u * kRound<In>, a.V);
+      at[u] = score[u].load(in, first + u * kRound<In>, V);
+      if (noise) more[u].load(noise, first + u * kRound<In>, V);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -616,7 +629,7 @@ __device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const R
         part += expf(z[j] - top);
         float y = noise ? z[j] + g[j] : z[j];
         y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
-        const u64 d = z[j] > -INFINITY ? (u64)key_of(y) << 32 | (uint32_t)~(at[u] + j) : 0;
+        const u64 d = z[j] > -INFINITY ? (u64)key_of(y) << 32 | (uint32_t)~(begin + at[u] + j) : 0;
         drawn = d > drawn ? d : drawn;
       }
       sum += (double)part;
@@ -631,19 +644,27 @@ __device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const R
   }
   __syncthreads();
   drawn = parts_all(kChooseWaves, sh, Max());
-  if (drawn == 0) return no_answer(a, n);
   const int l = threadIdx.x % kWave;
   const float best = value_of((uint32_t)wave_all(sh.tops[l % kChooseWaves], Max()));
-  sum *= (double)expf(top - best);
+  sum *= top > -INFINITY ? (double)expf(top - best) : 0.0;
   for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
   if (l == 0) sh.sums[threadIdx.x / kWave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0.0;
     for (int w = 0; w < kChooseWaves; ++w) sum += sh.sums[w];
-    const int i = (int)~(uint32_t)drawn;
+  }
+  return All{best, sum, drawn};
+}
+
+// Thread 0 writes the answer.
+template <typename In>
+__device__ __forceinline__ void from_all(const ChooseArgs& a, int64_t n, const Row<In>& row, const All& all) {
+  if (all.drawn == 0) return no_answer(a, n);
+  if (threadIdx.x == 0) {
+    const int i = (int)~(uint32_t)all.drawn;
     a.tokens[n] = i;
-    a.logprobs[n] = (row(i) - best) - logf((float)sum);
+    a.logprobs[n] = (row(i) - all.best) - logf((float)all.sum);
   }
 }
 
@@ -1079,45 +1100,138 @@ __device__ __forceinline__ void from_small(const ChooseArgs& a, int64_t n, int c
     }
 }
 
+// A row's filters.
+struct Filters {
+  float t, p, min;
+  int k;
+  bool bounded, seek;  // min_p holds; top_k is sought by a bound
+
+  __device__ __forceinline__ Filters(const ChooseArgs& a, int64_t n) {
+    t = a.temperature ? a.temperature[n] : 1.0f;
+    k = a.top_k ? a.top_k[n] : 0;
+    if (t <= 0.0f) {
+      t = 1.0f;
+      k = 1;
+    }
+    if (k >= a.V) k = 0;
+    p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
+    min = a.min_p ? a.min_p[n] : 0.0f;
+    bounded = min > 0.0f;
+    seek = k > 0 && k <= kMaxSeek;
+  }
+  __device__ __forceinline__ bool none() const { return k <= 0 && p >= 1.0f && !bounded; }
+};
+
+// Lists what may be kept of `V` scores (a row, or a slice, whose k-th largest and largest are no larger
+// than the row's), with a bound from their first `rounds` rounds; whether it fits.
+template <typename In>
+__device__ __forceinline__ bool list_kept(const In* in, int V, int rounds, const Filters& f, float& own,
+                                          ChooseShared& sh) {
+  own = own_most(in, V, rounds);
+  float least;
+  if (f.seek) {
+    const uint32_t bound = kth_of(key_of(own + 0.0f), f.k, sh);
+    least = bound > kNone ? with_equals(value_of(bound), f.t) : -INFINITY;
+  } else {
+    const float z = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), f.t);
+    const float low = z + logf(f.min);
+    least = with_equals((low <= z ? low : z) * f.t, f.t);
+  }
+  return list_from(in, V, least, own, sh);
+}
+
+// A CU reads about 40 GB/s here whatever is on its way, so a long row alone takes 13 us per 512 KB:
+// where rows are few, slices of them go to blocks of their own, which leave for the row's block
+// what they list (`count` entries; more than kSliceList, or a row whose filters no list serves: -1)
+// or, without filters, what all_of finds.
+constexpr int kSliceList = 512;
+struct Slice {
+  int count;
+  float best;
+  double sum;
+  u64 drawn;
+  u64 list[kSliceList];
+};
+
+template <typename In>
+__global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(4, 4))) void slice_kernel(
+    ChooseArgs a) {
+  __shared__ ChooseShared sh;
+  const int64_t n = blockIdx.y;
+  const int begin = blockIdx.x * a.each, end = begin + a.each < a.V ? begin + a.each : a.V;
+  const Filters f(a, n);
+  const Row<In> row{(const In*)a.scores + n * a.stride, f.t};
+  Slice& to = a.found[n * a.slices + blockIdx.x];
+  if (f.none()) {
+    const All all = all_of(a, n, row, begin, end, sh);
+    if (threadIdx.x == 0) {
+      to.best = all.best;
+      to.sum = all.sum;
+      to.drawn = all.drawn;
+    }
+    return;
+  }
+  int count = -1;
+  if (f.seek || f.bounded) {
+    float own;
+    const int rounds = (end - begin + kRound<In> - 1) / kRound<In>;
+    if (list_kept(row.in + begin, end - begin, rounds, f, own, sh) && sh.listed <= kSliceList) {
+      count = (int)sh.listed;
+      for (int i = threadIdx.x; i < count; i += kChooseThreads) to.list[i] = sh.list[i] - (uint32_t)begin;  // ~index
+    }
+  }
+  if (threadIdx.x == 0) to.count = count;
+}
+
 template <typename In>
 __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(4, 4))) void choose_kernel(
     ChooseArgs a) {
   __shared__ ChooseShared sh;
   const int64_t n = blockIdx.x;
   const int V = a.V;
-  float t = a.temperature ? a.temperature[n] : 1.0f;
-  int k = a.top_k ? a.top_k[n] : 0;
-  if (t <= 0.0f) {
-    t = 1.0f;
-    k = 1;
-  }
-  if (k >= V) k = 0;
-  const float p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
-  const bool bounded = a.min_p && a.min_p[n] > 0.0f;
+  const Filters filters(a, n);
+  const float t = filters.t, p = filters.p;
+  const int k = filters.k;
+  const bool bounded = filters.bounded;
   const Row<In> row{(const In*)a.scores + n * a.stride, t};
-  if (k <= 0 && p >= 1.0f && !bounded) return from_all(a, n, row, sh);
-  const int rounds = (V + kRound<In> - 1) / kRound<In>;
-  float own = -INFINITY;
-  const bool seek = k > 0 && k <= kMaxSeek;
-  if (seek || bounded) {  // a bound from a quarter of the row, and the list of what reaches it
-    own = own_most(row.in, V, (rounds + 3) / 4);
-    float least;
-    if (seek) {
-      const uint32_t bound = kth_of(key_of(own + 0.0f), k, sh);
-      least = bound > kNone ? with_equals(value_of(bound), t) : -INFINITY;
-    } else {  // no larger than that of the row's largest
-      const float z = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), t);
-      const float low = z + logf(a.min_p[n]);
-      least = with_equals((low <= z ? low : z) * t, t);
-    }
-    if (list_from(row.in, V, least, own, sh)) {
-      int count = (int)sh.listed;
-      if (seek && count > kSmall) count = shorten_list(count, t, k, sh);
-      return count <= kSmall ? from_small(a, n, count, t, k, sh) : from_list(a, n, row, count, k, sh);
-    }
-  } else {
-    own = own_most(row.in, V, rounds);
+  const Slice* slices = a.found + n * a.slices;
+  const auto from_entries = [&](int count) {
+    if (filters.seek && count > kSmall) count = shorten_list(count, t, k, sh);
+    return count <= kSmall ? from_small(a, n, count, t, k, sh) : from_list(a, n, row, count, k, sh);
+  };
+  if (filters.none()) {
+    if (a.slices == 0) return from_all(a, n, row, all_of(a, n, row, 0, V, sh));
+    if (threadIdx.x >= kWave) return;
+    const int l = threadIdx.x;  // a slice a lane
+    const bool real = l < a.slices;
+    const u64 drawn = wave_all(real ? slices[l].drawn : 0, Max());
+    const float top = real ? slices[l].best : -INFINITY;
+    const float best = value_of((uint32_t)wave_all(key_of(top), Max()));
+    double sum = top > -INFINITY ? slices[l].sum * (double)expf(top - best) : 0.0;
+    for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
+    return from_all(a, n, row, All{best, sum, drawn});
   }
+  float own = -INFINITY;
+  bool known = false;  // whether `own` covers the row
+  if (a.slices > 0 && (filters.seek || bounded)) {
+    const int l = threadIdx.x % kWave;
+    const int mine = l < a.slices ? slices[l].count : 0;
+    const u64 upto = wave_scan(mine > 0 ? mine : 0, Add());
+    const int count = (int)lane_value(upto, kWave - 1);
+    if (!__any(mine < 0) && count <= kList) {
+      for (int s = threadIdx.x / kWave; s < a.slices; s += kChooseWaves) {
+        const int many = __builtin_amdgcn_readlane(mine, s), to = (int)lane_value(upto, s) - many;
+        for (int i = l; i < many; i += kWave) sh.list[to + i] = slices[s].list[i];
+      }
+      __syncthreads();
+      return from_entries(count);
+    }
+  } else if (filters.seek || bounded) {
+    const int rounds = (V + kRound<In> - 1) / kRound<In>;
+    if (list_kept(row.in, V, (rounds + 3) / 4, filters, own, sh)) return from_entries((int)sh.listed);
+    known = true;
+  }
+  if (!known) own = own_most(row.in, V, (V + kRound<In> - 1) / kRound<In>);
   const float best = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), t);
   if (best == -INFINITY) return no_answer(a, n);
   Cut cut{kNone + 1u, V - 1};
@@ -1148,6 +1262,14 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   if ((k > 0 || p < 1.0f) && from_bins(a, n, row, each, best, k, p, cut, sh)) return;
   __syncthreads();
   from_row(a, n, row, best, k, p, cut, sh);
+}
+
+// Slices of each row: none where a row has less than 128 KB or the rows alone take a quarter of the
+// 256 CUs, else 32 KB each, up to 16 (16 lists of the largest top_k sought fit one of kList).
+int slices_of(int size, int64_t N, int64_t V) {
+  if (V * size < 128 * 1024 || N > 64) return 0;
+  const int64_t slices = (V * size + 32 * 1024 - 1) / (32 * 1024);
+  return slices < 16 ? (int)slices : 16;
 }
 
 }  // namespace
@@ -1186,9 +1308,16 @@ int ytm_adjust_scores(const void* scores, int dtype, int64_t stride, int64_t N, 
   return YTM_OK;
 }
 
+int ytm_choose_workspace(int dtype, int64_t N, int64_t V, int64_t* bytes) {
+  if (!bytes || !ytm::decode_float(dtype) || N < 0 || N > INT32_MAX || V < 0 || V > ytm::kMaxScores)
+    return fail(YTM_EINVAL, "bad choose_workspace arguments");
+  *bytes = N * ytm::slices_of(dtype == YTM_DTYPE_F32 ? 4 : 2, N, V) * (int64_t)sizeof(ytm::Slice);
+  return YTM_OK;
+}
+
 int ytm_choose(const void* scores, int dtype, int64_t stride, int64_t N, int64_t V, const float* temperature,
                const int32_t* top_k, const float* top_p, const float* min_p, const float* noise, int64_t noise_stride,
-               int32_t* tokens, float* logprobs, void* stream) {
+               int32_t* tokens, float* logprobs, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!ytm::decode_float(dtype)) return fail(YTM_EINVAL, "scores are float32, float16 or bfloat16");
   if (N < 0 || V < 0 || N > INT32_MAX || V > ytm::kMaxScores)
     return fail(YTM_EINVAL, "choose takes at most 8388608 scores a row");
@@ -1196,8 +1325,24 @@ int ytm_choose(const void* scores, int dtype, int64_t stride, int64_t N, int64_t
   if ((V > 0 && !scores) || !tokens || !logprobs) return fail(YTM_EINVAL, "bad choose arguments");
   if (N > 1 && (stride < V || (noise && noise_stride != 0 && noise_stride < V)))
     return fail(YTM_EINVAL, "choose: rows overlap");
-  ytm::ChooseArgs a{scores, stride, (int)V, temperature, top_k, top_p, min_p, noise, noise_stride, tokens, logprobs};
+  int64_t need = 0;
+  if (int rc = ytm_choose_workspace(dtype, N, V, &need)) return rc;
+  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+    return fail(YTM_EINVAL, "choose: the workspace is too small or not at a multiple of 16 bytes");
+  const int slices = ytm::slices_of(dtype == YTM_DTYPE_F32 ? 4 : 2, N, V);
+  const ytm::ChooseArgs a{scores, stride, (int)V, temperature, top_k, top_p, min_p, noise, noise_stride, tokens, logprobs,
+                          slices, slices ? (int)((V + slices - 1) / slices) : 0, (ytm::Slice*)workspace};
   hipStream_t s = (hipStream_t)stream;
+  if (slices) {
+    const dim3 grid(slices, (unsigned)N);
+    switch (dtype) {
+      case YTM_DTYPE_F16: ytm::slice_kernel<ytm::f16><<<grid, ytm::kChooseThreads, 0, s>>>(a); break;
+      case YTM_DTYPE_BF16: ytm::slice_kernel<ytm::bf16><<<grid, ytm::kChooseThreads, 0, s>>>(a); break;
+      default: ytm::slice_kernel<float><<<grid, ytm::kChooseThreads, 0, s>>>(a); break;
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(YTM_EHIP, std::string("choose failed: ") + hipGetErrorString(e));
+  }
   switch (dtype) {
     case YTM_DTYPE_F16: ytm::choose_kernel<ytm::f16><<<(unsigned)N, ytm::kChooseThreads, 0, s>>>(a); break;
     case YTM_DTYPE_BF16: ytm::choose_kernel<ytm::bf16><<<(unsigned)N, ytm::kChooseThreads, 0, s>>>(a); break;

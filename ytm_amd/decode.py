@@ -169,6 +169,15 @@ def _call(function, device: int, *args) -> None:
         check(rc)
 
 
+def _workspace(function, device: torch.device, *args) -> tuple[int, torch.Tensor | None]:
+    """The bytes that function(*args) asks for, and a tensor of them (None for 0)."""
+    need = ctypes.c_int64()
+    rc = function(*args, need)
+    if rc:
+        check(rc)
+    return need.value, torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+
+
 def readout(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: int = 32, clauses: int | None = None,
             out: torch.Tensor | None = None) -> torch.Tensor:
     """Class sums (N, K) of clause outputs x through weights in 4 bits (pack_weights).
@@ -202,13 +211,7 @@ def readout(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: i
     out, out_type = _result(out, (N, K), device)
     need, workspace = 0, None
     if N > 16 or C * N > 4096:  # fewer are held in one block's LDS
-        need = ctypes.c_int64()
-        rc = lib.ytm_readout_workspace(x_type, N, C, K, need)
-        if rc:
-            check(rc)
-        need = need.value
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        need, workspace = _workspace(lib.ytm_readout_workspace, x.device, x_type, N, C, K)
     _call(lib.ytm_readout, device, x.data_ptr(), x_type, x.stride(0), N, C, codes.data_ptr(), codes.stride(0),
           scales.data_ptr(), _FLOATS[scales.dtype], scales.stride(0), group, K, out.data_ptr(), out_type,
           out.stride(0), workspace.data_ptr() if need else None, need)
@@ -273,6 +276,9 @@ def choose(scores: torch.Tensor, temperature: torch.Tensor | None = None, top_k:
     where = scores.device
     tokens = torch.empty(N, dtype=torch.int32, device=where)
     logprobs = torch.empty(N, dtype=torch.float32, device=where)
+    need, workspace = 0, None
+    if V >= 32768 and N <= 64:  # fewer or more rows are not sliced
+        need, workspace = _workspace(lib.ytm_choose_workspace, where, dtype, N, V)
     _call(lib.ytm_choose, device, scores.data_ptr(), dtype, scores.stride(0), N, V, temperature, top_k, top_p, min_p,
-          noise, noise_stride, tokens.data_ptr(), logprobs.data_ptr())
+          noise, noise_stride, tokens.data_ptr(), logprobs.data_ptr(), workspace.data_ptr() if need else None, need)
     return tokens, logprobs
