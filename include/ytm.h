@@ -309,7 +309,7 @@ int ytm_adjust_scores(const void *scores, int dtype, int64_t stride, int64_t N, 
                       int64_t out_stride, void *stream);
 
 /* ytm_choose: one of V (at most 8388608) answers for each row.  With z = score / temperature[n]
- * (NULL: 1; 0 or less: temperature 1 and top_k 1; a NaN score counts as -inf, +inf as the
+ * (NULL: 1; 0 or less: temperature 1 and top_k 1; less than the smallest normal float: that; a NaN score counts as -inf, +inf as the
  * largest float) and the answers in the order of z descending, then index ascending, the filters keep
  * a first part of that order, the first answer always among it:
  *   min_p: z >= max z + log(min_p[n]);  top_k: the first top_k[n] of these (0 or less: all);

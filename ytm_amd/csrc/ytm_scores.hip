@@ -225,8 +225,13 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 constexpr uint32_t kNone = 0x007FFFFFu;  // key of -inf
 
+// score / t: the product with the reciprocal, corrected by its remainder, which rounds as the division
+// does (but for quotients below the normal floats) in half its instructions; t of a row is the
+// same for all its scores, so the reciprocal is made once.
 __device__ __forceinline__ float scaled(float score, float t) {
-  const float z = score / t;
+  const float r = 1.0f / t, q = score * r;
+  const float c = __builtin_fmaf(__builtin_fmaf(-q, t, score), r, q);
+  const float z = c == c ? c : q;  // infinities have no remainder
   return (z != z ? -INFINITY : fminf(z, FLT_MAX)) + 0.0f;
 }
 
@@ -237,7 +242,20 @@ struct Row {
   __device__ __forceinline__ float operator()(int i) const { return scaled(to_float(in[i]), t); }
 };
 
-__device__ __forceinline__ u64 mass_of(float z, float best) { return (u64)(expf(z - best) * kMass); }
+// exp(x) for x <= 0 as 2^(x log2 e), the rounding of that product put back: within two units in the last
+// place, 0 below 2^-126.
+__device__ __forceinline__ float exp_of(float x) {
+  const float y = x * 1.44269502f;
+  const float rest = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269502f, -y));
+  const float e = __builtin_amdgcn_exp2f(y);
+  return y > -INFINITY ? __builtin_fmaf(e, rest * 0.693147182f, e) : 0.0f;
+}
+
+__device__ __forceinline__ u64 mass_of(float z, float best) {
+  const float e = exp_of(z - best) * 256.0f;  // the upper 8 of 40 bits, then the lower 32
+  const uint32_t high = (uint32_t)e;
+  return (u64)high << 32 | (uint32_t)((e - (float)high) * 4294967296.0f);
+}
 
 __device__ __forceinline__ u64 drawn_of(float z, int i, const float* noise) {
   float y = noise ? z + noise[i] : z;
@@ -626,7 +644,7 @@ __device__ __forceinline__ All all_of(const ChooseArgs& a, int64_t n, const Row<
       float part = 0.0f;
 #pragma unroll
       for (int j = 0; j < P; ++j) {
-        part += expf(z[j] - top);
+        part += exp_of(z[j] - top);
         float y = noise ? z[j] + g[j] : z[j];
         y = y >= -FLT_MAX ? y + 0.0f : -FLT_MAX;
         const u64 d = z[j] > -INFINITY ? (u64)key_of(y) << 32 | (uint32_t)~(begin + at[u] + j) : 0;
@@ -1113,6 +1131,7 @@ struct Filters {
       t = 1.0f;
       k = 1;
     }
+    t = fmaxf(t, FLT_MIN);  // a smaller one has no reciprocal; a NaN too becomes it
     if (k >= a.V) k = 0;
     p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
     min = a.min_p ? a.min_p[n] : 0.0f;
@@ -1212,7 +1231,6 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
     return from_all(a, n, row, All{best, sum, drawn});
   }
   float own = -INFINITY;
-  bool known = false;  // whether `own` covers the row
   if (a.slices > 0 && (filters.seek || bounded)) {
     const int l = threadIdx.x % kWave;
     const int mine = l < a.slices ? slices[l].count : 0;
@@ -1226,12 +1244,13 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
       __syncthreads();
       return from_entries(count);
     }
-  } else if (filters.seek || bounded) {
+  }
+  if (filters.seek || bounded) {
     const int rounds = (V + kRound<In> - 1) / kRound<In>;
     if (list_kept(row.in, V, (rounds + 3) / 4, filters, own, sh)) return from_entries((int)sh.listed);
-    known = true;
+  } else {
+    own = own_most(row.in, V, (V + kRound<In> - 1) / kRound<In>);
   }
-  if (!known) own = own_most(row.in, V, (V + kRound<In> - 1) / kRound<In>);
   const float best = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), t);
   if (best == -INFINITY) return no_answer(a, n);
   Cut cut{kNone + 1u, V - 1};
