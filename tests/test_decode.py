@@ -63,6 +63,14 @@ def test_host_refusals(call):
         call()
 
 
+def test_clause_banks_refused():
+    class Banks:
+        coalesced = False
+
+    with pytest.raises(ValueError, match="banks"):
+        decode.pack_model(Banks(), device="cpu")
+
+
 def test_scale_type_refused():
     with pytest.raises(TypeError):
         decode.pack_weights(np.zeros((3, 2), np.float32), dtype=torch.float64, device="cpu")

@@ -166,13 +166,27 @@ def test_readout_of_a_model():
     tm.load_state_dict({"state": {"ta_state": ta, "clause_weights": w, "min_y": None, "max_y": None,
                                   "patch_weights": np.zeros((C, 1), np.int32)}})
     X = rng.integers(0, 2, (40, 60)).astype(np.uint32)
-    codes, scales = decode.pack_weights(tm.get_weights())
-    # transform lets clauses without literals fire, class sums leave them out
-    empty = (tm.get_literals().sum(1) == 0)
-    fires = tm.transform(X)
-    fires[:, empty] = 0
-    got = decode.readout(decode.pack_outputs(fires), codes, scales, clauses=C)
-    np.testing.assert_array_equal(got.cpu().numpy(), tm.score(X, False) if hasattr(tm, "score") else None)
+    codes, scales = decode.pack_model(tm)
+    got = decode.readout(decode.pack_outputs(tm.transform(X)), codes, scales, clauses=C)
+    np.testing.assert_array_equal(got.cpu().numpy(), tm.score(tm.encode(X), True))
+
+
+def test_example_goes_on_writing():
+    """The example's steps together: the grammar holds, and training shows."""
+    import sys
+    from pathlib import Path
+
+    sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "examples"))
+    import next_word
+
+    tm, after = next_word.train(samples=6000, epochs=3)
+    said = next_word.write(tm, texts=5, length=12)
+    assert said.shape == (5, 12 + next_word.CONTEXT) and (said >= 0).all() and (said < next_word.WORDS).all()
+    stops = said == next_word.STOP
+    assert not (stops[:, 1:] & stops[:, :-1]).any()
+    follows = (after[said[:, next_word.CONTEXT - 1:-1]] == said[:, next_word.CONTEXT:, None]).any(2)
+    assert follows.mean() > 0.5  # 4 of 60 words do
+    np.testing.assert_array_equal(said, next_word.write(tm, texts=5, length=12))
 
 
 # --------------------------------------------------------------------------- adjust_scores

@@ -2,7 +2,7 @@
 
 A model with many outputs, such as one a word of a vocabulary, answers in three steps:
 
-    codes, scales = decode.pack_weights(tm.get_weights())          # once: weights in 4 bits
+    codes, scales = decode.pack_model(tm)                          # once: weights in 4 bits
     bits = decode.pack_outputs(tm.transform(X))                    # clause outputs, packed
     scores = decode.readout(bits, codes, scales, clauses=C)        # class sums (N, K)
     scores = decode.adjust_scores(scores, tokens=said, ...)        # penalties, bias, grammar
@@ -10,7 +10,7 @@ A model with many outputs, such as one a word of a vocabulary, answers in three 
 
 readout, adjust_scores and choose take torch tensors on one GPU and put their work on the
 current stream of that GPU without waiting for it, as torch's own operations do (they may be
-captured into a graph); pack_weights and pack_outputs turn the framework's host arrays into such
+captured into a graph); pack_model, pack_weights and pack_outputs turn the framework's host arrays into such
 tensors.  Rows may be any distance apart; a row's elements follow one another.  A wrong argument
 raises TypeError or ValueError before anything is launched.  There are no gradients: clause
 outputs are bits made by automata and the codes are made from trained weights, so tensors that
@@ -59,6 +59,18 @@ def pack_weights(weights: np.ndarray, group: int = 32, dtype: torch.dtype = torc
     code = np.zeros((K, padded), np.uint8)
     code[:, :C] = np.searchsorted(_BETWEEN, np.abs(scaled), side="left") | (scaled < 0).astype(np.uint8) << 3
     return torch.from_numpy(code[:, 0::2] | code[:, 1::2] << 4).to(device), scales.to(device)
+
+
+def pack_model(tm, group: int = 32, dtype: torch.dtype = torch.float32,
+               device: str | torch.device = "cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """pack_weights of a model's clause weights, for the clause outputs that transform() gives:
+    clauses without literals, which transform() lets fire and class sums leave out, get zeros.
+    Models with clause banks (coalesced=False) are refused."""
+    if not tm.coalesced:
+        raise ValueError("pack_model takes coalesced models, not clause banks.")
+    weights = tm.get_weights()
+    weights[~tm.get_literals().any(axis=1)] = 0.0
+    return pack_weights(weights, group, dtype, device)
 
 
 def unpack_weights(codes: torch.Tensor, scales: torch.Tensor, clauses: int, group: int = 32) -> np.ndarray:
