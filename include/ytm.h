@@ -275,7 +275,8 @@ int ytm_collapse_bins(const uint32_t *B, int64_t rows, int64_t width, int kind, 
  * hipStream_t of the current device, NULL the default one) without waiting for it: what they
  * read must stay until the stream has passed, and results are there once it has.  They allocate
  * nothing and may be captured into a graph.  Rows may be any distance apart (strides in
- * elements, of codes in bytes); a row's elements follow one another.  Their errors are those
+ * elements, of codes in bytes; 0 in what is read: one row for all); a row's elements follow one
+ * another.  Their errors are those
  * of their arguments and of the launch.  Sums are made in f32 and rounded once; results do not
  * depend on the order in which blocks run.
  *

@@ -578,6 +578,25 @@ def test_captured_into_a_graph(N, C, K):
         assert same(want, out), seed
 
 
+def test_one_row_for_all():
+    """Rows that are one (stride 0) read as if they were copies."""
+    rng = np.random.default_rng(2)
+    codes, scales, _ = weights(rng, 300, 40, 32, "f32", True)
+    dev = [torch.from_numpy(codes).cuda(), scales.cuda()]
+    for N in (5, 40):
+        x = torch.randn(1, 300, device="cuda")
+        assert torch.equal(decode.readout(x.expand(N, 300), *dev), decode.readout(x.expand(N, 300).contiguous(), *dev))
+        s, t = torch.randn(1, 500, device="cuda"), torch.arange(9, dtype=torch.int32, device="cuda").view(1, 9)
+        rep, noise = torch.rand(N, device="cuda") + 1, torch.rand(500, device="cuda")
+        bias, ok = torch.randn(500, device="cuda"), words_of(rng.random((1, 500)) < 0.8)
+        a = decode.adjust_scores(s.expand(N, 500), tokens=t.expand(N, 9), repetition=rep, bias=bias, allowed=ok[0])
+        b = decode.adjust_scores(s.expand(N, 500).contiguous(), tokens=t.expand(N, 9).contiguous(), repetition=rep,
+                                 bias=bias.expand(N, 500).contiguous(), allowed=ok.expand(N, -1).contiguous())
+        assert torch.equal(a, b)
+        assert same(decode.choose(s.expand(N, 500), noise=noise, temperature=rep),
+                    decode.choose(s.expand(N, 500).contiguous(), noise=noise.expand(N, 500).contiguous(), temperature=rep))
+
+
 def test_refusals():
     f = lambda *shape, **kw: torch.zeros(*shape, device="cuda", **kw)  # noqa: E731
     i32, u8 = torch.int32, torch.uint8

@@ -1310,7 +1310,8 @@ int ytm_adjust_scores(const void* scores, int dtype, int64_t stride, int64_t N, 
     return fail(YTM_EINVAL, "adjust_scores takes at most 65535 rows of 8388608 scores");
   if (N == 0 || V == 0) return YTM_OK;
   if (!scores || !out || (T > 0 && !tokens)) return fail(YTM_EINVAL, "bad adjust_scores arguments");
-  if ((N > 1 && (stride < V || out_stride < V)) || (tokens && N > 1 && token_stride < T) ||
+  if ((N > 1 && ((stride != 0 && stride < V) || out_stride < V)) ||
+      (tokens && N > 1 && token_stride != 0 && token_stride < T) ||
       (bias && bias_stride != 0 && N > 1 && bias_stride < V) ||
       (allowed && allowed_stride != 0 && N > 1 && allowed_stride < (V + 31) / 32))
     return fail(YTM_EINVAL, "adjust_scores: rows overlap");
@@ -1342,7 +1343,7 @@ int ytm_choose(const void* scores, int dtype, int64_t stride, int64_t N, int64_t
     return fail(YTM_EINVAL, "choose takes at most 8388608 scores a row");
   if (N == 0) return YTM_OK;
   if ((V > 0 && !scores) || !tokens || !logprobs) return fail(YTM_EINVAL, "bad choose arguments");
-  if (N > 1 && (stride < V || (noise && noise_stride != 0 && noise_stride < V)))
+  if (N > 1 && ((stride != 0 && stride < V) || (noise && noise_stride != 0 && noise_stride < V)))
     return fail(YTM_EINVAL, "choose: rows overlap");
   int64_t need = 0;
   if (int rc = ytm_choose_workspace(dtype, N, V, &need)) return rc;
