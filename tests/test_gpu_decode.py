@@ -578,6 +578,26 @@ def test_captured_into_a_graph(N, C, K):
         assert same(want, out), seed
 
 
+@pytest.mark.parametrize("N", [1, 9, 20, 64, 100])
+@pytest.mark.parametrize("dtype", ["bits", "f16", "f32"])
+@pytest.mark.parametrize("C,group", [(40, 32), (200, 32), (200, 128), (1000, 256), (1090, 64)])
+def test_infinite_scale(dtype, N, C, group):
+    """An infinite scale makes its group's sum infinite, whatever pads the last group."""
+    K, groups = 20, -(-C // group)
+    codes = torch.full((K, 16 * -(-C // 32)), 0x22, dtype=torch.uint8, device="cuda")  # ones
+    scales = torch.ones(K, groups, device="cuda")
+    scales[3, groups - 1] = float("inf")
+    scales[4, 0] = -float("inf")
+    if dtype == "bits":
+        x = torch.full((N, -(-C // 32)), -1, dtype=torch.int32, device="cuda")
+        got = decode.readout(x, codes, scales, group=group, clauses=C)
+    else:
+        got = decode.readout(torch.ones(N, C, dtype=TYPES[dtype], device="cuda"), codes, scales, group=group)
+    want = torch.full((N, K), float(C), device="cuda")
+    want[:, 3], want[:, 4] = float("inf"), -float("inf")
+    assert torch.equal(got, want)
+
+
 def test_one_row_for_all():
     """Rows that are one (stride 0) read as if they were copies."""
     rng = np.random.default_rng(2)

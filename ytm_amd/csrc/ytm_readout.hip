@@ -235,8 +235,8 @@ struct Codes {
     const uint32_t q = __umulhi(step < steps ? step + 1 : steps, a.inverse);
     scale = *(const decltype(scale)*)(scales + (at + q * (uint32_t)sizeof scale));
   }
-  // scales of the four products
-  __device__ __forceinline__ void scaled(const ReadoutArgs& a, float (&f)[4]) const {
+  // scales of the four products, zero past the last clause: infinity by the zeros there would be NaN
+  __device__ __forceinline__ void scaled(const ReadoutArgs& a, int chunk, float (&f)[4]) const {
     uint32_t u;
     if constexpr (WIDE)
       u = __float_as_uint(scale);
@@ -244,7 +244,10 @@ struct Codes {
       u = __float_as_uint(scale_value(a, scale, scale));
     const v4u t = turn<GRAIN>(v4u{u, u, u, u});
 #pragma unroll
-    for (int s = 0; s < 4; ++s) f[s] = __uint_as_float(t[s]);
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t there = GRAIN == kChunk ? ~0u : (uint32_t)((chunk * 4 + s - (a.C + kStep - 1) / kStep) >> 31);
+      f[s] = __uint_as_float(t[s] & there);
+    }
   }
 };
 
@@ -318,34 +321,69 @@ __global__ __launch_bounds__(kPieces* kTile) void rows_kernel(ReadoutArgs a) {
         plane[p];
 }
 
-// A block takes 16 NT RW rows and 16 OB WO outputs; its waves are WK groups, each with chunks of
+// ---------------------------------------------------------------------- copies into LDS, and waits
+// A wave's copy from memory into LDS that passes no register: lane l's 16 bytes (4 or 2, which take
+// a word each) from `off` bytes after the uniform address `from`, to `at` (uniform) and on, lane after
+// lane.  The compiler knows nothing of them: await() waits for all but the wave's youngest LEFT copies
+// and for its reads of LDS, and then for the block's other waves.  What it loads itself meanwhile only
+// makes that wait longer.
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_to_lds(const void* from, uint32_t off, uint32_t at) {
+  if (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(from), "s"(at) : "memory", "m0");
+  else if (BYTES == 4)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(from), "s"(at) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1" ::"v"(off), "s"(from), "s"(at) : "memory", "m0");
+}
+template <int LEFT>
+__device__ __forceinline__ void await() {
+  static_assert(LEFT < 64, "what the counter of loads holds");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+// A block takes 16 NT RW rows and 16 OB WO outputs; its waves are WK groups, each with pairs of chunks of
 // clauses of its own, of WO x RW waves, each with NT tiles of rows and OB of outputs.  Lane l takes
 // the codes of output l % 16 as a product's second operand and gets sums of rows 4 (l / 16) .. + 3
 // of that output.
 //
-// A group keeps a chunk of its rows' operands in LDS, and two chunks of its outputs' codes and
-// scales: 128 bytes of codes in a row, which a wave that loaded its own 16 outputs' chunk would take
-// in halves, and twice where two waves have the same outputs.  (With each wave loading its own,
-// 512 rows x 20000 clauses x 10000 outputs took 340 us, of which 150 went without these loads.)
-// What comes next is on its way meanwhile: rows are asked for a chunk ahead, codes two.  The groups' sums are joined in LDS in their order.
+// A group's chunks pass through LDS: the rows' operands in a ring of three chunks (two where three do
+// not fit), the outputs' codes and scales in one of two pairs, of which each output's codes are 128
+// bytes in a row.  A wave has a chunk's operands in registers before the chunk begins, so that there
+// is one wait a chunk, at its start: for the next chunk to be in LDS, and for all waves to have read this
+// one, whose place then takes the chunk after the ring's last.  Copies are thus under way for
+// two chunks, which eight waves a CU, in step, have nothing else to hide.  A group's sums are scaled
+// beside the products of the next.
+//
+// 512 rows x 20000 clauses x 10000 outputs of bfloat16 (groups of 128): 200 us, 1.0 PFLOP/s; with loads
+// through registers a chunk ahead and LDS read where it was needed, 256.  Of the 200 about 40 go without
+// the copies; the rest is the matrix unit at the clock that it leaves, and vector work that shares
+// its issue: per product of 16 cycles two conversions, and one multiply-add and one other instruction.
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) {
   constexpr int kPlanes = Kind<X>::kPlanes;
-  constexpr int kGroupWaves = RW * WO, kGroupThreads = kWave * kGroupWaves;
+  constexpr bool kHalf = Kind<X>::kHalf;
+  constexpr int kGroupWaves = RW * WO;
   constexpr int kTiles = NT * RW;               // of rows
-  constexpr int kFrags = kPlanes * 4 * kTiles;  // operands of a chunk
-  constexpr int kEach = kFrags / kGroupWaves;   // that a wave loads
-  static_assert(kFrags % kGroupWaves == 0, "");
+  constexpr int kFrags = kPlanes * 4 * kTiles;  // operands of a chunk, 1 KB each
   constexpr int kOuts = kTile * OB * WO;
-  constexpr int kGrains = kChunk / GRAIN;                      // scales of a chunk
-  // 16-byte pieces of codes and scales a thread loads, the last of them twice where they do not come out even
-  constexpr int kCodes = (2 * 4 * kOuts + kGroupThreads - 1) / kGroupThreads;
-  constexpr int kScales = (2 * kGrains * kOuts + kGroupThreads - 1) / kGroupThreads;
+  constexpr int kGrains = kChunk / GRAIN;  // scales of a chunk
+  // copies a wave makes, the last of them twice where they do not come out even
+  constexpr int kRowCopies = kFrags / kGroupWaves;
+  constexpr int kCodeCopies = (kOuts / 8 + kGroupWaves - 1) / kGroupWaves;
+  constexpr int kScaleAll = 2 * kGrains * kOuts / kWave;
+  constexpr int kScaleCopies = (kScaleAll + kGroupWaves - 1) / kGroupWaves;
+  static_assert(kFrags % kGroupWaves == 0 && 2 * kGrains * kOuts % kWave == 0, "");
+  constexpr int kPairSpace = 2 * WK * (kOuts * 8 * 16 + 2 * kGrains * kOuts * 4);
+  constexpr int kSlots = 3 * WK * kFrags * 1024 + kPairSpace <= 160 * 1024 ? 3 : 2;
   constexpr int kJoin = (WK - 1) * kGroupWaves * NT * OB;
-  constexpr int kRowSpace = 2 * WK * kFrags;
-  __shared__ v4u lds[(kRowSpace > kJoin ? kRowSpace : kJoin) * kWave];
-  __shared__ v4u held_codes[2][WK][2][kOuts * 4];
-  __shared__ float held_scales[2][WK][2][kGrains][kOuts];
+  static_assert(kJoin <= kSlots * WK * kFrags, "");
+  __shared__ v4u held_rows[kSlots][WK][kFrags * kWave];
+  __shared__ v4u held_codes[2][WK][kOuts * 8];
+  __shared__ __attribute__((aligned(16))) uint32_t held_scales[2][WK][kOuts * 2 * kGrains];
 
   // blocks of the same outputs one after the other on the same XCD, whose L2 then has the codes
   const int row_blocks = (a.row_tiles + kTiles - 1) / kTiles;
@@ -354,120 +392,168 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   if (out_tile >= a.out_tiles) return;
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int group = wave / kGroupWaves, mine = wave % kGroupWaves, wo = mine / RW, rw = mine % RW;
-  const int t = threadIdx.x % kGroupThreads;
   const int block_out = out_tile * kOuts;
 
   // uniform addresses and 32-bit distances from them take fewer registers than addresses
-  const uint32_t size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  const bool wide = a.scale_dtype == YTM_DTYPE_F32;
+  const uint32_t size = wide ? 4 : 2;
   const uint8_t* codes = a.codes + block_out * a.code_stride;
   const char* scales = (const char*)a.scales + block_out * a.scale_stride * size;
   // outputs past the last take its codes and are not stored
   const auto output = [&](int o) { return (uint32_t)((block_out + o < a.K ? block_out + o : a.K - 1) - block_out); };
-  uint32_t code_off[kCodes], scale_off[kScales];
+  const auto code_copy = [&](int e) {  // which 8 outputs' codes
+    const int f = e * kGroupWaves + mine;
+    return f < kOuts / 8 ? f : kOuts / 8 - 1;
+  };
+  const auto scale_copy = [&](int e) {
+    const int f = e * kGroupWaves + mine;
+    return f < kScaleAll ? f : kScaleAll - 1;
+  };
+  // Piece p of output o's eight in a pair lies at place p ^ o % 8 of its 128 bytes, so that 16 outputs'
+  // same piece is in different banks.
+  uint32_t code_off[kCodeCopies], scale_off[kScaleCopies];
 #pragma unroll
-  for (int e = 0; e < kCodes; ++e) {
-    const int j = (e * kGroupThreads + t) / 8;
-    code_off[e] = output(j < kOuts ? j : 0) * (uint32_t)a.code_stride;
-  }
+  for (int e = 0; e < kCodeCopies; ++e) code_off[e] = output(code_copy(e) * 8 + l / 8) * (uint32_t)a.code_stride;
 #pragma unroll
-  for (int e = 0; e < kScales; ++e) {
-    const int j = (e * kGroupThreads + t) / (2 * kGrains);
-    scale_off[e] = output(j < kOuts ? j : 0) * (uint32_t)a.scale_stride * size;
-  }
-  // Chunks past the last are loaded too: whether to load would be a branch, after which every load
-  // has to be waited for.  Their rows are zero up to the last pair's end, and what is loaded past it is
-  // not used.
+  for (int e = 0; e < kScaleCopies; ++e)
+    scale_off[e] = output((scale_copy(e) * kWave + l) / (2 * kGrains)) * (uint32_t)a.scale_stride * size;
   const int all_pairs = (a.chunks + 2 * WK - 1) / (2 * WK);
   const int first_pair = blockIdx.y * a.part_chunks;  // of this part; part_chunks counts pairs here
   const int pairs = all_pairs - first_pair < a.part_chunks ? all_pairs - first_pair : a.part_chunks;
   const uint32_t steps = (a.C + kStep - 1) / kStep;
-  v4u code[kCodes];
-  uint16_t low[kScales], high[kScales];
-  const auto load_codes = [&](int pair) {
-    const uint32_t first = (uint32_t)((first_pair + pair) * WK + group) * 2 * 4;  // step
-#pragma unroll
-    for (int e = 0; e < kCodes; ++e) {
-      const uint32_t step = first + (e * kGroupThreads + t) % 8;
-      code[e] = *(const v4u*)(codes + (code_off[e] + 16 * (step < steps ? step : steps - 1)));
-    }
-#pragma unroll
-    for (int e = 0; e < kScales; ++e) {
-      const uint32_t step = first + (e * kGroupThreads + t) % (2 * kGrains) * (4 / kGrains);
-      const uint32_t at = scale_off[e] + __umulhi(step < steps ? step + 1 : steps, a.inverse) * size;
-      low[e] = *(const uint16_t*)(scales + at);
-      high[e] = *(const uint16_t*)(scales + (at + size - 2));
-    }
-  };
-  const auto keep_codes = [&](int pair) {
-#pragma unroll
-    for (int e = 0; e < kCodes; ++e) {
-      const int j = e * kGroupThreads + t;
-      if (j < 8 * kOuts) held_codes[pair % 2][group][j % 8 / 4][j / 8 * 4 + j % 4] = code[e];
-    }
-#pragma unroll
-    for (int e = 0; e < kScales; ++e) {
-      const int j = e * kGroupThreads + t, o = j / (2 * kGrains), i = j % (2 * kGrains);
-      if (o < kOuts) held_scales[pair % 2][group][i / kGrains][i % kGrains][o] = scale_value(a, low[e], high[e]);
-    }
-  };
   const int padded = all_pairs * 2 * WK;
-  struct Rows {
-    v4u x[kEach];
-  };
-  const auto load_rows = [&](int i, Rows& to) {  // of chunk i of this group's
-    const int own = ((first_pair + i / 2) * WK + group) * 2 + i % 2, chunk = own < padded ? own : padded - 1;
+  // What is copied past the part's end is not used: copies are made all the same, so that their
+  // number is known where they are waited for.  Rows are zero from the last clause to the last pair's end.
+  const auto chunk_of = [&](int i) { return ((first_pair + i / 2) * WK + group) * 2 + i % 2; };
+  const auto copy_rows = [&](int i, int to) {  // of the group's chunk i
+    const int own = chunk_of(i), chunk = own < padded ? own : padded - 1;
+    const uint32_t at = lds_address(held_rows) + (to * WK + group) * kFrags * 1024;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {  // row tiles past the last take its rows and are not stored
+    for (int e = 0; e < kRowCopies; ++e) {  // row tiles past the last take its rows and are not stored
       const int f = e * kGroupWaves + mine, tile = row_block * kTiles + f % kTiles;
       const v4u* from = a.frag + (((int64_t)chunk * kPlanes * 4 + f / kTiles) * a.row_tiles +
                                   (tile < a.row_tiles ? tile : a.row_tiles - 1)) * kWave;
-      to.x[e] = from[l];
+      copy_to_lds<16>(from, l * 16, at + f * 1024);
     }
   };
-  const auto keep_rows = [&](const Rows& of, int i) {
-    v4u* to = lds + (i % 2 * WK + group) * kFrags * kWave;
+  const auto copy_codes = [&](int pair) {
+    const uint32_t first = chunk_of(2 * pair) * 4;  // step
+    const int place = pair % 2 * WK + group;
+    const uint32_t step = first + (l % 8 ^ l / 8);
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) to[(e * kGroupWaves + mine) * kWave + l] = of.x[e];
+    for (int e = 0; e < kCodeCopies; ++e)
+      copy_to_lds<16>(codes, code_off[e] + 16 * (step < steps ? step : steps - 1),
+                      lds_address(held_codes) + place * kOuts * 128 + code_copy(e) * 1024);
+    const uint32_t at = lds_address(held_scales) + place * kOuts * 2 * kGrains * 4;
+#pragma unroll
+    for (int e = 0; e < kScaleCopies; ++e) {
+      const uint32_t of = first + l % (2 * kGrains) * (4 / kGrains);
+      const uint32_t off = scale_off[e] + __umulhi(of < steps ? of + 1 : steps, a.inverse) * size;
+      if (wide)
+        copy_to_lds<4>(scales, off, at + scale_copy(e) * 256);
+      else
+        copy_to_lds<2>(scales, off, at + scale_copy(e) * 256);
+    }
   };
 
   v4f total[NT][OB];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int b = 0; b < OB; ++b)
 #pragma unroll
-    for (int b = 0; b < OB; ++b) total[n][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  const auto add = [&](int pair, int half) {
-    const int o = wo * OB * kTile;
-    const v4u* w_from = held_codes[pair % 2][group][half] + (o + l % 16) * 4 + l / 16;
-    const float* s_from = held_scales[pair % 2][group][half][0] + o + l % 16;
-    add_chunk<X, GRAIN, NT, OB>(lds + ((half * WK + group) * kFrags + rw * NT) * kWave + l, 4 * kTiles * kWave,
-                                kTiles * kWave, kWave, total, [&](int b, v4u& w, float(&scale)[4]) {
-                                  w = w_from[b * kTile * 4];
-#pragma unroll
-                                  for (int s = 0; s < 4; ++s) scale[s] = s_from[s * kGrains / 4 * kOuts + b * kTile];
-                                });
+    for (int n = 0; n < NT; ++n) total[n][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  struct Operands {  // a wave's of a chunk
+    v4u x[4][kPlanes][NT], w[OB];
+    uint32_t scale[OB][kGrains];
   };
-  Rows next;
-  load_codes(0);
-  load_rows(0, next);
-  keep_codes(0);
-  keep_rows(next, 0);
-  for (int i = 0; i < pairs; ++i) {
-    __syncthreads();
-    load_codes(i + 1);
-    load_rows(2 * i + 1, next);
-    __builtin_amdgcn_sched_barrier(0);  // or the loads sink to where they are needed
-    add(i, 0);
-    keep_rows(next, 1);
-    __syncthreads();
-    load_rows(2 * i + 2, next);
-    __builtin_amdgcn_sched_barrier(0);
-    add(i, 1);
-    keep_rows(next, 0);
-    keep_codes(i + 1);
+  const auto read = [&](int i, int from, Operands& to) {
+#pragma unroll
+    for (int b = 0; b < OB; ++b) {
+      const int place = i / 2 % 2, half = i % 2, o = (wo * OB + b) * kTile + l % 16;
+      to.w[b] = held_codes[place][group][o * 8 + ((half * 4 + l / 16) ^ l % 8)];
+#pragma unroll
+      for (int g = 0; g < kGrains; ++g) to.scale[b][g] = held_scales[place][group][(o * 2 + half) * kGrains + g];
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          to.x[s][p][n] = held_rows[from][group][((p * 4 + s) * kTiles + rw * NT + n) * kWave + l];
+  };
+  const int shift = wide ? 0 : 16;
+  const uint32_t halves = a.scale_dtype == YTM_DTYPE_F16 ? ~0u : 0u;
+  v4f last[NT];  // the sums before these, and their scale
+  float due = 0.0f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) last[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto scaled = [&](int b) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) total[n][b][r] = __builtin_fmaf(due, last[n][r], total[n][b][r]);
+  };
+
+  Operands now[2];
+  copy_codes(0);
+  copy_rows(0, 0);
+#pragma unroll
+  for (int i = 1; i < kSlots; ++i) copy_rows(i, i);
+  copy_codes(1);
+  await<(kSlots - 1) * kRowCopies + kCodeCopies + kScaleCopies>();
+  read(0, 0, now[0]);
+  int at = 0;  // the chunk's place in the ring
+  for (int pair = 0; pair < pairs; ++pair) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int i = 2 * pair + half, next = at + 1 < kSlots ? at + 1 : 0;
+      // Of what is younger than the next chunk's: a chunk's rows in a ring of three, and where
+      // this chunk is the first of its pair, the codes that its predecessor asked for.
+      if (half == 0)
+        await<(kSlots - 2) * kRowCopies + kCodeCopies + kScaleCopies>();
+      else
+        await<(kSlots - 2) * kRowCopies>();
+      copy_rows(i + kSlots, at);
+      if (half == 1) copy_codes(pair + 2);
+      read(i + 1, next, now[1 - half]);
+      const Operands& o = now[half];
+      const uint32_t first = chunk_of(i) * 4;
+#pragma unroll
+      for (int b = 0; b < OB; ++b) {
+        const v4u w = turn<GRAIN>(o.w[b]);
+#pragma unroll
+        for (int g = 0; g < kGrains; ++g) {
+          v4f sum[NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) sum[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int s = 4 / kGrains * g; s < 4 / kGrains * (g + 1); ++s) {
+            const v4u y = codes_to_16<kHalf>(w[s]);
+#pragma unroll
+            for (int p = kPlanes - 1; p >= 0; --p)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) sum[n] = product<kHalf>(o.x[s][p][n], y, sum[n]);
+          }
+          scaled(g > 0 ? b : b > 0 ? b - 1 : OB - 1);
+          // Zero past the last clause, as in few rows.  By masks, since uniform choices become branches,
+          // which keep products and scaling apart.
+          const uint32_t u = o.scale[b][g];
+          const uint32_t half_bits = __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)u));
+          const uint32_t there = (uint32_t)((int32_t)(first + g * (4 / kGrains) - steps) >> 31);
+          due = __uint_as_float(((half_bits & halves) | (u << shift & ~halves)) & there);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) last[n] = sum[n];
+          // or the compiler puts the products of all groups first, whose sums take more registers than there are
+          if (kGrains > 1) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      at = next;
+    }
   }
-  v4f* join = (v4f*)lds;
+  scaled(OB - 1);
+  await<0>();  // no copy comes after the block's end, or into the sums to be joined
+  v4f* join = (v4f*)held_rows;
   if (WK > 1) {
-    __syncthreads();
     if (group > 0) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -514,16 +600,17 @@ hipError_t launch_parts(const ReadoutArgs& a, int parts, hipStream_t s) {
 
 // What a block of tile_kernel takes, by the number of rows: 32, 64, or 96 and 128, whichever leaves
 // fewer rows that are not there; float32, whose operands take three times the LDS, up to 64.  With
-// four scales a chunk (grain 32) 160 outputs do not fit the registers.
+// four scales a chunk (grain 32) a wave's groups of sums and their operands have to be fewer: what does not fit the registers costs three times
+// its time (512 rows x 10000 clauses x 10000 outputs: 704 us in blocks of 128 rows, 210 of 96).
 struct Tile {
   int rows, outs, groups;
 };
-constexpr Tile kTile32{32, 128, 2}, kTile64{64, 128, 2}, kTile96{96, 128, 1};
-constexpr Tile kWide32{32, 128, 1}, kWide64{64, 128, 1};
 Tile tile_of(int planes, int grain, int N) {
-  if (planes > 1) return N <= 32 ? kWide32 : kWide64;
-  if (N <= 64) return N <= 32 ? kTile32 : kTile64;
-  return (N + 95) / 96 * 96 < (N + 127) / 128 * 128 ? kTile96 : Tile{128, grain == kChunk ? 160 : 128, 1};
+  const bool whole = grain == kChunk;
+  if (planes > 1) return N <= 32 ? Tile{32, 128, 1} : Tile{64, whole ? 128 : 96, 1};
+  if (N <= 32) return Tile{32, 128, 2};
+  if (N <= 64) return Tile{64, 128, whole ? 2 : 1};
+  return !whole || (N + 95) / 96 * 96 < (N + 127) / 128 * 128 ? Tile{96, 128, 1} : Tile{128, 160, 1};
 }
 // Pairs of chunks in a part of the clauses: all, or where that leaves half of the 256 CUs without
 // a block, as many as give each CU one (103 rows x 10012 clauses x 22 outputs, one block: 909 us;
@@ -567,16 +654,16 @@ template <int X, int GRAIN>
 hipError_t launch_tiles(const ReadoutArgs& a, hipStream_t s) {
   const int rows = tile_of(Kind<X>::kPlanes, GRAIN, a.N).rows;
   if constexpr (Kind<X>::kPlanes > 1) {
-    return rows == 32 ? launch_tile<X, GRAIN, 2, 1, 2, 4, 1>(a, s) : launch_tile<X, GRAIN, 2, 2, 2, 4, 1>(a, s);
+    if (rows == 32) return launch_tile<X, GRAIN, 2, 1, 2, 4, 1>(a, s);
+    if constexpr (GRAIN == kChunk) return launch_tile<X, GRAIN, 2, 2, 2, 4, 1>(a, s);
+    else return launch_tile<X, GRAIN, 1, 4, 3, 2, 1>(a, s);
   } else {
-    switch (rows) {
-      case 32: return launch_tile<X, GRAIN, 2, 1, 2, 4, 2>(a, s);
-      case 64: return launch_tile<X, GRAIN, 4, 1, 2, 4, 2>(a, s);
-      case 96: return launch_tile<X, GRAIN, 3, 2, 2, 4, 1>(a, s);
-      default:
-        if constexpr (GRAIN == kChunk) return launch_tile<X, GRAIN, 2, 4, 5, 2, 1>(a, s);
-        else return launch_tile<X, GRAIN, 4, 2, 2, 4, 1>(a, s);
-    }
+    if (rows == 32) return launch_tile<X, GRAIN, 2, 1, 2, 4, 2>(a, s);
+    if (rows == 96) return launch_tile<X, GRAIN, 3, 2, 2, 4, 1>(a, s);
+    if constexpr (GRAIN == kChunk)
+      return rows == 64 ? launch_tile<X, GRAIN, 4, 1, 2, 4, 2>(a, s) : launch_tile<X, GRAIN, 2, 4, 5, 2, 1>(a, s);
+    else
+      return launch_tile<X, GRAIN, 2, 2, 2, 4, 1>(a, s);
   }
 }
 
@@ -662,7 +749,7 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
       add_chunk<X, GRAIN, 1, OB>(from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total,
                                  [&](int b, v4u& w, float(&scale)[4]) {
                                    w = now[u][b].w;
-                                   now[u][b].scaled(a, scale);
+                                   now[u][b].scaled(a, chunk, scale);
                                  });
     }
   }
