@@ -5,8 +5,9 @@
 //
 // A code is an E2M1 float (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), exact in float16 and
 // bfloat16, into which gfx950 converts two codes an instruction; so the inner sums run on the
-// matrix cores in f32 with operands that are no less exact than x: bits, float16 and bfloat16 as
-// they are, float32 as the sum of three bfloat16 (8 + 8 + 8 bits of its fraction), a product each.
+// matrix cores in f32 with operands that are no less exact than x: float16 and bfloat16 as they
+// are, float32 as the sum of three bfloat16 (8 + 8 + 8 bits of its fraction), a product each.  Bits
+// are E2M1 floats themselves, 0 and 1, which the matrix cores multiply with the codes as they are.
 // The scale multiplies each group's f32 sum.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -22,7 +23,7 @@ namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-typedef short v8s __attribute__((ext_vector_type(8)));
+typedef int v8i __attribute__((ext_vector_type(8)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -33,6 +34,7 @@ constexpr int kTile = 16;    // rows and outputs of a product
 constexpr int kStep = 32;    // clauses of a product
 constexpr int kChunk = 128;  // clauses of a 16-byte load of codes by each lane, four products
 constexpr int kPieces = 16;  // of 8 clauses, in a chunk: a lane's part of a product's row operand
+constexpr int kWords = 4;    // of 32 bits, in a chunk: the same of a product with bits, which takes a whole chunk
 
 struct ReadoutArgs {
   const void* x;
@@ -63,6 +65,8 @@ struct Kind<YTM_DTYPE_BITS> {
   static constexpr int kPlanes = 1;
   static constexpr bool kHalf = false;
 };
+template <int X>
+constexpr bool kBits = X == YTM_DTYPE_BITS;
 template <>
 struct Kind<YTM_DTYPE_F16> {
   static constexpr int kPlanes = 1;
@@ -79,8 +83,15 @@ struct Kind<YTM_DTYPE_F32> {
   static constexpr bool kHalf = false;
 };
 
+// Operands that 16 rows' clauses of a chunk make, 1 KB each.
+constexpr int operands_of(int x_dtype) {
+  return x_dtype == YTM_DTYPE_BITS ? 1 : x_dtype == YTM_DTYPE_F32 ? 12 : 4;
+}
+template <int X>
+constexpr int kOperands = operands_of(X);
+
 // ------------------------------------------------------------------------------- row operands
-// Eight clauses of a row as they are in memory, and as 16-bit operands: bits as 0 and 1, float32
+// Eight clauses of a row as they are in memory, and as 16-bit operands: float32
 // as the sum of three bfloat16, each cut (not rounded) to one, so that nothing overflows; where
 // the first is infinite or NaN the others are zero.
 //
@@ -89,16 +100,11 @@ struct Kind<YTM_DTYPE_F32> {
 // to its place, with zeros after it, when it becomes operands.
 template <int X>
 struct Piece {
-  static constexpr int kWords = X == YTM_DTYPE_F32 ? 8 : X == YTM_DTYPE_BITS ? 1 : 4;
+  static constexpr int kWords = X == YTM_DTYPE_F32 ? 8 : 4;
   uint32_t raw[kWords];
 
   // of the row `off` bytes from x's uniform address `x`, clauses c .. c + 7
   __device__ __forceinline__ void load(const ReadoutArgs& a, const char* x, uint32_t off, int c) {
-    if (X == YTM_DTYPE_BITS) {
-      const int at = c < a.C ? c : a.C - 1;
-      raw[0] = *(const uint32_t*)(x + (off + at / 32 * 4));
-      return;
-    }
     const int at = c < a.C - 8 ? c : a.C - 8;
     __builtin_memcpy(raw, x + (off + at * (X == YTM_DTYPE_F32 ? 4 : 2)), sizeof raw);
   }
@@ -106,16 +112,6 @@ struct Piece {
   // the operands of clauses c .. c + 7, which load() was asked for
   __device__ __forceinline__ void operands(const ReadoutArgs& a, int c, v4u (&plane)[Kind<X>::kPlanes]) const {
     const int over = c + 8 - a.C;  // of the eight, past the last clause
-    if (X == YTM_DTYPE_BITS) {
-      uint32_t bits = raw[0] >> (c % 32);
-      if (over > 0) bits = over < 8 ? bits & (255u >> over) : 0u;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t two = bits >> (2 * q);
-        plane[0][q] = ((two & 1u) | (two & 2u) << 15) * 0x3F80u;  // 1.0 at either half
-      }
-      return;
-    }
     uint32_t r[kWords];
 #pragma unroll
     for (int q = 0; q < kWords; ++q) r[q] = raw[q];
@@ -165,6 +161,26 @@ struct Piece {
   }
 };
 
+// Word i of a row's bits, and as E2M1 floats: a bit's 1 is 0010.
+__device__ __forceinline__ uint32_t load_bits(const ReadoutArgs& a, const char* x, uint32_t off, int i) {
+  const int last = (a.C - 1) / 32;
+  return *(const uint32_t*)(x + (off + 4 * (i < last ? i : last)));
+}
+__device__ __forceinline__ v4u bit_operand(const ReadoutArgs& a, uint32_t bits, int i) {
+  const int left = a.C - 32 * i;
+  bits = left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1u) : 0u;
+  v4u r;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {  // eight bits four places apart
+    uint32_t u = bits >> 8 * q & 0xFFu;
+    u = (u | u << 12) & 0x000F000Fu;
+    u = (u | u << 6) & 0x03030303u;
+    u = (u | u << 3) & 0x11111111u;
+    r[q] = u << 1;
+  }
+  return r;
+}
+
 // ------------------------------------------------------------------------------------ products
 template <bool HALF>
 __device__ __forceinline__ v4u codes_to_16(uint32_t w) {
@@ -190,11 +206,24 @@ __device__ __forceinline__ v4f product(v4u x, v4u w, v4f d) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x), __builtin_bit_cast(v8bf, w), d, 0, 0, 0);
 }
 
+// A whole chunk's product of bits and codes, each lane's 32 clauses of a row and of an output.
+__device__ __forceinline__ v4f bit_product(v4u x, v4u w) {
+  const v8i p = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+  const v8i q = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p, q, v4f{0.0f, 0.0f, 0.0f, 0.0f}, 4, 4, 0, 0, 0, 0);
+}
+
 // A lane of group g = l / 16 holds a chunk's clauses 32 g .. 32 g + 31 in four words of codes, and
 // a product takes one word of each lane.  Where a scale holds for the whole chunk (GRAIN 128),
 // product s takes word s as it is: clauses 32 g + 8 s .., the row operands' alike.  Where it does
 // not (GRAIN 32), the words are exchanged first so that product s has clauses 32 s + 8 g ..:
-// a 4 x 4 transposition in two exchanges of bits of (group, word).
+// a 4 x 4 transposition in two exchanges of bits of (group, word).  A product with bits takes all
+// four words, and where a scale does not hold for the chunk, one for each group of lanes, with zeros for
+// the other groups' bits: as many cycles as the four of 16-bit operands, without their conversion.
+__device__ __forceinline__ v4u only(v4u w, int group) {
+  const bool mine = threadIdx.x % kWave / 16 == group;
+  return v4u{mine ? w[0] : 0u, mine ? w[1] : 0u, mine ? w[2] : 0u, mine ? w[3] : 0u};
+}
 template <int GRAIN>
 __device__ __forceinline__ v4u turn(v4u w) {
   if (GRAIN == kChunk) return w;
@@ -307,6 +336,14 @@ __device__ __forceinline__ void add_chunk(const v4u* from, int plane, int step, 
 // (the grid's first axis) of a row tile, a thread a piece; 16 of them read 256 or 512 bytes in a row.
 template <int X, int GRAIN>
 __global__ __launch_bounds__(kPieces* kTile) void rows_kernel(ReadoutArgs a) {
+  if constexpr (kBits<X>) {  // frag[chunk][row tile][lane]: a block makes four chunks of a row tile
+    const int row = threadIdx.x / kPieces, i = threadIdx.x % kPieces, chunk = blockIdx.x * 4 + i / kWords;
+    const int tile = blockIdx.y, n = tile * kTile + row < a.N ? tile * kTile + row : a.N - 1;
+    const uint32_t bits = load_bits(a, (const char*)a.x + n * a.x_stride * 4, 0, blockIdx.x * kPieces + i);
+    a.frag[((int64_t)chunk * a.row_tiles + tile) * kWave + i % kWords * 16 + row] =
+        bit_operand(a, bits, blockIdx.x * kPieces + i);
+    return;
+  }
   constexpr int kPlanes = Kind<X>::kPlanes;
   const int chunk = blockIdx.x, tile = blockIdx.y, row = threadIdx.x / kPieces, i = threadIdx.x % kPieces;
   const int place = place_of<GRAIN>(i), c = chunk * kChunk + i * 8;
@@ -333,11 +370,14 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 template <int BYTES>
 __device__ __forceinline__ void copy_to_lds(const void* from, uint32_t off, uint32_t at) {
   if (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(from), "s"(at) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(from), "s"(at)
+                 : "memory", "m0");
   else if (BYTES == 4)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(from), "s"(at) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(from), "s"(at)
+                 : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1" ::"v"(off), "s"(from), "s"(at) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1" ::"v"(off), "s"(from), "s"(at)
+                 : "memory", "m0");
 }
 template <int LEFT>
 __device__ __forceinline__ void await() {
@@ -362,27 +402,30 @@ __device__ __forceinline__ void await() {
 // through registers a chunk ahead and LDS read where it was needed, 256.  Of the 200 about 40 go without
 // the copies; the rest is the matrix unit at the clock that it leaves, and vector work that shares
 // its issue: per product of 16 cycles two conversions, and one multiply-add and one other instruction.
+// Bits, with a quarter of the products and no conversion: 10000 x 10000, 512 rows 62 us (109 through 16 bits).
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) {
   constexpr int kPlanes = Kind<X>::kPlanes;
   constexpr bool kHalf = Kind<X>::kHalf;
   constexpr int kGroupWaves = RW * WO;
   constexpr int kTiles = NT * RW;               // of rows
-  constexpr int kFrags = kPlanes * 4 * kTiles;  // operands of a chunk, 1 KB each
+  constexpr int kFrags = kOperands<X> * kTiles;  // operands of a chunk, 1 KB each
   constexpr int kOuts = kTile * OB * WO;
   constexpr int kGrains = kChunk / GRAIN;  // scales of a chunk
   // copies a wave makes, the last of them twice where they do not come out even
-  constexpr int kRowCopies = kFrags / kGroupWaves;
+  constexpr int kRowCopies = (kFrags + kGroupWaves - 1) / kGroupWaves;
   constexpr int kCodeCopies = (kOuts / 8 + kGroupWaves - 1) / kGroupWaves;
   constexpr int kScaleAll = 2 * kGrains * kOuts / kWave;
   constexpr int kScaleCopies = (kScaleAll + kGroupWaves - 1) / kGroupWaves;
-  static_assert(kFrags % kGroupWaves == 0 && 2 * kGrains * kOuts % kWave == 0, "");
+  static_assert(2 * kGrains * kOuts % kWave == 0, "");
   constexpr int kPairSpace = 2 * WK * (kOuts * 8 * 16 + 2 * kGrains * kOuts * 4);
   constexpr int kSlots = 3 * WK * kFrags * 1024 + kPairSpace <= 160 * 1024 ? 3 : 2;
   constexpr int kJoin = (WK - 1) * kGroupWaves * NT * OB;
-  static_assert(kJoin <= kSlots * WK * kFrags, "");
-  __shared__ v4u held_rows[kSlots][WK][kFrags * kWave];
-  __shared__ v4u held_codes[2][WK][kOuts * 8];
+  static_assert(kJoin <= kSlots * WK * kFrags + 2 * WK * kOuts * 8 / kWave, "");
+  constexpr int kRowSpace = kSlots * WK * kFrags * kWave;
+  __shared__ v4u held[kRowSpace + 2 * WK * kOuts * 8];  // rows, then codes
+  v4u(*held_rows)[WK][kFrags * kWave] = (v4u(*)[WK][kFrags * kWave])held;
+  v4u(*held_codes)[WK][kOuts * 8] = (v4u(*)[WK][kOuts * 8])(held + kRowSpace);
   __shared__ __attribute__((aligned(16))) uint32_t held_scales[2][WK][kOuts * 2 * kGrains];
 
   // blocks of the same outputs one after the other on the same XCD, whose L2 then has the codes
@@ -404,6 +447,10 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   const auto code_copy = [&](int e) {  // which 8 outputs' codes
     const int f = e * kGroupWaves + mine;
     return f < kOuts / 8 ? f : kOuts / 8 - 1;
+  };
+  const auto row_copy = [&](int e) {
+    const int f = e * kGroupWaves + mine;
+    return f < kFrags ? f : kFrags - 1;
   };
   const auto scale_copy = [&](int e) {
     const int f = e * kGroupWaves + mine;
@@ -430,8 +477,8 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
     const uint32_t at = lds_address(held_rows) + (to * WK + group) * kFrags * 1024;
 #pragma unroll
     for (int e = 0; e < kRowCopies; ++e) {  // row tiles past the last take its rows and are not stored
-      const int f = e * kGroupWaves + mine, tile = row_block * kTiles + f % kTiles;
-      const v4u* from = a.frag + (((int64_t)chunk * kPlanes * 4 + f / kTiles) * a.row_tiles +
+      const int f = row_copy(e), tile = row_block * kTiles + f % kTiles;
+      const v4u* from = a.frag + (((int64_t)chunk * kOperands<X> + f / kTiles) * a.row_tiles +
                                   (tile < a.row_tiles ? tile : a.row_tiles - 1)) * kWave;
       copy_to_lds<16>(from, l * 16, at + f * 1024);
     }
@@ -462,7 +509,7 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
 #pragma unroll
     for (int n = 0; n < NT; ++n) total[n][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   struct Operands {  // a wave's of a chunk
-    v4u x[4][kPlanes][NT], w[OB];
+    v4u x[kOperands<X>][NT], w[OB];
     uint32_t scale[OB][kGrains];
   };
   const auto read = [&](int i, int from, Operands& to) {
@@ -474,12 +521,9 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
       for (int g = 0; g < kGrains; ++g) to.scale[b][g] = held_scales[place][group][(o * 2 + half) * kGrains + g];
     }
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int q = 0; q < kOperands<X>; ++q)
 #pragma unroll
-      for (int p = 0; p < kPlanes; ++p)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          to.x[s][p][n] = held_rows[from][group][((p * 4 + s) * kTiles + rw * NT + n) * kWave + l];
+      for (int n = 0; n < NT; ++n) to.x[q][n] = held_rows[from][group][(q * kTiles + rw * NT + n) * kWave + l];
   };
   const int shift = wide ? 0 : 16;
   const uint32_t halves = a.scale_dtype == YTM_DTYPE_F16 ? ~0u : 0u;
@@ -520,19 +564,25 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
       const uint32_t first = chunk_of(i) * 4;
 #pragma unroll
       for (int b = 0; b < OB; ++b) {
-        const v4u w = turn<GRAIN>(o.w[b]);
+        const v4u w = kBits<X> ? o.w[b] : turn<GRAIN>(o.w[b]);
 #pragma unroll
         for (int g = 0; g < kGrains; ++g) {
           v4f sum[NT];
+          if constexpr (kBits<X>) {
+            const v4u y = kGrains == 1 ? w : only(w, g);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) sum[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int n = 0; n < NT; ++n) sum[n] = bit_product(o.x[0][n], y);
+          } else {
 #pragma unroll
-          for (int s = 4 / kGrains * g; s < 4 / kGrains * (g + 1); ++s) {
-            const v4u y = codes_to_16<kHalf>(w[s]);
+            for (int n = 0; n < NT; ++n) sum[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int p = kPlanes - 1; p >= 0; --p)
+            for (int s = 4 / kGrains * g; s < 4 / kGrains * (g + 1); ++s) {
+              const v4u y = codes_to_16<kHalf>(w[s]);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) sum[n] = product<kHalf>(o.x[s][p][n], y, sum[n]);
+              for (int p = kPlanes - 1; p >= 0; --p)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sum[n] = product<kHalf>(o.x[p * 4 + s][n], y, sum[n]);
+            }
           }
           scaled(g > 0 ? b : b > 0 ? b - 1 : OB - 1);
           // Zero past the last clause, as in few rows.  By masks, since uniform choices become branches,
@@ -552,7 +602,7 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   }
   scaled(OB - 1);
   await<0>();  // no copy comes after the block's end, or into the sums to be joined
-  v4f* join = (v4f*)held_rows;
+  v4f* join = (v4f*)held;
   if (WK > 1) {
     if (group > 0) {
 #pragma unroll
@@ -598,51 +648,61 @@ hipError_t launch_parts(const ReadoutArgs& a, int parts, hipStream_t s) {
   return hipGetLastError();
 }
 
-// What a block of tile_kernel takes, by the number of rows: 32, 64, or 96 and 128, whichever leaves
-// fewer rows that are not there; float32, whose operands take three times the LDS, up to 64.  With
-// four scales a chunk (grain 32) a wave's groups of sums and their operands have to be fewer: what does not fit the registers costs three times
-// its time (512 rows x 10000 clauses x 10000 outputs: 704 us in blocks of 128 rows, 210 of 96).
+// What a block of tile_kernel takes: 32 or 64 rows where there are no more; float32, whose operands
+// take three times the LDS, up to 64; else 64, 96 or 128 rows by the rounds in which the 256 CUs take the
+// blocks, at 4, 5 and 7 units of time each (fewer blocks than half the CUs are cut into parts, and
+// count as what they are).  10000 clauses x 10000 outputs in groups of 32, blocks of 64 and of 96 rows:
+// 192 rows 86 and 106 us (one round each), 320 rows 129 and 160 (two), 500 rows 243 and 207 (three, two).
+// With four scales a chunk (grain 32) 128 rows' sums and operands do not fit the registers and take
+// three times as long.
 struct Tile {
   int rows, outs, groups;
 };
-Tile tile_of(int planes, int grain, int N) {
+Tile tile_of(int operands, int grain, int N, int K) {
   const bool whole = grain == kChunk;
-  if (planes > 1) return N <= 32 ? Tile{32, 128, 1} : Tile{64, whole ? 128 : 96, 1};
+  if (operands > 4) return N <= 32 ? Tile{32, 128, 1} : Tile{64, whole ? 128 : 96, 1};
   if (N <= 32) return Tile{32, 128, 2};
-  if (N <= 64) return Tile{64, 128, whole ? 2 : 1};
-  return !whole || (N + 95) / 96 * 96 < (N + 127) / 128 * 128 ? Tile{96, 128, 1} : Tile{128, 160, 1};
+  const Tile tiles[3] = {{64, 128, whole ? 2 : 1}, {96, 128, 1}, {128, 160, 1}};
+  constexpr int kTime[3] = {4, 5, 7};
+  int best = 0;
+  int64_t least = 0;
+  for (int i = 0; i < (N <= 64 ? 1 : whole ? 3 : 2); ++i) {
+    const int64_t blocks = (int64_t)((N + tiles[i].rows - 1) / tiles[i].rows) * ((K + tiles[i].outs - 1) / tiles[i].outs);
+    const int64_t time = (blocks > 128 ? (blocks + 255) / 256 * 256 : blocks) * kTime[i];
+    if (i == 0 || time < least) least = time, best = i;
+  }
+  return tiles[best];
 }
 // Pairs of chunks in a part of the clauses: all, or where that leaves half of the 256 CUs without
 // a block, as many as give each CU one (103 rows x 10012 clauses x 22 outputs, one block: 909 us;
-// two pairs a part: 25).
-int part_pairs_of(int planes, int grain, int N, int chunks, int K) {
-  const Tile t = tile_of(planes, grain, N);
+// two pairs a part: 21).
+int part_pairs_of(int operands, int grain, int N, int chunks, int K) {
+  const Tile t = tile_of(operands, grain, N, K);
   const int64_t blocks = (int64_t)((N + t.rows - 1) / t.rows) * ((K + t.outs - 1) / t.outs);
   const int pairs = (chunks + 2 * t.groups - 1) / (2 * t.groups);
   if (blocks > 128 || pairs < 4) return pairs;
   const int parts = (int)(256 / blocks) < pairs / 2 ? (int)(256 / blocks) : pairs / 2;
   return (pairs + parts - 1) / parts;
 }
-int tile_parts_of(int planes, int grain, int N, int chunks, int K) {
-  const Tile t = tile_of(planes, grain, N);
-  const int each = part_pairs_of(planes, grain, N, chunks, K);
+int tile_parts_of(int operands, int grain, int N, int chunks, int K) {
+  const Tile t = tile_of(operands, grain, N, K);
+  const int each = part_pairs_of(operands, grain, N, chunks, K);
   return ((chunks + 2 * t.groups - 1) / (2 * t.groups) + each - 1) / each;
 }
 // Chunks of the rows' operands: whole pairs for each group of waves, of which a block has up to two.
 int padded_of(int chunks) { return (chunks + 3) / 4 * 4; }
-int64_t frag_bytes(int planes, int N, int chunks) {
-  return (int64_t)(N + kTile - 1) / kTile * padded_of(chunks) * planes * 4 * kWave * 16;
+int64_t frag_bytes(int operands, int N, int chunks) {
+  return (int64_t)(N + kTile - 1) / kTile * padded_of(chunks) * operands * kWave * 16;
 }
 
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 hipError_t launch_tile(ReadoutArgs a, hipStream_t s) {
-  constexpr int kPlanes = Kind<X>::kPlanes;
   a.row_tiles = (a.N + kTile - 1) / kTile;
   a.out_tiles = (a.K + kTile * OB * WO - 1) / (kTile * OB * WO);
-  a.part_chunks = part_pairs_of(kPlanes, GRAIN, a.N, a.chunks, a.K);
-  a.parts = (float*)((char*)a.frag + frag_bytes(kPlanes, a.N, a.chunks));
-  const int parts = tile_parts_of(kPlanes, GRAIN, a.N, a.chunks, a.K);
-  rows_kernel<X, GRAIN><<<dim3(padded_of(a.chunks), a.row_tiles), kPieces * kTile, 0, s>>>(a);
+  a.part_chunks = part_pairs_of(kOperands<X>, GRAIN, a.N, a.chunks, a.K);
+  a.parts = (float*)((char*)a.frag + frag_bytes(kOperands<X>, a.N, a.chunks));
+  const int parts = tile_parts_of(kOperands<X>, GRAIN, a.N, a.chunks, a.K);
+  rows_kernel<X, GRAIN><<<dim3(padded_of(a.chunks) / (kBits<X> ? 4 : 1), a.row_tiles), kPieces * kTile, 0, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const unsigned grid = (unsigned)((a.out_tiles + 7) / 8 * 8 * ((a.row_tiles + NT * RW - 1) / (NT * RW)));
@@ -652,7 +712,7 @@ hipError_t launch_tile(ReadoutArgs a, hipStream_t s) {
 }
 template <int X, int GRAIN>
 hipError_t launch_tiles(const ReadoutArgs& a, hipStream_t s) {
-  const int rows = tile_of(Kind<X>::kPlanes, GRAIN, a.N).rows;
+  const int rows = tile_of(kOperands<X>, GRAIN, a.N, a.K).rows;
   if constexpr (Kind<X>::kPlanes > 1) {
     if (rows == 32) return launch_tile<X, GRAIN, 2, 1, 2, 4, 1>(a, s);
     if constexpr (GRAIN == kChunk) return launch_tile<X, GRAIN, 2, 2, 2, 4, 1>(a, s);
@@ -667,10 +727,13 @@ hipError_t launch_tiles(const ReadoutArgs& a, hipStream_t s) {
   }
 }
 
-// Few rows (up to 16): a block has 16 OB WO outputs and the clauses of one of the parts that the
+// Few rows (up to 16), bound by the codes' bytes: one row of 9973 bits x 10000 outputs takes 14.5 us,
+// 3.6 TB/s (through products of 16-bit operands 18.5: two thirds of the vector work was their
+// conversion).  A block has 16 OB WO outputs and the clauses of one of the parts that the
 // grid's second axis counts, whose row operands lie in LDS from the start (without those of rows
 // that are not there), so that nothing waits between its first and last chunk.  WK waves share
-// an output tile's chunks, two at a time (128 bytes of codes); each loads kAhead of them before the first is looked at.  With more
+// an output tile's chunks, two at a time (128 bytes of codes); each loads kAhead of them before the
+// first is looked at.  With more
 // than one part the sums go to the workspace, [part][row][output].
 template <int OB>
 constexpr int kAhead = OB == 1 ? 4 : 2;
@@ -680,7 +743,7 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
   constexpr int kDeep = kAhead<OB>;
   extern __shared__ v4u held[];
   __shared__ v4f join[WO * WK][OB][kWave];
-  const int l = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wo = wave / WK, wk = wave % WK;
   const int begin = blockIdx.y * a.part_chunks;
   const int end = begin + a.part_chunks < a.chunks ? begin + a.part_chunks : a.chunks;
@@ -707,9 +770,15 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
         code[u][b].load(a, codes, code_off[b], scales, scale_off[b], chunk_at(first, u));
   };
   load(begin + 2 * wk);
-  const int count = (end - begin) * kPieces;
+  const int count = (end - begin) * (kBits<X> ? kWords : kPieces);
   constexpr int kAtOnce = kPlanes == 1 ? 4 : 2;
-  for (int first = threadIdx.x; first < a.N * count; first += kAtOnce * kWave * WO * WK) {
+  if constexpr (kBits<X>) {
+    for (int j = threadIdx.x; j < a.N * count; j += kWave * WO * WK) {
+      const int n = j / count, i = j - n * count;
+      const uint32_t bits = load_bits(a, (const char*)a.x, n * (uint32_t)a.x_stride * 4, begin * kWords + i);
+      held[i * a.N + n] = bit_operand(a, bits, begin * kWords + i);
+    }
+  } else for (int first = threadIdx.x; first < a.N * count; first += kAtOnce * kWave * WO * WK) {
     Piece<X> piece[kAtOnce];
 #pragma unroll
     for (int e = 0; e < kAtOnce; ++e) {
@@ -746,6 +815,21 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
     for (int u = 0; u < kDeep; ++u) {
       const int chunk = chunk_at(first, u);
       if (chunk >= end) break;
+      if constexpr (kBits<X>) {
+        const v4u x = from[(chunk - begin) * kWords * a.N];
+#pragma unroll
+        for (int b = 0; b < OB; ++b) {
+          float scale[4];
+          now[u][b].scaled(a, chunk, scale);
+#pragma unroll
+          for (int g = 0; g < kChunk / GRAIN; ++g) {
+            const v4f sum = bit_product(GRAIN == kChunk ? x : only(x, g), now[u][b].w);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) total[0][b][r] = __builtin_fmaf(scale[g], sum[r], total[0][b][r]);
+          }
+        }
+        continue;
+      }
       add_chunk<X, GRAIN, 1, OB>(from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total,
                                  [&](int b, v4u& w, float(&scale)[4]) {
                                    w = now[u][b].w;
@@ -774,25 +858,27 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
   }
 }
 
-// A chunk's row operands take rows * kPlanes * 256 bytes of LDS; a part has as many chunks as
-// kHeldLimit takes, which leaves room for two blocks on a CU.
+// A chunk's row operands take 64 bytes of LDS a row for each operand of 16 rows; a part has as many
+// chunks as kHeldLimit takes, which leaves room for two blocks on a CU; bits, whose products leave
+// the codes' loads to wait for, half of that (16 rows x 20000 clauses x 10000 outputs: 64 KB 48 us, 32 KB
+// 38, 150 KB 64).
 constexpr int64_t kHeldLimit = 64 * 1024;
-int part_chunks_of(int planes, int N, int chunks) {
-  const int64_t most = kHeldLimit / ((int64_t)planes * N * kPieces * 16);
+int part_chunks_of(int operands, int N, int chunks) {
+  const int64_t most = kHeldLimit / (operands == 1 ? 2 : 1) / ((int64_t)operands * N * 64);
   if (most >= chunks) return chunks;
   const int64_t parts = (chunks + most - 1) / most;
   return (int)((chunks + parts - 1) / parts);
 }
-int parts_of(int planes, int N, int chunks) {
-  const int each = part_chunks_of(planes, N, chunks);
+int parts_of(int operands, int N, int chunks) {
+  const int each = part_chunks_of(operands, N, chunks);
   return (chunks + each - 1) / each;
 }
 
 template <int X, int GRAIN, int OB, int WO, int WK>
 hipError_t launch_held(ReadoutArgs a, hipStream_t s) {
-  const int parts = parts_of(Kind<X>::kPlanes, a.N, a.chunks);
-  a.part_chunks = part_chunks_of(Kind<X>::kPlanes, a.N, a.chunks);
-  const size_t lds = (size_t)a.N * Kind<X>::kPlanes * a.part_chunks * kPieces * 16;
+  const int parts = parts_of(kOperands<X>, a.N, a.chunks);
+  a.part_chunks = part_chunks_of(kOperands<X>, a.N, a.chunks);
+  const size_t lds = (size_t)a.N * kOperands<X> * a.part_chunks * 64;
   const dim3 grid((unsigned)((a.K + kTile * OB * WO - 1) / (kTile * OB * WO)), (unsigned)parts);
   if (a.scale_dtype == YTM_DTYPE_F32)
     held_kernel<X, GRAIN, OB, WO, WK, true><<<grid, kWave * WO * WK, lds, s>>>(a);
@@ -835,7 +921,15 @@ __global__ __launch_bounds__(256) void short_kernel(ReadoutArgs a) {
 template <int X, int GRAIN>
 hipError_t launch_rows(const ReadoutArgs& a, hipStream_t s) {
   if (a.N > kFewRows) return launch_tiles<X, GRAIN>(a, s);
-  if (a.K > 1024 && parts_of(Kind<X>::kPlanes, a.N, a.chunks) > 1) return launch_held<X, GRAIN, 2, 8, 1>(a, s);
+  // Parts of 16-bit operands in blocks of 256 outputs, so that fewer blocks lay out the same rows (8 rows x
+  // 20000 clauses x 5000 outputs, float32: 32 us, in blocks of 16 outputs 73), unless that makes few blocks
+  // (2 rows x 10027 clauses x 1792 outputs, float32: 14 blocks 40 us, blocks of 16 outputs 15).  Bits are
+  // laid out quickly (12 rows x 14000 clauses x 2000 outputs: 40 us, 15).
+  if constexpr (!kBits<X>) {
+    const int parts = parts_of(kOperands<X>, a.N, a.chunks);
+    if (parts > 1 && (int64_t)(a.K + 255) / 256 * parts >= 40) return launch_held<X, GRAIN, 2, 8, 1>(a, s);
+  }
+  // A block's waves share its 16 outputs' clauses: 16 where there are few outputs, or 4.
   return a.K <= 4096 ? launch_held<X, GRAIN, 1, 1, 16>(a, s) : launch_held<X, GRAIN, 1, 1, 4>(a, s);
 }
 
@@ -863,14 +957,14 @@ int ytm_readout_workspace(int x_dtype, int64_t N, int64_t C, int64_t K, int64_t*
     return fail(YTM_EINVAL, "bad readout_workspace arguments");
   *bytes = 0;
   if (N == 0 || K == 0 || C < 8) return YTM_OK;
-  const int planes = x_dtype == YTM_DTYPE_F32 ? 3 : 1, chunks = (int)((C + 127) / 128);
+  const int operands = ytm::operands_of(x_dtype), chunks = (int)((C + 127) / 128);
   if (N > ytm::kFewRows) {
-    *bytes = ytm::frag_bytes(planes, (int)N, chunks);
-    const int whole = ytm::tile_parts_of(planes, ytm::kChunk, (int)N, chunks, (int)K);
-    const int four = ytm::tile_parts_of(planes, ytm::kStep, (int)N, chunks, (int)K);
+    *bytes = ytm::frag_bytes(operands, (int)N, chunks);
+    const int whole = ytm::tile_parts_of(operands, ytm::kChunk, (int)N, chunks, (int)K);
+    const int four = ytm::tile_parts_of(operands, ytm::kStep, (int)N, chunks, (int)K);
     if (whole > 1 || four > 1) *bytes += (whole > four ? whole : four) * N * K * 4;
   } else {
-    const int parts = ytm::parts_of(planes, (int)N, chunks);
+    const int parts = ytm::parts_of(operands, (int)N, chunks);
     if (parts > 1) *bytes = parts * N * K * 4;
   }
   return YTM_OK;
