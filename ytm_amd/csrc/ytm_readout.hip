@@ -289,43 +289,35 @@ __device__ __forceinline__ void store_out(const ReadoutArgs& a, int n, int o, fl
   }
 }
 
-// A chunk's products of NT row tiles, whose operands lie at from[plane * .. + step * .. + tile * ..], and OB
-// output tiles, added to the sums so far.  One output tile after the other, so that the scaling
-// of one can go beside the products of the next; code(b, w, scale) gives tile b's codes and the
-// scales of its four products.
-template <int X, int GRAIN, int NT, int OB, typename Code>
-__device__ __forceinline__ void add_chunk(const v4u* from, int plane, int step, int tile, v4f (&total)[NT][OB],
-                                          Code code) {
+// A chunk's products of a row tile, whose operands lie at from[plane * .. + step * ..], and OB output
+// tiles, added to the sums so far.  One output tile after the other, so that the scaling of one can go
+// beside the products of the next; code(b, w, scale) gives tile b's codes and the scales of its four
+// products.
+template <int X, int GRAIN, int OB, typename Code>
+__device__ __forceinline__ void add_chunk(const v4u* from, int plane, int step, v4f (&total)[OB], Code code) {
   constexpr int kPlanes = Kind<X>::kPlanes;
   constexpr bool kHalf = Kind<X>::kHalf;
-  v4u x[4][kPlanes][NT];
+  v4u x[4][kPlanes];
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int p = 0; p < kPlanes; ++p)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) x[s][p][n] = from[p * plane + s * step + n * tile];
+    for (int p = 0; p < kPlanes; ++p) x[s][p] = from[p * plane + s * step];
 #pragma unroll
   for (int b = 0; b < OB; ++b) {
     v4u w;
     float scale[4];
     code(b, w, scale);
     w = turn<GRAIN>(w);
-    v4f sum[NT];
+    v4f sum;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const v4u y = codes_to_16<kHalf>(w[s]);
+      if (s * kStep % GRAIN == 0) sum = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (s * kStep % GRAIN == 0) sum[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int p = kPlanes - 1; p >= 0; --p) sum[n] = product<kHalf>(x[s][p][n], y, sum[n]);
-      }
+      for (int p = kPlanes - 1; p >= 0; --p) sum = product<kHalf>(x[s][p], y, sum);
       if ((s + 1) * kStep % GRAIN == 0) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) total[n][b][r] = __builtin_fmaf(scale[s], sum[n][r], total[n][b][r]);
+        for (int r = 0; r < 4; ++r) total[b][r] = __builtin_fmaf(scale[s], sum[r], total[b][r]);
       }
     }
   }
@@ -667,7 +659,8 @@ Tile tile_of(int operands, int grain, int N, int K) {
   int best = 0;
   int64_t least = 0;
   for (int i = 0; i < (N <= 64 ? 1 : whole ? 3 : 2); ++i) {
-    const int64_t blocks = (int64_t)((N + tiles[i].rows - 1) / tiles[i].rows) * ((K + tiles[i].outs - 1) / tiles[i].outs);
+    const int64_t blocks =
+        (int64_t)((N + tiles[i].rows - 1) / tiles[i].rows) * ((K + tiles[i].outs - 1) / tiles[i].outs);
     const int64_t time = (blocks > 128 ? (blocks + 255) / 256 * 256 : blocks) * kTime[i];
     if (i == 0 || time < least) least = time, best = i;
   }
@@ -778,32 +771,34 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
       const uint32_t bits = load_bits(a, (const char*)a.x, n * (uint32_t)a.x_stride * 4, begin * kWords + i);
       held[i * a.N + n] = bit_operand(a, bits, begin * kWords + i);
     }
-  } else for (int first = threadIdx.x; first < a.N * count; first += kAtOnce * kWave * WO * WK) {
-    Piece<X> piece[kAtOnce];
+  } else {
+    for (int first = threadIdx.x; first < a.N * count; first += kAtOnce * kWave * WO * WK) {
+      Piece<X> piece[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < kAtOnce; ++e) {
-      const int j = first + e * kWave * WO * WK;
-      const int n = j < a.N * count ? j / count : 0;
-      piece[e].load(a, (const char*)a.x, n * (uint32_t)a.x_stride * kSize<X>,
-                    begin * kChunk + 8 * (j < a.N * count ? j - n * count : 0));
-    }
+      for (int e = 0; e < kAtOnce; ++e) {
+        const int j = first + e * kWave * WO * WK;
+        const int n = j < a.N * count ? j / count : 0;
+        piece[e].load(a, (const char*)a.x, n * (uint32_t)a.x_stride * kSize<X>,
+                      begin * kChunk + 8 * (j < a.N * count ? j - n * count : 0));
+      }
 #pragma unroll
-    for (int e = 0; e < kAtOnce; ++e) {
-      const int j = first + e * kWave * WO * WK;
-      if (j >= a.N * count) break;
-      const int n = j / count, i = j - n * count;
-      v4u plane[kPlanes];
-      piece[e].operands(a, begin * kChunk + 8 * i, plane);
-      const int place = i / kPieces * kPieces + place_of<GRAIN>(i % kPieces);
+      for (int e = 0; e < kAtOnce; ++e) {
+        const int j = first + e * kWave * WO * WK;
+        if (j >= a.N * count) break;
+        const int n = j / count, i = j - n * count;
+        v4u plane[kPlanes];
+        piece[e].operands(a, begin * kChunk + 8 * i, plane);
+        const int place = i / kPieces * kPieces + place_of<GRAIN>(i % kPieces);
 #pragma unroll
-      for (int p = 0; p < kPlanes; ++p) held[(p * count + place) * a.N + n] = plane[p];
+        for (int p = 0; p < kPlanes; ++p) held[(p * count + place) * a.N + n] = plane[p];
+      }
     }
   }
   __syncthreads();
   const v4u* from = held + l / 16 * a.N + (l % 16 < a.N ? l % 16 : 0);
-  v4f total[1][OB];
+  v4f total[OB];
 #pragma unroll
-  for (int b = 0; b < OB; ++b) total[0][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int b = 0; b < OB; ++b) total[b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   for (int first = begin + 2 * wk; first < end; first += kDeep * WK) {
     Codes<GRAIN, WIDE> now[kDeep][OB];
 #pragma unroll
@@ -825,25 +820,25 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
           for (int g = 0; g < kChunk / GRAIN; ++g) {
             const v4f sum = bit_product(GRAIN == kChunk ? x : only(x, g), now[u][b].w);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) total[0][b][r] = __builtin_fmaf(scale[g], sum[r], total[0][b][r]);
+            for (int r = 0; r < 4; ++r) total[b][r] = __builtin_fmaf(scale[g], sum[r], total[b][r]);
           }
         }
         continue;
       }
-      add_chunk<X, GRAIN, 1, OB>(from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, 0, total,
-                                 [&](int b, v4u& w, float(&scale)[4]) {
-                                   w = now[u][b].w;
-                                   now[u][b].scaled(a, chunk, scale);
-                                 });
+      add_chunk<X, GRAIN, OB>(from + (chunk - begin) * kPieces * a.N, count * a.N, 4 * a.N, total,
+                              [&](int b, v4u& w, float(&scale)[4]) {
+                                w = now[u][b].w;
+                                now[u][b].scaled(a, chunk, scale);
+                              });
     }
   }
 #pragma unroll
-  for (int b = 0; b < OB; ++b) join[wave][b][l] = total[0][b];
+  for (int b = 0; b < OB; ++b) join[wave][b][l] = total[b];
   __syncthreads();
   if (wk > 0) return;
 #pragma unroll
   for (int b = 0; b < OB; ++b) {
-    v4f v = total[0][b];
+    v4f v = total[b];
     for (int w = 1; w < WK; ++w) v += join[wave + w][b][l];
     const int o = first_out + b * kTile;
 #pragma unroll
