@@ -1,0 +1,93 @@
+"""What the answering operators refuse of their operands, before anything is launched.
+
+Tensors here are on the CPU and say that they are on a GPU; the library's entries only count their
+calls, so a call that is let through is seen and reads nothing.
+"""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from ytm_amd import decode  # noqa: E402
+
+
+class OnGpu(torch.Tensor):
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return 0
+
+
+def on_gpu(*shape, dtype=torch.float32, grad=False):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnGpu).requires_grad_(grad)
+
+
+class Entries:
+    """The library's entries: how often one that launches was called."""
+
+    launched = 0
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.launched += not name.endswith("_workspace")
+            return 0
+
+        return entry
+
+
+@pytest.fixture
+def entries(monkeypatch):
+    e = Entries()
+    monkeypatch.setattr(decode, "lib", e)
+    monkeypatch.setattr(decode, "_device_now", lambda: 0)
+    monkeypatch.setattr(decode, "_stream_of", lambda device: 0)
+    return e
+
+
+def readout(**kw):
+    a = dict(x=on_gpu(2, 64), codes=on_gpu(3, 32, dtype=torch.uint8), scales=on_gpu(3, 2), out=on_gpu(2, 3))
+    return decode.readout(**{**a, **kw})
+
+
+def adjust(**kw):
+    a = dict(scores=on_gpu(2, 10), tokens=on_gpu(2, 4, dtype=torch.int32), out=on_gpu(2, 10))
+    return decode.adjust_scores(**{**a, **kw})
+
+
+def choose(**kw):
+    return decode.choose(**{**dict(scores=on_gpu(2, 10)), **kw})
+
+
+FLOATS = [
+    (readout, "x", (2, 64)), (readout, "scales", (3, 2)), (readout, "out", (2, 3)),
+    (adjust, "scores", (2, 10)), (adjust, "repetition", (2,)), (adjust, "frequency", (2,)),
+    (adjust, "presence", (2,)), (adjust, "bias", (2, 10)), (adjust, "bias", (10,)), (adjust, "out", (2, 10)),
+    (choose, "scores", (2, 10)), (choose, "temperature", (2,)), (choose, "top_p", (2,)), (choose, "min_p", (2,)),
+    (choose, "noise", (2, 10)), (choose, "noise", (10,)),
+]
+
+
+@pytest.mark.parametrize("call,name,shape", FLOATS)
+def test_operands_that_require_a_gradient(entries, call, name, shape):
+    """Refused where gradients are recorded, taken where none are: what a trained module's parameters are."""
+    with pytest.raises(ValueError, match="gradient"):
+        call(**{name: on_gpu(*shape, grad=True)})
+    assert entries.launched == 0
+    with torch.no_grad():
+        call(**{name: on_gpu(*shape, grad=True)})
+    assert entries.launched == 1
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("call,name,shape", [
+    (readout, "scales", (3, 1)), (readout, "scales", (1, 2)), (readout, "out", (1, 1)), (readout, "out", (2, 4)),
+    (adjust, "repetition", (1,)), (adjust, "frequency", (3,)), (adjust, "presence", (1,)), (adjust, "bias", (9,)),
+    (adjust, "bias", (1, 5)), (adjust, "bias", (1, 10)), (adjust, "out", (1, 1)), (adjust, "out", (2, 9)),
+    (choose, "temperature", (1,)), (choose, "top_p", (3,)), (choose, "min_p", (1,)), (choose, "noise", (9,)),
+    (choose, "noise", (1, 10)), (choose, "noise", (2, 9)),
+])
+def test_wrong_shapes_without_gradients_recorded(entries, call, name, shape, grad):
+    """A size that does not fit is refused under no_grad too, whether or not the operand requires a gradient."""
+    with torch.no_grad(), pytest.raises(ValueError, match=f"^{name} must have shape"):
+        call(**{name: on_gpu(*shape, grad=grad)})
+    assert entries.launched == 0

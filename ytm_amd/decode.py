@@ -101,8 +101,8 @@ _stream_of = torch._C._cuda_getCurrentRawStream
 
 
 def _refuse(t, name: str, dims: tuple, dtype, shape: str, device: int) -> None:
-    """Raises what is wrong with operand t (nothing where it only requires a gradient and none
-    is recorded)."""
+    """Raises what is wrong with operand t; `shape` says what its shape must be where it does not fit.
+    Nothing where t only requires a gradient and none is recorded."""
     if not isinstance(t, _Tensor):
         raise TypeError(f"{name} must be a torch tensor.")
     if not t.is_cuda:
@@ -116,11 +116,10 @@ def _refuse(t, name: str, dims: tuple, dtype, shape: str, device: int) -> None:
         raise TypeError(f"{name} must be {' or '.join(str(d).removeprefix('torch.') for d in names)}, not {t.dtype}.")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}'s rows must be contiguous.")
-    if t.requires_grad:
-        if torch.is_grad_enabled():
-            raise ValueError(f"{name} requires a gradient; this operator has none.")
-    elif shape:
+    if shape:
         raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}.")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient; this operator has none.")
 
 
 def _rows_of(t, name: str, types: dict) -> tuple[int, int, int, int]:
