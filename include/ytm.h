@@ -310,16 +310,18 @@ int ytm_adjust_scores(const void *scores, int dtype, int64_t stride, int64_t N, 
                       int64_t out_stride, void *stream);
 
 /* ytm_choose: one of V (at most 8388608) answers for each row.  With z = score / temperature[n]
- * (NULL: 1; 0 or less: temperature 1 and top_k 1; less than the smallest normal float: that; a NaN score counts as -inf, +inf as the
- * largest float) and the answers in the order of z descending, then index ascending, the filters keep
- * a first part of that order, the first answer always among it:
- *   min_p: z >= max z + log(min_p[n]);  top_k: the first top_k[n] of these (0 or less: all);
+ * (NULL: 1; 0 or less: temperature 1 and top_k 1; less than the smallest normal float, or NaN:
+ * that; a z that is NaN counts as -inf, one of +inf as the largest float) and the answers in the
+ * order of z descending, then index ascending, the filters keep a first part of that order, the
+ * first answer always among it:
+ *   min_p: z >= max z + log(min_p[n]) (0 or less, or NaN: all);
+ *   top_k: the first top_k[n] of these (0 or less: all);
  *   top_p: of these, with masses exp(z - max z), those before which less than top_p[n] of the mass
- *   stands (1 or more: all).
+ *   stands (1 or more, or NaN: all).
  * tokens[n] = the index of the largest z + noise[n][v] (NULL: of z) of the kept answers, the
  * lowest of equal ones, and logprobs[n] = z of it - log of the kept answers' sum of exp(z).
  * With standard Gumbel noise -log(-log(u)) that is a draw from softmax(z) over the kept
- * answers.  Noise is finite.  -1 and -inf where no score is above -inf.  workspace: device memory
+ * answers.  Noise is finite.  -1 and -inf where no z is above -inf.  workspace: device memory
  * of ytm_choose_workspace's bytes at a multiple of 16 bytes, for the time of the call's work (NULL
  * where that is 0: rows that are short or many). */
 int ytm_choose_workspace(int dtype, int64_t N, int64_t V, int64_t *bytes);

@@ -1,0 +1,38 @@
+"""The answering operators at the ends of what their operands may be."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+ytm_amd = pytest.importorskip("ytm_amd")
+from ytm_amd import decode  # noqa: E402
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# few answers, hundreds of them kept, thousands of equal ones, a row long enough to be sliced
+LENGTHS = [4, 100, 3000, 20001, 40000]
+
+
+def ties(V):
+    """Two rows in which most of the answers are the best, answer 1 the first of them."""
+    x = torch.zeros(2, V, device="cuda")
+    x[:, 0] = -1.0
+    x[1, V // 2:] = -3.0
+    return x, torch.linspace(0, 2, V, device="cuda")  # noise that likes the last answers
+
+
+@pytest.mark.parametrize("V", LENGTHS)
+@pytest.mark.parametrize("kept", [2, 50, 200, 1000, 0])
+def test_choose_top_p_not_a_number(V, kept):
+    """No bound, as 1 is, however many answers the other filters leave."""
+    x, noise = ties(V)
+    x = x + torch.arange(V, device="cuda") % 7 * 0.125
+    k = torch.full((2,), kept, dtype=torch.int32, device="cuda")
+    m = torch.full((2,), 0.1, device="cuda")
+    p = torch.full((2,), float("nan"), device="cuda")
+    for more in ({}, {"min_p": m}):
+        assert same(decode.choose(x, top_k=k, top_p=p, noise=noise, **more),
+                    decode.choose(x, top_k=k, noise=noise, **more))

@@ -827,11 +827,36 @@ __device__ __forceinline__ bool from_bins(const ChooseArgs& a, int64_t n, const 
   return true;
 }
 
+// A row's filters, as every path below takes them: a bound that is not a number is none.
+struct Filters {
+  float t, p, min;
+  int k;
+  bool bounded, seek;  // min_p holds; top_k is sought by a bound
+
+  __device__ __forceinline__ Filters(const ChooseArgs& a, int64_t n) {
+    t = a.temperature ? a.temperature[n] : 1.0f;
+    k = a.top_k ? a.top_k[n] : 0;
+    if (t <= 0.0f) {
+      t = 1.0f;
+      k = 1;
+    }
+    t = fmaxf(t, FLT_MIN);  // a smaller one has no reciprocal; a NaN too becomes it
+    if (k >= a.V) k = 0;
+    p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
+    min = a.min_p ? a.min_p[n] : 0.0f;
+    bounded = min > 0.0f;
+    seek = k > 0 && k <= kMaxSeek;
+  }
+  __device__ __forceinline__ bool none() const { return k <= 0 && p >= 1.0f && !bounded; }
+};
+
 // The answer from a list (of key of score, ~index) that holds every answer the filters may keep:
 // from a histogram over it, or from the whole list sorted where a slice holds too many.
 template <typename In>
-__device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, const Row<In>& row, int count, int k,
-                                          ChooseShared& sh) {
+__device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, const Row<In>& row, int count,
+                                          const Filters& filters, ChooseShared& sh) {
+  const int k = filters.k;
+  const float p = filters.p;
   u64 first = 0;
   for (int i = threadIdx.x; i < count; i += kChooseThreads) {
     const u64 e = sh.list[i];
@@ -843,12 +868,11 @@ __device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, const 
   if (top <= kNone) return no_answer(a, n);
   const float best = value_of(top);
   uint32_t least = kNone + 1u;
-  if (a.min_p && a.min_p[n] > 0.0f) {
-    const float z = best + logf(a.min_p[n]);
+  if (filters.bounded) {
+    const float z = best + logf(filters.min);
     const uint32_t key = key_of((z <= best ? z : best) + 0.0f);
     if (key > least) least = key;
   }
-  const float p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
   const auto each = [&](float, bool, auto f) {
     for (int i = threadIdx.x; i < count; i += kChooseThreads)
       f(value_of((uint32_t)(sh.list[i] >> 32)), (int)~(uint32_t)sh.list[i]);
@@ -1071,9 +1095,11 @@ __device__ __forceinline__ int shorten_list(int count, float t, int k, ChooseSha
 }
 
 // from_list for up to kSmall entries: one wave, in registers, without a barrier.
-__device__ __forceinline__ void from_small(const ChooseArgs& a, int64_t n, int count, float t, int k,
+__device__ __forceinline__ void from_small(const ChooseArgs& a, int64_t n, int count, const Filters& filters,
                                            ChooseShared& sh) {
   if (threadIdx.x >= kWave) return;
+  const float t = filters.t, p = filters.p;
+  const int k = filters.k;
   const int l = threadIdx.x;
   u64 v[4];
 #pragma unroll
@@ -1087,12 +1113,11 @@ __device__ __forceinline__ void from_small(const ChooseArgs& a, int64_t n, int c
   if (top <= kNone) return no_answer(a, n);
   const float best = value_of(top);
   uint32_t least = kNone + 1u;
-  if (a.min_p && a.min_p[n] > 0.0f) {
-    const float z = best + logf(a.min_p[n]);
+  if (filters.bounded) {
+    const float z = best + logf(filters.min);
     const uint32_t key = key_of((z <= best ? z : best) + 0.0f);
     if (key > least) least = key;
   }
-  const float p = a.top_p ? a.top_p[n] : 1.0f;
   const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
   u64 mass[4], own = 0;
   bool in[4];
@@ -1128,29 +1153,6 @@ __device__ __forceinline__ void from_small(const ChooseArgs& a, int64_t n, int c
       a.logprobs[n] = (z[r] - best) - logf((float)sum * (1.0f / kMass));
     }
 }
-
-// A row's filters.
-struct Filters {
-  float t, p, min;
-  int k;
-  bool bounded, seek;  // min_p holds; top_k is sought by a bound
-
-  __device__ __forceinline__ Filters(const ChooseArgs& a, int64_t n) {
-    t = a.temperature ? a.temperature[n] : 1.0f;
-    k = a.top_k ? a.top_k[n] : 0;
-    if (t <= 0.0f) {
-      t = 1.0f;
-      k = 1;
-    }
-    t = fmaxf(t, FLT_MIN);  // a smaller one has no reciprocal; a NaN too becomes it
-    if (k >= a.V) k = 0;
-    p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
-    min = a.min_p ? a.min_p[n] : 0.0f;
-    bounded = min > 0.0f;
-    seek = k > 0 && k <= kMaxSeek;
-  }
-  __device__ __forceinline__ bool none() const { return k <= 0 && p >= 1.0f && !bounded; }
-};
 
 // Lists what may be kept of `V` scores (a row, or a slice, whose k-th largest and largest are no larger
 // than the row's), with a bound from their first `rounds` rounds; whether it fits.
@@ -1227,7 +1229,7 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   const Slice* slices = a.found + n * a.slices;
   const auto from_entries = [&](int count) {
     if (filters.seek && count > kSmall) count = shorten_list(count, t, k, sh);
-    return count <= kSmall ? from_small(a, n, count, t, k, sh) : from_list(a, n, row, count, k, sh);
+    return count <= kSmall ? from_small(a, n, count, filters, sh) : from_list(a, n, row, count, filters, sh);
   };
   if (filters.none()) {
     if (a.slices == 0) return from_all(a, n, row, all_of(a, n, row, 0, V, sh));
@@ -1266,7 +1268,7 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   if (best == -INFINITY) return no_answer(a, n);
   Cut cut{kNone + 1u, V - 1};
   if (bounded) {
-    const float low = best + logf(a.min_p[n]);
+    const float low = best + logf(filters.min);
     const uint32_t key = key_of((low <= best ? low : best) + 0.0f);
     if (key > cut.key) cut.key = key;
   }
