@@ -314,7 +314,7 @@ int ytm_adjust_scores(const void *scores, int dtype, int64_t stride, int64_t N, 
  * that; a z that is NaN counts as -inf, one of +inf as the largest float) and the answers in the
  * order of z descending, then index ascending, the filters keep a first part of that order, the
  * first answer always among it:
- *   min_p: z >= max z + log(min_p[n]) (0 or less, or NaN: all);
+ *   min_p: z >= max z + log(min_p[n]) (0 or less, or NaN: all; above 1: the first answer alone);
  *   top_k: the first top_k[n] of these (0 or less: all);
  *   top_p: of these, with masses exp(z - max z), those before which less than top_p[n] of the mass
  *   stands (1 or more, or NaN: all).

@@ -36,3 +36,16 @@ def test_choose_top_p_not_a_number(V, kept):
     for more in ({}, {"min_p": m}):
         assert same(decode.choose(x, top_k=k, top_p=p, noise=noise, **more),
                     decode.choose(x, top_k=k, noise=noise, **more))
+
+
+@pytest.mark.parametrize("V", LENGTHS)
+@pytest.mark.parametrize("share", [1.0000001, 2.0, float("inf")])
+def test_choose_min_p_above_one(V, share):
+    """No answer reaches more than the best one's share: the first answer alone is kept."""
+    x, noise = ties(V)
+    for more in ({}, {"top_p": torch.full((2,), 0.9, device="cuda")},
+                 {"top_k": torch.full((2,), 300, dtype=torch.int32, device="cuda")}):
+        index, log = decode.choose(x, min_p=torch.full((2,), share, device="cuda"), noise=noise, **more)
+        assert index.tolist() == [1, 1] and log.tolist() == [0.0, 0.0]
+    index, _ = decode.choose(x, min_p=torch.ones(2, device="cuda"), noise=noise)  # all of the best ones
+    assert index.tolist() == [V - 1, V // 2 - 1]

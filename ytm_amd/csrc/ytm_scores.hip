@@ -841,9 +841,13 @@ struct Filters {
       k = 1;
     }
     t = fmaxf(t, FLT_MIN);  // a smaller one has no reciprocal; a NaN too becomes it
+    min = a.min_p ? a.min_p[n] : 0.0f;
+    if (min > 1.0f) {  // not even the first answer reaches it, which alone is kept all the same
+      min = 0.0f;
+      k = 1;
+    }
     if (k >= a.V) k = 0;
     p = a.top_p && a.top_p[n] < 1.0f ? a.top_p[n] : 1.0f;
-    min = a.min_p ? a.min_p[n] : 0.0f;
     bounded = min > 0.0f;
     seek = k > 0 && k <= kMaxSeek;
   }
@@ -869,8 +873,7 @@ __device__ __forceinline__ void from_list(const ChooseArgs& a, int64_t n, const 
   const float best = value_of(top);
   uint32_t least = kNone + 1u;
   if (filters.bounded) {
-    const float z = best + logf(filters.min);
-    const uint32_t key = key_of((z <= best ? z : best) + 0.0f);
+    const uint32_t key = key_of(best + logf(filters.min) + 0.0f);
     if (key > least) least = key;
   }
   const auto each = [&](float, bool, auto f) {
@@ -1114,8 +1117,7 @@ __device__ __forceinline__ void from_small(const ChooseArgs& a, int64_t n, int c
   const float best = value_of(top);
   uint32_t least = kNone + 1u;
   if (filters.bounded) {
-    const float z = best + logf(filters.min);
-    const uint32_t key = key_of((z <= best ? z : best) + 0.0f);
+    const uint32_t key = key_of(best + logf(filters.min) + 0.0f);
     if (key > least) least = key;
   }
   const float* noise = a.noise ? a.noise + n * a.noise_stride : nullptr;
@@ -1166,8 +1168,7 @@ __device__ __forceinline__ bool list_kept(const In* in, int V, int rounds, const
     least = bound > kNone ? with_equals(value_of(bound), f.t) : -INFINITY;
   } else {
     const float z = scaled(value_of((uint32_t)block_max(key_of(own + 0.0f), sh)), f.t);
-    const float low = z + logf(f.min);
-    least = with_equals((low <= z ? low : z) * f.t, f.t);
+    least = with_equals((z + logf(f.min)) * f.t, f.t);
   }
   return list_from(in, V, least, own, sh);
 }
@@ -1268,8 +1269,7 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   if (best == -INFINITY) return no_answer(a, n);
   Cut cut{kNone + 1u, V - 1};
   if (bounded) {
-    const float low = best + logf(filters.min);
-    const uint32_t key = key_of((low <= best ? low : best) + 0.0f);
+    const uint32_t key = key_of(best + logf(filters.min) + 0.0f);
     if (key > cut.key) cut.key = key;
   }
   // Where a bound leaves few scores, the threads mark them and go through their marks: every lane
