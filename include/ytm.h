@@ -309,7 +309,7 @@ int ytm_adjust_scores(const void *scores, int dtype, int64_t stride, int64_t N, 
                       int64_t bias_stride, const uint32_t *allowed, int64_t allowed_stride, void *out, int out_dtype,
                       int64_t out_stride, void *stream);
 
-/* ytm_choose: one of V (at most 8388608) answers for each row.  With z = score / temperature[n]
+/* ytm_choose: one of V (at most 8388608) answers for each of N (2147483647) rows.  With z = score / temperature[n]
  * (NULL: 1; 0 or less: temperature 1 and top_k 1; less than the smallest normal float, or NaN:
  * that; a z that is NaN counts as -inf, one of +inf as the largest float) and the answers in the
  * order of z descending, then index ascending, the filters keep a first part of that order, the

@@ -49,3 +49,15 @@ def test_choose_min_p_above_one(V, share):
         assert index.tolist() == [1, 1] and log.tolist() == [0.0, 0.0]
     index, _ = decode.choose(x, min_p=torch.ones(2, device="cuda"), noise=noise)  # all of the best ones
     assert index.tolist() == [V - 1, V // 2 - 1]
+
+
+def test_choose_more_rows_than_a_launch_takes():
+    N, V = (1 << 22) + 5, 3
+    x = torch.randint(-8, 9, (N, V), device="cuda").float()
+    index, log = decode.choose(x)
+    best = torch.where(x == x.amax(1, keepdim=True), torch.arange(V, device="cuda"), V).amin(1)
+    assert torch.equal(index.long(), best)
+    assert bool(((log.double() - torch.log_softmax(x.double(), 1).amax(1)).abs() <= 2.0**-18).all())
+    k = torch.ones(N, dtype=torch.int32, device="cuda")
+    first, none = decode.choose(x, top_k=k)
+    assert torch.equal(index, first) and not bool(none.any())

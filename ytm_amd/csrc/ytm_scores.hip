@@ -204,6 +204,7 @@ struct ChooseArgs {
   int64_t noise_stride;
   int32_t* tokens;
   float* logprobs;
+  int64_t first;     // row of the launch's first block
   int slices, each;  // of a row, and scores in one (0: rows are not sliced)
   struct Slice* found;
 };
@@ -1220,7 +1221,7 @@ template <typename In>
 __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(4, 4))) void choose_kernel(
     ChooseArgs a) {
   __shared__ ChooseShared sh;
-  const int64_t n = blockIdx.x;
+  const int64_t n = a.first + blockIdx.x;
   const int V = a.V;
   const Filters filters(a, n);
   const float t = filters.t, p = filters.p;
@@ -1296,6 +1297,24 @@ __global__ __launch_bounds__(kChooseThreads) __attribute__((amdgpu_waves_per_eu(
   from_row(a, n, row, best, k, p, cut, sh);
 }
 
+// A row a block.  A launch counts its threads in 32 bits, and one of more leaves blocks out without an
+// error, so more rows than that take several.
+template <typename In>
+hipError_t launch_choose(ChooseArgs a, int64_t N, hipStream_t s) {
+  if (a.slices) {
+    slice_kernel<In><<<dim3(a.slices, (unsigned)N), kChooseThreads, 0, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  constexpr int64_t kMost = UINT32_MAX / kChooseThreads;
+  for (a.first = 0; a.first < N; a.first += kMost) {
+    choose_kernel<In><<<(unsigned)(N - a.first < kMost ? N - a.first : kMost), kChooseThreads, 0, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 // Slices of each row: none where a row has less than 128 KB or the rows alone take a quarter of the
 // 256 CUs, else 32 KB each, up to 16 (16 lists of the largest top_k sought fit one of kList).
 int slices_of(int size, int64_t N, int64_t V) {
@@ -1353,7 +1372,7 @@ int ytm_choose(const void* scores, int dtype, int64_t stride, int64_t N, int64_t
                int32_t* tokens, float* logprobs, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!ytm::decode_float(dtype)) return fail(YTM_EINVAL, "scores are float32, float16 or bfloat16");
   if (N < 0 || V < 0 || N > INT32_MAX || V > ytm::kMaxScores)
-    return fail(YTM_EINVAL, "choose takes at most 8388608 scores a row");
+    return fail(YTM_EINVAL, "choose takes at most 2147483647 rows of 8388608 scores");
   if (N == 0) return YTM_OK;
   if ((V > 0 && !scores) || !tokens || !logprobs) return fail(YTM_EINVAL, "bad choose arguments");
   if (N > 1 && ((stride != 0 && stride < V) || (noise && noise_stride != 0 && noise_stride < V)))
@@ -1364,24 +1383,14 @@ int ytm_choose(const void* scores, int dtype, int64_t stride, int64_t N, int64_t
     return fail(YTM_EINVAL, "choose: the workspace is too small or not at a multiple of 16 bytes");
   const int slices = ytm::slices_of(dtype == YTM_DTYPE_F32 ? 4 : 2, N, V);
   const ytm::ChooseArgs a{scores, stride, (int)V, temperature, top_k, top_p, min_p, noise, noise_stride, tokens, logprobs,
-                          slices, slices ? (int)((V + slices - 1) / slices) : 0, (ytm::Slice*)workspace};
+                          0, slices, slices ? (int)((V + slices - 1) / slices) : 0, (ytm::Slice*)workspace};
   hipStream_t s = (hipStream_t)stream;
-  if (slices) {
-    const dim3 grid(slices, (unsigned)N);
-    switch (dtype) {
-      case YTM_DTYPE_F16: ytm::slice_kernel<ytm::f16><<<grid, ytm::kChooseThreads, 0, s>>>(a); break;
-      case YTM_DTYPE_BF16: ytm::slice_kernel<ytm::bf16><<<grid, ytm::kChooseThreads, 0, s>>>(a); break;
-      default: ytm::slice_kernel<float><<<grid, ytm::kChooseThreads, 0, s>>>(a); break;
-    }
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return fail(YTM_EHIP, std::string("choose failed: ") + hipGetErrorString(e));
-  }
+  hipError_t e;
   switch (dtype) {
-    case YTM_DTYPE_F16: ytm::choose_kernel<ytm::f16><<<(unsigned)N, ytm::kChooseThreads, 0, s>>>(a); break;
-    case YTM_DTYPE_BF16: ytm::choose_kernel<ytm::bf16><<<(unsigned)N, ytm::kChooseThreads, 0, s>>>(a); break;
-    default: ytm::choose_kernel<float><<<(unsigned)N, ytm::kChooseThreads, 0, s>>>(a); break;
+    case YTM_DTYPE_F16: e = ytm::launch_choose<ytm::f16>(a, N, s); break;
+    case YTM_DTYPE_BF16: e = ytm::launch_choose<ytm::bf16>(a, N, s); break;
+    default: e = ytm::launch_choose<float>(a, N, s); break;
   }
-  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(YTM_EHIP, std::string("choose failed: ") + hipGetErrorString(e));
   return YTM_OK;
 }
