@@ -61,3 +61,23 @@ def test_choose_more_rows_than_a_launch_takes():
     k = torch.ones(N, dtype=torch.int32, device="cuda")
     first, none = decode.choose(x, top_k=k)
     assert torch.equal(index, first) and not bool(none.any())
+
+
+def test_readout_more_outputs_than_a_launch_takes():
+    """65535 rows x 786433 outputs of float16."""
+    N, C, K = 65535, 8, 786433
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 160 << 30:
+        pytest.skip("takes 103 GB of device memory")
+    codes = torch.zeros(K, 16, dtype=torch.uint8, device="cuda")
+    codes[:, :4] = torch.randint(0, 256, (K, 4), device="cuda", dtype=torch.uint8)
+    x = torch.randint(-4, 5, (N, C), device="cuda").float()
+    scales = torch.ones(K, 1, device="cuda")
+    out = torch.empty(N, K, dtype=torch.float16, device="cuda")
+    decode.readout(x, codes, scales, out=out)
+    values = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], device="cuda")
+    w = values[torch.stack((codes[:, :4] & 15, codes[:, :4] >> 4), 2).view(K, C).int()].t().contiguous()
+    wrong = sum(int((out[n:n + 1024] != (x[n:n + 1024] @ w).half()).any()) for n in range(0, N, 1024))
+    del out
+    torch.cuda.empty_cache()
+    assert wrong == 0

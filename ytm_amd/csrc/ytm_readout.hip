@@ -691,17 +691,31 @@ int64_t frag_bytes(int operands, int N, int chunks) {
 template <int X, int GRAIN, int NT, int RW, int OB, int WO, int WK>
 hipError_t launch_tile(ReadoutArgs a, hipStream_t s) {
   a.row_tiles = (a.N + kTile - 1) / kTile;
-  a.out_tiles = (a.K + kTile * OB * WO - 1) / (kTile * OB * WO);
   a.part_chunks = part_pairs_of(kOperands<X>, GRAIN, a.N, a.chunks, a.K);
   a.parts = (float*)((char*)a.frag + frag_bytes(kOperands<X>, a.N, a.chunks));
   const int parts = tile_parts_of(kOperands<X>, GRAIN, a.N, a.chunks, a.K);
   rows_kernel<X, GRAIN><<<dim3(padded_of(a.chunks) / (kBits<X> ? 4 : 1), a.row_tiles), kPieces * kTile, 0, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const unsigned grid = (unsigned)((a.out_tiles + 7) / 8 * 8 * ((a.row_tiles + NT * RW - 1) / (NT * RW)));
-  tile_kernel<X, GRAIN, NT, RW, OB, WO, WK><<<dim3(grid, parts), kWave * RW * WO * WK, 0, s>>>(a);
-  e = hipGetLastError();
-  return e != hipSuccess || parts == 1 ? e : launch_parts(a, parts, s);
+  // A launch counts its threads in 32 bits, and one of more leaves blocks out without an error, so more
+  // outputs than that take several (never in parts, which few blocks are cut into).
+  constexpr int kThreads = kWave * RW * WO * WK, kOuts = kTile * OB * WO;
+  const int64_t row_blocks = (a.row_tiles + NT * RW - 1) / (NT * RW), K = a.K;
+  const int64_t most = (int64_t)UINT32_MAX / kThreads / row_blocks / 8 * 8 * kOuts;
+  const int out_size = a.out_dtype == YTM_DTYPE_F32 ? 4 : 2, scale_size = a.scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  for (int64_t done = 0; done < K; done += most) {
+    a.K = (int)(K - done < most ? K - done : most);
+    a.out_tiles = (a.K + kOuts - 1) / kOuts;
+    const unsigned grid = (unsigned)((a.out_tiles + 7) / 8 * 8 * row_blocks);
+    tile_kernel<X, GRAIN, NT, RW, OB, WO, WK><<<dim3(grid, parts), kThreads, 0, s>>>(a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (done + most >= K) break;  // and the addresses stay within their tensors
+    a.codes += most * a.code_stride;
+    a.scales = (const char*)a.scales + most * a.scale_stride * scale_size;
+    a.out = (char*)a.out + most * out_size;
+  }
+  return parts == 1 ? e : launch_parts(a, parts, s);
 }
 template <int X, int GRAIN>
 hipError_t launch_tiles(const ReadoutArgs& a, hipStream_t s) {
