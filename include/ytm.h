@@ -275,10 +275,10 @@ int ytm_collapse_bins(const uint32_t *B, int64_t rows, int64_t width, int kind, 
  * hipStream_t of the current device, NULL the default one) without waiting for it: what they
  * read must stay until the stream has passed, and results are there once it has.  They allocate
  * nothing and may be captured into a graph.  Rows may be any distance apart (strides in
- * elements, of codes in bytes; 0 in what is read: one row for all); a row's elements follow one
- * another.  Their errors are those
- * of their arguments and of the launch.  Sums are made in f32 and rounded once; results do not
- * depend on the order in which blocks run.
+ * elements, of codes in bytes; 0 in what is read: one row, or one output's codes or scales, for
+ * all); a row's elements follow one another.  Their errors are those of their arguments and of the
+ * launch.  Sums are made in f32 and rounded once; results do not depend on the order in which
+ * blocks run.
  *
  * ytm_readout: out[n][o] = sum over clauses c of x[n][c] * value(code[o][c]) * scale[o][c / group]
  * for N rows (at most 65535), C clauses (2097120) and K outputs (8388608).  x: YTM_DTYPE_BITS (clause outputs,

@@ -81,3 +81,15 @@ def test_readout_more_outputs_than_a_launch_takes():
     del out
     torch.cuda.empty_cache()
     assert wrong == 0
+
+
+@pytest.mark.parametrize("N", [1, 5, 40])
+@pytest.mark.parametrize("C", [5, 300])
+def test_readout_one_row_of_codes_or_scales_for_all(N, C):
+    """Codes or scales that are the same for all outputs (stride 0) read as if they were copies."""
+    K = 37
+    codes = torch.randint(0, 256, (K, 16 * -(-C // 32)), device="cuda", dtype=torch.uint8)
+    scales, x = torch.rand(K, -(-C // 32), device="cuda"), torch.randn(N, C, device="cuda")
+    for c, s in ((codes[:1].expand(K, -1), scales), (codes, scales[:1].expand(K, -1)),
+                 (codes[:1].expand(K, -1), scales[:1].expand(K, -1))):
+        assert torch.equal(decode.readout(x, c, s), decode.readout(x, c.contiguous(), s.contiguous()))

@@ -995,7 +995,8 @@ int ytm_readout(const void* x, int x_dtype, int64_t x_stride, int64_t N, int64_t
   if (C > 0 && ((uintptr_t)codes | (K > 1 ? (uint64_t)code_stride : 0u)) % 16)
     return fail(YTM_EINVAL, "readout codes start at multiples of 16 bytes, every output's");
   const int64_t width = x_dtype == YTM_DTYPE_BITS ? (C + 31) / 32 : C;
-  if ((K > 1 && (code_stride < (C + 31) / 32 * 16 || scale_stride < (C + group - 1) / group)) ||
+  if ((K > 1 && ((code_stride != 0 && code_stride < (C + 31) / 32 * 16) ||
+                 (scale_stride != 0 && scale_stride < (C + group - 1) / group))) ||
       (N > 1 && ((x_stride != 0 && x_stride < width) || out_stride < K)))
     return fail(YTM_EINVAL, "readout: rows overlap");
   const int64_t x_size = x_dtype == YTM_DTYPE_BITS || x_dtype == YTM_DTYPE_F32 ? 4 : 2;
