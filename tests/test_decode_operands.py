@@ -8,7 +8,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from ytm_amd import decode  # noqa: E402
+from ytm_amd import _lib, decode  # noqa: E402
 
 
 class OnGpu(torch.Tensor):
@@ -91,3 +91,21 @@ def test_wrong_shapes_without_gradients_recorded(entries, call, name, shape, gra
     with torch.no_grad(), pytest.raises(ValueError, match=f"^{name} must have shape"):
         call(**{name: on_gpu(*shape, grad=grad)})
     assert entries.launched == 0
+
+
+# The C boundary; addresses here are never read.
+P = 1 << 30
+READOUT = dict(x=P, x_dtype=7, x_stride=64, N=2, C=64, codes=2 * P, code_stride=32, scales=3 * P, scale_dtype=7,
+               scale_stride=2, group=32, K=3, out=4 * P, out_dtype=7, out_stride=3, workspace=None, workspace_bytes=0,
+               stream=None)
+
+
+def entry(name, base, **wrong):
+    return getattr(_lib.lib, name)(*{**base, **wrong}.values())
+
+
+@pytest.mark.parametrize("wrong", [dict(x_stride=1 << 62), dict(x_stride=(1 << 61) + 64), dict(x_dtype=9, x_stride=1 << 62),
+                                   dict(scale_stride=1 << 62), dict(scale_dtype=10, scale_stride=(1 << 62) + 2)])
+def test_strides_whose_bytes_pass_64_bits(wrong):
+    assert entry("ytm_readout", READOUT, **wrong) == _lib.YTM_EINVAL
+    assert b"apart" in _lib.lib.ytm_last_error()

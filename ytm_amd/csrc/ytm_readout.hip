@@ -1003,7 +1003,7 @@ int ytm_readout(const void* x, int x_dtype, int64_t x_stride, int64_t N, int64_t
   const int64_t scale_size = scale_dtype == YTM_DTYPE_F32 ? 4 : 2;
   if (N == 1) x_stride = 0;
   if (K == 1) code_stride = scale_stride = 0;
-  if (x_stride * x_size > ytm::kMaxApart || code_stride > ytm::kMaxApart || scale_stride * scale_size > ytm::kMaxApart)
+  if (x_stride > ytm::kMaxApart / x_size || code_stride > ytm::kMaxApart || scale_stride > ytm::kMaxApart / scale_size)
     return fail(YTM_EINVAL, "readout rows, codes and scales are at most 8 MiB apart");
   int64_t need = 0;
   if (int rc = ytm_readout_workspace(x_dtype, N, C, K, &need)) return rc;
