@@ -295,8 +295,8 @@ int ytm_readout(const void *x, int x_dtype, int64_t x_stride, int64_t N, int64_t
                 void *stream);
 
 /* ytm_adjust_scores: for row n (at most 65535 rows) and answer v of V (at most 8388608), with h
- * the first lengths[n] (NULL: T) entries of tokens[n] (N, T), c the number of h's entries from
- * prompt[n] on (NULL: 0) that are v:
+ * the first lengths[n] (NULL: T) entries of tokens[n] (N, T; T at most 2147483647), c the number of
+ * h's entries from prompt[n] on (NULL: 0) that are v:
  *   s = score; if v is in h: s = s > 0 ? s / repetition[n] : s * repetition[n];
  *   s = s - frequency[n] * c - presence[n] * (c > 0); s = s + bias[v];
  *   s = -inf if bit v % 32 of allowed word v / 32 is 0.

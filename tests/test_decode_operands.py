@@ -109,3 +109,13 @@ def entry(name, base, **wrong):
 def test_strides_whose_bytes_pass_64_bits(wrong):
     assert entry("ytm_readout", READOUT, **wrong) == _lib.YTM_EINVAL
     assert b"apart" in _lib.lib.ytm_last_error()
+
+
+ADJUST = dict(scores=P, dtype=7, stride=8, N=2, V=8, tokens=2 * P, token_stride=4, T=4, lengths=None, prompt=None,
+              repetition=None, frequency=None, presence=None, bias=3 * P, bias_stride=8, allowed=4 * P,
+              allowed_stride=1, out=5 * P, out_dtype=7, out_stride=8, stream=None)
+
+
+def test_history_whose_counts_pass_31_bits():
+    assert entry("ytm_adjust_scores", ADJUST, T=1 << 31, token_stride=1 << 31, tokens=1 << 40) == _lib.YTM_EINVAL
+    assert b"history" in _lib.lib.ytm_last_error()

@@ -1340,6 +1340,8 @@ int ytm_adjust_scores(const void* scores, int dtype, int64_t stride, int64_t N, 
     return fail(YTM_EINVAL, "scores are float32, float16 or bfloat16");
   if (N < 0 || V < 0 || T < 0 || N > ytm::kDecodeRows || V > ytm::kMaxScores)
     return fail(YTM_EINVAL, "adjust_scores takes at most 65535 rows of 8388608 scores");
+  if (T > INT32_MAX)  // the top bit of an answer's count says that it was given
+    return fail(YTM_EINVAL, "adjust_scores takes a history of at most 2147483647 answers");
   if (N == 0 || V == 0) return YTM_OK;
   if (!scores || !out || (T > 0 && !tokens)) return fail(YTM_EINVAL, "bad adjust_scores arguments");
   if ((N > 1 && ((stride != 0 && stride < V) || out_stride < V)) ||
