@@ -119,3 +119,10 @@ ADJUST = dict(scores=P, dtype=7, stride=8, N=2, V=8, tokens=2 * P, token_stride=
 def test_history_whose_counts_pass_31_bits():
     assert entry("ytm_adjust_scores", ADJUST, T=1 << 31, token_stride=1 << 31, tokens=1 << 40) == _lib.YTM_EINVAL
     assert b"history" in _lib.lib.ytm_last_error()
+
+
+@pytest.mark.parametrize("group", [2**64 + 32, 2**63, -32, 0, 33])
+def test_groups_that_are_none(entries, group):
+    with pytest.raises(ValueError, match="group"):
+        readout(scales=on_gpu(3, 1), group=group)
+    assert entries.launched == 0

@@ -206,7 +206,7 @@ def readout(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: i
         if clauses is not None and int(clauses) != C:
             raise ValueError(f"x must have {clauses} columns, not {C}.")
     group = int(group)
-    if group < 32 or group % 32:
+    if not 32 <= group < 1 << 63 or group % 32:  # the library takes 64 bits
         raise ValueError("group must be a multiple of 32.")
     if not (isinstance(codes, _Tensor) and codes.dtype is torch.uint8 and codes.get_device() == device
             and codes.dim() == 2 and (codes.stride(1) == 1 or codes.shape[1] < 2)):
