@@ -126,3 +126,36 @@ def test_groups_that_are_none(entries, group):
     with pytest.raises(ValueError, match="group"):
         readout(scales=on_gpu(3, 1), group=group)
     assert entries.launched == 0
+
+
+CHOOSE = dict(scores=P, dtype=7, stride=8, N=2, V=8, temperature=2 * P, top_k=3 * P, top_p=4 * P, min_p=5 * P,
+              noise=6 * P, noise_stride=8, tokens=7 * P, logprobs=8 * P, workspace=None, workspace_bytes=0, stream=None)
+PENALTIES = dict(lengths=6 * P, prompt=7 * P, repetition=8 * P, frequency=9 * P, presence=10 * P)
+SLICED = dict(V=100000, stride=100000, noise_stride=100000, workspace_bytes=1 << 30)
+MANY = dict(N=20, x_stride=64, out_stride=3, workspace=9 * P, workspace_bytes=1 << 30)
+
+
+@pytest.mark.parametrize("name,base,wrong", [
+    ("ytm_readout", READOUT, dict(out=P)), ("ytm_readout", READOUT, dict(out=P + 4 * 127)),
+    ("ytm_readout", READOUT, dict(out=P - 4 * 5)), ("ytm_readout", READOUT, dict(out=2 * P + 64)),
+    ("ytm_readout", READOUT, dict(out=3 * P + 8)),
+    ("ytm_readout", READOUT, dict(out=P + 4 * 64, x_stride=70, out_stride=70, N=3, K=7)),
+    ("ytm_readout", READOUT, {**MANY, "workspace": P}), ("ytm_readout", READOUT, {**MANY, "workspace": 2 * P + 32}),
+    ("ytm_readout", READOUT, {**MANY, "workspace": 3 * P - 16}), ("ytm_readout", READOUT, {**MANY, "out": 9 * P + 64}),
+    # scores' own place, but of another size, distance, or one row for all; then a part of them
+    ("ytm_adjust_scores", ADJUST, dict(out=P, out_dtype=9)), ("ytm_adjust_scores", ADJUST, dict(out=P, out_stride=9)),
+    ("ytm_adjust_scores", ADJUST, dict(out=P, stride=0)), ("ytm_adjust_scores", ADJUST, dict(out=P + 4)),
+    ("ytm_adjust_scores", ADJUST, dict(out=P + 4 * 15)), ("ytm_adjust_scores", ADJUST, dict(out=P - 4 * 15)),
+    ("ytm_adjust_scores", ADJUST, dict(out=P + 4 * 8, stride=15, out_stride=15)),
+    ("ytm_adjust_scores", ADJUST, dict(out=2 * P + 28)), ("ytm_adjust_scores", ADJUST, dict(out=3 * P + 60)),
+    ("ytm_adjust_scores", ADJUST, dict(out=4 * P + 4)), ("ytm_adjust_scores", ADJUST, dict(out=3 * P, bias_stride=0)),
+    *(("ytm_adjust_scores", dict(ADJUST, **PENALTIES), dict(out=p + 4)) for p in PENALTIES.values()),
+    *(("ytm_choose", CHOOSE, {w: CHOOSE[r]}) for w in ("tokens", "logprobs")
+      for r in ("scores", "temperature", "top_k", "top_p", "min_p", "noise")),
+    ("ytm_choose", CHOOSE, dict(tokens=8 * P + 4)),
+    *(("ytm_choose", dict(CHOOSE, **SLICED), dict(workspace=p)) for p in (P, 2 * P, 6 * P, 7 * P, 8 * P)),
+])
+def test_written_over_what_is_read(name, base, wrong):
+    """Blocks run in no order, so one would read what another has written."""
+    assert entry(name, base, **wrong) == _lib.YTM_EINVAL
+    assert b"overlaps" in _lib.lib.ytm_last_error()

@@ -93,3 +93,29 @@ def test_readout_one_row_of_codes_or_scales_for_all(N, C):
     for c, s in ((codes[:1].expand(K, -1), scales), (codes, scales[:1].expand(K, -1)),
                  (codes[:1].expand(K, -1), scales[:1].expand(K, -1))):
         assert torch.equal(decode.readout(x, c, s), decode.readout(x, c.contiguous(), s.contiguous()))
+
+
+def test_written_between_what_is_read():
+    """Rows of the output that lie between rows of an input are no overlap; a part of the scores is."""
+    N, V = 6, 100
+    want = torch.randn(N, V, device="cuda")
+    bias = torch.randn(V, device="cuda")
+    both = torch.zeros(N, 2 * V, device="cuda")
+    both[:, :V] = want
+    decode.adjust_scores(both[:, :V], bias=bias, out=both[:, V:])
+    assert torch.equal(both, torch.cat((want, want + bias), 1))
+    x, ones = torch.ones(N, 32, device="cuda"), torch.ones(V, 1, device="cuda")
+    both = torch.ones(N, 32 + V, device="cuda")
+    codes = torch.full((V, 16), 0x22, dtype=torch.uint8, device="cuda")
+    decode.readout(both[:, :32], codes, ones, out=both[:, 32:])
+    assert torch.equal(both, torch.cat((x, 32 * torch.ones(N, V, device="cuda")), 1))
+    half = torch.randn(N, 2 * V, device="cuda").half()
+    want = half[:, :V].bfloat16() + bias.bfloat16().float()  # in place, from one type of 16 bits to another
+    scores = half.view(torch.bfloat16)
+    scores[:, :V] = half[:, :V].bfloat16()
+    decode.adjust_scores(scores[:, :V], bias=bias.bfloat16().float(), out=half[:, :V])
+    assert torch.equal(half[:, :V], want.half())
+    big = torch.randn(2 * N, V, device="cuda")
+    for out in (big[1:N + 1], big.as_strided((N, V), (V, 1), 3), big.view(torch.float16)[:N, :V]):
+        with pytest.raises(ValueError, match="overlaps"):
+            decode.adjust_scores(big[:N], bias=bias, out=out)

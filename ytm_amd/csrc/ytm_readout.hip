@@ -1009,6 +1009,15 @@ int ytm_readout(const void* x, int x_dtype, int64_t x_stride, int64_t N, int64_t
   if (int rc = ytm_readout_workspace(x_dtype, N, C, K, &need)) return rc;
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(YTM_EINVAL, "readout: the workspace is too small or not at a multiple of 16 bytes");
+  const ytm::Rows written[] = {ytm::rows_of(out, N, K, out_stride, out_dtype == YTM_DTYPE_F32 ? 4 : 2),
+                               ytm::block_of(workspace, need)};
+  const ytm::Rows read[] = {ytm::rows_of(x, N, width, x_stride, x_size),
+                            ytm::rows_of(codes, K, (C + 31) / 32 * 16, code_stride, 1),
+                            ytm::rows_of(scales, K, (C + group - 1) / group, scale_stride, scale_size)};
+  bool overlap = ytm::share_bytes(written[0], written[1]);
+  for (const ytm::Rows& w : written)
+    for (const ytm::Rows& r : read) overlap |= ytm::share_bytes(w, r);
+  if (overlap) return fail(YTM_EINVAL, "readout: what is written overlaps what is read");
   const int64_t steps = (C + 31) / 32, units = group / 32;
   // (step + 1) * floor((2^32 - 1) / units) >> 32 is step / units while (step + 1) * units < 2^32
   const uint32_t inverse = units >= steps ? 0u : (uint32_t)(0xFFFFFFFFu / units);

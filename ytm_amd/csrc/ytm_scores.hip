@@ -1349,6 +1349,18 @@ int ytm_adjust_scores(const void* scores, int dtype, int64_t stride, int64_t N, 
       (bias && bias_stride != 0 && N > 1 && bias_stride < V) ||
       (allowed && allowed_stride != 0 && N > 1 && allowed_stride < (V + 31) / 32))
     return fail(YTM_EINVAL, "adjust_scores: rows overlap");
+  const int size = dtype == YTM_DTYPE_F32 ? 4 : 2, out_size = out_dtype == YTM_DTYPE_F32 ? 4 : 2;
+  const bool in_place = out == scores && size == out_size && (N == 1 || stride == out_stride);
+  const ytm::Rows written = ytm::rows_of(out, N, V, out_stride, out_size);
+  const ytm::Rows read[] = {ytm::rows_of(in_place ? nullptr : scores, N, V, stride, size),
+                            ytm::rows_of(tokens, N, T, token_stride, 4), ytm::rows_of(bias, N, V, bias_stride, 4),
+                            ytm::rows_of(allowed, N, (V + 31) / 32, allowed_stride, 4),
+                            ytm::block_of(lengths, 4 * N), ytm::block_of(prompt, 4 * N),
+                            ytm::block_of(repetition, 4 * N), ytm::block_of(frequency, 4 * N),
+                            ytm::block_of(presence, 4 * N)};
+  for (const ytm::Rows& r : read)
+    if (ytm::share_bytes(written, r))
+      return fail(YTM_EINVAL, "adjust_scores: out overlaps an input, and is not the scores' own place");
   ytm::AdjustArgs a{scores, stride, V, T > 0 ? tokens : nullptr, token_stride, T, lengths, prompt, repetition,
                     frequency, presence, bias, bias_stride, allowed, allowed_stride, out, out_stride};
   hipStream_t s = (hipStream_t)stream;
@@ -1383,6 +1395,16 @@ int ytm_choose(const void* scores, int dtype, int64_t stride, int64_t N, int64_t
   if (int rc = ytm_choose_workspace(dtype, N, V, &need)) return rc;
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(YTM_EINVAL, "choose: the workspace is too small or not at a multiple of 16 bytes");
+  const ytm::Rows written[] = {ytm::block_of(tokens, 4 * N), ytm::block_of(logprobs, 4 * N),
+                               ytm::block_of(workspace, need)};
+  const ytm::Rows read[] = {ytm::rows_of(scores, N, V, stride, dtype == YTM_DTYPE_F32 ? 4 : 2),
+                            ytm::rows_of(noise, N, V, noise_stride, 4), ytm::block_of(temperature, 4 * N),
+                            ytm::block_of(top_k, 4 * N), ytm::block_of(top_p, 4 * N), ytm::block_of(min_p, 4 * N)};
+  bool overlap = ytm::share_bytes(written[0], written[1]) || ytm::share_bytes(written[0], written[2]) ||
+                 ytm::share_bytes(written[1], written[2]);
+  for (const ytm::Rows& w : written)
+    for (const ytm::Rows& r : read) overlap |= ytm::share_bytes(w, r);
+  if (overlap) return fail(YTM_EINVAL, "choose: what is written overlaps what is read");
   const int slices = ytm::slices_of(dtype == YTM_DTYPE_F32 ? 4 : 2, N, V);
   const ytm::ChooseArgs a{scores, stride, (int)V, temperature, top_k, top_p, min_p, noise, noise_stride, tokens, logprobs,
                           0, slices, slices ? (int)((V + slices - 1) / slices) : 0, (ytm::Slice*)workspace};
