@@ -8,6 +8,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import torch.autograd.forward_ad as forward_ad  # noqa: E402
+
 from ytm_amd import _lib, decode  # noqa: E402
 
 
@@ -159,3 +161,21 @@ def test_written_over_what_is_read(name, base, wrong):
     """Blocks run in no order, so one would read what another has written."""
     assert entry(name, base, **wrong) == _lib.YTM_EINVAL
     assert b"overlaps" in _lib.lib.ytm_last_error()
+
+
+def dual(*shape):
+    return forward_ad.make_dual(torch.zeros(*shape), torch.ones(*shape)).as_subclass(OnGpu)
+
+
+@pytest.mark.parametrize("call,name,shape", FLOATS)
+def test_operands_with_a_tangent(entries, call, name, shape):
+    """Forward-mode derivatives would be dropped: refused, where they are recorded."""
+    with forward_ad.dual_level():
+        t = dual(*shape)
+        with torch.no_grad(), pytest.raises(ValueError, match=f"^{name} .*tangent"):
+            call(**{name: t})
+        assert entries.launched == 0
+        call()
+        with torch.inference_mode():
+            call(**{name: t})
+        assert entries.launched == 2

@@ -10,12 +10,12 @@ A model with many outputs, such as one a word of a vocabulary, answers in three 
 
 readout, adjust_scores and choose take torch tensors on one GPU and put their work on the
 current stream of that GPU without waiting for it, as torch's own operations do (they may be
-captured into a graph); pack_model, pack_weights and pack_outputs turn the framework's host arrays into such
-tensors.  Rows may be any distance apart; a row's elements follow one another.  A wrong argument
-raises TypeError or ValueError before anything is launched.  There are no gradients: clause
-outputs are bits made by automata and the codes are made from trained weights, so tensors that
-require a gradient are refused.  The formulas are at ytm_readout, ytm_adjust_scores and ytm_choose
-in include/ytm.h.
+captured into a graph); pack_model, pack_weights and pack_outputs turn the framework's host arrays
+into such tensors.  Rows may be any distance apart; a row's elements follow one another.  A wrong
+argument raises TypeError or ValueError before anything is launched.  There are no gradients:
+clause outputs are bits made by automata and the codes are made from trained weights, so tensors
+that require a gradient, or have a tangent of forward mode, are refused.  The formulas are at
+ytm_readout, ytm_adjust_scores and ytm_choose in include/ytm.h.
 """
 from __future__ import annotations
 
@@ -23,6 +23,7 @@ import ctypes
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from ._lib import DTYPE_BF16, DTYPE_BITS, DTYPE_F16, DTYPE_F32, check, lib
 
@@ -122,6 +123,14 @@ def _refuse(t, name: str, dims: tuple, dtype, shape: str, device: int) -> None:
         raise ValueError(f"{name} requires a gradient; this operator has none.")
 
 
+def _no_tangents(**operands) -> None:
+    """Refuses operands whose forward-mode derivative would be dropped."""
+    if torch._C._is_fwd_grad_enabled():
+        for name, t in operands.items():
+            if isinstance(t, _Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has a tangent; this operator has no derivative.")
+
+
 def _rows_of(t, name: str, types: dict) -> tuple[int, int, int, int]:
     """(type code, rows, width, device) of an operator's first operand."""
     if not (isinstance(t, _Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in types and not t.requires_grad
@@ -196,6 +205,8 @@ def readout(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: i
     x: bits, int32 (N, ceil(C/32)) as pack_outputs gives them, C being `clauses` (default: every
     bit); or float32, float16 or bfloat16 (N, C), outputs averaged over models or patches.
     out: where the sums go, float32, float16 or bfloat16 (default: a new float32 tensor)."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents(x=x, scales=scales, out=out)
     x_type, N, width, device = _rows_of(x, "x", _CLAUSES)
     if x_type == DTYPE_BITS:
         C = 32 * width if clauses is None else int(clauses)
@@ -245,6 +256,8 @@ def adjust_scores(scores: torch.Tensor, tokens: torch.Tensor | None = None, leng
     where answer v may be given; the others get -inf, whatever their score.
     out: where the scores go, any of the three types, `scores` itself too (default: a new float32
     tensor)."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents(scores=scores, repetition=repetition, frequency=frequency, presence=presence, bias=bias, out=out)
     dtype, N, V, device = _rows_of(scores, "scores", _FLOATS)
     T, said, token_stride = 0, None, 0
     if tokens is not None:
@@ -278,6 +291,8 @@ def choose(scores: torch.Tensor, temperature: torch.Tensor | None = None, top_k:
     noise of these, the lowest of equal ones, the log probability that of a draw among them.
     noise: float32 (N, V) or (V,), finite; standard Gumbel draws -log(-log(u)) make the answer a
     draw, None the best one.  A row without a score above -inf gets -1 and -inf."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents(scores=scores, temperature=temperature, top_p=top_p, min_p=min_p, noise=noise)
     dtype, N, V, device = _rows_of(scores, "scores", _FLOATS)
     noise, noise_stride = _matrix(noise, "noise", torch.float32, N, V, device)
     temperature = _per_row(temperature, "temperature", torch.float32, N, device)
