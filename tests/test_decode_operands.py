@@ -179,3 +179,14 @@ def test_operands_with_a_tangent(entries, call, name, shape):
         with torch.inference_mode():
             call(**{name: t})
         assert entries.launched == 2
+
+
+@pytest.mark.parametrize("call,shape", [(readout, (2, 3)), (adjust, (2, 10))])
+def test_outputs_count_as_changed(entries, call, shape):
+    """A backward pass that has kept `out` sees that it was written to; one made in inference mode has no count."""
+    out = on_gpu(*shape)
+    for n in range(3):
+        assert out._version == n
+        assert call(out=out) is out
+    with torch.inference_mode():
+        call(out=on_gpu(*shape))

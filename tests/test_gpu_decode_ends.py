@@ -95,6 +95,19 @@ def test_readout_one_row_of_codes_or_scales_for_all(N, C):
         assert torch.equal(decode.readout(x, c, s), decode.readout(x, c.contiguous(), s.contiguous()))
 
 
+def test_written_tensors_are_known_to_autograd():
+    """What a backward pass has kept is not used once an operator has written to it."""
+    scores, w = torch.randn(3, 40, device="cuda"), torch.ones(3, 40, device="cuda", requires_grad=True)
+    codes, scales = torch.full((40, 16), 0x22, dtype=torch.uint8, device="cuda"), torch.ones(40, 1, device="cuda")
+    for write in (lambda out: decode.adjust_scores(scores, out=out),
+                  lambda out: decode.readout(torch.ones(3, 32, device="cuda"), codes, scales, out=out)):
+        kept = torch.randn(3, 40, device="cuda")
+        y = (w * kept).sum()
+        write(kept)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
 def test_written_between_what_is_read():
     """Rows of the output that lie between rows of an input are no overlap; a part of the scores is."""
     N, V = 6, 100

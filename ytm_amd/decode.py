@@ -99,6 +99,7 @@ def pack_outputs(outputs: np.ndarray, device: str | torch.device = "cuda") -> to
 _Tensor = torch.Tensor
 _device_now = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream
+_changed = torch._C._increment_version  # what torch.autograd.graph.increment_version calls
 
 
 def _refuse(t, name: str, dims: tuple, dtype, shape: str, device: int) -> None:
@@ -175,6 +176,7 @@ def _result(out, shape: tuple[int, int], device: int) -> tuple[torch.Tensor, int
             and (out.stride(1) == 1 or shape[1] < 2) and not out.requires_grad):
         fits = isinstance(out, _Tensor) and tuple(out.shape) == shape
         _refuse(out, "out", (2,), _FLOATS, "" if fits else str(shape), device)
+    _changed((out,))  # for a backward pass that has kept it
     return out, _FLOATS[out.dtype]
 
 
