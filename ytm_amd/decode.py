@@ -39,10 +39,15 @@ def pack_weights(weights: np.ndarray, group: int = 32, dtype: torch.dtype = torc
     """Clause weights (C, K), as get_weights() gives them, in 4 bits for readout: codes uint8
     (K, 16 ceil(C/32)) and scales (K, ceil(C/group)) of `dtype`.  A group's largest weight becomes
     6 (a code's largest value) times its scale, the others the nearest code, ties to the smaller
-    magnitude.  Runs on the host."""
-    w = np.asarray(weights, dtype=np.float32)
+    magnitude; where that scale would be 0, it is the least positive one and all weights become the
+    nearest code.  Weights whose scale `dtype` does not hold (in float16 those above 393000) are
+    refused.  Runs on the host."""
+    with np.errstate(over="ignore"):  # refused below
+        w = np.asarray(weights, dtype=np.float32)
     if w.ndim != 2:
         raise ValueError("weights must have shape (clauses, outputs).")
+    if not np.isfinite(w).all():
+        raise ValueError("weights must be finite in float32.")
     if group < 32 or group % 32:
         raise ValueError("group must be a multiple of 32.")
     if dtype not in _FLOATS:
@@ -53,8 +58,11 @@ def pack_weights(weights: np.ndarray, group: int = 32, dtype: torch.dtype = torc
     for q in range(groups):
         largest[:, q] = np.abs(w[q * group:(q + 1) * group]).max(0)
     scales = torch.from_numpy(largest / 6.0).to(dtype)
-    # a scale that its type holds as 0 or infinity has no codes; 1 leaves zeros as they are
-    scales = torch.where((scales > 0) & torch.isfinite(scales), scales, torch.ones((), dtype=dtype))
+    if not torch.isfinite(scales).all():
+        raise ValueError(f"weights of {largest.max():g} are past what {dtype} scales hold.".replace("torch.", ""))
+    least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    scales = torch.where(scales > 0, scales, torch.tensor(least, dtype=dtype))
+    scales[torch.from_numpy(largest) == 0] = 1.0  # whatever it is, their codes are 0
     per_clause = scales.double().numpy().repeat(group, axis=1)[:, :C]
     scaled = w.T / per_clause  # in float64, so that the nearest code is
     code = np.zeros((K, padded), np.uint8)
