@@ -281,13 +281,14 @@ int ytm_collapse_bins(const uint32_t *B, int64_t rows, int64_t width, int kind, 
  * made in f32 and rounded once; results do not depend on the order in which blocks run.
  *
  * ytm_readout: out[n][o] = sum over clauses c of x[n][c] * value(code[o][c]) * scale[o][c / group]
- * for N rows (at most 65535), C clauses (2097120) and K outputs (8388608).  x: YTM_DTYPE_BITS (clause outputs,
- * (N, ceil(C/32)) words; bits past C are ignored), F32, F16 or BF16 (N, C).  codes: E2M1 floats (codes 0..7
- * are 0, 0.5, 1, 1.5, 2, 3, 4, 6; 8..15 their negatives), two a byte, the even clause in the
- * low half, 16 ceil(C/32) bytes an output, each output's at a multiple of 16 bytes (codes
- * past C are ignored).  scales: (K, ceil(C/group)), group a multiple of 32.  scales and out: F32, F16 or
- * BF16.  Rows of x, codes and scales are at most 8 MiB apart.  workspace: device memory of ytm_readout_workspace's bytes at a multiple of 16 bytes, for
- * the time of the call's work (NULL where that is 0). */
+ * for N rows (at most 65535), C clauses (2097120) and K outputs (8388608).  x: YTM_DTYPE_BITS
+ * (clause outputs, (N, ceil(C/32)) words; bits past C are ignored), F32 (whose parts below 2^-133
+ * are ignored), F16 or BF16 (N, C).  codes: E2M1 floats (codes 0..7 are 0, 0.5, 1, 1.5, 2, 3, 4, 6;
+ * 8..15 their negatives), two a byte, the even clause in the low half, 16 ceil(C/32) bytes an
+ * output, each output's at a multiple of 16 bytes (codes past C are ignored).  scales:
+ * (K, ceil(C/group)), group a multiple of 32.  scales and out: F32, F16 or BF16.  Rows of x, codes
+ * and scales are at most 8 MiB apart.  workspace: device memory of ytm_readout_workspace's bytes at
+ * a multiple of 16 bytes, for the time of the call's work (NULL where that is 0). */
 int ytm_readout_workspace(int x_dtype, int64_t N, int64_t C, int64_t K, int64_t *bytes);
 int ytm_readout(const void *x, int x_dtype, int64_t x_stride, int64_t N, int64_t C, const uint8_t *codes,
                 int64_t code_stride, const void *scales, int scale_dtype, int64_t scale_stride, int64_t group,

@@ -132,3 +132,18 @@ def test_written_between_what_is_read():
     for out in (big[1:N + 1], big.as_strided((N, V), (V, 1), 3), big.view(torch.float16)[:N, :V]):
         with pytest.raises(ValueError, match="overlaps"):
             decode.adjust_scores(big[:N], bias=bias, out=out)
+
+
+@pytest.mark.parametrize("N", [1, 20])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("dtype,least", [("float16", -24), ("bfloat16", -133), ("float32", -133)])
+def test_readout_least_values(dtype, least, group, N):
+    """Rows' subnormal values count; of float32 those down to the least of bfloat16."""
+    at = torch.arange(least, least + 24)
+    x = torch.zeros(N, 128, dtype=torch.float64)
+    x[:, torch.arange(24) * 5] = torch.exp2(at.double())
+    codes = torch.full((3, 64), 0x22, dtype=torch.uint8, device="cuda")
+    scales = torch.full((3, 128 // group), 2.0 ** (100 if least < -100 else 0), device="cuda")
+    got = decode.readout(x.to(getattr(torch, dtype)).cuda(), codes, scales, group=group)
+    want = torch.exp2(at.double()).sum() * scales[0, 0].item()  # 24 bits
+    assert bool((got.double().cpu() == want).all())

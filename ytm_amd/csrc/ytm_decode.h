@@ -43,8 +43,10 @@ constexpr int64_t kMaxScores = 1 << 23;
 // Clauses of a readout: fewer than 65536 steps of 32.
 constexpr int64_t kMaxClauses = 65535 * 32;
 
-// Bytes from a row to the next of a readout's operands: a block's rows, 192 at most, lie within 2^31.
+// Bytes from a row to the next of a readout's operands: a block's rows or outputs lie within 2^31.
 constexpr int64_t kMaxApart = 8 << 20;
+constexpr int kMaxTogether = 256;
+static_assert(kMaxApart * kMaxTogether <= (int64_t)1 << 31, "");
 
 // An operand's `n` rows of `width` bytes, each `stride` after the one before (0: one row for all).
 struct Rows {

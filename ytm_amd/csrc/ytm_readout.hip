@@ -93,7 +93,8 @@ constexpr int kOperands = operands_of(X);
 // ------------------------------------------------------------------------------- row operands
 // Eight clauses of a row as they are in memory, and as 16-bit operands: float32
 // as the sum of three bfloat16, each cut (not rounded) to one, so that nothing overflows; where
-// the first is infinite or NaN the others are zero.
+// the first is infinite or NaN the others are zero.  What a float has below 2^-133, the least bfloat16,
+// is left out.
 //
 // The load has no branch (rows have eight clauses or more), so that others can follow it before
 // it is there: a piece that would pass the row's end is taken from its last eight clauses, and moved
@@ -403,6 +404,7 @@ __global__ __launch_bounds__(kWave* RW* WO* WK) void tile_kernel(ReadoutArgs a) 
   constexpr int kTiles = NT * RW;               // of rows
   constexpr int kFrags = kOperands<X> * kTiles;  // operands of a chunk, 1 KB each
   constexpr int kOuts = kTile * OB * WO;
+  static_assert(kOuts <= kMaxTogether, "32-bit distances of codes and scales");
   constexpr int kGrains = kChunk / GRAIN;  // scales of a chunk
   // copies a wave makes, the last of them twice where they do not come out even
   constexpr int kRowCopies = (kFrags + kGroupWaves - 1) / kGroupWaves;
@@ -756,6 +758,7 @@ __global__ __launch_bounds__(kWave* WO* WK) void held_kernel(ReadoutArgs a) {
   const int end = begin + a.part_chunks < a.chunks ? begin + a.part_chunks : a.chunks;
   const int first_out = (blockIdx.x * WO + wo) * OB * kTile + l % 16;
   const int block_out = blockIdx.x * WO * OB * kTile;
+  static_assert(WO * OB * kTile <= kMaxTogether, "32-bit distances of codes and scales");
   constexpr int size = WIDE ? 4 : 2;
   const uint8_t* codes = a.codes + block_out * a.code_stride;
   const char* scales = (const char*)a.scales + block_out * a.scale_stride * size;
