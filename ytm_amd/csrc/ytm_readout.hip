@@ -941,7 +941,8 @@ hipError_t launch_rows(const ReadoutArgs& a, hipStream_t s) {
     const int parts = parts_of(kOperands<X>, a.N, a.chunks);
     if (parts > 1 && (int64_t)(a.K + 255) / 256 * parts >= 40) return launch_held<X, GRAIN, 2, 8, 1>(a, s);
   }
-  // A block's waves share its 16 outputs' clauses: 16 where there are few outputs, or 4.
+  // A block's waves share its 16 outputs' clauses: 16 where there are few outputs, or 4.  With float32 and
+  // groups of 32, 16 waves leave too few registers and 48 to 52 are spilled.
   return a.K <= 4096 ? launch_held<X, GRAIN, 1, 1, 16>(a, s) : launch_held<X, GRAIN, 1, 1, 4>(a, s);
 }
 

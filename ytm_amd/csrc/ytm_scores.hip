@@ -188,11 +188,12 @@ hipError_t launch_adjust_out(int out_dtype, const AdjustArgs& a, int64_t N, hipS
 //  - where a list overflows (thousands of equal scores): the cut's key eight bits at a time, from
 //    histograms over the whole row.
 //
-// 256 x 131072 float32 with noise: no filter 66 us (4.1 TB/s), top_k 60 (the noise of what is dropped is
-// not read), all three 85, min_p alone 155 and top_p alone 173, where most of a row passes the bound and
-// goes through the histogram.  With filters a row's steps (bound, pass, list, sort, cuts, draw) follow one
-// another, and most read little: 64 x 32001 bfloat16 takes 20 us, of which its 64 KB a row are two.
-// 1 x 10000 without filters 5.7 us, three waits for memory and the block's joins.
+// 256 x 131072 float32 with noise: no filter 67 us (4.0 TB/s), top_k 62 (the noise of what is dropped is
+// not read), all three 86 to 98 over several cards, min_p alone 160 and top_p alone 174, where most of a
+// row passes the bound and goes through the histogram.  With filters a row's steps (bound, pass, list,
+// sort, cuts, draw) follow one another, and most read little: 64 x 32001 bfloat16 takes 21 us, of which
+// its 64 KB a row are two.  1 x 10000 without filters 5.7 us, three waits for memory and the block's joins.
+// Rows of ties: 64 x 4096 scores of about 60 whole numbers 22 us, 64 x 32001, whose lists overflow, 61.
 struct ChooseArgs {
   const void* scores;
   int64_t stride;
@@ -1315,8 +1316,12 @@ hipError_t launch_choose(ChooseArgs a, int64_t N, hipStream_t s) {
   return hipSuccess;
 }
 
-// Slices of each row: none where a row has less than 128 KB or the rows alone take a quarter of the
-// 256 CUs, else 32 KB each, up to 16 (16 lists of the largest top_k sought fit one of kList).
+// Slices of each row: none where a row has less than 128 KB or the rows alone take more than a quarter
+// of the 256 CUs, else 32 KB each, up to 16 (16 lists of the largest top_k sought fit one of kList).
+// 131072 float32 with noise, us, 16 and 64 rows in slices and 65 rows a block each: no filter 17, 35 and 46;
+// top_k 21, 48 and 45; all three filters 38, 105 and 45.  A row whose min_p leaves more than a slice's list
+// holds has its slices read in vain, and so do rows of min_p alone (29, 147 and 114): up to a few dozen
+// rows slices are the faster side, at 64 only without filters.
 int slices_of(int size, int64_t N, int64_t V) {
   if (V * size < 128 * 1024 || N > 64) return 0;
   const int64_t slices = (V * size + 32 * 1024 - 1) / (32 * 1024);

@@ -1,6 +1,7 @@
 """From clause outputs to an answer, on the GPU (not in the reference).
 
-A model with many outputs, such as one a word of a vocabulary, answers in three steps:
+A model with many outputs, such as one a word of a vocabulary (up to 4096; more with weights from
+elsewhere), answers in three steps:
 
     codes, scales = decode.pack_model(tm)                          # once: weights in 4 bits
     bits = decode.pack_outputs(tm.transform(X))                    # clause outputs, packed
