@@ -277,7 +277,7 @@ int ytm_collapse_bins(const uint32_t *B, int64_t rows, int64_t width, int kind, 
  * nothing and may be captured into a graph.  Rows may be any distance apart (strides in
  * elements, of codes in bytes; 0 in what is read: one row, or one output's codes or scales, for
  * all); a row's elements follow one another.  Their errors are those of their arguments and of the
- * launch.  What they write must not overlap what they read (adjust_scores' scores apart).  Sums are
+ * launch.  What they write must not overlap what they read (adjust_scores in place apart).  Sums are
  * made in f32 and rounded once; results do not depend on the order in which blocks run.
  *
  * ytm_readout: out[n][o] = sum over clauses c of x[n][c] * value(code[o][c]) * scale[o][c / group]
@@ -303,8 +303,8 @@ int ytm_readout(const void *x, int x_dtype, int64_t x_stride, int64_t N, int64_t
  *   s = -inf if bit v % 32 of allowed word v / 32 is 0.
  * Entries outside 0..V-1 stand for no answer.  Anything NULL is left out; bias_stride or
  * allowed_stride 0: one row for all.  A lengths[n] above T counts as T.  scores and out: F32,
- * F16 or BF16, each its own; out may be scores itself, with elements of the same size and rows of the
- * same distance. */
+ * F16 or BF16, each its own; out may be scores or bias itself, with elements of the same size and rows
+ * of the same distance. */
 int ytm_adjust_scores(const void *scores, int dtype, int64_t stride, int64_t N, int64_t V, const int32_t *tokens,
                       int64_t token_stride, int64_t T, const int32_t *lengths, const int32_t *prompt,
                       const float *repetition, const float *frequency, const float *presence, const float *bias,

@@ -147,3 +147,12 @@ def test_readout_least_values(dtype, least, group, N):
     got = decode.readout(x.to(getattr(torch, dtype)).cuda(), codes, scales, group=group)
     want = torch.exp2(at.double()).sum() * scales[0, 0].item()  # 24 bits
     assert bool((got.double().cpu() == want).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", [(1, 50), (7, 9001)])
+def test_adjust_over_the_bias(N, V, dtype):
+    scores, bias = torch.randn(N, V, device="cuda").to(dtype), torch.randn(N, V, device="cuda")
+    want = scores.float() + bias
+    assert decode.adjust_scores(scores, bias=bias, out=bias) is bias
+    assert torch.equal(bias, want)

@@ -1355,17 +1355,21 @@ int ytm_adjust_scores(const void* scores, int dtype, int64_t stride, int64_t N, 
       (allowed && allowed_stride != 0 && N > 1 && allowed_stride < (V + 31) / 32))
     return fail(YTM_EINVAL, "adjust_scores: rows overlap");
   const int size = dtype == YTM_DTYPE_F32 ? 4 : 2, out_size = out_dtype == YTM_DTYPE_F32 ? 4 : 2;
-  const bool in_place = out == scores && size == out_size && (N == 1 || stride == out_stride);
+  // a block reads its own part of these before it writes it
+  const auto in_place = [&](const void* p, int64_t distance, int bytes) {
+    return out == p && out_size == bytes && (N == 1 || distance == out_stride);
+  };
   const ytm::Rows written = ytm::rows_of(out, N, V, out_stride, out_size);
-  const ytm::Rows read[] = {ytm::rows_of(in_place ? nullptr : scores, N, V, stride, size),
-                            ytm::rows_of(tokens, N, T, token_stride, 4), ytm::rows_of(bias, N, V, bias_stride, 4),
+  const ytm::Rows read[] = {ytm::rows_of(in_place(scores, stride, size) ? nullptr : scores, N, V, stride, size),
+                            ytm::rows_of(in_place(bias, bias_stride, 4) ? nullptr : bias, N, V, bias_stride, 4),
+                            ytm::rows_of(tokens, N, T, token_stride, 4),
                             ytm::rows_of(allowed, N, (V + 31) / 32, allowed_stride, 4),
                             ytm::block_of(lengths, 4 * N), ytm::block_of(prompt, 4 * N),
                             ytm::block_of(repetition, 4 * N), ytm::block_of(frequency, 4 * N),
                             ytm::block_of(presence, 4 * N)};
   for (const ytm::Rows& r : read)
     if (ytm::share_bytes(written, r))
-      return fail(YTM_EINVAL, "adjust_scores: out overlaps an input, and is not the scores' own place");
+      return fail(YTM_EINVAL, "adjust_scores: out overlaps an input, and is not the scores' or the bias's own place");
   ytm::AdjustArgs a{scores, stride, V, T > 0 ? tokens : nullptr, token_stride, T, lengths, prompt, repetition,
                     frequency, presence, bias, bias_stride, allowed, allowed_stride, out, out_stride};
   hipStream_t s = (hipStream_t)stream;

@@ -265,8 +265,8 @@ def adjust_scores(scores: torch.Tensor, tokens: torch.Tensor | None = None, leng
     the answers loses `frequency` for each time and `presence` once.  bias: float32 (N, V) or
     (V,), added.  allowed: int32 (N, ceil(V/32)) or (ceil(V/32),), bit v % 32 of word v / 32 set
     where answer v may be given; the others get -inf, whatever their score.
-    out: where the scores go, any of the three types, `scores` itself too (default: a new float32
-    tensor)."""
+    out: where the scores go, any of the three types, `scores` or `bias` itself too (default: a new
+    float32 tensor)."""
     if _forward_ad._current_level >= 0:
         _no_tangents(scores=scores, repetition=repetition, frequency=frequency, presence=presence, bias=bias, out=out)
     dtype, N, V, device = _rows_of(scores, "scores", _FLOATS)
