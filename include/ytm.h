@@ -331,6 +331,102 @@ int ytm_choose(const void *scores, int dtype, int64_t stride, int64_t N, int64_t
                const int32_t *top_k, const float *top_p, const float *min_p, const float *noise, int64_t noise_stride,
                int32_t *tokens, float *logprobs, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ---- Adapting a model's answers and learning from them (not in the reference): low-rank
+ * adapters beside ytm_readout, losses of answers with the gradient of the scores, and a step of the
+ * adapters.  Device pointers, streams, strides, errors and graphs as above.  Sums and states are made in
+ * f32 and rounded once; results do not depend on the order in which blocks run.
+ *
+ * ytm_adapt: with a = which[n] one of M (at most 65535) adapters of rank r (1 to 256),
+ *   hidden[n][j] = sum over clauses c of x[n][c] * down[a][j][c]
+ *   out[n][o] = scores[n][o] + scale * sum over j of up[a][o][j] * hidden[n][j]
+ * for N rows (at most 65535), C clauses (2097120) and K outputs (8388608); where which[n] is outside
+ * 0..M-1 the row has no adapter, out is its scores and hidden 0.  x as for ytm_readout (bits past C are
+ * ignored).  down: (M, r, C), up: (M, K, r), both of w_dtype, a distance from an adapter to the next and
+ * from a row to the next; scores, out and adapters: F32, F16 or BF16.  hidden: f32 (N, r), or NULL.  out
+ * may be scores itself, with elements of the same size and rows of the same distance.  workspace: device
+ * memory of ytm_adapt_workspace's bytes at a multiple of 16 bytes, for the time of the call's work. */
+int ytm_adapt_workspace(int64_t N, int64_t C, int64_t M, int64_t r, int64_t *bytes);
+int ytm_adapt(const void *scores, int dtype, int64_t stride, int64_t N, int64_t K, const void *x, int x_dtype,
+              int64_t x_stride, int64_t C, const void *down, int64_t down_adapter, int64_t down_rank, const void *up,
+              int64_t up_adapter, int64_t up_output, int w_dtype, int64_t M, int64_t r, const int32_t *which,
+              float scale, float *hidden, int64_t hidden_stride, void *out, int out_dtype, int64_t out_stride,
+              void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ytm_adapt_gradient: of a loss whose gradient by out is grad (N, K), with hidden as ytm_adapt gave it:
+ *   d_up[a][o][j] = scale * sum over rows n of a of grad[n][o] * hidden[n][j]
+ *   d_down[a][j][c] = sum over rows n of a of x[n][c] * scale * sum over o of grad[n][o] * up[a][o][j]
+ * 0 for adapters that no row names.  (The gradient by scores is grad itself.)  d_down (M, r, C) and d_up
+ * (M, K, r) are of w_dtype; grad F32, F16 or BF16.  Bounds and workspace as for ytm_adapt. */
+int ytm_adapt_gradient_workspace(int64_t N, int64_t K, int64_t M, int64_t r, int64_t *bytes);
+int ytm_adapt_gradient(const void *grad, int dtype, int64_t stride, int64_t N, int64_t K, const void *x, int x_dtype,
+                       int64_t x_stride, int64_t C, const void *up, int64_t up_adapter, int64_t up_output, int w_dtype,
+                       int64_t M, int64_t r, const int32_t *which, float scale, const float *hidden,
+                       int64_t hidden_stride, void *d_down, int64_t d_down_adapter, int64_t d_down_rank, void *d_up,
+                       int64_t d_up_adapter, int64_t d_up_output, void *workspace, int64_t workspace_bytes,
+                       void *stream);
+
+/* Both losses take N rows (at most 65535) of V scores (8388608), F32, F16 or BF16, the answer tokens[n]
+ * of each, and a temperature (NULL: 1; 0 or less counts as 1, less than the smallest normal float or NaN
+ * as that).  A score that is NaN counts as -inf, one of +inf as the largest float.  With p = softmax(score
+ * / temperature) and lp = log p[tokens[n]], grad (F32, F16 or BF16; scores itself too, with elements of the
+ * same size and rows of the same distance) becomes the gradient of the losses' sum by the scores.  A
+ * row whose answer is outside 0..V-1 or has a score of -inf is left out: its lp and loss are 0, and so is
+ * its gradient.
+ *
+ * ytm_policy_loss: with ratio = exp(lp - old[n]), d = reference[n] - lp,
+ *   losses[n] = weights[n] * (kl * (exp(d) - d - 1)
+ *               - min(ratio * advantages[n], clamp(ratio, 1 - low, 1 + high) * advantages[n]))
+ * (where the two are equal, the first counts); weights NULL: 1 / N; reference NULL: kl must be 0.
+ * logprobs[n] = lp.
+ *
+ * ytm_preference_loss: rows starts[s] .. starts[s + 1] - 1 are sequence s of 2 pairs (at most 65535),
+ * starts (2 pairs + 1) not falling, between 0 and N (elsewhere cut to that; where they fall,
+ * results are unspecified).  With l[s] the sum of its rows' lp, of pair p
+ *   m = beta * ((l[2p] - reference[2p]) - (l[2p+1] - reference[2p+1]))
+ *   losses[p] = ((1 - smoothing) * log(1 + exp(-m)) + smoothing * log(1 + exp(m))) / pairs
+ * logprobs[s] = l[s].  Rows of no sequence are left out.
+ *
+ * workspace: device memory of the _workspace's bytes at a multiple of 16 bytes, for the time of the
+ * call's work (NULL where that is 0). */
+int ytm_policy_loss_workspace(int64_t N, int64_t V, int64_t *bytes);
+int ytm_policy_loss(const void *scores, int dtype, int64_t stride, int64_t N, int64_t V, const int32_t *tokens,
+                    const float *old, const float *advantages, const float *reference, float kl, float low, float high,
+                    const float *weights, const float *temperature, float *losses, float *logprobs, void *grad,
+                    int grad_dtype, int64_t grad_stride, void *workspace, int64_t workspace_bytes, void *stream);
+int ytm_preference_loss_workspace(int64_t N, int64_t V, int64_t *bytes);
+int ytm_preference_loss(const void *scores, int dtype, int64_t stride, int64_t N, int64_t V, const int32_t *tokens,
+                        const int32_t *starts, int64_t pairs, const float *reference, float beta, float smoothing,
+                        const float *temperature, float *losses, float *logprobs, void *grad, int grad_dtype,
+                        int64_t grad_stride, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ytm_adamw: a step of AdamW on n (at most 16777216) tensors at once.  Of tensor i it is the step k =
+ * ++steps[i], for each element with gradient g
+ *   m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2
+ *   p = (1 - rate decay) p - rate / (1 - beta1^k) * m / (sqrt(v / (1 - beta2^k)) + eps)
+ * and none where active[i] (NULL: all are) is 0.  rate_at (or NULL) has the rate instead of `rate`.
+ * steps, active, rate_at: device.  The tensors are in a table
+ * that ytm_adamw_table writes to host memory (NULL: says only its bytes and its chunks, which ytm_adamw
+ * takes) and that the caller copies to device memory at a multiple of 16 bytes; ytm_adamw writes to it,
+ * so two steps of one table follow each other.  parameter: F32, F16 or BF16; gradient: of the same type or
+ * F32.  With bits 32 first (m) and second (v) are f32.  With bits 8 they are E4M3 floats (sign, four bits
+ * of exponent with bias 7, three of fraction, 127 a NaN) times a power of two for each 256 elements in a
+ * row, m itself and v as its root.  What is stored in fewer bits than f32 is rounded up or down at random,
+ * with the chances that keep the mean of parameters, of m and of v, from `seed`, the step and the
+ * element's place (each tensor before it counts as a multiple of 256 long); a v above 0 stays above 0, what is
+ * not finite becomes NaN in 8 bits.  The operands of different tensors must not overlap. */
+typedef struct {
+  void *parameter;
+  const void *gradient;
+  void *first, *second;
+  float *first_scales, *second_scales; /* bits 8: (ceil(count / 256)) each */
+  int64_t count;
+  int32_t parameter_dtype, gradient_dtype;
+} ytm_adamw_tensor;
+int ytm_adamw_table(const ytm_adamw_tensor *tensors, int64_t n, int bits, void *table, int64_t *bytes,
+                    int64_t *chunks);
+int ytm_adamw(void *table, int64_t n, int64_t chunks, int bits, int64_t *steps, const uint8_t *active, double rate,
+              const float *rate_at, double beta1, double beta2, double eps, double decay, uint32_t seed, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

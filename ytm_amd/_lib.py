@@ -105,7 +105,34 @@ SIGNATURES = {
                                          _I64, _P, _I64, _P, ctypes.c_int, _I64, _P]),
     "ytm_choose_workspace": (ctypes.c_int, [ctypes.c_int, _I64, _I64, ctypes.POINTER(_I64)]),
     "ytm_choose": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _P]),
+    "ytm_adapt_workspace": (ctypes.c_int, [_I64, _I64, _I64, _I64, ctypes.POINTER(_I64)]),
+    "ytm_adapt": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, ctypes.c_int, _I64, _I64, _P, _I64, _I64, _P,
+                                 _I64, _I64, ctypes.c_int, _I64, _I64, _P, ctypes.c_float, _P, _I64, _P, ctypes.c_int,
+                                 _I64, _P, _I64, _P]),
+    "ytm_adapt_gradient_workspace": (ctypes.c_int, [_I64, _I64, _I64, _I64, ctypes.POINTER(_I64)]),
+    "ytm_adapt_gradient": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, ctypes.c_int, _I64, _I64, _P, _I64,
+                                          _I64, ctypes.c_int, _I64, _I64, _P, ctypes.c_float, _P, _I64, _P, _I64, _I64,
+                                          _P, _I64, _I64, _P, _I64, _P]),
+    "ytm_policy_loss_workspace": (ctypes.c_int, [_I64, _I64, ctypes.POINTER(_I64)]),
+    "ytm_policy_loss": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, ctypes.c_float,
+                                       ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _P, ctypes.c_int, _I64, _P, _I64,
+                                       _P]),
+    "ytm_preference_loss_workspace": (ctypes.c_int, [_I64, _I64, ctypes.POINTER(_I64)]),
+    "ytm_preference_loss": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _I64, _P, ctypes.c_float,
+                                           ctypes.c_float, _P, _P, _P, _P, ctypes.c_int, _I64, _P, _I64, _P]),
+    "ytm_adamw_table": (ctypes.c_int, [_P, _I64, ctypes.c_int, _P, ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
+    "ytm_adamw": (ctypes.c_int, [_P, _I64, _I64, ctypes.c_int, _P, _P, ctypes.c_double, _P, ctypes.c_double,
+                                 ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_uint32, _P]),
 }
+
+
+class AdamWTensor(ctypes.Structure):
+    """ytm_adamw_tensor"""
+
+    _fields_ = [("parameter", _P), ("gradient", _P), ("first", _P), ("second", _P), ("first_scales", _P),
+                ("second_scales", _P), ("count", _I64), ("parameter_dtype", ctypes.c_int32),
+                ("gradient_dtype", ctypes.c_int32)]
+
 
 # Element types of the answering operators (YTM_DTYPE_* of include/ytm.h).
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_BITS = 7, 9, 10, 11

@@ -113,7 +113,7 @@ _changed = torch._C._increment_version  # what torch.autograd.graph.increment_ve
 
 def _refuse(t, name: str, dims: tuple, dtype, shape: str, device: int) -> None:
     """Raises what is wrong with operand t; `shape` says what its shape must be where it does not fit.
-    Nothing where t only requires a gradient and none is recorded."""
+    Nothing where t only requires a gradient and none is recorded, or is empty with odd strides."""
     if not isinstance(t, _Tensor):
         raise TypeError(f"{name} must be a torch tensor.")
     if not t.is_cuda:
@@ -125,7 +125,7 @@ def _refuse(t, name: str, dims: tuple, dtype, shape: str, device: int) -> None:
     if dtype is not None and t.dtype not in (dtype if isinstance(dtype, (tuple, dict)) else (dtype,)):
         names = dtype if isinstance(dtype, (tuple, dict)) else (dtype,)
         raise TypeError(f"{name} must be {' or '.join(str(d).removeprefix('torch.') for d in names)}, not {t.dtype}.")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
         raise ValueError(f"{name}'s rows must be contiguous.")
     if shape:
         raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}.")
