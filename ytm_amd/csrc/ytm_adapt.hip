@@ -13,6 +13,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ytm_decode.h"
 #include "ytm_internal.h"
 
@@ -55,9 +57,13 @@ struct AdaptArgs {
   int64_t d_up_adapter, d_up_output;
   int windows, slots;     // slots: blocks that share a window's segments
   int parts, part_steps;  // of a sum over clauses or outputs
-  float* part;            // [parts][N in order][r]
-  float* back;            // [N in order][r]
-  int32_t* order;         // [N] rows, then [N] keys, of more than kInline rows
+  int padded;             // r, to whole tiles
+  float* part;            // [parts][N in order][padded]
+  float* back;            // [back_parts][N in order][padded]
+  int back_parts;
+  uint32_t* order;  // [N], of more than kInline rows
+  int w_dtype;
+  int first;  // adapter of a launch of gradients
 };
 
 // ----------------------------------------------------------------------------------- elements
@@ -77,24 +83,17 @@ struct Element<YTM_DTYPE_BF16> {
 };
 
 // E values in a row at p, of which `left` are there, as float; the others are 0.
-template <int E, typename T>
+// WHOLE: all are, which leaves no branch, so that other loads can follow before these are there.
+template <int E, bool WHOLE = false, typename T>
 __device__ __forceinline__ void load_floats(const T* p, int left, float (&v)[E]) {
   T raw[E];
-  if (left >= E) {
+  if (WHOLE || left >= E) {
     __builtin_memcpy(raw, p, sizeof raw);
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = to_float(raw[e]);
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = e < left ? to_float(p[e]) : 0.0f;
-  }
-}
-template <int E>
-__device__ __forceinline__ void load_floats(const void* p, int64_t at, int dtype, int left, float (&v)[E]) {
-  switch (dtype) {
-    case YTM_DTYPE_F16: load_floats<E>((const f16*)p + at, left, v); break;
-    case YTM_DTYPE_BF16: load_floats<E>((const bf16*)p + at, left, v); break;
-    default: load_floats<E>((const float*)p + at, left, v); break;
   }
 }
 template <int E, typename T>
@@ -120,362 +119,600 @@ __device__ __forceinline__ void store_floats(void* p, int64_t at, int dtype, int
 }
 
 // Clauses c .. c + E - 1 of row n (E divides 32, c a multiple of E), 0 past the last clause.
-template <int X, int E>
+template <int X, int E, bool WHOLE = false>
 __device__ __forceinline__ void load_clauses(const AdaptArgs& a, int64_t n, int c, float (&v)[E]) {
   const int left = a.C - c;
   if constexpr (X == YTM_DTYPE_BITS) {
-    const uint32_t word = left > 0 ? ((const uint32_t*)a.x)[n * a.x_stride + c / 32] >> c % 32 : 0u;
+    const uint32_t word = WHOLE || left > 0 ? ((const uint32_t*)a.x)[n * a.x_stride + c / 32] >> c % 32 : 0u;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = e < left ? (float)(word >> e & 1u) : 0.0f;
+    for (int e = 0; e < E; ++e) v[e] = WHOLE || e < left ? (float)(word >> e & 1u) : 0.0f;
   } else {
-    load_floats<E>((const typename Element<X>::type*)a.x + n * a.x_stride + c, left, v);
+    load_floats<E, WHOLE>((const typename Element<X>::type*)a.x + n * a.x_stride + c, left, v);
   }
 }
+
+// What is loaded before stays before the products after it.
+__device__ __forceinline__ void loads_first() { __builtin_amdgcn_sched_barrier(0); }
 
 __device__ __forceinline__ v4f product(float a, float b, v4f d) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, d, 0, 0, 0);
 }
 
 // ---------------------------------------------------------------------------------- the order
-// A row's place among the rows is the number of those of a smaller key, or of the same key before it;
-// the key is the row's adapter, M where it has none.
-__device__ __forceinline__ int key_of(const AdaptArgs& a, int n) {
+// A row's place among the rows is the number of smaller codes, a code being the row's adapter (M where it
+// has none) above its number; both have 16 bits.
+__device__ __forceinline__ uint32_t code_of(const AdaptArgs& a, int n) {
   const uint32_t w = (uint32_t)a.which[n];
-  return w < (uint32_t)a.M ? (int)w : a.M;
+  return (w < (uint32_t)a.M ? w : (uint32_t)a.M) << 16 | (uint32_t)n;
+}
+__device__ __forceinline__ int key_of(uint32_t code) { return (int)(code >> 16); }
+__device__ __forceinline__ int row_of(uint32_t code) { return (int)(code & 0xFFFFu); }
+
+// How many of four codes are smaller.
+__device__ __forceinline__ int smaller(uint4 v, uint32_t mine) {
+  return (v.x < mine) + (v.y < mine) + (v.z < mine) + (v.w < mine);
 }
 
-__global__ __launch_bounds__(kThreads) void order_kernel(AdaptArgs a) {
-  __shared__ int keys[4 * kThreads];
-  const int n = blockIdx.x * kThreads + threadIdx.x;
-  const int mine = n < a.N ? key_of(a, n) : 0;
+// More than kInline rows: a block places 64 of them, its waves share the codes that they are compared with.
+constexpr int kOrderThreads = 1024;
+__global__ __launch_bounds__(kOrderThreads) void order_kernel(AdaptArgs a) {
+  __shared__ uint4 codes[kOrderThreads];
+  __shared__ int places[kOrderThreads / kWave][kWave];
+  const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int n = blockIdx.x * kWave + l;
+  const uint32_t mine = n < a.N ? code_of(a, n) : 0u;
   int place = 0;
-  for (int first = 0; first < a.N; first += 4 * kThreads) {
-    __syncthreads();
+  for (int first = 0; first < a.N; first += 4 * kOrderThreads) {
+    uint32_t v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int m = first + q * kThreads + threadIdx.x;
-      keys[q * kThreads + threadIdx.x] = m < a.N ? key_of(a, m) : INT32_MAX;
+      const int m = first + 4 * threadIdx.x + q;
+      v[q] = m < a.N ? code_of(a, m) : UINT32_MAX;
     }
     __syncthreads();
-#pragma unroll 8
-    for (int m = 0; m < 4 * kThreads; ++m) {
-      const int key = keys[m];
-      place += key < mine || (key == mine && first + m < n);
-    }
+    codes[threadIdx.x] = uint4{v[0], v[1], v[2], v[3]};
+    __syncthreads();
+    const int left = (a.N - first + 3) / 4, last = left < kOrderThreads ? left : kOrderThreads;
+#pragma unroll 4
+    for (int m = wave; m < last; m += kOrderThreads / kWave) place += smaller(codes[m], mine);
   }
-  if (n < a.N) {
-    a.order[place] = n;
-    a.order[a.N + place] = mine;
-  }
+  places[wave][l] = place;
+  __syncthreads();
+  if (wave > 0 || n >= a.N) return;
+  place = 0;
+#pragma unroll
+  for (int w = 0; w < kOrderThreads / kWave; ++w) place += places[w][l];
+  a.order[place] = mine;
 }
 
-// `count` rows (at most kInline) of the order from `first` on, and their keys.
-template <int COUNT>
-struct Taken {
-  int row[COUNT], key[COUNT];
-  int keys[kInline];  // of all rows
+// What a block knows of the order: with at most kInline rows all of it, made by itself.
+struct Order {
+  uint32_t code[kInline];
+  __attribute__((aligned(16))) uint32_t all[kInline];
 
-  __device__ __forceinline__ void take(const AdaptArgs& a, int first) {
-    if (a.N > kInline) {
-      for (int i = threadIdx.x; i < COUNT; i += kThreads) {
-        const bool there = first + i < a.N;
-        row[i] = there ? a.order[first + i] : -1;
-        key[i] = there ? a.order[a.N + first + i] : INT32_MAX;
-      }
-    } else {
-      const int n = threadIdx.x;
-      const int mine = n < a.N ? key_of(a, n) : INT32_MAX;
-      keys[n] = mine;
-      for (int i = n; i < COUNT; i += kThreads) {
-        row[i] = -1;
-        key[i] = INT32_MAX;
-      }
-      __syncthreads();
-      int place = 0;
-#pragma unroll 4
-      for (int m = 0; m < a.N; ++m) place += keys[m] < mine || (keys[m] == mine && m < n);
-      if (n < a.N && place >= first && place < first + COUNT) {
-        row[place - first] = n;
-        key[place - first] = mine;
-      }
+  __device__ __forceinline__ void make(const AdaptArgs& a) {
+    const int n = threadIdx.x;
+    const uint32_t mine = n < a.N ? code_of(a, n) : UINT32_MAX;
+    if (n < kInline) {
+      all[n] = mine;
+      code[n] = UINT32_MAX;
     }
     __syncthreads();
+    int place = 0;
+#pragma unroll 4
+    for (int m = 0; m < (a.N + 3) / 4; ++m) place += smaller(((const uint4*)all)[m], mine);
+    if (n < a.N) code[place] = mine;
+    __syncthreads();
+  }
+  // the codes of a window, at code[0 ..]; past the last row none
+  __device__ __forceinline__ const uint32_t* window(const AdaptArgs& a, int w) {
+    if (a.N <= kInline) {
+      make(a);
+      return code + w * kTile;
+    }
+    if (threadIdx.x < kTile) {
+      const int i = w * kTile + threadIdx.x;
+      code[threadIdx.x] = i < a.N ? a.order[i] : UINT32_MAX;
+    }
+    __syncthreads();
+    return code;
+  }
+  // where adapter `key` begins: the number of codes of smaller keys; after make() where the block makes it
+  __device__ __forceinline__ int begin(const AdaptArgs& a, int key) const {
+    const uint32_t* from = a.N <= kInline ? code : a.order;
+    const uint64_t least = (uint64_t)key << 16;
+    int low = 0, high = a.N;
+    while (low < high) {
+      const int mid = (low + high) / 2;
+      if (from[mid] < least)
+        low = mid + 1;
+      else
+        high = mid;
+    }
+    return low;
   }
 };
 
-// Where adapter `key` begins in the order of all rows: the number of smaller keys.
-__device__ __forceinline__ int begin_of(const AdaptArgs& a, int key, const int* keys) {
-  if (a.N <= kInline) {
-    int before = 0;
-    for (int m = 0; m < a.N; ++m) before += keys[m] < key;
-    return before;
-  }
-  int low = 0, high = a.N;
-  while (low < high) {
-    const int mid = (low + high) / 2;
-    if (a.order[a.N + mid] < key)
-      low = mid + 1;
-    else
-      high = mid;
-  }
-  return low;
-}
-
 // The segments of a window that block `slot` of `slots` takes: body(key, first place, end).
 template <typename Body>
-__device__ __forceinline__ void segments(const int* key, int slot, int slots, Body body) {
-  for (int i = 0, s = 0; i < kTile && key[i] != INT32_MAX; ++s) {
+__device__ __forceinline__ void segments(const uint32_t* code, int slot, int slots, Body body) {
+  for (int i = 0, s = 0; i < kTile && code[i] != UINT32_MAX; ++s) {
+    const int key = __builtin_amdgcn_readfirstlane(key_of(code[i]));
     int end = i + 1;
-    while (end < kTile && key[end] == key[i]) ++end;
-    if (s % slots == slot) body(__builtin_amdgcn_readfirstlane(key[i]), i, end);
+    while (end < kTile && code[end] != UINT32_MAX && key_of(code[end]) == key) ++end;
+    end = __builtin_amdgcn_readfirstlane(end);
+    if (s % slots == slot) body(key, i, end);
     i = end;
   }
 }
 
+// Of each wave's sums of RT tiles of ranks and 16 rows the block's, written to the part's place: rank
+// RT c + t of tile t's column c, so that a lane's are in a row.
+template <int RT>
+__device__ __forceinline__ void write_part(const AdaptArgs& a, int p, int window, int first, int end, int ranks,
+                                           const v4f (&sum)[RT], v4f (*join)[RT][kWave]) {
+  const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < RT; ++t) join[wave][t][l] = sum[t];
+  __syncthreads();
+  // wave w takes row 4 (l / 16) + w of each tile
+  const int i = l / kTile * 4 + wave, j = ranks + l % kTile * RT;
+  if (i < first || i >= end) return;
+  float v[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    v[t] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v[t] += ((const float*)&join[w][t][l])[wave];
+    if (j + t >= a.r) v[t] = 0.0f;  // not another rank's infinity
+  }
+  __builtin_memcpy(a.part + ((int64_t)p * a.N + window * kTile + i) * a.padded + j, v, sizeof v);
+}
+
 // ------------------------------------------------------------------------------------ forward
-// Sums over a part of the clauses of 16 rows with 16 RT ranks of a segment's adapter.  Lane l has row and
-// rank l % 16 and eight clauses in a row of every 32, one of them a product; a block's waves take 32 clauses in
-// turn and are joined in LDS.
+// Clauses and weights of one 16-bit type (bits have any) are multiplied as they are, 32 clauses a product,
+// each exact in f32; all else as f32, 4 clauses a product.
+template <int X, int W>
+constexpr bool kHalves = W != YTM_DTYPE_F32 && (X == W || X == YTM_DTYPE_BITS);
+template <int X, int W>
+constexpr int kChunk = kHalves<X, W> ? 128 : 64;  // clauses that a wave's lanes load at once, a quarter a lane
+
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+template <int W>
+__device__ __forceinline__ v4f half_product(v4u x, v4u w, v4f d) {
+  if (W == YTM_DTYPE_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, x), __builtin_bit_cast(v8h, w), d, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x), __builtin_bit_cast(v8bf, w), d, 0, 0, 0);
+}
+
+// Eight 16-bit values at p, of which `left` are there.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ v4u load_halves(const T* p, int left) {
+  v4u r;
+  if (WHOLE || left >= 8) {
+    __builtin_memcpy(&r, p, sizeof r);
+    return r;
+  }
+  uint16_t v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = 0;
+    if (e < left) __builtin_memcpy(&v[e], p + e, 2);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) r[q] = (uint32_t)v[2 * q + 1] << 16 | v[2 * q];
+  return r;
+}
+
+// Sums over a part of the clauses of 16 rows with 16 RT ranks of a segment's adapter.  Lane l has row l % 16, the
+// ranks RT (l % 16) + t and a quarter of a chunk's clauses in a row, all loaded before the first product; a
+// block's waves take chunks in turn.
 template <int X, int W, int RT>
 __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
   typedef typename Element<W>::type T;
-  __shared__ Taken<kTile> taken;
-  __shared__ v4f join[kWaves - 1][RT][kWave];
+  constexpr int kOwn = kChunk<X, W> / 4;
+  __shared__ Order order;
+  __shared__ v4f join[kWaves][RT][kWave];
   const int slot = blockIdx.x % a.slots, window = blockIdx.x / a.slots, p = blockIdx.y, ranks = blockIdx.z * RT * kTile;
-  taken.take(a, window * kTile);
+  const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int row = taken.row[l % kTile] < 0 ? taken.row[0] : taken.row[l % kTile];
-  segments(taken.key, slot, a.slots, [&](int key, int first, int end) {
+  const int64_t row = row_of(code[l % kTile] == UINT32_MAX ? code[0] : code[l % kTile]);
+  segments(code, slot, a.slots, [&](int key, int first, int end) {
     if (key == a.M) return;
-    const T* down = (const T*)a.down + key * a.down_adapter;
     v4f sum[RT];
+    const T* down[RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) sum[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const int steps = (a.C + 31) / 32, last = (p + 1) * a.part_steps < steps ? (p + 1) * a.part_steps : steps;
-    for (int step = p * a.part_steps + wave; step < last; step += kWaves) {
-      const int c = step * 32 + l / kTile * 8;
-      float x[8], w[RT][8];
-      load_clauses<X, 8>(a, row, c, x);
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const int j = ranks + t * kTile + l % kTile;
-        load_floats<8>(down + (j < a.r ? j : a.r - 1) * a.down_rank + c, a.C - c, w[t]);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int t = 0; t < RT; ++t) sum[t] = product(x[e], w[t][e], sum[t]);
+    for (int t = 0; t < RT; ++t) {
+      sum[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      const int j = ranks + l % kTile * RT + t;
+      down[t] = (const T*)a.down + key * a.down_adapter + (int64_t)(j < a.r ? j : a.r - 1) * a.down_rank;
     }
-    if (wave > 0)
+    // a chunk's operands, as they are in memory
+    struct Operands {
+      v4u x[kHalves<X, W> ? 4 : 1], w[kHalves<X, W> ? RT : 1][4];
+      uint32_t word;
+      float fx[kHalves<X, W> ? 1 : 4][4], fw[kHalves<X, W> ? 1 : RT][4][4];
+    };
+    const auto load = [&](int at, auto all, Operands& o) {
+      constexpr bool kWhole = decltype(all)::value;
+      const int c = at * kChunk<X, W> + l / kTile * kOwn;
+      if constexpr (kHalves<X, W>) {
+        if constexpr (X == YTM_DTYPE_BITS) {
+          const int left = a.C - c;
+          o.word = kWhole || left > 0 ? ((const uint32_t*)a.x)[row * a.x_stride + c / 32] : 0u;
+          if (!kWhole && left > 0 && left < 32) o.word &= (1u << left) - 1u;
+        } else {
 #pragma unroll
-      for (int t = 0; t < RT; ++t) join[wave - 1][t][l] = sum[t];
-    __syncthreads();
-    if (wave == 0) {
+          for (int i = 0; i < 4; ++i)
+            o.x[i] = load_halves<T, kWhole>((const T*)a.x + row * a.x_stride + c + 8 * i, a.C - c - 8 * i);
+        }
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        for (int w = 0; w < kWaves - 1; ++w) sum[t] += join[w][t][l];
-        const int j = ranks + t * kTile + l % kTile;
+        for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int i = l / kTile * 4 + q;
-          if (i >= first && i < end && j < a.r) a.part[((int64_t)p * a.N + window * kTile + i) * a.r + j] = sum[t][q];
+          for (int i = 0; i < 4; ++i) o.w[t][i] = load_halves<T, kWhole>(down[t] + c + 8 * i, a.C - c - 8 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          load_clauses<X, 4, kWhole>(a, row, c + 4 * i, o.fx[i]);
+#pragma unroll
+          for (int t = 0; t < RT; ++t) load_floats<4, kWhole>(down[t] + c + 4 * i, a.C - c - 4 * i, o.fw[t][i]);
         }
       }
+    };
+    const auto multiply = [&](const Operands& o) {
+      if constexpr (kHalves<X, W>) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v4u x = o.x[i];
+          if constexpr (X == YTM_DTYPE_BITS) {
+            constexpr uint32_t one = W == YTM_DTYPE_F16 ? 0x3C00u : 0x3F80u;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t two = o.word >> (8 * i + 2 * q);
+              x[q] = ((two & 1u) | (two & 2u) << 15) * one;
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < RT; ++t) sum[t] = half_product<W>(x, o.w[t][i], sum[t]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) sum[t] = product(o.fx[i][e], o.fw[t][i][e], sum[t]);
+      }
+    };
+    const int whole = a.C / kChunk<X, W>, last = (p + 1) * a.part_steps < whole ? (p + 1) * a.part_steps : whole;
+    int at = p * a.part_steps + wave;
+    if (at < last) {
+      Operands now;
+      load(at, std::true_type{}, now);
+      for (; at + kWaves < last; at += kWaves) {
+        Operands next;
+        load(at + kWaves, std::true_type{}, next);
+        loads_first();
+        multiply(now);
+        now = next;
+      }
+      multiply(now);
     }
-    __syncthreads();
+    if (whole * kChunk<X, W> < a.C && whole / a.part_steps == p && whole % kWaves == wave) {
+      Operands end_of_row;
+      load(whole, std::false_type{}, end_of_row);
+      multiply(end_of_row);
+    }
+    write_part<RT>(a, p, window, first, end, ranks, sum, join);
   });
 }
 
-// 64 outputs a wave of 16 rows.  Lane l has output l % 16 of a tile and row l % 16, and four ranks of every
-// 16; it gets sums of four outputs in a row of row l % 16.
-template <int W>
+// 64 outputs a wave at a time of 16 rows.  Lane l has output l % 16 of a tile and row l % 16, and four ranks of
+// every 16; it gets sums of four outputs in a row of row l % 16.
+template <int W, int S>
 __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
   typedef typename Element<W>::type T;
+  typedef typename Element<S>::type In;
   constexpr int kTiles = 4;
-  __shared__ Taken<kTile> taken;
-  __shared__ float hidden[kTile][kMaxRank + 4];
+  __shared__ Order order;
+  __shared__ __attribute__((aligned(16))) float hidden[kTile][kMaxRank + 4];
   const int slot = blockIdx.x % a.slots, window = blockIdx.x / a.slots;
-  taken.take(a, window * kTile);
+  const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int outputs = (blockIdx.y * kWaves + wave) * kTiles * kTile;
-  const int padded = (a.r + kTile - 1) / kTile * kTile;
-  segments(taken.key, slot, a.slots, [&](int key, int first, int end) {
-    for (int i = threadIdx.x; i < kTile * padded; i += kThreads) {
-      const int at = i / padded, j = i % padded;
-      float sum = 0.0f;
-      if (at >= first && at < end && j < a.r) {
-        if (key < a.M)
-          for (int p = 0; p < a.parts; ++p) sum += a.part[((int64_t)p * a.N + window * kTile + at) * a.r + j];
-        if (a.hidden && blockIdx.y == 0) a.hidden[taken.row[at] * a.hidden_stride + j] = sum;
+  const int at = l % kTile;
+  segments(code, slot, a.slots, [&](int key, int first, int end) {
+    // the parts' sums, in a row of four ranks a thread
+    __syncthreads();
+    for (int i = threadIdx.x; i < kTile * a.padded / 4; i += kThreads) {
+      const int n = i / (a.padded / 4), j = i % (a.padded / 4) * 4;
+      float4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+      if (n >= first && n < end && key < a.M) {
+        const float* from = a.part + ((int64_t)window * kTile + n) * a.padded + j;
+        const int64_t part = (int64_t)a.N * a.padded;
+        for (int p = 0; p < a.parts; p += 8) {
+          float4 v[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = *(const float4*)(from + (p + q < a.parts ? p + q : p) * part);
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (p + q < a.parts) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
+        }
       }
-      hidden[at][j] = sum;
+      *(float4*)&hidden[n][j] = sum;
+      if (a.hidden && blockIdx.y == 0 && n >= first && n < end) {
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        store_floats<4>(a.hidden + row_of(code[n]) * a.hidden_stride + j, a.r - j, v);
+      }
     }
     __syncthreads();
-    v4f sum[kTiles];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) sum[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    if (key < a.M) {
-      const T* up = (const T*)a.up + key * a.up_adapter;
-      for (int j = l / kTile * 4; j < padded; j += kTile) {
-        float h[4], w[kTiles][4];
-        __builtin_memcpy(h, &hidden[l % kTile][j], sizeof h);
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          const int o = outputs + t * kTile + l % kTile;
-          load_floats<4>(up + (o < a.K ? o : a.K - 1) * a.up_output + j, o < a.K ? a.r - j : 0, w[t]);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) sum[t] = product(w[t][e], h[e], sum[t]);
-      }
-    }
-    const int at = l % kTile;
-    if (at >= first && at < end) {
-      const int64_t row = taken.row[at];
+    const bool mine = at >= first && at < end;
+    const int64_t row = row_of(code[mine ? at : first]);
+    const T* up = (const T*)a.up + key * a.up_adapter;
+    const In* scores = (const In*)a.scores + row * a.stride;
+    const auto outputs = [&](int o0, auto all) {
+      constexpr bool kWhole = decltype(all)::value;
+      float v[kTiles][4];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        const int o = outputs + t * kTile + l / kTile * 4;
-        if (o >= a.K) continue;
-        float v[4];
-        load_floats<4>(a.scores, row * a.stride + o, a.dtype, a.K - o, v);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = key < a.M ? __builtin_fmaf(a.scale, sum[t][q], v[q]) : v[q];
-        store_floats<4>(a.out, row * a.out_stride + o, a.out_dtype, a.K - o, v);
+        const int o = o0 + t * kTile + l / kTile * 4;
+        load_floats<4, kWhole>(scores + o, a.K - o, v[t]);
       }
+      v4f sum[kTiles];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) sum[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      if (key < a.M) {
+        for (int j = l / kTile * 4; j < a.padded; j += kTile) {
+          float h[4], w[kTiles][4];
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            const int o = o0 + t * kTile + at;
+            load_floats<4, kWhole>(up + (int64_t)(o < a.K ? o : a.K - 1) * a.up_output + j, a.r - j, w[t]);
+          }
+          __builtin_memcpy(h, &hidden[at][j], sizeof h);
+          loads_first();
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) sum[t] = product(w[t][e], h[e], sum[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[t][q] = __builtin_fmaf(a.scale, sum[t][q], v[t][q]);
+      }
+      if (!mine) return;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const int o = o0 + t * kTile + l / kTile * 4;
+        if (kWhole || o < a.K) store_floats<4>(a.out, row * a.out_stride + o, a.out_dtype, kWhole ? 4 : a.K - o, v[t]);
+      }
+    };
+    for (int o0 = (blockIdx.y * kWaves + wave) * kTiles * kTile; o0 < a.K; o0 += gridDim.y * kWaves * kTiles * kTile) {
+      if (o0 + kTiles * kTile <= a.K && a.r % kTile == 0)
+        outputs(o0, std::true_type{});
+      else
+        outputs(o0, std::false_type{});
     }
-    __syncthreads();
   });
 }
 
 // ----------------------------------------------------------------------------------- gradients
-// back, a part of the outputs: lane l has row l % 16 and four outputs in a row of every 16, whose weights of
-// rank l % 16 it reads one after the other.
-template <int W, int RT>
-__global__ __launch_bounds__(kThreads) void back_kernel(AdaptArgs a) {
+// back, a part of the outputs: lane l has row l % 16 and eight outputs in a row of every 32, whose weights of
+// ranks RT (l % 16) + t it reads one output after the other.
+template <int G, int W, int RT>
+__device__ __forceinline__ void back_block(const AdaptArgs& a, int block, int p, int ranks, Order& order,
+                                           v4f (*join)[RT][kWave]) {
   typedef typename Element<W>::type T;
-  __shared__ Taken<kTile> taken;
-  __shared__ v4f join[kWaves - 1][RT][kWave];
-  const int slot = blockIdx.x % a.slots, window = blockIdx.x / a.slots, p = blockIdx.y, ranks = blockIdx.z * RT * kTile;
-  taken.take(a, window * kTile);
+  typedef typename Element<G>::type S;
+  const int slot = block % a.slots, window = block / a.slots;
+  const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t row = taken.row[l % kTile] < 0 ? taken.row[0] : taken.row[l % kTile];
-  segments(taken.key, slot, a.slots, [&](int key, int first, int end) {
+  const int64_t row = row_of(code[l % kTile] == UINT32_MAX ? code[0] : code[l % kTile]);
+  const S* grad = (const S*)a.scores + row * a.stride;
+  segments(code, slot, a.slots, [&](int key, int first, int end) {
     if (key == a.M) return;
-    const T* up = (const T*)a.up + key * a.up_adapter;
+    const int j = ranks + l % kTile * RT;
+    const T* up = (const T*)a.up + key * a.up_adapter + j;
     v4f sum[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) sum[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const int steps = (a.K + 15) / 16, last = (p + 1) * a.part_steps < steps ? (p + 1) * a.part_steps : steps;
-    for (int step = p * a.part_steps + wave; step < last; step += kWaves) {
-      const int o = step * 16 + l / kTile * 4;
-      float g[4];
-      load_floats<4>(a.scores, row * a.stride + o, a.dtype, a.K - o, g);
+    struct Operands {
+      float g[8], w[8][RT];
+    };
+    const auto load = [&](int step, auto all, Operands& v) {
+      constexpr bool kWhole = decltype(all)::value;
+      const int o = step * 32 + l / kTile * 8;
+      load_floats<8, kWhole>(grad + o, a.K - o, v.g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 8; ++e)
+        load_floats<RT, kWhole>(up + (int64_t)(o + e) * a.up_output, o + e < a.K ? a.r - j : 0, v.w[e]);
+    };
+    const auto multiply = [&](const Operands& v) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const int j = ranks + t * kTile + l % kTile;
-          const float w = o + e < a.K ? to_float(up[(o + e) * a.up_output + (j < a.r ? j : a.r - 1)]) : 0.0f;
-          sum[t] = product(g[e], w, sum[t]);
-        }
-    }
-    if (wave > 0)
+      for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int t = 0; t < RT; ++t) join[wave - 1][t][l] = sum[t];
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        for (int w = 0; w < kWaves - 1; ++w) sum[t] += join[w][t][l];
-        const int j = ranks + t * kTile + l % kTile;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int i = l / kTile * 4 + q;
-          if (i >= first && i < end && j < a.r) a.part[((int64_t)p * a.N + window * kTile + i) * a.r + j] = sum[t][q];
-        }
+        for (int t = 0; t < RT; ++t) sum[t] = product(v.g[e], v.w[e][t], sum[t]);
+    };
+    // whole steps of whole ranks have the next one's operands on their way
+    const int steps = (a.K + 31) / 32, last = (p + 1) * a.part_steps < steps ? (p + 1) * a.part_steps : steps;
+    const int whole = ranks + RT * kTile <= a.r ? (last < a.K / 32 ? last : a.K / 32) : 0;
+    int step = p * a.part_steps + wave;
+    if (step < whole) {
+      Operands now;
+      load(step, std::true_type{}, now);
+      for (; step + kWaves < whole; step += kWaves) {
+        Operands next;
+        load(step + kWaves, std::true_type{}, next);
+        loads_first();
+        multiply(now);
+        now = next;
       }
+      multiply(now);
+      step += kWaves;
     }
-    __syncthreads();
+    for (; step < last; step += kWaves) {
+      Operands now;
+      load(step, std::false_type{}, now);
+      multiply(now);
+    }
+    write_part<RT>(a, p, window, first, end, ranks, sum, join);
   });
 }
 
 __global__ __launch_bounds__(kThreads) void back_join_kernel(AdaptArgs a) {
-  const int64_t each = (int64_t)a.N * a.r;
-  for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < each; i += (int64_t)gridDim.x * kThreads) {
-    float sum = 0.0f;
-    for (int p = 0; p < a.parts; ++p) sum += a.part[p * each + i];
-    a.back[i] = a.scale * sum;
+  const int64_t each = (int64_t)a.N * a.padded;
+  for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < each / 4; i += (int64_t)gridDim.x * kThreads) {
+    float4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int p = 0; p < a.parts; ++p) {
+      const float4 v = ((const float4*)(a.part + p * each))[i];
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    ((float4*)a.back)[i] = sum;
   }
 }
 
-// A gradient's tile of 64 columns (outputs or clauses) and 16 RT ranks: the sum over an adapter's rows of a
-// row's value at the column times its value at the rank.  A lane has four columns in a row of one of four
-// rows, each of them a product's operand; a block's waves take four rows in turn and are joined in LDS.
+// A gradient's tile of 128 columns (outputs or clauses) and 16 RT ranks: the sum over an adapter's rows of a
+// row's value at the column times its value at the rank.  A lane has eight columns in a row of one of four
+// rows, each of them a product's operand, and the ranks RT (l % 16) + t; a block's waves take sixteen rows in
+// turn and are joined in LDS.  X: what a row's values at the columns are.
+constexpr int kColumns = 128;
 template <int X, int RT, bool UP>
-__global__ __launch_bounds__(kThreads) void outer_kernel(AdaptArgs a, int w_dtype) {
-  __shared__ Taken<kInline> taken;
-  __shared__ v4f join[kWaves - 1][RT][4][kWave];
-  const int key = blockIdx.y, first_column = blockIdx.x * 64, ranks = blockIdx.z * RT * kTile;
+__device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int key, int ranks, Order& order,
+                                            v4f (*join)[8][kWave]) {
+  constexpr int kSteps = 4;
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (a.N <= kInline) taken.take(a, 0);
-  const int begin = begin_of(a, key, taken.keys), end = begin_of(a, key + 1, taken.keys);
-  v4f sum[RT][4];
+  if (a.N <= kInline) order.make(a);
+  const uint32_t* from = a.N <= kInline ? order.code : a.order;
+  const int begin = __builtin_amdgcn_readfirstlane(order.begin(a, key));
+  const int end = __builtin_amdgcn_readfirstlane(order.begin(a, key + 1));
+  v4f sum[RT][8];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum[t][e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  const int column = first_column + l % kTile * 4, columns = UP ? a.K : a.C;
-  for (int first = begin + wave * 4; first < end; first += kWaves * 4) {
-    const int place = first + l / kTile;
-    const bool there = place < end;
-    const int at = there ? place : end - 1;
-    const int64_t row = a.N <= kInline ? taken.row[at] : a.order[at];
-    float v[4];
-    if constexpr (UP)
-      load_floats<4>(a.scores, row * a.stride + column, a.dtype, there ? columns - column : 0, v);
-    else
-      load_clauses<X, 4>(a, row, column, v);
+    for (int e = 0; e < 8; ++e) sum[t][e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const int column = tile * kColumns + l % kTile * 8, columns = UP ? a.K : a.C, j = ranks + l % kTile * RT;
+  struct Operands {
+    float v[kSteps][8], h[kSteps][RT];
+  };
+  const auto load = [&](int first, auto all, Operands& o) {
+    constexpr bool kWhole = decltype(all)::value;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int j = ranks + t * kTile + l % kTile;
-      float h = 0.0f;
-      if (there && j < a.r) h = UP ? a.hidden[row * a.hidden_stride + j] : a.back[(int64_t)at * a.r + j];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        sum[t][e] = UP ? product(v[e], h, sum[t][e]) : product(h, there ? v[e] : 0.0f, sum[t][e]);
-    }
-  }
-  if (wave > 0)
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) join[wave - 1][t][e][l] = sum[t][e];
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      for (int w = 0; w < kWaves - 1; ++w) sum[t][e] += join[w][t][e][l];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if constexpr (UP) {  // outputs first_column + 4 i + e of product e's row i, rank l % 16
-        const int j = ranks + t * kTile + l % kTile;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int o = first_column + 4 * (l / kTile * 4 + q) + e;
-          const float v[1] = {a.scale * sum[t][e][q]};
-          if (j < a.r && o < a.K) store_floats<1>(a.out, key * a.d_up_adapter + o * a.d_up_output + j, w_dtype, 1, v);
-        }
+    for (int s = 0; s < kSteps; ++s) {
+      const int place = first + 4 * s + l / kTile;
+      const bool there = kWhole || place < end;
+      const int at = there ? place : end - 1;
+      const int64_t row = row_of(from[at]);
+      if constexpr (UP) {
+        load_floats<8, kWhole>((const typename Element<X>::type*)a.scores + row * a.stride + column,
+                               there ? columns - column : 0, o.v[s]);
+        load_floats<RT, kWhole>(a.hidden + row * a.hidden_stride + j, there ? a.r - j : 0, o.h[s]);
       } else {
-        const int j = ranks + t * kTile + l / kTile * 4 + q;
-        const float v[4] = {sum[t][0][q], sum[t][1][q], sum[t][2][q], sum[t][3][q]};
-        if (j < a.r && column < a.C)
-          store_floats<4>(a.d_down, key * a.d_down_adapter + j * a.d_down_rank + column, w_dtype, a.C - column, v);
+        load_clauses<X, 8, kWhole>(a, row, there ? column : a.C, o.v[s]);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) o.h[s][t] = 0.0f;
+        if (kWhole || there) {
+          const int64_t part = (int64_t)a.N * a.padded;
+          for (int p = 0; p < a.back_parts; ++p) {
+            float one[RT];
+            __builtin_memcpy(one, a.back + p * part + (int64_t)at * a.padded + j, sizeof one);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) o.h[s][t] += one[t];
+          }
+        }
       }
     }
+  };
+  const auto multiply = [&](const Operands& o) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          sum[t][e] = UP ? product(o.v[s][e], o.h[s][t], sum[t][e]) : product(o.h[s][t], o.v[s][e], sum[t][e]);
+  };
+  constexpr int kRows = kWaves * 4 * kSteps;
+  int first = begin + wave * 4 * kSteps;
+  if ((tile + 1) * kColumns <= columns && (!UP || ranks + RT * kTile <= a.r) && first + 4 * kSteps <= end) {
+    Operands now;
+    load(first, std::true_type{}, now);
+    for (; first + kRows + 4 * kSteps <= end; first += kRows) {
+      Operands next;
+      load(first + kRows, std::true_type{}, next);
+      loads_first();
+      multiply(now);
+      now = next;
+    }
+    multiply(now);
+    first += kRows;
   }
+  for (; first < end; first += kRows) {
+    Operands now;
+    load(first, std::false_type{}, now);
+    multiply(now);
+  }
+  // wave w takes row 4 (l / 16) + w of each product: outputs 8 (4 (l / 16) + w) + e, or ranks
+  float total[RT][8];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) join[wave][e][l] = sum[t][e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      total[t][e] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) total[t][e] += ((const float*)&join[w][e][l])[wave];
+      total[t][e] *= a.scale;
+    }
+  }
+  if constexpr (UP) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int o = tile * kColumns + 8 * (l / kTile * 4 + wave) + e;
+      float v[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) v[t] = total[t][e];
+      if (o < a.K && j < a.r)
+        store_floats<RT>(a.out, key * a.d_up_adapter + o * a.d_up_output + j, a.w_dtype, a.r - j, v);
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int rank = ranks + (l / kTile * 4 + wave) * RT + t;
+      if (rank < a.r && column < a.C)
+        store_floats<8>(a.d_down, key * a.d_down_adapter + rank * a.d_down_rank + column, a.w_dtype, a.C - column,
+                        total[t]);
+    }
+  }
+}
+
+// What reads the scores' gradient: the first blocks of a launch make back, the others the gradient of up.
+template <int G, int W, int RT>
+__global__ __launch_bounds__(kThreads) void grad_kernel(AdaptArgs a) {
+  __shared__ Order order;
+  __shared__ v4f join[kWaves][RT > 8 ? RT : 8][kWave];
+  const int back = a.windows * a.slots * a.parts, ranks = blockIdx.y * RT * kTile;
+  if ((int)blockIdx.x < back) {
+    const int p = blockIdx.x % a.parts;
+    back_block<G, W, RT>(a, blockIdx.x / a.parts, p, ranks, order, (v4f(*)[RT][kWave])join);
+  } else {
+    const int i = blockIdx.x - back, tiles = (a.K + kColumns - 1) / kColumns;
+    outer_block<G, RT, true>(a, i % tiles, a.first + i / tiles, ranks, order, join);
+  }
+}
+
+template <int X, int RT>
+__global__ __launch_bounds__(kThreads) void clauses_kernel(AdaptArgs a) {
+  __shared__ Order order;
+  __shared__ v4f join[kWaves][8][kWave];
+  outer_block<X, RT, false>(a, blockIdx.x, blockIdx.y, blockIdx.z * RT * kTile, order, join);
 }
 
 // --------------------------------------------------------------------------------------- host
@@ -483,31 +720,43 @@ struct Split {
   int windows, slots, parts, part_steps;
 };
 
-// Parts of a sum over `steps`, so that about 512 blocks share it, each with a step a wave at least, and
-// slots that share a window's segments where there are still few blocks.
-Split split_of(int64_t N, int64_t M, int64_t steps) {
+// Parts of a sum over `steps` (of `block` rows in a row), so that about 512 blocks share it, each with a step a
+// wave at least, and slots that share a window's segments where there are still few blocks.
+Split split_of(int64_t N, int64_t M, int64_t steps, int64_t most_parts) {
   Split s;
   s.windows = (int)((N + kTile - 1) / kTile);
   const int64_t most = steps > kWaves ? (steps + kWaves - 1) / kWaves : 1;
   int64_t parts = 512 / s.windows;
-  parts = parts < 1 ? 1 : parts > 32 ? 32 : parts;
+  parts = parts < 1 ? 1 : parts > most_parts ? most_parts : parts;
   parts = parts < most ? parts : most;
   s.part_steps = (int)((steps + parts - 1) / parts);
-  s.parts = s.part_steps ? (int)((steps + s.part_steps - 1) / s.part_steps) : 1;
-  int64_t slots = 2048 / ((int64_t)s.windows * s.parts);
+  s.part_steps = s.part_steps ? s.part_steps : 1;
+  s.parts = steps ? (int)((steps + s.part_steps - 1) / s.part_steps) : 1;
+  int64_t slots = 1024 / ((int64_t)s.windows * s.parts);
   const int64_t segments = M + 1 < kTile ? M + 1 : kTile;
   slots = slots < 1 ? 1 : slots < segments ? slots : segments;
   s.slots = (int)slots;
   return s;
 }
+Split down_split(int64_t N, int64_t M, int64_t C, bool halves) {
+  const int64_t chunk = halves ? 128 : 64;
+  return split_of(N, M, (C + chunk - 1) / chunk, 16);
+}
+// Few rows: eight parts at most, which the blocks that use back add up themselves.
+Split back_split(int64_t N, int64_t M, int64_t K) {
+  return split_of(N, M, (K + 31) / 32, N <= kInline ? 8 : 16);
+}
+bool joins_back(int64_t N, const Split& s) { return N > kInline && s.parts > 1; }
 
 int64_t aligned(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+int64_t padded_of(int64_t r) { return (r + kTile - 1) / kTile * kTile <= 32 ? (r + kTile - 1) / kTile * kTile
+                                                                            : (r + 63) / 64 * 64; }
 
 int rank_tiles(int r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; }
 
 hipError_t launch_order(const AdaptArgs& a, hipStream_t s) {
   if (a.N <= kInline) return hipSuccess;
-  order_kernel<<<(a.N + kThreads - 1) / kThreads, kThreads, 0, s>>>(a);
+  order_kernel<<<(a.N + kWave - 1) / kWave, kOrderThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -534,54 +783,81 @@ hipError_t launch_adapt(const AdaptArgs& a, int x_dtype, hipStream_t s) {
     default: e = launch_down<YTM_DTYPE_F32, W>(a, s); break;
   }
   if (e != hipSuccess) return e;
-  const unsigned tiles = a.K > 0 ? (unsigned)((a.K + 4 * kThreads / 4 - 1) / (4 * kThreads / 4)) : 1;
-  up_kernel<W><<<dim3(a.windows * a.slots, tiles), kThreads, 0, s>>>(a);
-  return hipGetLastError();
-}
-
-template <int X, bool UP>
-hipError_t launch_outer(const AdaptArgs& a, int w_dtype, hipStream_t s) {
-  const int t = rank_tiles(a.r), columns = UP ? a.K : a.C;
-  if (columns == 0) return hipSuccess;
-  const dim3 grid((columns + 63) / 64, a.M, (a.r + t * kTile - 1) / (t * kTile));
-  switch (t) {
-    case 1: outer_kernel<X, 1, UP><<<grid, kThreads, 0, s>>>(a, w_dtype); break;
-    case 2: outer_kernel<X, 2, UP><<<grid, kThreads, 0, s>>>(a, w_dtype); break;
-    default: outer_kernel<X, 4, UP><<<grid, kThreads, 0, s>>>(a, w_dtype); break;
+  // a block takes so many times 256 outputs that there are about 2048 of them
+  const int64_t tiles = a.K > 0 ? (a.K + 255) / 256 : 1, blocks = (int64_t)a.windows * a.slots;
+  const int64_t each = (tiles * blocks + 2047) / 2048;
+  const dim3 grid((unsigned)blocks, (unsigned)((tiles + each - 1) / each));
+  switch (a.dtype) {
+    case YTM_DTYPE_F16: up_kernel<W, YTM_DTYPE_F16><<<grid, kThreads, 0, s>>>(a); break;
+    case YTM_DTYPE_BF16: up_kernel<W, YTM_DTYPE_BF16><<<grid, kThreads, 0, s>>>(a); break;
+    default: up_kernel<W, YTM_DTYPE_F32><<<grid, kThreads, 0, s>>>(a); break;
   }
   return hipGetLastError();
 }
 
-template <int W>
-hipError_t launch_back(const AdaptArgs& a, hipStream_t s) {
+template <int G, int W>
+hipError_t launch_grad(AdaptArgs a, hipStream_t s) {
   const int t = rank_tiles(a.r);
-  const dim3 grid(a.windows * a.slots, a.parts, (a.r + t * kTile - 1) / (t * kTile));
-  switch (t) {
-    case 1: back_kernel<W, 1><<<grid, kThreads, 0, s>>>(a); break;
-    case 2: back_kernel<W, 2><<<grid, kThreads, 0, s>>>(a); break;
-    default: back_kernel<W, 4><<<grid, kThreads, 0, s>>>(a); break;
+  const int64_t tiles = (a.K + kColumns - 1) / kColumns, most = tiles ? ((int64_t)1 << 23) / tiles : 1;
+  // a launch counts its threads in 32 bits: more adapters than it holds take several
+  for (int64_t first = 0; first < a.M; first += most) {
+    a.first = (int)first;
+    const int64_t back = first ? 0 : (int64_t)a.windows * a.slots * a.parts;
+    const int64_t blocks = back + tiles * (a.M - first < most ? a.M - first : most);
+    const dim3 grid((unsigned)blocks, (a.r + t * kTile - 1) / (t * kTile));
+    if (blocks == 0) return hipSuccess;
+    if (first) a.windows = 0;
+    switch (t) {
+      case 1: grad_kernel<G, W, 1><<<grid, kThreads, 0, s>>>(a); break;
+      case 2: grad_kernel<G, W, 2><<<grid, kThreads, 0, s>>>(a); break;
+      default: grad_kernel<G, W, 4><<<grid, kThreads, 0, s>>>(a); break;
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const int64_t blocks = ((int64_t)a.N * a.r + kThreads - 1) / kThreads;
-  back_join_kernel<<<(unsigned)(blocks < 2048 ? blocks : 2048), kThreads, 0, s>>>(a);
+  return hipSuccess;
+}
+template <int G>
+hipError_t launch_grad_of(const AdaptArgs& a, hipStream_t s) {
+  switch (a.w_dtype) {
+    case YTM_DTYPE_F16: return launch_grad<G, YTM_DTYPE_F16>(a, s);
+    case YTM_DTYPE_BF16: return launch_grad<G, YTM_DTYPE_BF16>(a, s);
+    default: return launch_grad<G, YTM_DTYPE_F32>(a, s);
+  }
+}
+
+template <int X>
+hipError_t launch_clauses(const AdaptArgs& a, hipStream_t s) {
+  const int t = rank_tiles(a.r);
+  if (a.C == 0) return hipSuccess;
+  const dim3 grid((a.C + kColumns - 1) / kColumns, a.M, (a.r + t * kTile - 1) / (t * kTile));
+  switch (t) {
+    case 1: clauses_kernel<X, 1><<<grid, kThreads, 0, s>>>(a); break;
+    case 2: clauses_kernel<X, 2><<<grid, kThreads, 0, s>>>(a); break;
+    default: clauses_kernel<X, 4><<<grid, kThreads, 0, s>>>(a); break;
+  }
   return hipGetLastError();
 }
 
-hipError_t launch_gradient(const AdaptArgs& a, int x_dtype, int w_dtype, hipStream_t s) {
+hipError_t launch_gradient(AdaptArgs a, int x_dtype, hipStream_t s) {
   hipError_t e = launch_order(a, s);
-  if (e == hipSuccess && a.N > 0) switch (w_dtype) {
-      case YTM_DTYPE_F16: e = launch_back<YTM_DTYPE_F16>(a, s); break;
-      case YTM_DTYPE_BF16: e = launch_back<YTM_DTYPE_BF16>(a, s); break;
-      default: e = launch_back<YTM_DTYPE_F32>(a, s); break;
-    }
-  if (e == hipSuccess) e = launch_outer<YTM_DTYPE_BITS, true>(a, w_dtype, s);
+  if (e != hipSuccess) return e;
+  switch (a.dtype) {
+    case YTM_DTYPE_F16: e = launch_grad_of<YTM_DTYPE_F16>(a, s); break;
+    case YTM_DTYPE_BF16: e = launch_grad_of<YTM_DTYPE_BF16>(a, s); break;
+    default: e = launch_grad_of<YTM_DTYPE_F32>(a, s); break;
+  }
+  if (e == hipSuccess && a.back != a.part) {
+    const int64_t blocks = ((int64_t)a.N * a.padded / 4 + kThreads - 1) / kThreads;
+    back_join_kernel<<<(unsigned)(blocks < 2048 ? blocks : 2048), kThreads, 0, s>>>(a);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess) return e;
   switch (x_dtype) {
-    case YTM_DTYPE_BITS: return launch_outer<YTM_DTYPE_BITS, false>(a, w_dtype, s);
-    case YTM_DTYPE_F16: return launch_outer<YTM_DTYPE_F16, false>(a, w_dtype, s);
-    case YTM_DTYPE_BF16: return launch_outer<YTM_DTYPE_BF16, false>(a, w_dtype, s);
-    default: return launch_outer<YTM_DTYPE_F32, false>(a, w_dtype, s);
+    case YTM_DTYPE_BITS: return launch_clauses<YTM_DTYPE_BITS>(a, s);
+    case YTM_DTYPE_F16: return launch_clauses<YTM_DTYPE_F16>(a, s);
+    case YTM_DTYPE_BF16: return launch_clauses<YTM_DTYPE_BF16>(a, s);
+    default: return launch_clauses<YTM_DTYPE_F32>(a, s);
   }
 }
 
@@ -616,7 +892,7 @@ const char* wrong_operands(int dtype, int64_t stride, int64_t N, int64_t K, int 
   return nullptr;
 }
 
-int64_t order_bytes(int64_t N) { return N > kInline ? aligned(8 * N) : 0; }
+int64_t order_bytes(int64_t N) { return N > kInline ? aligned(4 * N) : 0; }
 
 }  // namespace
 
@@ -632,8 +908,12 @@ int ytm_adapt_workspace(int64_t N, int64_t C, int64_t M, int64_t r, int64_t* byt
     return fail(YTM_EINVAL, "bad adapt_workspace arguments");
   *bytes = 0;
   if (N == 0) return YTM_OK;
-  const ytm::Split s = ytm::split_of(N, M, (C + 31) / 32);
-  *bytes = ytm::order_bytes(N) + s.parts * N * r * 4;
+  int64_t parts = 1;  // the most of the types'
+  for (bool halves : {false, true}) {
+    const ytm::Split s = ytm::down_split(N, M, C, halves);
+    parts = s.parts > parts ? s.parts : parts;
+  }
+  *bytes = ytm::order_bytes(N) + parts * N * ytm::padded_of(r) * 4;
   return YTM_OK;
 }
 
@@ -672,17 +952,19 @@ int ytm_adapt(const void* scores, int dtype, int64_t stride, int64_t N, int64_t 
   if (in_place)  // what else is written must still not lie in the scores
     for (int i = 1; i < 3; ++i) overlap |= ytm::share_bytes(written[i], ytm::rows_of(scores, N, K, stride, size));
   if (overlap) return fail(YTM_EINVAL, "adapt: what is written overlaps what is read, and is not the scores' own place");
-  const ytm::Split split = ytm::split_of(N, M, (C + 31) / 32);
+  const bool halves = w_dtype != YTM_DTYPE_F32 && (x_dtype == w_dtype || x_dtype == YTM_DTYPE_BITS);
+  const ytm::Split split = ytm::down_split(N, M, C, halves);
   ytm::AdaptArgs a{};
   a.scores = scores, a.dtype = dtype, a.stride = stride, a.N = (int)N, a.K = (int)K;
   a.x = x, a.x_stride = x_stride, a.C = (int)C;
   a.down = down, a.down_adapter = down_adapter, a.down_rank = down_rank;
   a.up = up, a.up_adapter = up_adapter, a.up_output = up_output;
-  a.M = (int)M, a.r = (int)r, a.which = which, a.scale = scale;
+  a.M = (int)M, a.r = (int)r, a.w_dtype = w_dtype, a.which = which, a.scale = scale;
   a.hidden = hidden, a.hidden_stride = hidden_stride;
   a.out = out, a.out_dtype = out_dtype, a.out_stride = out_stride;
   a.windows = split.windows, a.slots = split.slots, a.parts = split.parts, a.part_steps = split.part_steps;
-  a.order = (int32_t*)workspace;
+  a.padded = (int)ytm::padded_of(r);
+  a.order = (uint32_t*)workspace;
   a.part = (float*)((char*)workspace + ytm::order_bytes(N));
   hipStream_t s = (hipStream_t)stream;
   hipError_t e;
@@ -701,8 +983,8 @@ int ytm_adapt_gradient_workspace(int64_t N, int64_t K, int64_t M, int64_t r, int
     return fail(YTM_EINVAL, "bad adapt_gradient_workspace arguments");
   *bytes = 0;
   if (N == 0 || M == 0) return YTM_OK;
-  const ytm::Split s = ytm::split_of(N, M, (K + 15) / 16);
-  *bytes = ytm::order_bytes(N) + ytm::aligned(s.parts * N * r * 4) + N * r * 4;
+  const ytm::Split s = ytm::back_split(N, M, K);
+  *bytes = ytm::order_bytes(N) + (s.parts + ytm::joins_back(N, s)) * N * ytm::padded_of(r) * 4;
   return YTM_OK;
 }
 
@@ -745,20 +1027,23 @@ int ytm_adapt_gradient(const void* grad, int dtype, int64_t stride, int64_t N, i
   if (overlap) return fail(YTM_EINVAL, "adapt_gradient: what is written overlaps what is read");
   ytm::AdaptArgs a{};
   if (N > 0) {
-    const ytm::Split split = ytm::split_of(N, M, (K + 15) / 16);
+    const ytm::Split split = ytm::back_split(N, M, K);
+    const bool joins = ytm::joins_back(N, split);
     a.windows = split.windows, a.slots = split.slots, a.parts = split.parts, a.part_steps = split.part_steps;
-    a.order = (int32_t*)workspace;
+    a.padded = (int)ytm::padded_of(r);
+    a.order = (uint32_t*)workspace;
     a.part = (float*)((char*)workspace + ytm::order_bytes(N));
-    a.back = (float*)((char*)a.part + ytm::aligned(split.parts * N * r * 4));
+    a.back = joins ? a.part + split.parts * N * a.padded : a.part;
+    a.back_parts = joins ? 1 : split.parts;
   }
   a.scores = grad, a.dtype = dtype, a.stride = stride, a.N = (int)N, a.K = (int)K;
   a.x = x, a.x_stride = x_stride, a.C = (int)C;
   a.up = up, a.up_adapter = up_adapter, a.up_output = up_output;
-  a.M = (int)M, a.r = (int)r, a.which = which, a.scale = scale;
+  a.M = (int)M, a.r = (int)r, a.w_dtype = w_dtype, a.which = which, a.scale = scale;
   a.hidden = const_cast<float*>(hidden), a.hidden_stride = hidden_stride;
   a.out = d_up, a.d_up_adapter = d_up_adapter, a.d_up_output = d_up_output;
   a.d_down = d_down, a.d_down_adapter = d_down_adapter, a.d_down_rank = d_down_rank;
-  const hipError_t e = ytm::launch_gradient(a, x_dtype, w_dtype, (hipStream_t)stream);
+  const hipError_t e = ytm::launch_gradient(a, x_dtype, (hipStream_t)stream);
   if (e != hipSuccess) return fail(YTM_EHIP, std::string("adapt_gradient failed: ") + hipGetErrorString(e));
   return YTM_OK;
 }
