@@ -357,7 +357,7 @@ int ytm_adapt(const void *scores, int dtype, int64_t stride, int64_t N, int64_t 
  *   d_down[a][j][c] = sum over rows n of a of x[n][c] * scale * sum over o of grad[n][o] * up[a][o][j]
  * 0 for adapters that no row names.  (The gradient by scores is grad itself.)  d_down (M, r, C) and d_up
  * (M, K, r) are of w_dtype; grad F32, F16 or BF16.  Bounds and workspace as for ytm_adapt. */
-int ytm_adapt_gradient_workspace(int64_t N, int64_t K, int64_t M, int64_t r, int64_t *bytes);
+int ytm_adapt_gradient_workspace(int64_t N, int64_t C, int64_t K, int64_t M, int64_t r, int64_t *bytes);
 int ytm_adapt_gradient(const void *grad, int dtype, int64_t stride, int64_t N, int64_t K, const void *x, int x_dtype,
                        int64_t x_stride, int64_t C, const void *up, int64_t up_adapter, int64_t up_output, int w_dtype,
                        int64_t M, int64_t r, const int32_t *which, float scale, const float *hidden,

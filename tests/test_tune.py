@@ -270,7 +270,8 @@ def test_workspaces():
     for name, good, wrong in (
             ("adapt", (65535, 2097120, 65535, 256), ((-1, 1, 1, 1), (65536, 1, 1, 1), (1, -1, 1, 1), (1, 1, 65536, 1), (1, 1, 1, 0),
                                                      (1, 1, 1, 257))),
-            ("adapt_gradient", (65535, 1 << 23, 65535, 256), ((-1, 1, 1, 1), (1, 1 + (1 << 23), 1, 1), (1, 1, -1, 1), (1, 1, 1, 0))),
+            ("adapt_gradient", (65535, 2097120, 1 << 23, 65535, 256), ((-1, 1, 1, 1, 1), (1, 1, 1 + (1 << 23), 1, 1), (1, 1, 1, -1, 1),
+                                                                        (1, 1, 1, 1, 0), (1, 2097121, 1, 1, 1))),
             ("policy_loss", (1, 1 << 23), ((-1, 1), (65536, 1), (1, -1), (1, 1 + (1 << 23)))),
             ("preference_loss", (65535, 1 << 23), ((-1, 1), (65536, 1), (1, -1), (1, 1 + (1 << 23))))):
         ask = getattr(_lib.lib, f"ytm_{name}_workspace")

@@ -109,7 +109,7 @@ SIGNATURES = {
     "ytm_adapt": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, ctypes.c_int, _I64, _I64, _P, _I64, _I64, _P,
                                  _I64, _I64, ctypes.c_int, _I64, _I64, _P, ctypes.c_float, _P, _I64, _P, ctypes.c_int,
                                  _I64, _P, _I64, _P]),
-    "ytm_adapt_gradient_workspace": (ctypes.c_int, [_I64, _I64, _I64, _I64, ctypes.POINTER(_I64)]),
+    "ytm_adapt_gradient_workspace": (ctypes.c_int, [_I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_I64)]),
     "ytm_adapt_gradient": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, ctypes.c_int, _I64, _I64, _P, _I64,
                                           _I64, ctypes.c_int, _I64, _I64, _P, ctypes.c_float, _P, _I64, _P, _I64, _I64,
                                           _P, _I64, _I64, _P, _I64, _P]),

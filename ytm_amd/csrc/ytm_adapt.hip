@@ -32,6 +32,13 @@ constexpr int kInline = kThreads;  // rows that every block sorts by itself
 constexpr int kMaxRank = 256;
 constexpr int64_t kMaxAdapters = 65535;
 
+// A gradient's sums over many rows: windows of `rows` rows of the order, whose adapters `slots` blocks share;
+// what a window has of an adapter that others have rows of goes to `partial`.
+struct RowWindows {
+  int count, rows, slots;
+  float* partial;
+};
+
 struct AdaptArgs {
   const void* scores;  // or their gradient
   int dtype;
@@ -61,9 +68,11 @@ struct AdaptArgs {
   float* part;            // [parts][N in order][padded]
   float* back;            // [back_parts][N in order][padded]
   int back_parts;
-  uint32_t* order;  // [N], of more than kInline rows
+  uint32_t* order;  // [N], of more than kInline rows; then [begins] where adapters begin
+  int begins;       // M + 1 where they are asked for
   int w_dtype;
   int first;  // adapter of a launch of gradients
+  RowWindows up_windows, down_windows;
 };
 
 // ----------------------------------------------------------------------------------- elements
@@ -153,14 +162,15 @@ __device__ __forceinline__ int smaller(uint4 v, uint32_t mine) {
   return (v.x < mine) + (v.y < mine) + (v.z < mine) + (v.w < mine);
 }
 
-// More than kInline rows: a block places 64 of them, its waves share the codes that they are compared with.
+// More than kInline rows: a block places 64 of them, its waves share the codes that they are compared with.  After
+// the rows come the adapters, as codes before all of theirs, whose places are where their rows begin.
 constexpr int kOrderThreads = 1024;
 __global__ __launch_bounds__(kOrderThreads) void order_kernel(AdaptArgs a) {
   __shared__ uint4 codes[kOrderThreads];
   __shared__ int places[kOrderThreads / kWave][kWave];
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n = blockIdx.x * kWave + l;
-  const uint32_t mine = n < a.N ? code_of(a, n) : 0u;
+  const uint32_t mine = n < a.N ? code_of(a, n) : (uint32_t)(n - a.N) << 16;
   int place = 0;
   for (int first = 0; first < a.N; first += 4 * kOrderThreads) {
     uint32_t v[4];
@@ -178,11 +188,14 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(AdaptArgs a) {
   }
   places[wave][l] = place;
   __syncthreads();
-  if (wave > 0 || n >= a.N) return;
+  if (wave > 0 || n >= a.N + a.begins) return;
   place = 0;
 #pragma unroll
   for (int w = 0; w < kOrderThreads / kWave; ++w) place += places[w][l];
-  a.order[place] = mine;
+  if (n < a.N)
+    a.order[place] = mine;
+  else
+    a.order[n] = (uint32_t)place;
 }
 
 // What a block knows of the order: with at most kInline rows all of it, made by itself.
@@ -219,17 +232,11 @@ struct Order {
   }
   // where adapter `key` begins: the number of codes of smaller keys; after make() where the block makes it
   __device__ __forceinline__ int begin(const AdaptArgs& a, int key) const {
-    const uint32_t* from = a.N <= kInline ? code : a.order;
-    const uint64_t least = (uint64_t)key << 16;
-    int low = 0, high = a.N;
-    while (low < high) {
-      const int mid = (low + high) / 2;
-      if (from[mid] < least)
-        low = mid + 1;
-      else
-        high = mid;
-    }
-    return low;
+    if (a.N > kInline) return __builtin_amdgcn_readfirstlane((int)a.order[a.N + key]);
+    const uint32_t least = (uint32_t)key << 16;
+    int before = 0;
+    for (int i = 0; i < a.N; i += kWave) before += __popcll(__ballot(i + threadIdx.x % kWave < a.N && code[(i + threadIdx.x % kWave) % kInline] < least));
+    return before;
   }
 };
 
@@ -502,12 +509,14 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
 
 // ----------------------------------------------------------------------------------- gradients
 // back, a part of the outputs: lane l has row l % 16 and eight outputs in a row of every 32, whose weights of
-// ranks RT (l % 16) + t it reads one output after the other.
+// ranks RT (l % 16) + t it reads one output after the other.  Gradients and weights of one 16-bit type are
+// multiplied as they are.
 template <int G, int W, int RT>
 __device__ __forceinline__ void back_block(const AdaptArgs& a, int block, int p, int ranks, Order& order,
                                            v4f (*join)[RT][kWave]) {
   typedef typename Element<W>::type T;
   typedef typename Element<G>::type S;
+  constexpr bool kHalf = G == W && W != YTM_DTYPE_F32;
   const int slot = block % a.slots, window = block / a.slots;
   const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -521,21 +530,50 @@ __device__ __forceinline__ void back_block(const AdaptArgs& a, int block, int p,
 #pragma unroll
     for (int t = 0; t < RT; ++t) sum[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     struct Operands {
-      float g[8], w[8][RT];
+      v4u x;
+      uint16_t h[kHalf ? 8 : 1][RT];
+      float g[kHalf ? 1 : 8], w[kHalf ? 1 : 8][RT];
     };
     const auto load = [&](int step, auto all, Operands& v) {
       constexpr bool kWhole = decltype(all)::value;
       const int o = step * 32 + l / kTile * 8;
-      load_floats<8, kWhole>(grad + o, a.K - o, v.g);
+      if constexpr (kHalf) {
+        v.x = load_halves<S, kWhole>(grad + o, a.K - o);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        load_floats<RT, kWhole>(up + (int64_t)(o + e) * a.up_output, o + e < a.K ? a.r - j : 0, v.w[e]);
+        for (int e = 0; e < 8; ++e) {
+          const T* from = up + (int64_t)(o + e) * a.up_output;
+          if (kWhole) {
+            __builtin_memcpy(v.h[e], from, sizeof v.h[e]);
+          } else {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+              v.h[e][t] = 0;
+              if (o + e < a.K && j + t < a.r) __builtin_memcpy(&v.h[e][t], from + t, 2);
+            }
+          }
+        }
+      } else {
+        load_floats<8, kWhole>(grad + o, a.K - o, v.g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          load_floats<RT, kWhole>(up + (int64_t)(o + e) * a.up_output, o + e < a.K ? a.r - j : 0, v.w[e]);
+      }
     };
     const auto multiply = [&](const Operands& v) {
+      if constexpr (kHalf) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+        for (int t = 0; t < RT; ++t) {
+          v4u w;
 #pragma unroll
-        for (int t = 0; t < RT; ++t) sum[t] = product(v.g[e], v.w[e][t], sum[t]);
+          for (int q = 0; q < 4; ++q) w[q] = (uint32_t)v.h[2 * q + 1][t] << 16 | v.h[2 * q][t];
+          sum[t] = half_product<W>(v.x, w, sum[t]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) sum[t] = product(v.g[e], v.w[e][t], sum[t]);
+      }
     };
     // whole steps of whole ranks have the next one's operands on their way
     const int steps = (a.K + 31) / 32, last = (p + 1) * a.part_steps < steps ? (p + 1) * a.part_steps : steps;
@@ -577,102 +615,49 @@ __global__ __launch_bounds__(kThreads) void back_join_kernel(AdaptArgs a) {
 }
 
 // A gradient's tile of 128 columns (outputs or clauses) and 16 RT ranks: the sum over an adapter's rows of a
-// row's value at the column times its value at the rank.  A lane has eight columns in a row of one of four
-// rows, each of them a product's operand, and the ranks RT (l % 16) + t; a block's waves take sixteen rows in
-// turn and are joined in LDS.  X: what a row's values at the columns are.
-constexpr int kColumns = 128;
-template <int X, int RT, bool UP>
-__device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int key, int ranks, Order& order,
-                                            v4f (*join)[8][kWave]) {
-  constexpr int kSteps = 4;
-  const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (a.N <= kInline) order.make(a);
-  const uint32_t* from = a.N <= kInline ? order.code : a.order;
-  const int begin = __builtin_amdgcn_readfirstlane(order.begin(a, key));
-  const int end = __builtin_amdgcn_readfirstlane(order.begin(a, key + 1));
-  v4f sum[RT][8];
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum[t][e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  const int column = tile * kColumns + l % kTile * 8, columns = UP ? a.K : a.C, j = ranks + l % kTile * RT;
-  struct Operands {
-    float v[kSteps][8], h[kSteps][RT];
+// row's value at the column times its value at the rank (hidden or back, f32).  The rows are taken 128 at a
+// time: their values at the ranks go through LDS, those at the columns are loaded by the wave that has the
+// row, eight columns in a row a lane.
+//
+// PLANES 0: f32 operands.  Lane l has a row of every four and eight columns, each a product's operand.
+// PLANES 3: values at the columns that bfloat16 holds (bits, bfloat16).  Lane l has eight rows of 32, whose
+// values are exchanged to eight rows of a column, an operand of 32 rows; the values at the ranks are the
+// sum of three bfloat16 (8 + 8 + 8 bits of a float32's fraction), a product each.
+constexpr int kColumns = 128, kBatch = 128;
+template <int X, int RT, int PLANES>
+struct OuterShared {
+  static constexpr int kPitch = kBatch + 8;  // of a rank's rows, so that 16 ranks' are in different banks
+  static constexpr int kValues = PLANES ? PLANES * RT * kTile * kPitch / 2 : kBatch * (RT * kTile + 4);
+  union {
+    float values[kValues];
+    uint16_t planes[2 * kValues];
+    v4f join[kWaves][8][kWave];
   };
-  const auto load = [&](int first, auto all, Operands& o) {
-    constexpr bool kWhole = decltype(all)::value;
+};
+
+// The 32 bits of a f32 as the sum of bfloat16: each cut, not rounded, so that nothing overflows; where the first is
+// infinite or NaN the others are zero.
+template <int PLANES>
+__device__ __forceinline__ void split(float v, uint16_t (&part)[PLANES]) {
+  const uint32_t u = __float_as_uint(v);
+  const bool finite = (u & 0x7F800000u) != 0x7F800000u;
+  part[0] = (uint16_t)((finite || (u & 0x007FFFFFu) == 0u ? u : u | 0x00400000u) >> 16);  // a NaN stays one
+  float rest = finite ? v - __uint_as_float(u & 0xFFFF0000u) : 0.0f;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int place = first + 4 * s + l / kTile;
-      const bool there = kWhole || place < end;
-      const int at = there ? place : end - 1;
-      const int64_t row = row_of(from[at]);
-      if constexpr (UP) {
-        load_floats<8, kWhole>((const typename Element<X>::type*)a.scores + row * a.stride + column,
-                               there ? columns - column : 0, o.v[s]);
-        load_floats<RT, kWhole>(a.hidden + row * a.hidden_stride + j, there ? a.r - j : 0, o.h[s]);
-      } else {
-        load_clauses<X, 8, kWhole>(a, row, there ? column : a.C, o.v[s]);
-#pragma unroll
-        for (int t = 0; t < RT; ++t) o.h[s][t] = 0.0f;
-        if (kWhole || there) {
-          const int64_t part = (int64_t)a.N * a.padded;
-          for (int p = 0; p < a.back_parts; ++p) {
-            float one[RT];
-            __builtin_memcpy(one, a.back + p * part + (int64_t)at * a.padded + j, sizeof one);
-#pragma unroll
-            for (int t = 0; t < RT; ++t) o.h[s][t] += one[t];
-          }
-        }
-      }
-    }
-  };
-  const auto multiply = [&](const Operands& o) {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-          sum[t][e] = UP ? product(o.v[s][e], o.h[s][t], sum[t][e]) : product(o.h[s][t], o.v[s][e], sum[t][e]);
-  };
-  constexpr int kRows = kWaves * 4 * kSteps;
-  int first = begin + wave * 4 * kSteps;
-  if ((tile + 1) * kColumns <= columns && (!UP || ranks + RT * kTile <= a.r) && first + 4 * kSteps <= end) {
-    Operands now;
-    load(first, std::true_type{}, now);
-    for (; first + kRows + 4 * kSteps <= end; first += kRows) {
-      Operands next;
-      load(first + kRows, std::true_type{}, next);
-      loads_first();
-      multiply(now);
-      now = next;
-    }
-    multiply(now);
-    first += kRows;
+  for (int p = 1; p < PLANES; ++p) {
+    const uint32_t w = __float_as_uint(rest);
+    part[p] = (uint16_t)(w >> 16);
+    rest -= __uint_as_float(w & 0xFFFF0000u);
   }
-  for (; first < end; first += kRows) {
-    Operands now;
-    load(first, std::false_type{}, now);
-    multiply(now);
-  }
-  // wave w takes row 4 (l / 16) + w of each product: outputs 8 (4 (l / 16) + w) + e, or ranks
-  float total[RT][8];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) join[wave][e][l] = sum[t][e];
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      total[t][e] = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) total[t][e] += ((const float*)&join[w][e][l])[wave];
-      total[t][e] *= a.scale;
-    }
-  }
+}
+
+// Writes a block's sums total[t][e]: wave w has row 4 (l / 16) + w of each product, of outputs 8 (4 (l / 16) + w) + e
+// or of ranks.
+template <int RT, bool UP>
+__device__ __forceinline__ void store_outer(const AdaptArgs& a, int tile, int key, int ranks, const float (&total)[RT][8]) {
+  const int l = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   if constexpr (UP) {
+    const int j = ranks + l % kTile * RT;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int o = tile * kColumns + 8 * (l / kTile * 4 + wave) + e;
@@ -683,6 +668,7 @@ __device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int ke
         store_floats<RT>(a.out, key * a.d_up_adapter + o * a.d_up_output + j, a.w_dtype, a.r - j, v);
     }
   } else {
+    const int column = tile * kColumns + l % kTile * 8;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int rank = ranks + (l / kTile * 4 + wave) * RT + t;
@@ -693,26 +679,256 @@ __device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int ke
   }
 }
 
-// What reads the scores' gradient: the first blocks of a launch make back, the others the gradient of up.
-template <int G, int W, int RT>
-__global__ __launch_bounds__(kThreads) void grad_kernel(AdaptArgs a) {
-  __shared__ Order order;
-  __shared__ v4f join[kWaves][RT > 8 ? RT : 8][kWave];
-  const int back = a.windows * a.slots * a.parts, ranks = blockIdx.y * RT * kTile;
-  if ((int)blockIdx.x < back) {
-    const int p = blockIdx.x % a.parts;
-    back_block<G, W, RT>(a, blockIdx.x / a.parts, p, ranks, order, (v4f(*)[RT][kWave])join);
-  } else {
-    const int i = blockIdx.x - back, tiles = (a.K + kColumns - 1) / kColumns;
-    outer_block<G, RT, true>(a, i % tiles, a.first + i / tiles, ranks, order, join);
+// The place of a block's partial sums, by slot (two a window), block of ranks and tile.
+template <int RT>
+__device__ __forceinline__ float* partial_of(float* from, int slot, int ranks, int tiles, int tile, int r) {
+  const int64_t blocks = (r + RT * kTile - 1) / (RT * kTile);
+  return from + ((slot * blocks + ranks / (RT * kTile)) * tiles + tile) * (RT * 8 * kThreads);
+}
+
+// The sums over rows begin .. end - 1 of the order, all of adapter `key`; to the gradient, or to `partial`.
+template <int X, int RT, bool UP, int PLANES>
+__device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int key, int begin, int end, int ranks,
+                                            Order& order, OuterShared<X, RT, PLANES>& sh, float* partial) {
+  typedef OuterShared<X, RT, PLANES> Shared;
+  constexpr int kRanks = RT * kTile;
+  const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  v4f sum[RT][8];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[t][e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const int column = tile * kColumns + l % kTile * 8, columns = UP ? a.K : a.C;
+  const bool whole_tile = (tile + 1) * kColumns <= columns;
+  for (int first = begin; first < end; first += kBatch) {
+    const int rows = end - first < kBatch ? end - first : kBatch;
+    __syncthreads();
+    if (a.N > kInline && threadIdx.x < kBatch)  // rows past the last are it
+      order.code[threadIdx.x] = a.order[first + ((int)threadIdx.x < rows ? (int)threadIdx.x : rows - 1)];
+    __syncthreads();
+    const uint32_t* code = a.N > kInline ? order.code : order.code + first;
+    // 32 rows a wave: its lane's eight (of four, RANK by RANK, with f32 operands)
+    const bool work = wave * 32 < rows;
+    int mine[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = wave * 32 + (PLANES ? l / kTile * 8 + i : i * 4 + l / kTile);
+      mine[i] = at < rows ? row_of(code[at]) : -1;
+    }
+    v4u raw[PLANES && X != YTM_DTYPE_BITS ? 8 : 1];
+    uint32_t bits[8];
+    float v[PLANES ? 1 : 8][8];
+    const auto load = [&](auto all) {
+      constexpr bool kWhole = decltype(all)::value;
+      const int last = row_of(code[rows - 1]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool there = kWhole || mine[i] >= 0;
+        const int64_t row = there ? mine[i] : last;
+        const int left = there ? columns - column : 0;
+        if constexpr (X == YTM_DTYPE_BITS && PLANES) {
+          bits[i] = 0u;
+          if (kWhole || left > 0)
+            bits[i] = ((const uint8_t*)((const uint32_t*)a.x + row * a.x_stride))[column / 8];
+          if (!kWhole && left > 0 && left < 8) bits[i] &= (1u << left) - 1u;
+        } else if constexpr (PLANES > 0) {
+          const bf16* from = UP ? (const bf16*)a.scores + row * a.stride : (const bf16*)a.x + row * a.x_stride;
+          raw[i] = load_halves<bf16, kWhole>(from + column, left);
+        } else if constexpr (UP) {
+          load_floats<8, kWhole>((const typename Element<X>::type*)a.scores + row * a.stride + column, left, v[i]);
+        } else {
+          load_clauses<X, 8, kWhole>(a, row, there ? column : a.C, v[i]);
+        }
+      }
+    };
+    if (work) {
+      if (whole_tile && wave * 32 + 32 <= rows)
+        load(std::true_type{});
+      else
+        load(std::false_type{});
+    }
+    loads_first();
+    // the rows' values at the ranks: two threads a row
+    {
+      const int i = threadIdx.x % kBatch, half = threadIdx.x / kBatch * (kRanks / 2);
+      float h[kRanks / 2];
+#pragma unroll
+      for (int q = 0; q < kRanks / 2; ++q) h[q] = 0.0f;
+      if (i < rows) {
+        if constexpr (UP) {
+          const float* from = a.hidden + row_of(code[i]) * a.hidden_stride + ranks + half;
+          if (ranks + kRanks <= a.r) {
+            load_floats<kRanks / 2, true>(from, 0, h);
+          } else {
+#pragma unroll
+            for (int q = 0; q < kRanks / 2; ++q) h[q] = ranks + half + q < a.r ? from[q] : 0.0f;
+          }
+        } else {
+          const float* from = a.back + (int64_t)(first + i) * a.padded + ranks + half;
+          const int64_t part = (int64_t)a.N * a.padded;
+#pragma unroll 4
+          for (int p = 0; p < a.back_parts; ++p) {
+            float one[kRanks / 2];
+            __builtin_memcpy(one, from + p * part, sizeof one);
+#pragma unroll
+            for (int q = 0; q < kRanks / 2; ++q) h[q] += one[q];
+          }
+        }
+      }
+      if constexpr (PLANES > 0) {
+#pragma unroll
+        for (int q = 0; q < kRanks / 2; ++q) {
+          uint16_t part[PLANES > 0 ? PLANES : 1];
+          split(h[q], part);
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p) sh.planes[(p * kRanks + half + q) * Shared::kPitch + i] = part[p];
+        }
+      } else {
+        __builtin_memcpy(&sh.values[i * (kRanks + 4) + half], h, sizeof h);
+      }
+    }
+    __syncthreads();
+    if (!work) continue;
+    if constexpr (PLANES > 0) {
+      v4u h[RT][PLANES > 0 ? PLANES : 1];
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p)
+          h[t][p] = *(const v4u*)&sh.planes[(p * kRanks + l % kTile * RT + t) * Shared::kPitch + wave * 32 + l / kTile * 8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v4u x;  // eight rows of column e
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (X == YTM_DTYPE_BITS)
+            x[q] = ((bits[2 * q] >> e & 1u) | (bits[2 * q + 1] >> e & 1u) << 16) * 0x3F80u;
+          else
+            x[q] = __builtin_amdgcn_perm(raw[2 * q + 1][e / 2], raw[2 * q][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+        }
+#pragma unroll
+        for (int p = PLANES - 1; p >= 0; --p)
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+            sum[t][e] = UP ? half_product<YTM_DTYPE_BF16>(x, h[t][p], sum[t][e])
+                           : half_product<YTM_DTYPE_BF16>(h[t][p], x, sum[t][e]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float h[RT];
+        __builtin_memcpy(h, &sh.values[(wave * 32 + i * 4 + l / kTile) * (kRanks + 4) + l % kTile * RT], sizeof h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+            sum[t][e] = UP ? product(v[i][e], h[t], sum[t][e]) : product(h[t], v[i][e], sum[t][e]);
+      }
+    }
+  }
+  float total[RT][8];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sh.join[wave][e][l] = sum[t][e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      total[t][e] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) total[t][e] += ((const float*)&sh.join[w][e][l])[wave];
+      if (partial)
+        partial[(t * 8 + e) * kThreads + threadIdx.x] = total[t][e];
+      else
+        total[t][e] *= a.scale;
+    }
+  }
+  if (!partial) store_outer<RT, UP>(a, tile, key, ranks, total);
+}
+
+// Block `block` of a gradient: of at most kInline rows a tile of an adapter, all of its rows; of more a tile,
+// a window of the order and every slots-th adapter of it, one of whose rows pass the window's ends giving
+// partial sums.
+template <int X, int RT, bool UP, int PLANES>
+__device__ __forceinline__ void outer_blocks(const AdaptArgs& a, int block, int ranks, Order& order,
+                                             OuterShared<X, RT, PLANES>& sh) {
+  const int tiles = ((UP ? a.K : a.C) + kColumns - 1) / kColumns, tile = block % tiles;
+  block /= tiles;
+  if (a.N <= kInline) {
+    const int key = a.first + block;
+    order.make(a);
+    const int begin = order.begin(a, key), end = order.begin(a, key + 1);
+    outer_block<X, RT, UP, PLANES>(a, tile, key, begin, end, ranks, order, sh, nullptr);
+    return;
+  }
+  const RowWindows& w = UP ? a.up_windows : a.down_windows;
+  const int window = block / w.slots, from = window * w.rows, to = from + w.rows < a.N ? from + w.rows : a.N;
+  const int first = key_of(a.order[from]), last = key_of(a.order[to - 1]);
+  for (int key = first + block % w.slots; key <= last && key < a.M; key += w.slots) {
+    const int begin = order.begin(a, key), end = order.begin(a, key + 1);
+    if (begin == end) continue;
+    float* partial = nullptr;
+    if (begin < from || end > to) partial = partial_of<RT>(w.partial, 2 * window + (begin >= from), ranks, tiles, tile, a.r);
+    outer_block<X, RT, UP, PLANES>(a, tile, key, begin < from ? from : begin, end > to ? to : end, ranks, order, sh,
+                                   partial);
   }
 }
 
-template <int X, int RT>
+// After both gradients of more than kInline rows: zeros for adapters that no row names, the sums of the
+// parts for those that several windows have rows of.
+template <int RT, bool UP>
+__device__ __forceinline__ void join_block(const AdaptArgs& a, int tile, int tiles, int key, int ranks) {
+  const RowWindows& w = UP ? a.up_windows : a.down_windows;
+  const int begin = (int)a.order[a.N + key], end = (int)a.order[a.N + key + 1];
+  const int first = begin / w.rows, last = (end - 1) / w.rows;
+  if (begin < end && first == last) return;
+  float total[RT][8] = {};
+  if (begin < end)
+    for (int window = first; window <= last; ++window) {
+      const float* partial = partial_of<RT>(w.partial, 2 * window + (window == first), ranks, tiles, tile, a.r);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) total[t][e] += partial[(t * 8 + e) * kThreads + threadIdx.x];
+    }
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) total[t][e] *= a.scale;
+  store_outer<RT, UP>(a, tile, key, ranks, total);
+}
+template <int RT>
+__global__ __launch_bounds__(kThreads) void join_kernel(AdaptArgs a) {
+  const int ups = (a.K + kColumns - 1) / kColumns, downs = (a.C + kColumns - 1) / kColumns, tile = blockIdx.x;
+  for (int key = blockIdx.y; key < a.M; key += gridDim.y) {
+    if (tile < ups)
+      join_block<RT, true>(a, tile, ups, key, blockIdx.z * RT * kTile);
+    else
+      join_block<RT, false>(a, tile - ups, downs, key, blockIdx.z * RT * kTile);
+  }
+}
+
+// What reads the scores' gradient: the first blocks of a launch make back, the others the gradient of up.
+template <int G, int W, int RT>
+__global__ __launch_bounds__(kThreads) void grad_kernel(AdaptArgs a) {
+  constexpr int kPlanes = G == YTM_DTYPE_BF16 ? 3 : 0;
+  __shared__ Order order;
+  __shared__ OuterShared<G, RT, kPlanes> sh;
+  const int back = a.windows * a.slots * a.parts, ranks = blockIdx.y * RT * kTile;
+  if ((int)blockIdx.x < back) {
+    const int p = blockIdx.x % a.parts;
+    back_block<G, W, RT>(a, blockIdx.x / a.parts, p, ranks, order, (v4f(*)[RT][kWave])sh.join);
+  } else {
+    outer_blocks<G, RT, true, kPlanes>(a, blockIdx.x - back, ranks, order, sh);
+  }
+}
+
+template <int X, int RT, int PLANES>
 __global__ __launch_bounds__(kThreads) void clauses_kernel(AdaptArgs a) {
   __shared__ Order order;
-  __shared__ v4f join[kWaves][8][kWave];
-  outer_block<X, RT, false>(a, blockIdx.x, blockIdx.y, blockIdx.z * RT * kTile, order, join);
+  __shared__ OuterShared<X, RT, PLANES> sh;
+  outer_blocks<X, RT, false, PLANES>(a, blockIdx.x, blockIdx.y * RT * kTile, order, sh);
 }
 
 // --------------------------------------------------------------------------------------- host
@@ -748,6 +964,28 @@ Split back_split(int64_t N, int64_t M, int64_t K) {
 }
 bool joins_back(int64_t N, const Split& s) { return N > kInline && s.parts > 1; }
 
+// Windows of a gradient's rows: 256 rows or more, so that about 1024 blocks share them and their sums'
+// parts take at most some 64 MB; slots that share the adapters a window has on average.
+RowWindows windows_of(int64_t N, int64_t M, int64_t columns, int64_t r) {
+  RowWindows w{};
+  if (N <= kInline || columns == 0) return w;
+  const int64_t ranks = r <= 16 ? 16 : r <= 32 ? 32 : 64;
+  const int64_t tiles = (columns + kColumns - 1) / kColumns * ((r + ranks - 1) / ranks);
+  int64_t count = (N + 255) / 256;
+  const int64_t most = tiles < 1024 ? 1024 / tiles : 1;
+  if (count > most) count = most;
+  w.rows = (int)((N + count - 1) / count);
+  w.count = (int)((N + w.rows - 1) / w.rows);
+  const int64_t slots = 2 * (M * w.rows / N);
+  w.slots = (int)(slots < 1 ? 1 : slots > 64 ? 64 : slots);
+  return w;
+}
+int64_t partial_bytes(const RowWindows& w, int64_t columns, int64_t r) {
+  if (w.count < 2) return 0;  // one window has all of an adapter's rows
+  const int64_t ranks = r <= 16 ? 16 : r <= 32 ? 32 : 64;
+  return 2 * w.count * ((columns + kColumns - 1) / kColumns) * ((r + ranks - 1) / ranks) * (ranks / 2 * kThreads * 4);
+}
+
 int64_t aligned(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 int64_t padded_of(int64_t r) { return (r + kTile - 1) / kTile * kTile <= 32 ? (r + kTile - 1) / kTile * kTile
                                                                             : (r + 63) / 64 * 64; }
@@ -756,7 +994,7 @@ int rank_tiles(int r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; }
 
 hipError_t launch_order(const AdaptArgs& a, hipStream_t s) {
   if (a.N <= kInline) return hipSuccess;
-  order_kernel<<<(a.N + kWave - 1) / kWave, kOrderThreads, 0, s>>>(a);
+  order_kernel<<<(a.N + a.begins + kWave - 1) / kWave, kOrderThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -795,27 +1033,35 @@ hipError_t launch_adapt(const AdaptArgs& a, int x_dtype, hipStream_t s) {
   return hipGetLastError();
 }
 
+// A launch counts its threads in 32 bits: launch(first adapter or 0, blocks) for each of as many launches as
+// that takes for the blocks of a gradient.
+template <typename Launch>
+hipError_t launch_outer(const AdaptArgs& a, int64_t columns, const RowWindows& w, Launch launch) {
+  const int64_t tiles = (columns + kColumns - 1) / kColumns, most = tiles ? ((int64_t)1 << 23) / tiles : 1;
+  if (a.N > kInline) return launch(0, tiles * w.count * w.slots);
+  for (int64_t first = 0; first < a.M; first += most) {
+    const hipError_t e = launch((int)first, tiles * (a.M - first < most ? a.M - first : most));
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <int G, int W>
 hipError_t launch_grad(AdaptArgs a, hipStream_t s) {
   const int t = rank_tiles(a.r);
-  const int64_t tiles = (a.K + kColumns - 1) / kColumns, most = tiles ? ((int64_t)1 << 23) / tiles : 1;
-  // a launch counts its threads in 32 bits: more adapters than it holds take several
-  for (int64_t first = 0; first < a.M; first += most) {
-    a.first = (int)first;
-    const int64_t back = first ? 0 : (int64_t)a.windows * a.slots * a.parts;
-    const int64_t blocks = back + tiles * (a.M - first < most ? a.M - first : most);
-    const dim3 grid((unsigned)blocks, (a.r + t * kTile - 1) / (t * kTile));
+  return launch_outer(a, a.K, a.up_windows, [&](int first, int64_t blocks) {
+    a.first = first;
+    if (first) a.windows = 0;  // back is there
+    blocks += (int64_t)a.windows * a.slots * a.parts;
     if (blocks == 0) return hipSuccess;
-    if (first) a.windows = 0;
+    const dim3 grid((unsigned)blocks, (a.r + t * kTile - 1) / (t * kTile));
     switch (t) {
       case 1: grad_kernel<G, W, 1><<<grid, kThreads, 0, s>>>(a); break;
       case 2: grad_kernel<G, W, 2><<<grid, kThreads, 0, s>>>(a); break;
       default: grad_kernel<G, W, 4><<<grid, kThreads, 0, s>>>(a); break;
     }
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
+    return hipGetLastError();
+  });
 }
 template <int G>
 hipError_t launch_grad_of(const AdaptArgs& a, hipStream_t s) {
@@ -826,15 +1072,30 @@ hipError_t launch_grad_of(const AdaptArgs& a, hipStream_t s) {
   }
 }
 
-template <int X>
-hipError_t launch_clauses(const AdaptArgs& a, hipStream_t s) {
+template <int X, int PLANES>
+hipError_t launch_clauses(AdaptArgs a, hipStream_t s) {
   const int t = rank_tiles(a.r);
-  if (a.C == 0) return hipSuccess;
-  const dim3 grid((a.C + kColumns - 1) / kColumns, a.M, (a.r + t * kTile - 1) / (t * kTile));
+  return launch_outer(a, a.C, a.down_windows, [&](int first, int64_t blocks) {
+    a.first = first;
+    const dim3 grid((unsigned)blocks, (a.r + t * kTile - 1) / (t * kTile));
+    switch (t) {
+      case 1: clauses_kernel<X, 1, PLANES><<<grid, kThreads, 0, s>>>(a); break;
+      case 2: clauses_kernel<X, 2, PLANES><<<grid, kThreads, 0, s>>>(a); break;
+      default: clauses_kernel<X, 4, PLANES><<<grid, kThreads, 0, s>>>(a); break;
+    }
+    return hipGetLastError();
+  });
+}
+
+hipError_t launch_join(const AdaptArgs& a, hipStream_t s) {
+  const int t = rank_tiles(a.r);
+  const unsigned tiles = (a.K + kColumns - 1) / kColumns + (a.C + kColumns - 1) / kColumns;
+  if (a.N <= kInline || tiles == 0) return hipSuccess;
+  const dim3 grid(tiles, a.M < 1024 ? a.M : 1024, (a.r + t * kTile - 1) / (t * kTile));
   switch (t) {
-    case 1: clauses_kernel<X, 1><<<grid, kThreads, 0, s>>>(a); break;
-    case 2: clauses_kernel<X, 2><<<grid, kThreads, 0, s>>>(a); break;
-    default: clauses_kernel<X, 4><<<grid, kThreads, 0, s>>>(a); break;
+    case 1: join_kernel<1><<<grid, kThreads, 0, s>>>(a); break;
+    case 2: join_kernel<2><<<grid, kThreads, 0, s>>>(a); break;
+    default: join_kernel<4><<<grid, kThreads, 0, s>>>(a); break;
   }
   return hipGetLastError();
 }
@@ -853,12 +1114,13 @@ hipError_t launch_gradient(AdaptArgs a, int x_dtype, hipStream_t s) {
     e = hipGetLastError();
   }
   if (e != hipSuccess) return e;
-  switch (x_dtype) {
-    case YTM_DTYPE_BITS: return launch_clauses<YTM_DTYPE_BITS>(a, s);
-    case YTM_DTYPE_F16: return launch_clauses<YTM_DTYPE_F16>(a, s);
-    case YTM_DTYPE_BF16: return launch_clauses<YTM_DTYPE_BF16>(a, s);
-    default: return launch_clauses<YTM_DTYPE_F32>(a, s);
-  }
+  if (a.C > 0) switch (x_dtype) {
+      case YTM_DTYPE_BITS: e = launch_clauses<YTM_DTYPE_BITS, 3>(a, s); break;
+      case YTM_DTYPE_BF16: e = launch_clauses<YTM_DTYPE_BF16, 3>(a, s); break;
+      case YTM_DTYPE_F16: e = launch_clauses<YTM_DTYPE_F16, 0>(a, s); break;
+      default: e = launch_clauses<YTM_DTYPE_F32, 0>(a, s); break;
+    }
+  return e == hipSuccess ? launch_join(a, s) : e;
 }
 
 int size_of(int dtype) { return dtype == YTM_DTYPE_F32 || dtype == YTM_DTYPE_BITS ? 4 : 2; }
@@ -892,7 +1154,7 @@ const char* wrong_operands(int dtype, int64_t stride, int64_t N, int64_t K, int 
   return nullptr;
 }
 
-int64_t order_bytes(int64_t N) { return N > kInline ? aligned(4 * N) : 0; }
+int64_t order_bytes(int64_t N, int64_t begins) { return N > kInline ? aligned(4 * (N + begins)) : 0; }
 
 }  // namespace
 
@@ -913,7 +1175,7 @@ int ytm_adapt_workspace(int64_t N, int64_t C, int64_t M, int64_t r, int64_t* byt
     const ytm::Split s = ytm::down_split(N, M, C, halves);
     parts = s.parts > parts ? s.parts : parts;
   }
-  *bytes = ytm::order_bytes(N) + parts * N * ytm::padded_of(r) * 4;
+  *bytes = ytm::order_bytes(N, 0) + parts * N * ytm::padded_of(r) * 4;
   return YTM_OK;
 }
 
@@ -965,7 +1227,7 @@ int ytm_adapt(const void* scores, int dtype, int64_t stride, int64_t N, int64_t 
   a.windows = split.windows, a.slots = split.slots, a.parts = split.parts, a.part_steps = split.part_steps;
   a.padded = (int)ytm::padded_of(r);
   a.order = (uint32_t*)workspace;
-  a.part = (float*)((char*)workspace + ytm::order_bytes(N));
+  a.part = (float*)((char*)workspace + ytm::order_bytes(N, 0));
   hipStream_t s = (hipStream_t)stream;
   hipError_t e;
   switch (w_dtype) {
@@ -977,14 +1239,15 @@ int ytm_adapt(const void* scores, int dtype, int64_t stride, int64_t N, int64_t 
   return YTM_OK;
 }
 
-int ytm_adapt_gradient_workspace(int64_t N, int64_t K, int64_t M, int64_t r, int64_t* bytes) {
-  if (!bytes || N < 0 || K < 0 || M < 0 || r < 1 || N > ytm::kDecodeRows || K > ytm::kMaxScores ||
-      M > ytm::kMaxAdapters || r > ytm::kMaxRank)
+int ytm_adapt_gradient_workspace(int64_t N, int64_t C, int64_t K, int64_t M, int64_t r, int64_t* bytes) {
+  if (!bytes || N < 0 || C < 0 || K < 0 || M < 0 || r < 1 || N > ytm::kDecodeRows || C > ytm::kMaxClauses ||
+      K > ytm::kMaxScores || M > ytm::kMaxAdapters || r > ytm::kMaxRank)
     return fail(YTM_EINVAL, "bad adapt_gradient_workspace arguments");
   *bytes = 0;
   if (N == 0 || M == 0) return YTM_OK;
   const ytm::Split s = ytm::back_split(N, M, K);
-  *bytes = ytm::order_bytes(N) + (s.parts + ytm::joins_back(N, s)) * N * ytm::padded_of(r) * 4;
+  *bytes = ytm::order_bytes(N, M + 1) + (s.parts + ytm::joins_back(N, s)) * N * ytm::padded_of(r) * 4 +
+           ytm::partial_bytes(ytm::windows_of(N, M, K, r), K, r) + ytm::partial_bytes(ytm::windows_of(N, M, C, r), C, r);
   return YTM_OK;
 }
 
@@ -1008,7 +1271,7 @@ int ytm_adapt_gradient(const void* grad, int dtype, int64_t stride, int64_t N, i
       (M > 1 && (d_down_adapter < (r - 1) * d_down_rank + C || (K > 0 && d_up_adapter < (K - 1) * d_up_output + r))))
     return fail(YTM_EINVAL, "adapt_gradient: rows overlap");
   int64_t need = 0;
-  if (int rc = ytm_adapt_gradient_workspace(N, K, M, r, &need)) return rc;
+  if (int rc = ytm_adapt_gradient_workspace(N, C, K, M, r, &need)) return rc;
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(YTM_EINVAL, "adapt_gradient: the workspace is too small or not at a multiple of 16 bytes");
   const int64_t width = x_dtype == YTM_DTYPE_BITS ? (C + 31) / 32 : C;
@@ -1032,9 +1295,14 @@ int ytm_adapt_gradient(const void* grad, int dtype, int64_t stride, int64_t N, i
     a.windows = split.windows, a.slots = split.slots, a.parts = split.parts, a.part_steps = split.part_steps;
     a.padded = (int)ytm::padded_of(r);
     a.order = (uint32_t*)workspace;
-    a.part = (float*)((char*)workspace + ytm::order_bytes(N));
+    a.part = (float*)((char*)workspace + ytm::order_bytes(N, M + 1));
     a.back = joins ? a.part + split.parts * N * a.padded : a.part;
     a.back_parts = joins ? 1 : split.parts;
+    a.begins = (int)M + 1;
+    a.up_windows = ytm::windows_of(N, M, K, r);
+    a.down_windows = ytm::windows_of(N, M, C, r);
+    a.up_windows.partial = a.back + a.back_parts * N * a.padded;
+    a.down_windows.partial = a.up_windows.partial + ytm::partial_bytes(a.up_windows, K, r) / 4;
   }
   a.scores = grad, a.dtype = dtype, a.stride = stride, a.N = (int)N, a.K = (int)K;
   a.x = x, a.x_stride = x_stride, a.C = (int)C;

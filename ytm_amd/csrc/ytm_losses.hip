@@ -12,6 +12,8 @@
 #include <float.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ytm_decode.h"
 #include "ytm_internal.h"
 
@@ -20,7 +22,6 @@ namespace ytm {
 namespace {
 
 constexpr int kWave = 64;
-constexpr int kMaxThreads = 1024;
 constexpr int kMaxSlices = 32;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -47,12 +48,20 @@ struct LossArgs {
   float* slope;       // [N]: c, of preferences
 };
 
-// A score that is NaN counts as -inf, one of +inf as the largest float.
+// A score that is NaN counts as -inf, one of +inf as the largest float: the median of three, which is the least of
+// the others beside a NaN.  (The compiler would make a minimum of it, which is not, if it knew the -inf.)
+__device__ __forceinline__ float score_of(float v) {
+  float least = -INFINITY;
+  asm("" : "+s"(least));
+  return __builtin_amdgcn_fmed3f(v, least, FLT_MAX);
+}
 template <typename In>
 __device__ __forceinline__ float score_of(In v) {
-  const float s = to_float(v);
-  return s != s ? -INFINITY : fminf(s, FLT_MAX);
+  return score_of(to_float(v));
 }
+
+// 2^x, to one unit in its last place; what is less than the smallest normal float is 0.
+__device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 1 / temperature as choose() takes it: 0 or less counts as 1, less than the smallest normal float or NaN as that.
 __device__ __forceinline__ float cooling(const LossArgs& a, int n) {
@@ -67,45 +76,107 @@ struct Stats {
   __device__ __forceinline__ void add(const Stats& o, float scale) {
     if (o.max == -INFINITY) return;
     if (o.max > max) {
-      sum = sum * exp2f((max - o.max) * scale) + o.sum;  // max may be -inf, sum is 0 then
+      sum = sum * power((max - o.max) * scale) + o.sum;  // max may be -inf, sum is 0 then
       max = o.max;
     } else {
-      sum += o.sum * exp2f((o.max - max) * scale);
+      sum += o.sum * power((o.max - max) * scale);
     }
   }
 };
 
-template <int E, typename T>
-__device__ __forceinline__ void load_scores(const T* p, float (&v)[E]) {
-  T raw[E];
-  __builtin_memcpy(raw, p, sizeof raw);
-#pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = score_of(raw[e]);
-}
-
-// Of the scores first .. last - 1 of a row, each thread's own.
+// A thread's part of a row: R times 16 bytes, as they are in memory, every thread's one after the other; past
+// the last score -inf.  All are asked for before the first is used, and a row that fits is read
+// once.
 template <typename In>
+constexpr int kEach = 16 / sizeof(In);
+template <typename In>
+constexpr uint32_t kNothing = 0xFF800000u;
+template <>
+constexpr uint32_t kNothing<f16> = 0xFC00u;
+template <>
+constexpr uint32_t kNothing<bf16> = 0xFF80u;
+__device__ __forceinline__ float half_of(uint32_t u, int i, f16) {
+  return (float)__builtin_bit_cast(f16, (uint16_t)(i ? u >> 16 : u));
+}
+__device__ __forceinline__ float half_of(uint32_t u, int i, bf16) {
+  return __uint_as_float(i ? u & 0xFFFF0000u : u << 16);
+}
+__device__ __forceinline__ float half_of(uint32_t u, int, float) { return __uint_as_float(u); }
+
+template <typename In, int R>
+struct Part {
+  static constexpr int E = kEach<In>, kPerWord = E / 4;
+  uint32_t v[R][4];
+
+  // from the uniform score `first` on, up to `last`
+  __device__ __forceinline__ void load(const In* row, int first, int last) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int from = first + r * (int)blockDim.x * E, i = from + (int)threadIdx.x * E;
+      if (from + (int)blockDim.x * E <= last) {
+        __builtin_memcpy(v[r], row + i, sizeof v[r]);
+      } else {
+        uint32_t one[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          one[e] = kNothing<In>;
+          if (i + e < last) {
+            In at = row[i + e];
+            one[e] = 0u;
+            __builtin_memcpy(&one[e], &at, sizeof at);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[r][q] = kPerWord == 1 ? one[q] : one[2 * q] | one[2 * q + 1] << 16;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __device__ __forceinline__ float score(int r, int e) const {
+    return score_of(half_of(v[r][e / kPerWord], e % kPerWord, In{}));
+  }
+  // Scores are made from what is in memory each time that they are used: kept, they would not fit the registers.
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) asm volatile("" : "+v"(v[r][q]));
+  }
+  // whether any thread has scores in place r
+  __device__ __forceinline__ static bool has(int r, int first, int last) { return first + r * (int)blockDim.x * E < last; }
+
+  __device__ __forceinline__ Stats stats(int first, int last, float scale) {
+    float max = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (has(r, first, last)) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) max = fmaxf(max, score(r, e));
+      }
+    Stats s{max, 0.0f};
+    again();
+    if (max == -INFINITY) return s;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (has(r, first, last)) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e % 4] += power((score(r, e) - max) * scale);
+      }
+    s.sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    again();
+    return s;
+  }
+};
+
+// Of the scores first .. last - 1 of a row, each thread's own, part after part.
+template <typename In, int R>
 __device__ __forceinline__ Stats own_stats(const In* row, int first, int last, float scale) {
-  constexpr int E = 16 / sizeof(In);
   Stats s{-INFINITY, 0.0f};
-  for (int i = first + threadIdx.x * E; i < last; i += blockDim.x * E) {
-    float v[E];
-    if (i + E <= last) {
-      load_scores<E>(row + i, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = i + e < last ? score_of(row[i + e]) : -INFINITY;
-    }
-    float max = v[0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) max = fmaxf(max, v[e]);
-    if (max == -INFINITY) continue;
-    if (max > s.max) {
-      s.sum *= exp2f((s.max - max) * scale);
-      s.max = max;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) s.sum += exp2f((v[e] - s.max) * scale);
+  for (int from = first; from < last; from += R * (int)blockDim.x * kEach<In>) {
+    Part<In, R> part;
+    part.load(row, from, last);
+    s.add(part.stats(from, last, scale), scale);
   }
   return s;
 }
@@ -124,14 +195,14 @@ __device__ __forceinline__ Stats block_stats(Stats s, float scale, Stats* part) 
   return all;
 }
 
-template <typename In>
-__global__ __launch_bounds__(kMaxThreads) void stats_kernel(LossArgs a) {
-  __shared__ Stats part[kMaxThreads / kWave];
+template <typename In, int THREADS, int R>
+__global__ __launch_bounds__(THREADS) void stats_kernel(LossArgs a) {
+  __shared__ Stats part[THREADS / kWave];
   const int n = blockIdx.y, slice = blockIdx.x;
   const In* row = (const In*)a.scores + n * a.stride;
   const int first = slice * a.slice, last = first + a.slice < a.V ? first + a.slice : a.V;
   const float scale = cooling(a, n) * kLog2e;
-  const Stats s = block_stats(own_stats(row, first, last, scale), scale, part);
+  const Stats s = block_stats(own_stats<In, R>(row, first, last, scale), scale, part);
   if (threadIdx.x != 0) return;
   a.stats[(int64_t)n * a.slices + slice] = float2{s.max, s.sum};
   const int t = a.tokens[n];
@@ -186,47 +257,77 @@ __device__ __forceinline__ Loss policy(const LossArgs& a, int n, const Answer& r
   return Loss{w * value, w * slope};
 }
 
-// The gradient of a row's scores first .. last - 1; c is 0 where the row takes no part.
-template <typename In, typename Out>
-__device__ __forceinline__ void write_grad(const LossArgs& a, int n, int first, int last, const Answer& r, float c) {
-  constexpr int E = 8;
-  const In* row = (const In*)a.scores + n * a.stride;
-  Out* to = (Out*)a.grad + n * a.grad_stride;
-  const int t = a.tokens[n];
-  const bool any = r.there && c != 0.0f;
-  const float by = any ? c * r.cooling : 0.0f, each = any ? -by / r.all.sum : 0.0f, scale = r.cooling * kLog2e;
-  for (int i = first + threadIdx.x * E; i < last; i += blockDim.x * E) {
+// Two values to the gradient's type.
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+template <typename Out>
+__device__ __forceinline__ void to_out(float a, float b, Out* to) {
+  to[0] = from_float<Out>(a), to[1] = from_float<Out>(b);
+}
+template <>
+__device__ __forceinline__ void to_out<bf16>(float a, float b, bf16* to) {
+  const v2bf v = __builtin_convertvector((v2f{a, b}), v2bf);
+  __builtin_memcpy(to, &v, 4);
+}
+
+// The gradient of a row's scores first .. last - 1, of which `part` holds the first (whole: all); c is 0 where
+// the row takes no part.
+struct Slope {
+  float by, each, max, scale;
+  int t;
+  bool any;
+  __device__ __forceinline__ Slope(const LossArgs& a, int n, const Answer& r, float c) {
+    any = r.there && c != 0.0f;
+    by = any ? c * r.cooling : 0.0f;
+    each = any ? -by / r.all.sum : 0.0f;
+    max = r.all.max, scale = r.cooling * kLog2e, t = a.tokens[n];
+  }
+};
+template <typename In, typename Out, int R>
+__device__ __forceinline__ void write_part(const Part<In, R>& part, const Slope& s, Out* to, int first, int last) {
+  constexpr int E = kEach<In>;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int from = first + r * (int)blockDim.x * E, i = from + (int)threadIdx.x * E;
+    if (!Part<In, R>::has(r, first, last)) continue;
     float v[E];
-    const bool whole = i + E <= last;
-    if (!any) {
+    if (s.any) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = s.each * power((part.score(r, e) - s.max) * s.scale);
+      if (s.t >= i && s.t < i + E) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] += i + e == s.t ? s.by : 0.0f;
+      }
+    } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = 0.0f;
-    } else {
-      if (whole) {
-        load_scores<E>(row + i, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = i + e < last ? score_of(row[i + e]) : -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = each * exp2f((v[e] - r.all.max) * scale) + (i + e == t ? by : 0.0f);
     }
-    Out raw[E];
+    Out out[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) raw[e] = from_float<Out>(v[e]);
-    if (whole) {
-      __builtin_memcpy(to + i, raw, sizeof raw);
+    for (int e = 0; e < E; e += 2) to_out<Out>(v[e], v[e + 1], out + e);
+    if (from + (int)blockDim.x * E <= last) {
+      __builtin_memcpy(to + i, out, sizeof out);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (i + e < last) to[i + e] = raw[e];
+        if (i + e < last) to[i + e] = out[e];
     }
+  }
+}
+template <typename In, typename Out, int R>
+__device__ __forceinline__ void write_grad(const LossArgs& a, int n, int first, int last, const Slope& s) {
+  const In* row = (const In*)a.scores + n * a.stride;
+  Out* to = (Out*)a.grad + n * a.grad_stride;
+  for (int from = first; from < last; from += R * (int)blockDim.x * kEach<In>) {
+    Part<In, R> part;
+    if (s.any) part.load(row, from, last);
+    write_part<In, Out, R>(part, s, to, from, last);
   }
 }
 
 // A slice of a row, after stats_kernel, and after pair_kernel for preferences.
-template <typename In, typename Out, bool POLICY>
-__global__ __launch_bounds__(kMaxThreads) void grad_kernel(LossArgs a) {
+template <typename In, typename Out, bool POLICY, int THREADS, int R>
+__global__ __launch_bounds__(THREADS) void grad_kernel(LossArgs a) {
   const int n = blockIdx.y, first = blockIdx.x * a.slice, last = first + a.slice < a.V ? first + a.slice : a.V;
   const Answer r = answer_of(a, n);
   float c;
@@ -240,26 +341,37 @@ __global__ __launch_bounds__(kMaxThreads) void grad_kernel(LossArgs a) {
   } else {
     c = a.slope[n];
   }
-  write_grad<In, Out>(a, n, first, last, r, c);
+  write_grad<In, Out, R>(a, n, first, last, Slope(a, n, r, c));
 }
 
-// A policy loss's whole row.
-template <typename In, typename Out>
-__global__ __launch_bounds__(kMaxThreads) void policy_kernel(LossArgs a) {
-  __shared__ Stats part[kMaxThreads / kWave];
+// A policy loss's whole row; ONCE: it is in the threads' registers from its one reading to its gradient.
+template <typename In, typename Out, int THREADS, int R, bool ONCE>
+__global__ __launch_bounds__(THREADS) void policy_kernel(LossArgs a) {
+  __shared__ Stats part[THREADS / kWave];
   const int n = blockIdx.x;
   const In* row = (const In*)a.scores + n * a.stride;
   const int t = a.tokens[n];
   const float scale = cooling(a, n) * kLog2e;
   const float z = t >= 0 && t < a.V ? score_of(row[t]) : -INFINITY;
-  const Stats all = block_stats(own_stats(row, 0, a.V, scale), scale, part);
-  const Answer r = answer_of(a, n, z, all);
+  Part<In, R> held;
+  Stats own;
+  if (ONCE) {
+    held.load(row, 0, a.V);
+    own = held.stats(0, a.V, scale);
+  } else {
+    own = own_stats<In, R>(row, 0, a.V, scale);
+  }
+  const Answer r = answer_of(a, n, z, block_stats(own, scale, part));
   const Loss loss = policy(a, n, r);
   if (threadIdx.x == 0) {
     a.losses[n] = loss.value;
     a.logprobs[n] = r.lp;
   }
-  write_grad<In, Out>(a, n, 0, a.V, r, loss.slope);
+  const Slope s(a, n, r, loss.slope);
+  if (ONCE)
+    write_part<In, Out, R>(held, s, (Out*)a.grad + n * a.grad_stride, 0, a.V);
+  else
+    write_grad<In, Out, R>(a, n, 0, a.V, s);
 }
 
 // A pair of sequences a block: their log probabilities, the loss, and its derivative for their rows.
@@ -308,7 +420,20 @@ __global__ __launch_bounds__(kPairThreads) void pair_kernel(LossArgs a) {
 }
 
 // --------------------------------------------------------------------------------------- host
-int threads_of(int64_t scores) { return scores <= 1024 ? 64 : scores <= 16384 ? 256 : 1024; }
+// launch(threads, 16 bytes that each has of a row at once, whether that is all of it).
+template <typename In, typename Launch>
+hipError_t shaped(int64_t scores, Launch launch) {
+  const int64_t pieces = (scores + kEach<In> - 1) / kEach<In>;
+  if (pieces <= 64 * 4) return launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{}, std::true_type{});
+  if (pieces <= 256 * 4) return launch(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{}, std::true_type{});
+  if (pieces <= 256 * 16)
+    return launch(std::integral_constant<int, 256>{}, std::integral_constant<int, 16>{}, std::true_type{});
+  if (pieces <= 512 * 16)
+    return launch(std::integral_constant<int, 512>{}, std::integral_constant<int, 16>{}, std::true_type{});
+  if (pieces <= 512 * 32)
+    return launch(std::integral_constant<int, 512>{}, std::integral_constant<int, 32>{}, std::true_type{});
+  return launch(std::integral_constant<int, 512>{}, std::integral_constant<int, 16>{}, std::false_type{});
+}
 
 // Slices of a row: rows alone fill the 256 CUs, or a slice would have less than 4096 scores.
 int slices_of(int64_t N, int64_t V) {
@@ -320,22 +445,27 @@ int slices_of(int64_t N, int64_t V) {
 int64_t workspace_bytes_of(int64_t N, int64_t slices) { return N * (slices * 8 + 8); }
 
 template <typename In, typename Out, bool POLICY>
-hipError_t launch_loss(LossArgs a, hipStream_t s) {
-  if (POLICY && a.slices == 1) {
-    policy_kernel<In, Out><<<a.N, threads_of(a.V), 0, s>>>(a);
-    return hipGetLastError();
-  }
+hipError_t launch_loss(const LossArgs& a, hipStream_t s) {
+  if (POLICY && a.slices == 1)
+    return shaped<In>(a.V, [&](auto threads, auto r, auto once) {
+      constexpr int T = decltype(threads)::value, R = decltype(r)::value;
+      policy_kernel<In, Out, T, R, decltype(once)::value><<<a.N, T, 0, s>>>(a);
+      return hipGetLastError();
+    });
   const dim3 grid(a.slices, a.N);
-  const int threads = threads_of(a.slice);
-  stats_kernel<In><<<grid, threads, 0, s>>>(a);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && !POLICY) {
-    pair_kernel<<<a.pairs, kPairThreads, 0, s>>>(a);
-    e = hipGetLastError();
-  }
-  if (e != hipSuccess) return e;
-  grad_kernel<In, Out, POLICY><<<grid, threads, 0, s>>>(a);
-  return hipGetLastError();
+  return shaped<In>(a.slice, [&](auto threads, auto r, auto) {
+    constexpr int T = decltype(threads)::value, R = decltype(r)::value > 16 ? 16 : decltype(r)::value;
+    stats_kernel<In, T, R><<<grid, T, 0, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && !POLICY) {
+      pair_kernel<<<a.pairs, kPairThreads, 0, s>>>(a);
+      e = hipGetLastError();
+    }
+    if (e != hipSuccess) return e;
+    constexpr int G = R > 8 ? 8 : R;  // nothing is kept: fewer registers, more blocks
+    grad_kernel<In, Out, POLICY, T, G><<<grid, T, 0, s>>>(a);
+    return hipGetLastError();
+  });
 }
 
 template <typename In, bool POLICY>

@@ -128,7 +128,7 @@ def adapt_gradient(grad: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: 
     d_down_adapter, d_down_rank = _adapters(d_down, "out[0]", w, (M, r, C), device)
     d_up_adapter, d_up_output = _adapters(d_up, "out[1]", w, (M, K, r), device)
     _changed((d_down, d_up))
-    need, workspace = _workspace(lib.ytm_adapt_gradient_workspace, grad.device, N, K, M, r)
+    need, workspace = _workspace(lib.ytm_adapt_gradient_workspace, grad.device, N, C, K, M, r)
     _call(lib.ytm_adapt_gradient, device, grad.data_ptr(), dtype, grad.stride(0), N, K, x.data_ptr(), x_type,
           x.stride(0), C, up.data_ptr(), up_adapter, up_output, _FLOATS[w], M, r, which, scale, hidden.data_ptr(),
           hidden.stride(0), d_down.data_ptr(), d_down_adapter, d_down_rank, d_up.data_ptr(), d_up_adapter, d_up_output,
