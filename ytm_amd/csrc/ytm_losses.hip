@@ -70,13 +70,14 @@ __device__ __forceinline__ float cooling(const LossArgs& a, int n) {
   return t <= 0.0f ? 1.0f : 1.0f / (t >= FLT_MIN ? t : FLT_MIN);
 }
 
-// A row's maximum and its sum of exp((score - maximum) / temperature), in powers of two.
+// Of some of a row's scores: one of them, or near them, and their sum of exp((score - it) / temperature), in powers of
+// two; -inf and 0 where none is above -inf.
 struct Stats {
   float max, sum;
   __device__ __forceinline__ void add(const Stats& o, float scale) {
     if (o.max == -INFINITY) return;
     if (o.max > max) {
-      sum = sum * power((max - o.max) * scale) + o.sum;  // max may be -inf, sum is 0 then
+      sum = max == -INFINITY ? o.sum : sum * power((max - o.max) * scale) + o.sum;
       max = o.max;
     } else {
       sum += o.sum * power((o.max - max) * scale);
@@ -87,6 +88,7 @@ struct Stats {
 // A thread's part of a row: R times 16 bytes, as they are in memory, every thread's one after the other; past
 // the last score -inf.  All are asked for before the first is used, and a row that fits is read
 // once.
+constexpr float kWholes = 0x1p22f;  // whole numbers below it are exact, and their neighbours a quarter apart
 template <typename In>
 constexpr int kEach = 16 / sizeof(In);
 template <typename In>
@@ -145,25 +147,41 @@ struct Part {
   // whether any thread has scores in place r
   __device__ __forceinline__ static bool has(int r, int first, int last) { return first + r * (int)blockDim.x * E < last; }
 
+  // The sum is made relative to the largest of the thread's first few scores, or to 0, in one pass and with one rounding
+  // of each exponent: score * scale less a whole number near that score's.  Where that loses it (a NaN, an
+  // infinity, scores far above or all far below: a sum above 2^60 or below 2^-60), relative to the largest.
   __device__ __forceinline__ Stats stats(int first, int last, float scale) {
-    float max = -INFINITY;
+    float near = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (has(r, first, last)) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) max = fmaxf(max, score(r, e));
-      }
-    Stats s{max, 0.0f};
-    again();
-    if (max == -INFINITY) return s;
+    for (int e = 0; e < E; ++e) near = fmaxf(near, half_of(v[0][e / kPerWord], e % kPerWord, In{}));
+    near = near == -INFINITY ? 0.0f : near;
+    const float whole = rintf(near * scale);
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int r = 0; r < R; ++r)
       if (has(r, first, last)) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum[e % 4] += power((score(r, e) - max) * scale);
+        for (int e = 0; e < E; ++e)
+          sum[e % 4] += power(__builtin_fmaf(half_of(v[r][e / kPerWord], e % kPerWord, In{}), scale, -whole));
       }
-    s.sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    Stats s{near, ((sum[0] + sum[1]) + (sum[2] + sum[3])) * power(__builtin_fmaf(-near, scale, whole))};
+    again();
+    if (s.sum > 0x1p-60f && s.sum < 0x1p60f && fabsf(whole) < kWholes) return s;
+    s = Stats{-INFINITY, 0.0f};
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (has(r, first, last)) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s.max = fmaxf(s.max, score(r, e));
+      }
+    again();
+    if (s.max == -INFINITY) return s;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (has(r, first, last)) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s.sum += power((score(r, e) - s.max) * scale);
+      }
     again();
     return s;
   }
@@ -173,11 +191,17 @@ struct Part {
 template <typename In, int R>
 __device__ __forceinline__ Stats own_stats(const In* row, int first, int last, float scale) {
   Stats s{-INFINITY, 0.0f};
-  for (int from = first; from < last; from += R * (int)blockDim.x * kEach<In>) {
-    Part<In, R> part;
-    part.load(row, from, last);
-    s.add(part.stats(from, last, scale), scale);
+  if (first >= last) return s;
+  const int step = R * (int)blockDim.x * kEach<In>;
+  Part<In, R> now;
+  now.load(row, first, last);
+  for (; first + step < last; first += step) {  // the next part is on its way
+    Part<In, R> next;
+    next.load(row, first + step, last);
+    s.add(now.stats(first, last, scale), scale);
+    now = next;
   }
+  s.add(now.stats(first, last, scale), scale);
   return s;
 }
 
@@ -273,14 +297,17 @@ __device__ __forceinline__ void to_out<bf16>(float a, float b, bf16* to) {
 // The gradient of a row's scores first .. last - 1, of which `part` holds the first (whole: all); c is 0 where
 // the row takes no part.
 struct Slope {
-  float by, each, max, scale;
+  float by, each, max, scale, whole;
   int t;
-  bool any;
+  bool any, far;  // far: an exponent is no float's, and only differences are
   __device__ __forceinline__ Slope(const LossArgs& a, int n, const Answer& r, float c) {
     any = r.there && c != 0.0f;
     by = any ? c * r.cooling : 0.0f;
     each = any ? -by / r.all.sum : 0.0f;
     max = r.all.max, scale = r.cooling * kLog2e, t = a.tokens[n];
+    whole = rintf(max * scale);
+    far = !(fabsf(whole) < kWholes);
+    if (!far) each *= power(__builtin_fmaf(-max, scale, whole));
   }
 };
 template <typename In, typename Out, int R>
@@ -292,8 +319,13 @@ __device__ __forceinline__ void write_part(const Part<In, R>& part, const Slope&
     if (!Part<In, R>::has(r, first, last)) continue;
     float v[E];
     if (s.any) {
+      if (s.far) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = s.each * power((part.score(r, e) - s.max) * s.scale);
+        for (int e = 0; e < E; ++e) v[e] = s.each * power((part.score(r, e) - s.max) * s.scale);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = s.each * power(__builtin_fmaf(part.score(r, e), s.scale, -s.whole));
+      }
       if (s.t >= i && s.t < i + E) {
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] += i + e == s.t ? s.by : 0.0f;
@@ -454,8 +486,8 @@ hipError_t launch_loss(const LossArgs& a, hipStream_t s) {
     });
   const dim3 grid(a.slices, a.N);
   return shaped<In>(a.slice, [&](auto threads, auto r, auto) {
-    constexpr int T = decltype(threads)::value, R = decltype(r)::value > 16 ? 16 : decltype(r)::value;
-    stats_kernel<In, T, R><<<grid, T, 0, s>>>(a);
+    constexpr int T = decltype(threads)::value, R = decltype(r)::value;
+    stats_kernel<In, T, 4><<<grid, T, 0, s>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && !POLICY) {
       pair_kernel<<<a.pairs, kPairThreads, 0, s>>>(a);
