@@ -22,6 +22,7 @@ namespace ytm {
 namespace {
 
 constexpr int kWave = 64;
+constexpr int kMaxWaves = 8;  // of a block
 constexpr int kMaxSlices = 32;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -357,20 +358,104 @@ __device__ __forceinline__ void write_grad(const LossArgs& a, int n, int first, 
   }
 }
 
-// A slice of a row, after stats_kernel, and after pair_kernel for preferences.
-template <typename In, typename Out, bool POLICY, int THREADS, int R>
+// A pair of sequences: their rows and log probabilities, made by the whole block, the loss, and its derivative by
+// the log probability of the first.
+struct Pair {
+  int begin[2], end[2];
+  double said[2];
+  float loss, slope;
+  __device__ __forceinline__ Pair(const LossArgs& a, int pair, double (*part)[kMaxWaves]) {
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      begin[side] = a.starts[2 * pair + side];
+      end[side] = a.starts[2 * pair + side + 1];
+      begin[side] = begin[side] < 0 ? 0 : begin[side];
+      end[side] = end[side] > a.N ? a.N : end[side];
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      double sum = 0.0;
+      for (int64_t n = begin[side] + (int64_t)threadIdx.x; n < end[side]; n += blockDim.x)
+        sum += (double)answer_of(a, (int)n).lp;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
+      if (threadIdx.x % kWave == 0) part[side][threadIdx.x / kWave] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      said[side] = 0.0;
+      for (int w = 0; w < (int)blockDim.x / kWave; ++w) said[side] += part[side][w];
+    }
+    const float* ref = a.sequence_reference + 2 * pair;
+    const float m = (float)((double)a.beta * ((said[0] - (double)ref[0]) - (said[1] - (double)ref[1])));
+    const float small = expf(-fabsf(m));  // softplus(m) = max(m, 0) + log(1 + exp(-|m|)), sigmoid(m) alike
+    const float share = 1.0f / (float)a.pairs, log1 = log1pf(small);
+    const float won = (m >= 0.0f ? 1.0f : small) / (1.0f + small), lost = (m >= 0.0f ? small : 1.0f) / (1.0f + small);
+    slope = share * a.beta * (a.smoothing * won - (1.0f - a.smoothing) * lost);
+    loss = share * ((1.0f - a.smoothing) * (fmaxf(-m, 0.0f) + log1) + a.smoothing * (fmaxf(m, 0.0f) + log1));
+  }
+  __device__ __forceinline__ void write(const LossArgs& a, int pair) const {
+    if (threadIdx.x != 0) return;
+    a.losses[pair] = loss;
+    a.logprobs[2 * pair] = (float)said[0];
+    a.logprobs[2 * pair + 1] = (float)said[1];
+  }
+};
+
+constexpr int kPairThreads = 256;
+__global__ __launch_bounds__(kPairThreads) void pair_kernel(LossArgs a) {
+  __shared__ double part[2][kMaxWaves];
+  const Pair pair(a, blockIdx.x, part);
+  pair.write(a, blockIdx.x);
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+    for (int64_t n = pair.begin[side] + (int64_t)threadIdx.x; n < pair.end[side]; n += kPairThreads)
+      a.slope[n] = side ? -pair.slope : pair.slope;
+}
+
+// Row n's sequence: the last that begins at or before it; 2 pairs or -1 where it is in none.
+__device__ __forceinline__ int sequence_of(const LossArgs& a, int n, int* count) {
+  int before = 0;
+  for (int i = threadIdx.x; i < 2 * a.pairs + 1; i += blockDim.x) before += a.starts[i] <= n;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) before += __shfl_xor(before, d);
+  if (threadIdx.x % kWave == 0) count[threadIdx.x / kWave] = before;
+  __syncthreads();
+  int all = 0;
+  for (int w = 0; w < (int)blockDim.x / kWave; ++w) all += count[w];
+  return __builtin_amdgcn_readfirstlane(all) - 1;
+}
+
+// A slice of a row, after stats_kernel.  What its loss is to it: a policy's, that of a preference after pair_kernel,
+// or that of a preference whose pair each of its blocks looks at itself, with a block more for each pair.
+enum Kind { kPolicy, kPreference, kFewPreferences };
+template <typename In, typename Out, Kind KIND, int THREADS, int R>
 __global__ __launch_bounds__(THREADS) void grad_kernel(LossArgs a) {
   const int n = blockIdx.y, first = blockIdx.x * a.slice, last = first + a.slice < a.V ? first + a.slice : a.V;
+  float c = 0.0f;
+  if constexpr (KIND == kFewPreferences) {
+    __shared__ double part[2][kMaxWaves];
+    __shared__ int count[kMaxWaves];
+    if (n >= a.N) {
+      if (blockIdx.x == 0) Pair(a, n - a.N, part).write(a, n - a.N);
+      return;
+    }
+    const int sequence = sequence_of(a, n, count);
+    if (sequence >= 0 && sequence < 2 * a.pairs) {
+      const Pair pair(a, sequence / 2, part);
+      c = sequence % 2 ? -pair.slope : pair.slope;
+    }
+  }
   const Answer r = answer_of(a, n);
-  float c;
-  if (POLICY) {
+  if constexpr (KIND == kPolicy) {
     const Loss loss = policy(a, n, r);
     c = loss.slope;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
       a.losses[n] = loss.value;
       a.logprobs[n] = r.lp;
     }
-  } else {
+  } else if constexpr (KIND == kPreference) {
     c = a.slope[n];
   }
   write_grad<In, Out, R>(a, n, first, last, Slope(a, n, r, c));
@@ -406,51 +491,6 @@ __global__ __launch_bounds__(THREADS) void policy_kernel(LossArgs a) {
     write_grad<In, Out, R>(a, n, 0, a.V, s);
 }
 
-// A pair of sequences a block: their log probabilities, the loss, and its derivative for their rows.
-constexpr int kPairThreads = 256;
-__global__ __launch_bounds__(kPairThreads) void pair_kernel(LossArgs a) {
-  __shared__ double part[2][kPairThreads / kWave];
-  const int pair = blockIdx.x;
-  int begin[2], end[2];
-  double said[2];
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    begin[side] = a.starts[2 * pair + side];
-    end[side] = a.starts[2 * pair + side + 1];
-    begin[side] = begin[side] < 0 ? 0 : begin[side];
-    end[side] = end[side] > a.N ? a.N : end[side];
-    double sum = 0.0;
-    for (int64_t n = begin[side] + (int64_t)threadIdx.x; n < end[side]; n += kPairThreads)
-      sum += (double)answer_of(a, (int)n).lp;
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d);
-    if (threadIdx.x % kWave == 0) part[side][threadIdx.x / kWave] = sum;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    said[side] = 0.0;
-    for (int w = 0; w < kPairThreads / kWave; ++w) said[side] += part[side][w];
-  }
-  const float* ref = a.sequence_reference + 2 * pair;
-  const float m = (float)((double)a.beta * ((said[0] - (double)ref[0]) - (said[1] - (double)ref[1])));
-  const float small = expf(-fabsf(m));  // softplus(m) = max(m, 0) + log(1 + exp(-|m|)), sigmoid(m) alike
-  const float share = 1.0f / (float)a.pairs;
-  const float won = (m >= 0.0f ? 1.0f : small) / (1.0f + small), lost = (m >= 0.0f ? small : 1.0f) / (1.0f + small);
-  const float c = share * a.beta * (a.smoothing * won - (1.0f - a.smoothing) * lost);
-  if (threadIdx.x == 0) {
-    const float log1 = log1pf(small);
-    a.losses[pair] =
-        share * ((1.0f - a.smoothing) * (fmaxf(-m, 0.0f) + log1) + a.smoothing * (fmaxf(m, 0.0f) + log1));
-    a.logprobs[2 * pair] = (float)said[0];
-    a.logprobs[2 * pair + 1] = (float)said[1];
-  }
-#pragma unroll
-  for (int side = 0; side < 2; ++side)
-    for (int64_t n = begin[side] + (int64_t)threadIdx.x; n < end[side]; n += kPairThreads)
-      a.slope[n] = side ? -c : c;
-}
-
 // --------------------------------------------------------------------------------------- host
 // launch(threads, 16 bytes that each has of a row at once, whether that is all of it).
 template <typename In, typename Launch>
@@ -467,12 +507,16 @@ hipError_t shaped(int64_t scores, Launch launch) {
   return launch(std::integral_constant<int, 512>{}, std::integral_constant<int, 16>{}, std::false_type{});
 }
 
-// Slices of a row: rows alone fill the 256 CUs, or a slice would have less than 4096 scores.
+// Slices of a row: rows alone fill the 256 CUs, or a slice would have less than 8192 scores; a row of fewer than 32768
+// is one block's.
 int slices_of(int64_t N, int64_t V) {
-  int64_t slices = N > 0 ? 512 / N : 1;
-  if (slices > V / 4096) slices = V / 4096;
+  int64_t slices = N > 0 && V >= 32768 ? 512 / N : 1;
+  if (slices > V / 8192) slices = V / 8192;
   return slices < 1 ? 1 : slices > kMaxSlices ? kMaxSlices : (int)slices;
 }
+
+// Whether each row's block finds its pair's loss by itself, which saves a launch.
+bool few_pairs(int64_t N, int64_t pairs) { return N <= 256 && pairs <= 128; }
 
 int64_t workspace_bytes_of(int64_t N, int64_t slices) { return N * (slices * 8 + 8); }
 
@@ -489,13 +533,18 @@ hipError_t launch_loss(const LossArgs& a, hipStream_t s) {
     constexpr int T = decltype(threads)::value, R = decltype(r)::value;
     stats_kernel<In, T, 4><<<grid, T, 0, s>>>(a);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess && !POLICY) {
-      pair_kernel<<<a.pairs, kPairThreads, 0, s>>>(a);
-      e = hipGetLastError();
-    }
     if (e != hipSuccess) return e;
     constexpr int G = R > 8 ? 8 : R;  // nothing is kept: fewer registers, more blocks
-    grad_kernel<In, Out, POLICY, T, G><<<grid, T, 0, s>>>(a);
+    if (POLICY) {
+      grad_kernel<In, Out, kPolicy, T, G><<<grid, T, 0, s>>>(a);
+    } else if (few_pairs(a.N, a.pairs)) {
+      grad_kernel<In, Out, kFewPreferences, T, G><<<dim3(a.slices, a.N + a.pairs), T, 0, s>>>(a);
+    } else {
+      pair_kernel<<<a.pairs, kPairThreads, 0, s>>>(a);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      grad_kernel<In, Out, kPreference, T, G><<<grid, T, 0, s>>>(a);
+    }
     return hipGetLastError();
   });
 }

@@ -22,28 +22,29 @@ ytm_preference_loss and ytm_adamw in include/ytm.h.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 from torch.autograd import forward_ad as _forward_ad
 
 from ._lib import DTYPE_BITS, AdamWTensor, check, lib
-from .decode import (_call, _changed, _CLAUSES, _FLOATS, _no_tangents, _per_row, _refuse, _result, _rows_of, _Tensor,
-                     _workspace)
+from .decode import (_call, _changed, _CLAUSES, _FLOATS, _no_tangents, _per_row, _refuse, _result, _rows_of, _Tensor)
 
 _BLOCK = 256  # elements of a state in 8 bits that share a scale
 
 
-def _adapters(t, name: str, dtype: torch.dtype | None, shape: tuple, device: int) -> tuple[int, int]:
-    """(distance from an adapter to the next, from a row to the next) of adapters (M, rows, width); `shape` says
-    None where any size fits."""
-    if not (isinstance(t, _Tensor) and t.get_device() == device and t.dim() == 3
-            and (t.dtype is dtype or dtype is None and t.dtype in _FLOATS)
-            and all(n is None or n == m for n, m in zip(shape, t.shape))
-            and (t.stride(2) == 1 or t.shape[2] < 2) and not t.requires_grad):
-        fits = isinstance(t, _Tensor) and t.dim() == 3 and all(n is None or n == m for n, m in zip(shape, t.shape))
-        said = str(shape).replace("None", "*")
-        _refuse(t, name, (3,), _FLOATS if dtype is None else dtype, "" if fits else said, device)
+def _adapters(t, name: str, dtype: torch.dtype | None, shape: tuple | None, device: int) -> tuple[int, int]:
+    """(distance from an adapter to the next, from a row to the next) of adapters (M, rows, width); any where
+    `dtype` or `shape` is None."""
+    if isinstance(t, _Tensor) and t.get_device() == device and t.dim() == 3 and not t.requires_grad:
+        per_adapter, per_row, one = t.stride()
+        adapters, rows, width = size = t.shape
+        if ((size == shape or shape is None) and (t.dtype is dtype or dtype is None and t.dtype in _FLOATS)
+                and (one == 1 or width < 2)):
+            return (per_adapter if adapters > 1 else 0), (per_row if rows > 1 else 0)
+    fits = shape is None or isinstance(t, _Tensor) and tuple(t.shape) == shape
+    _refuse(t, name, (3,), _FLOATS if dtype is None else dtype, "" if fits else str(shape), device)
     return (t.stride(0) if t.shape[0] > 1 else 0), (t.stride(1) if t.shape[1] > 1 else 0)
 
 
@@ -55,6 +56,21 @@ def _clauses(x, C: int, rows: int, device: int) -> int:
         fits = isinstance(x, _Tensor) and tuple(x.shape) == (rows, width)
         _refuse(x, "x", (2,), _CLAUSES, "" if fits else f"({rows}, {width})", device)
     return _CLAUSES[x.dtype]
+
+
+@functools.lru_cache(maxsize=4096)
+def _bytes(name: str, *args: int) -> int:
+    """What the library's `name` says that a workspace takes."""
+    need = ctypes.c_int64()
+    check(getattr(lib, name)(*args, need))
+    return need.value
+
+
+def _hidden(t, rows: int, rank: int, device: int) -> None:
+    if not (isinstance(t, _Tensor) and t.dtype is torch.float32 and t.get_device() == device and t.shape == (rows, rank)
+            and (t.stride(1) == 1 or rank < 2) and not t.requires_grad):
+        fits = isinstance(t, _Tensor) and tuple(t.shape) == (rows, rank)
+        _refuse(t, "hidden", (2,), torch.float32, "" if fits else f"({rows}, {rank})", device)
 
 
 def _number(v, name: str) -> float:
@@ -76,7 +92,7 @@ def adapt(scores: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.T
     if _forward_ad._current_level >= 0:
         _no_tangents(scores=scores, x=x, down=down, up=up, hidden=hidden, out=out)
     dtype, N, K, device = _rows_of(scores, "scores", _FLOATS)
-    down_adapter, down_rank = _adapters(down, "down", None, (None, None, None), device)
+    down_adapter, down_rank = _adapters(down, "down", None, None, device)
     M, r, C = down.shape
     up_adapter, up_output = _adapters(up, "up", down.dtype, (M, K, r), device)
     x_type = _clauses(x, C, N, device)
@@ -84,13 +100,11 @@ def adapt(scores: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.T
     if which is None:
         raise TypeError("which must be a torch tensor.")
     if hidden is not None:
-        if not (isinstance(hidden, _Tensor) and hidden.dtype is torch.float32 and hidden.get_device() == device
-                and hidden.shape == (N, r) and (hidden.stride(1) == 1 or r < 2) and not hidden.requires_grad):
-            fits = isinstance(hidden, _Tensor) and tuple(hidden.shape) == (N, r)
-            _refuse(hidden, "hidden", (2,), torch.float32, "" if fits else f"({N}, {r})", device)
+        _hidden(hidden, N, r, device)
         _changed((hidden,))
     out, out_type = _result(out, (N, K), device)
-    need, workspace = _workspace(lib.ytm_adapt_workspace, scores.device, N, C, M, r)
+    need = _bytes("ytm_adapt_workspace", N, C, M, r)
+    workspace = torch.empty(need, dtype=torch.uint8, device=scores.device) if need else None
     _call(lib.ytm_adapt, device, scores.data_ptr(), dtype, scores.stride(0), N, K, x.data_ptr(), x_type, x.stride(0), C,
           down.data_ptr(), down_adapter, down_rank, up.data_ptr(), up_adapter, up_output, _FLOATS[down.dtype], M, r,
           which, scale, None if hidden is None else hidden.data_ptr(), 0 if hidden is None else hidden.stride(0),
@@ -110,7 +124,7 @@ def adapt_gradient(grad: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: 
         if out is not None:
             _no_tangents(down_gradient=out[0], up_gradient=out[1])
     dtype, N, K, device = _rows_of(grad, "grad", _FLOATS)
-    _adapters(down, "down", None, (None, None, None), device)
+    _adapters(down, "down", None, None, device)
     M, r, C = down.shape
     w = down.dtype
     up_adapter, up_output = _adapters(up, "up", w, (M, K, r), device)
@@ -118,17 +132,15 @@ def adapt_gradient(grad: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: 
     which = _per_row(which, "which", torch.int32, N, device)
     if which is None:
         raise TypeError("which must be a torch tensor.")
-    if not (isinstance(hidden, _Tensor) and hidden.dtype is torch.float32 and hidden.get_device() == device
-            and hidden.shape == (N, r) and (hidden.stride(1) == 1 or r < 2) and not hidden.requires_grad):
-        fits = isinstance(hidden, _Tensor) and tuple(hidden.shape) == (N, r)
-        _refuse(hidden, "hidden", (2,), torch.float32, "" if fits else f"({N}, {r})", device)
+    _hidden(hidden, N, r, device)
     if out is None:
         out = torch.empty((M, r, C), dtype=w, device=grad.device), torch.empty((M, K, r), dtype=w, device=grad.device)
     d_down, d_up = out
     d_down_adapter, d_down_rank = _adapters(d_down, "out[0]", w, (M, r, C), device)
     d_up_adapter, d_up_output = _adapters(d_up, "out[1]", w, (M, K, r), device)
     _changed((d_down, d_up))
-    need, workspace = _workspace(lib.ytm_adapt_gradient_workspace, grad.device, N, C, K, M, r)
+    need = _bytes("ytm_adapt_gradient_workspace", N, C, K, M, r)
+    workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
     _call(lib.ytm_adapt_gradient, device, grad.data_ptr(), dtype, grad.stride(0), N, K, x.data_ptr(), x_type,
           x.stride(0), C, up.data_ptr(), up_adapter, up_output, _FLOATS[w], M, r, which, scale, hidden.data_ptr(),
           hidden.stride(0), d_down.data_ptr(), d_down_adapter, d_down_rank, d_up.data_ptr(), d_up_adapter, d_up_output,
@@ -167,8 +179,9 @@ def policy_loss(scores: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, a
         raise ValueError("kl needs a reference.")
     out, out_type = _result(out, (N, V), device)
     where = scores.device
-    losses, logprobs = torch.empty(N, device=where), torch.empty(N, device=where)
-    need, workspace = _workspace(lib.ytm_policy_loss_workspace, where, N, V)
+    losses, logprobs = (torch.empty(N, dtype=torch.float32, device=where) for _ in range(2))
+    need = _bytes("ytm_policy_loss_workspace", N, V)
+    workspace = torch.empty(need, dtype=torch.uint8, device=where) if need else None
     _call(lib.ytm_policy_loss, device, scores.data_ptr(), dtype, scores.stride(0), N, V, tokens, old, advantages,
           reference, kl, clip, clip if clip_high is None else clip_high, weights, temperature, losses.data_ptr(),
           logprobs.data_ptr(), out.data_ptr(), out_type, out.stride(0), workspace.data_ptr() if need else None, need)
@@ -201,8 +214,9 @@ def preference_loss(scores: torch.Tensor, tokens: torch.Tensor, starts: torch.Te
     temperature = _per_row(temperature, "temperature", torch.float32, N, device)
     out, out_type = _result(out, (N, V), device)
     where = scores.device
-    losses, logprobs = torch.empty(pairs, device=where), torch.empty(2 * pairs, device=where)
-    need, workspace = _workspace(lib.ytm_preference_loss_workspace, where, N, V)
+    losses, logprobs = (torch.empty(n, dtype=torch.float32, device=where) for n in (pairs, 2 * pairs))
+    need = _bytes("ytm_preference_loss_workspace", N, V)
+    workspace = torch.empty(need, dtype=torch.uint8, device=where) if need else None
     _call(lib.ytm_preference_loss, device, scores.data_ptr(), dtype, scores.stride(0), N, V, tokens, starts, pairs,
           reference, beta, smoothing, temperature, losses.data_ptr(), logprobs.data_ptr(), out.data_ptr(), out_type,
           out.stride(0), workspace.data_ptr() if need else None, need)
