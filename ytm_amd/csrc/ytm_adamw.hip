@@ -59,6 +59,13 @@ __device__ __forceinline__ uint32_t mixed(uint32_t h) {
   return h ^ h >> 16;
 }
 
+__device__ double power(double x, int64_t k) {
+  double r = 1.0;
+  for (; k > 0; k >>= 1, x *= x)
+    if (k & 1) r *= x;
+  return r;
+}
+
 // Counts the steps of the tensors that take one, and what follows from it, in double.
 __global__ __launch_bounds__(kThreads) void step_kernel(Tensor* tensors, int n, int64_t* steps, const uint8_t* active,
                                                         double rate, const float* rate_at, double beta1, double beta2,
@@ -72,173 +79,273 @@ __global__ __launch_bounds__(kThreads) void step_kernel(Tensor* tensors, int n, 
     if (rate_at) rate = *rate_at;
     s.beta1 = (float)beta1, s.rest1 = (float)(1.0 - beta1), s.beta2 = (float)beta2, s.rest2 = (float)(1.0 - beta2);
     s.keep = (float)(1.0 - rate * decay);
-    s.rate = (float)(rate / (1.0 - pow(beta1, (double)k)));
-    s.cool = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)k)));
+    s.rate = (float)(rate / (1.0 - power(beta1, k)));
+    s.cool = (float)(1.0 / sqrt(1.0 - power(beta2, k)));
     s.eps = (float)eps;
     s.key = mixed(mixed((uint32_t)k) ^ seed);
   }
   tensors[i].step = s;
 }
 
-// Random bits of element `place` in this step: 16 for each state, 16 for the parameter.
+// Random bits of element `place` + e (of four in a row, the first a multiple of four) in this step, 16 for
+// each state and for the parameter.
 struct Chances {
-  float first, second, parameter;
+  uint32_t first, second, parameter;
 };
-__device__ __forceinline__ Chances chances_of(uint64_t place, uint32_t key) {
-  const uint32_t a = mixed((uint32_t)place ^ key ^ (uint32_t)(place >> 32) * 0xC2B2AE35u), b = a * 0x9E3779B9u;
-  constexpr float k = 1.0f / 65536.0f;
-  return Chances{(float)(a & 0xFFFFu) * k, (float)(a >> 16) * k, (float)(b >> 16) * k};
+__device__ __forceinline__ Chances chances_of(uint64_t place, int e, uint32_t key) {
+  const uint32_t a = mixed((uint32_t)place + e ^ key ^ (uint32_t)(place >> 32) * 0xC2B2AE35u), b = a * 0x9E3779B9u;
+  return Chances{a & 0xFFFFu, a >> 16, b >> 16};
 }
-
-// The distance of the numbers of `fraction` bits and of at least 2^least at x >= 0, and its reciprocal.
-__device__ __forceinline__ void step_of(float x, int fraction, int least, float& step, float& inverse) {
-  int e = (int)(__float_as_uint(x) >> 23) - 127;
-  e = e < least ? least : e;
-  step = ldexpf(1.0f, e - fraction);
-  inverse = ldexpf(1.0f, fraction - e);
-}
+__device__ __forceinline__ float share_of(uint32_t chance) { return (float)chance * (1.0f / 65536.0f); }
 
 // x to a number of `fraction` bits and at least 2^least: down, or up with the chance of what is cut off.
-__device__ __forceinline__ float drawn_to(float x, float chance, int fraction, int least) {
-  float step, inverse;
-  step_of(fabsf(x), fraction, least, step, inverse);
-  return copysignf(floorf(fabsf(x) * inverse + chance) * step, x);
+__device__ __forceinline__ float drawn_to(float x, uint32_t chance, int fraction, int least) {
+  int e = (int)(__float_as_uint(x) >> 23 & 255u) - 127;
+  e = e < least ? least : e;
+  const float up = floorf(ldexpf(fabsf(x), fraction - e) + share_of(chance));
+  return copysignf(ldexpf(up, e - fraction), x);
 }
 
-__device__ __forceinline__ float stored(float v, float, float) { return v; }
-__device__ __forceinline__ f16 stored(float v, float chance, f16) {
+__device__ __forceinline__ float stored(float v, uint32_t, float) { return v; }
+__device__ __forceinline__ f16 stored(float v, uint32_t chance, f16) {
   return (f16)(v - v == 0.0f ? drawn_to(v, chance, 10, -14) : v);
 }
-__device__ __forceinline__ bf16 stored(float v, float chance, bf16) {
-  return from_float<bf16>(v - v == 0.0f ? drawn_to(v, chance, 7, -126) : v);
+// A bfloat16 is a float's upper half, subnormal numbers too: what the sum carries into it.
+__device__ __forceinline__ bf16 stored(float v, uint32_t chance, bf16) {
+  return v - v == 0.0f ? bf16{(uint16_t)(__float_as_uint(v) + chance >> 16)} : from_float<bf16>(v);
 }
+
+// Addresses from a table: of device memory, at a multiple of an element's size.
+#define YTM_DEVICE __attribute__((address_space(1)))
+template <typename T>
+__device__ __forceinline__ YTM_DEVICE T* device(const void* p) {
+  return (YTM_DEVICE T*)p;
+}
+template <int BYTES>
+struct Four;  // elements
+template <>
+struct Four<1> {
+  typedef uint8_t one;
+  typedef uint32_t type __attribute__((aligned(1)));
+};
+template <>
+struct Four<2> {
+  typedef uint16_t one;
+  typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2)));
+};
+template <>
+struct Four<4> {
+  typedef uint32_t one;
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
 
 template <typename T>
-__device__ __forceinline__ void load_each(const T* p, int left, float (&v)[kEach]) {
-  T raw[kEach];
+__device__ __forceinline__ void load_raw(YTM_DEVICE T* p, int left, T (&raw)[kEach]) {
+  typedef typename Four<sizeof(T)>::one One;
   if (left >= kEach) {
-    __builtin_memcpy(raw, p, sizeof raw);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) v[e] = to_float(raw[e]);
+    const auto v = *(YTM_DEVICE typename Four<sizeof(T)>::type*)p;
+    __builtin_memcpy(raw, &v, sizeof raw);
   } else {
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) v[e] = e < left ? to_float(p[e]) : 0.0f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store_each(T* p, int left, const T (&v)[kEach]) {
-  if (left >= kEach) {
-    __builtin_memcpy(p, v, sizeof v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      if (e < left) p[e] = v[e];
-  }
-}
-
-// An E4M3 float (sign, four bits of exponent, three of fraction; 2^-9 the least, 448 the largest, 127 a
-// NaN) of a number that is one, and back.
-__device__ __forceinline__ uint8_t code_of(float v) {
-  const uint32_t sign = __float_as_uint(v) >> 24 & 0x80u;
-  const float x = fabsf(v);
-  if (!(x <= 448.0f)) return (uint8_t)(sign | 0x7Fu);
-  if (x < 0.015625f) return (uint8_t)(sign | (uint32_t)(x * 512.0f));
-  return (uint8_t)(sign | ((__float_as_uint(x) >> 20) - (120u << 3)));
-}
-__device__ __forceinline__ float value_of(uint8_t c) {
-  const uint32_t m = c & 0x7Fu;
-  const float x = m == 0x7Fu ? __uint_as_float(0x7FC00000u)
-                  : m < 8    ? (float)m * (1.0f / 512.0f)
-                             : __uint_as_float((m + (120u << 3)) << 20);
-  return c & 0x80u ? -x : x;
-}
-
-// The exponent of a block's scale: 2^e 448 is the least such number that its largest magnitude does not
-// pass, and at least 2^-98, so that no product leaves what float32 holds.  What is not finite has no part.
-__device__ __forceinline__ int exponent_of(const float (&v)[kEach]) {
-  uint32_t most = 0;
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const uint32_t u = __float_as_uint(v[e]) & 0x7FFFFFFFu;
-    if (u < 0x7F800000u && u > most) most = u;
-  }
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const uint32_t o = __shfl_xor(most, d);
-    most = o > most ? o : most;
-  }
-  const int bits = (int)((most + 0x1FFFFFu) >> 23);
-  return (bits < 37 ? 37 : bits) - 135;
-}
-
-template <int BITS, typename P, typename G>
-__device__ __forceinline__ void update(const Tensor& t, const Step& s, int64_t i, int left) {
-  float p[kEach], g[kEach], m[kEach], v[kEach], root[kEach];
-  load_each((const P*)t.parameter + i, left, p);
-  load_each((const G*)t.gradient + i, left, g);
-  if (BITS == 32) {
-    load_each((const float*)t.first + i, left, m);
-    load_each((const float*)t.second + i, left, v);
-  } else {
-    uint8_t c[2][kEach] = {};
-    float scale[2] = {0.0f, 0.0f};
-    if (left > 0) {
-      scale[0] = t.first_scales[i / kBlock];
-      scale[1] = t.second_scales[i / kBlock];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const uint8_t* from = (const uint8_t*)(q ? t.second : t.first) + i;
-        if (left >= kEach) {
-          __builtin_memcpy(c[q], from, kEach);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kEach; ++e)
-            if (e < left) c[q][e] = from[e];
-        }
-      }
-    }
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      m[e] = value_of(c[0][e]) * scale[0];
-      v[e] = value_of(c[1][e]) * scale[1];
+      One v = 0;
+      if (e < left) v = ((YTM_DEVICE One*)p)[e];
+      __builtin_memcpy(&raw[e], &v, sizeof v);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load_each(YTM_DEVICE T* p, int left, float (&v)[kEach]) {
+  T raw[kEach];
+  load_raw(p, left, raw);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) v[e] = to_float(raw[e]);
+}
+template <typename T>
+__device__ __forceinline__ void store_each(YTM_DEVICE T* p, int left, const T (&v)[kEach]) {
+  typedef typename Four<sizeof(T)>::one One;
+  typename Four<sizeof(T)>::type all;
+  __builtin_memcpy(&all, v, sizeof v);
+  if (left >= kEach) {
+    *(YTM_DEVICE typename Four<sizeof(T)>::type*)p = all;
+  } else {
+    One one[kEach];
+    __builtin_memcpy(one, v, sizeof v);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (e < left) ((YTM_DEVICE One*)p)[e] = one[e];
+  }
+}
+
+// Four E4M3 floats (sign, four bits of exponent, three of fraction; 2^-9 the least, 448 the largest, 127 a NaN).
+__device__ __forceinline__ void values_of(const uint8_t (&from)[kEach], float (&v)[kEach]) {
+  uint32_t codes;
+  __builtin_memcpy(&codes, from, sizeof codes);
+  const auto low = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+  const auto high = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  v[0] = low[0], v[1] = low[1], v[2] = high[0], v[3] = high[1];
+}
+
+// Codes of a magnitude x up to 448: that below it, and whether it is one of the equally spaced ones near 0.  A normal
+// one's bits are the float's from its third of fraction on, less 120 of exponent.
+constexpr float kNormal = 0.015625f;
+__device__ __forceinline__ uint32_t normal_code(uint32_t bits) { return (bits >> 20) - (120u << 3); }
+
+// Down, or up with the chance of what is cut off.
+__device__ __forceinline__ uint32_t first_code(float m, uint32_t chance) {
+  const uint32_t u = __float_as_uint(m), x = u & 0x7FFFFFFFu;
+  const uint32_t normal = normal_code(x + (chance << 4));
+  const uint32_t small = (uint32_t)(__uint_as_float(x) * 512.0f + share_of(chance));
+  const uint32_t code = __uint_as_float(x) < kNormal ? small : normal;
+  return x < 0x7F800000u ? code | u >> 24 & 0x80u : 0x7Fu;
+}
+
+// x is the root of a number between the squares of two codes: up with the chance that keeps the square's mean;
+// above zero it stays above.
+__device__ __forceinline__ uint32_t second_code(float x, uint32_t chance) {
+  const uint32_t u = __float_as_uint(x);
+  const bool tiny = x < kNormal;
+  const uint32_t code = tiny ? (uint32_t)(x * 512.0f) : normal_code(u);
+  const float low = tiny ? (float)code * (1.0f / 512.0f) : __uint_as_float(u & 0xFFF00000u);
+  const float step = tiny ? 1.0f / 512.0f : __uint_as_float((u & 0x7F800000u) - (3u << 23)), high = low + step;
+  const bool up = x * x - low * low > share_of(chance) * (high * high - low * low) || (code == 0u && x > 0.0f);
+  return u < 0x7F800000u ? code + up : 0x7Fu;
+}
+
+// The roots of v >= 0: an estimate of 1 / root to a unit in its last place and one step to the root
+// nearest to v; outside the normal floats the library's.
+__device__ __forceinline__ void roots_of(const float (&v)[kEach], float (&root)[kEach]) {
+  bool normal = true;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const float y = __builtin_amdgcn_rsqf(v[e]), s = v[e] * y;
+    root[e] = __builtin_fmaf(__builtin_fmaf(-s, s, v[e]), 0.5f * y, s);
+    normal &= v[e] >= 0x1p-126f && v[e] < INFINITY;
+  }
+  if (normal) return;
+#pragma unroll 1
+  for (int e = 0; e < kEach; ++e) {
+    float one = 0.0f;
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) one = q == e ? v[q] : one;
+    one = sqrtf(one);
+#pragma unroll
+    for (int q = 0; q < kEach; ++q) root[q] = q == e ? one : root[q];
+  }
+}
+
+// Exponents of a block's two scales: 2^e 448 is the least such number that its largest magnitude does not
+// pass, and at least 2^-98, so that no product leaves what float32 holds.  What is not finite has no part.
+typedef uint16_t v2h __attribute__((ext_vector_type(2)));
+template <int CONTROL>
+__device__ __forceinline__ v2h larger_of_row(v2h v) {
+  const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CONTROL, 0xF, 0xF, false);
+  return __builtin_elementwise_max(v, __builtin_bit_cast(v2h, o));
+}
+__device__ __forceinline__ void exponents_of(const float (&m)[kEach], const float (&root)[kEach], int& first, int& second) {
+  uint32_t most[2] = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const uint32_t a = __float_as_uint(m[e]) & 0x7FFFFFFFu, b = __float_as_uint(root[e]) & 0x7FFFFFFFu;
+    most[0] = a > most[0] ? a : most[0];
+    most[1] = b > most[1] ? b : most[1];
+  }
+  if (__any(most[0] >= 0x7F800000u || most[1] >= 0x7F800000u)) {
+    most[0] = most[1] = 0u;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const uint32_t a = __float_as_uint(m[e]) & 0x7FFFFFFFu, b = __float_as_uint(root[e]) & 0x7FFFFFFFu;
+      most[0] = a > most[0] && a < 0x7F800000u ? a : most[0];
+      most[1] = b > most[1] && b < 0x7F800000u ? b : most[1];
+    }
+  }
+  // the exponent of what comes after 1.75 times a power of two is the next
+  v2h v = {(uint16_t)(most[0] + 0x1FFFFFu >> 23), (uint16_t)(most[1] + 0x1FFFFFu >> 23)};
+  v = __builtin_elementwise_max(v, (v2h{37, 37}));
+  v = larger_of_row<0x128>(v);  // of the 16 lanes of a row, turned by 8, 4, 2 and 1
+  v = larger_of_row<0x124>(v);
+  v = larger_of_row<0x122>(v);
+  v = larger_of_row<0x121>(v);
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  v = __builtin_elementwise_max(__builtin_bit_cast(v2h, (uint32_t)rows[0]), __builtin_bit_cast(v2h, (uint32_t)rows[1]));
+  const uint32_t w = __builtin_bit_cast(uint32_t, v);
+  const auto halves = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  v = __builtin_elementwise_max(__builtin_bit_cast(v2h, (uint32_t)halves[0]),
+                                __builtin_bit_cast(v2h, (uint32_t)halves[1]));
+  first = (int)v[0] - 135, second = (int)v[1] - 135;
+}
+
+__device__ __forceinline__ float power_of(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Four elements from i on, of which `left` are there (WHOLE: all of the wave's are).
+template <int BITS, bool WHOLE, typename P, typename G>
+__device__ __forceinline__ void update(const Tensor& t, const Step& s, int64_t i, int some) {
+  const int left = WHOLE ? kEach : some;
+  const auto at = device<P>(t.parameter) + i;
+  const auto first = device<uint8_t>(t.first) + i, second = device<uint8_t>(t.second) + i;
+  float p[kEach], g[kEach], m[kEach], v[kEach], root[kEach];
+  if (BITS == 32) {
+    load_each(device<float>(t.first) + i, left, m);
+    load_each(device<float>(t.second) + i, left, v);
+    load_each(at, left, p);
+    load_each(device<G>(t.gradient) + i, left, g);
+  } else {
+    uint8_t codes[2][kEach];
+    load_raw(first, left, codes[0]);
+    load_raw(second, left, codes[1]);
+    float scale[2] = {0.0f, 0.0f};  // lanes past the end have a part in the wave's exponents
+    if (left > 0) {
+      scale[0] = device<float>(t.first_scales)[i / kBlock];
+      scale[1] = device<float>(t.second_scales)[i / kBlock];
+    }
+    load_each(at, left, p);
+    load_each(device<G>(t.gradient) + i, left, g);
+    values_of(codes[0], m);
+    values_of(codes[1], v);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      m[e] *= scale[0];
+      v[e] *= scale[1];
       v[e] *= v[e];
     }
   }
-  P out[kEach];
-  Chances chance[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     m[e] = s.beta1 * m[e] + s.rest1 * g[e];
     v[e] = s.beta2 * v[e] + s.rest2 * (g[e] * g[e]);
-    root[e] = sqrtf(v[e]);
-    if (BITS == 8 || sizeof(P) == 2) chance[e] = chances_of(t.place + i + e, s.key);
-    const float next = p[e] * s.keep - s.rate * m[e] / (root[e] * s.cool + s.eps);
-    out[e] = stored(next, chance[e].parameter, P{});
+    if (BITS == 32) root[e] = sqrtf(v[e]);
   }
-  store_each((P*)t.parameter + i, left, out);
-  if (BITS == 32) {
-    store_each((float*)t.first + i, left, m);
-    store_each((float*)t.second + i, left, v);
-    return;
-  }
-  uint8_t c[2][kEach];
-  const int e1 = exponent_of(m), e2 = exponent_of(root);
+  if (BITS == 8) roots_of(v, root);
+  P out[kEach];
+  Chances chance[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    c[0][e] = m[e] - m[e] == 0.0f ? code_of(drawn_to(ldexpf(m[e], -e1), chance[e].first, 3, -6)) : (uint8_t)0x7F;
-    // v between the squares of two codes: up with the chance that keeps its mean; above zero it stays above
-    const float x = ldexpf(root[e], -e2);
-    float step, inverse;
-    step_of(x, 3, -6, step, inverse);
-    const float low = floorf(x * inverse) * step, high = low + step;
-    const bool up = x * x - low * low > chance[e].second * (high * high - low * low) || (low == 0.0f && x > 0.0f);
-    c[1][e] = x - x == 0.0f ? code_of(up ? high : low) : (uint8_t)0x7F;
+    if (BITS == 8 || sizeof(P) == 2) chance[e] = chances_of(t.place + i, e, s.key);
+    // the quotient to two units in its last place
+    const float next = p[e] * s.keep - s.rate * m[e] * __builtin_amdgcn_rcpf(root[e] * s.cool + s.eps);
+    out[e] = stored(next, chance[e].parameter, P{});
   }
-  store_each((uint8_t*)t.first + i, left, c[0]);
-  store_each((uint8_t*)t.second + i, left, c[1]);
+  store_each(at, left, out);
+  if (BITS == 32) {
+    store_each(device<float>(t.first) + i, left, m);
+    store_each(device<float>(t.second) + i, left, v);
+    return;
+  }
+  int e1, e2;
+  exponents_of(m, root, e1, e2);
+  const float by1 = power_of(-e1), by2 = power_of(-e2);
+  uint8_t c[2][kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    c[0][e] = (uint8_t)first_code(m[e] * by1, chance[e].first);
+    c[1][e] = (uint8_t)second_code(root[e] * by2, chance[e].second);
+  }
+  store_each(first, left, c[0]);
+  store_each(second, left, c[1]);
   if (i % kBlock == 0 && left > 0) {
-    t.first_scales[i / kBlock] = ldexpf(1.0f, e1);
-    t.second_scales[i / kBlock] = ldexpf(1.0f, e2);
+    device<float>(t.first_scales)[i / kBlock] = power_of(e1);
+    device<float>(t.second_scales)[i / kBlock] = power_of(e2);
   }
 }
 
@@ -246,9 +353,14 @@ template <int BITS, typename P, typename G>
 __device__ __forceinline__ void update_chunk(const Tensor& t, const Step& s, int64_t first) {
   for (int64_t i = first + threadIdx.x * kEach; i < first + kChunk; i += kThreads * kEach) {
     // a wave goes on together: its lanes share a scale
-    if (i - threadIdx.x % kWave * kEach >= t.count) return;
+    const int64_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * kBlock + (i - threadIdx.x * kEach);
+    if (wave >= t.count) return;
+    if (wave + kBlock <= t.count) {
+      update<BITS, true, P, G>(t, s, i, kEach);
+      continue;
+    }
     const int64_t left = t.count - i;
-    update<BITS, P, G>(t, s, i, left < 0 ? 0 : left > kEach ? kEach : (int)left);
+    update<BITS, false, P, G>(t, s, i, left < 0 ? 0 : left > kEach ? kEach : (int)left);
   }
 }
 
