@@ -240,16 +240,20 @@ struct Order {
   }
 };
 
-// The segments of a window that block `slot` of `slots` takes: body(key, first place, end).
+// The segments of a window that block `slot` of `slots` takes: body(key, first place, end).  A place begins one
+// where its key is not that of the place before.
 template <typename Body>
 __device__ __forceinline__ void segments(const uint32_t* code, int slot, int slots, Body body) {
-  for (int i = 0, s = 0; i < kTile && code[i] != UINT32_MAX; ++s) {
-    const int key = __builtin_amdgcn_readfirstlane(key_of(code[i]));
-    int end = i + 1;
-    while (end < kTile && code[end] != UINT32_MAX && key_of(code[end]) == key) ++end;
-    end = __builtin_amdgcn_readfirstlane(end);
-    if (s % slots == slot) body(key, i, end);
-    i = end;
+  const int i = threadIdx.x % kTile;
+  const uint32_t mine = code[i], before = code[i ? i - 1 : 0];
+  const uint64_t there = __ballot(mine != UINT32_MAX) & 0xFFFFu;
+  const int rows = __popcll(there);
+  uint32_t begins = (uint32_t)(__ballot(mine != UINT32_MAX && (i == 0 || key_of(mine) != key_of(before))) & 0xFFFFu);
+  for (int s = 0; begins; ++s) {
+    const int first = __ffs(begins) - 1;
+    begins &= begins - 1;
+    if (s % slots == slot)
+      body(__builtin_amdgcn_readlane((int)key_of(mine), first), first, begins ? __ffs(begins) - 1 : rows);
   }
 }
 
@@ -419,91 +423,150 @@ __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
 }
 
 // 64 outputs a wave at a time of 16 rows.  Lane l has output l % 16 of a tile and row l % 16, and four ranks of
-// every 16; it gets sums of four outputs in a row of row l % 16.
-template <int W, int S>
+// every 16; it gets sums of four outputs in a row of row l % 16.  RANKS: those of a.padded, or the most.
+template <int W, int S, int RANKS>
 __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
   typedef typename Element<W>::type T;
   typedef typename Element<S>::type In;
-  constexpr int kTiles = 4;
+  constexpr int kTiles = 4, kOutputs = kTiles * kTile;
+  constexpr int kSteps = RANKS > 32 ? 1 : RANKS / kTile;  // of 16 ranks, at once
+  constexpr int kGroups = RANKS > 32 ? 1 : kThreads / (kTile * RANKS / 4);
   __shared__ Order order;
-  __shared__ __attribute__((aligned(16))) float hidden[kTile][kMaxRank + 4];
+  __shared__ __attribute__((aligned(16))) float hidden[kTile][RANKS + 4];
+  __shared__ __attribute__((aligned(16))) float group_sums[kGroups > 1 ? kGroups : 1][kGroups > 1 ? kTile : 1][RANKS + 4];
   const int slot = blockIdx.x % a.slots, window = blockIdx.x / a.slots;
   const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int at = l % kTile;
+  const int at = l % kTile, four = l / kTile * 4;
+  const int padded = RANKS <= 32 ? RANKS : a.padded;
   segments(code, slot, a.slots, [&](int key, int first, int end) {
-    // the parts' sums, in a row of four ranks a thread
-    __syncthreads();
-    for (int i = threadIdx.x; i < kTile * a.padded / 4; i += kThreads) {
-      const int n = i / (a.padded / 4), j = i % (a.padded / 4) * 4;
-      float4 sum{0.0f, 0.0f, 0.0f, 0.0f};
-      if (n >= first && n < end && key < a.M) {
-        const float* from = a.part + ((int64_t)window * kTile + n) * a.padded + j;
-        const int64_t part = (int64_t)a.N * a.padded;
-        for (int p = 0; p < a.parts; p += 8) {
-          float4 v[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] = *(const float4*)(from + (p + q < a.parts ? p + q : p) * part);
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (p + q < a.parts) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
-        }
-      }
-      *(float4*)&hidden[n][j] = sum;
-      if (a.hidden && blockIdx.y == 0 && n >= first && n < end) {
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        store_floats<4>(a.hidden + row_of(code[n]) * a.hidden_stride + j, a.r - j, v);
-      }
-    }
-    __syncthreads();
-    const bool mine = at >= first && at < end;
+    const bool mine = at >= first && at < end, some = key < a.M;
     const int64_t row = row_of(code[mine ? at : first]);
     const T* up = (const T*)a.up + key * a.up_adapter;
     const In* scores = (const In*)a.scores + row * a.stride;
-    const auto outputs = [&](int o0, auto all) {
-      constexpr bool kWhole = decltype(all)::value;
-      float v[kTiles][4];
+    // whole blocks of 64 outputs and 16 ranks: the scores and the first ranks' weights, as they are in memory
+    struct Operands {
+      In v[kTiles][4];
+      T w[kSteps][kTiles][4];
+    };
+    const uint32_t lane = (uint32_t)(at * a.up_output + four) * sizeof(T);  // rows are at most 8 MiB apart
+    const auto weights = [&](int o0, int j, T (&w)[kTiles][4]) {
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        const int o = o0 + t * kTile + l / kTile * 4;
-        load_floats<4, kWhole>(scores + o, a.K - o, v[t]);
-      }
+      for (int t = 0; t < kTiles; ++t)
+        __builtin_memcpy(w[t], (const char*)(up + (o0 + t * kTile) * a.up_output + j) + lane, sizeof w[t]);
+    };
+    const auto load = [&](int o0, Operands& x) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) weights(o0, s * kTile, x.w[s]);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) __builtin_memcpy(x.v[t], scores + o0 + t * kTile + four, sizeof x.v[t]);
+    };
+    const auto multiply = [&](int j, const T (&w)[kTiles][4], v4f (&sum)[kTiles]) {
+      float h[4];
+      __builtin_memcpy(h, &hidden[at][j + four], sizeof h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) sum[t] = product(to_float(w[t][e]), h[e], sum[t]);
+    };
+    const auto finish = [&](int o0, const Operands& x) {
       v4f sum[kTiles];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) sum[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-      if (key < a.M) {
-        for (int j = l / kTile * 4; j < a.padded; j += kTile) {
-          float h[4], w[kTiles][4];
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            const int o = o0 + t * kTile + at;
-            load_floats<4, kWhole>(up + (int64_t)(o < a.K ? o : a.K - 1) * a.up_output + j, a.r - j, w[t]);
-          }
-          __builtin_memcpy(h, &hidden[at][j], sizeof h);
-          loads_first();
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) sum[t] = product(w[t][e], h[e], sum[t]);
-        }
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) v[t][q] = __builtin_fmaf(a.scale, sum[t][q], v[t][q]);
+      for (int s = 0; s < kSteps; ++s) multiply(s * kTile, x.w[s], sum);
+      for (int j = kSteps * kTile; RANKS > 32 && j < padded; j += kTile) {
+        T w[kTiles][4];
+        weights(o0, j, w);
+        multiply(j, w, sum);
       }
       if (!mine) return;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        const int o = o0 + t * kTile + l / kTile * 4;
-        if (kWhole || o < a.K) store_floats<4>(a.out, row * a.out_stride + o, a.out_dtype, kWhole ? 4 : a.K - o, v[t]);
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = __builtin_fmaf(a.scale, sum[t][q], to_float(x.v[t][q]));
+        store_floats<4>(a.out, row * a.out_stride + o0 + t * kTile + four, a.out_dtype, 4, v);
       }
     };
-    for (int o0 = (blockIdx.y * kWaves + wave) * kTiles * kTile; o0 < a.K; o0 += gridDim.y * kWaves * kTiles * kTile) {
-      if (o0 + kTiles * kTile <= a.K && a.r % kTile == 0)
-        outputs(o0, std::true_type{});
-      else
-        outputs(o0, std::false_type{});
+    // any 16 outputs
+    const auto guarded = [&](int o0) {
+      v4f sum = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      const int o = o0 + at < a.K ? o0 + at : a.K - 1;
+      for (int j = four; some && j < padded; j += kTile) {
+        float w[4], h[4];
+        load_floats<4>(up + o * a.up_output + j, a.r - j, w);
+        __builtin_memcpy(h, &hidden[at][j], sizeof h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = product(w[e], h[e], sum);
+      }
+      if (!mine || o0 + four >= a.K) return;
+      float v[4];
+      load_floats<4>(scores + o0 + four, a.K - o0 - four, v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = some ? __builtin_fmaf(a.scale, sum[q], v[q]) : v[q];
+      store_floats<4>(a.out, row * a.out_stride + o0 + four, a.out_dtype, a.K - o0 - four, v);
+    };
+    const int whole = some && a.r % kTile == 0 ? a.K / kOutputs : 0;
+    int block = blockIdx.y * kWaves + wave;
+    Operands x;
+    const bool early = block < whole;  // on their way beside the parts
+    if (early) load(block * kOutputs, x);
+    loads_first();
+    __syncthreads();
+    // the parts' sums: four ranks of a row a thread, and where that leaves threads every kGroups-th part
+    const int each = kTile * padded / 4;
+    for (int i = threadIdx.x; i < each * kGroups; i += kThreads) {
+      const int g = i / each, n = i % each / (padded / 4), j = i % (padded / 4) * 4;
+      float4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+      if (n >= first && n < end && some) {
+        const float* from = a.part + ((int64_t)window * kTile + n) * padded + j;
+        const int64_t part = (int64_t)a.N * padded;
+        for (int p = g; p < a.parts; p += 4 * kGroups) {
+          float4 v[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            v[q] = *(const float4*)(from + (p + q * kGroups < a.parts ? p + q * kGroups : p) * part);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (p + q * kGroups < a.parts) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
+        }
+      }
+      *(float4*)&(kGroups > 1 ? group_sums[g][n][j] : hidden[n][j]) = sum;
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < each; i += kThreads) {
+      const int n = i / (padded / 4), j = i % (padded / 4) * 4;
+      if (kGroups > 1) {
+        float4 sum = *(const float4*)&group_sums[0][n][j];
+#pragma unroll
+        for (int g = 1; g < kGroups; ++g) {
+          const float4 v = *(const float4*)&group_sums[g][n][j];
+          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        *(float4*)&hidden[n][j] = sum;
+      }
+      if (a.hidden && blockIdx.y == 0 && n >= first && n < end) {
+        float v[4];
+        __builtin_memcpy(v, &hidden[n][j], sizeof v);
+        store_floats<4>(a.hidden + row_of(code[n]) * a.hidden_stride + j, a.r - j, v);
+      }
+    }
+    __syncthreads();
+    const int step = gridDim.y * kWaves;
+    if (early)
+      for (;;) {
+        Operands next;
+        const bool more = block + step < whole;
+        if (more) load((block + step) * kOutputs, next);
+        loads_first();
+        finish(block * kOutputs, x);
+        block += step;
+        if (!more) break;
+        x = next;
+      }
+    for (; block * kOutputs < a.K; block += step)
+      for (int o0 = block * kOutputs; o0 < a.K && o0 < (block + 1) * kOutputs; o0 += kTile) guarded(o0);
   });
 }
 
@@ -1010,6 +1073,16 @@ hipError_t launch_down(const AdaptArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <int W, int S>
+hipError_t launch_up(const AdaptArgs& a, dim3 grid, hipStream_t s) {
+  switch (a.padded) {
+    case 16: up_kernel<W, S, 16><<<grid, kThreads, 0, s>>>(a); break;
+    case 32: up_kernel<W, S, 32><<<grid, kThreads, 0, s>>>(a); break;
+    default: up_kernel<W, S, kMaxRank><<<grid, kThreads, 0, s>>>(a); break;
+  }
+  return hipGetLastError();
+}
+
 template <int W>
 hipError_t launch_adapt(const AdaptArgs& a, int x_dtype, hipStream_t s) {
   hipError_t e = launch_order(a, s);
@@ -1021,16 +1094,15 @@ hipError_t launch_adapt(const AdaptArgs& a, int x_dtype, hipStream_t s) {
     default: e = launch_down<YTM_DTYPE_F32, W>(a, s); break;
   }
   if (e != hipSuccess) return e;
-  // a block takes so many times 256 outputs that there are about 2048 of them
+  // a block takes so many times 256 outputs that there are about 1024 of them
   const int64_t tiles = a.K > 0 ? (a.K + 255) / 256 : 1, blocks = (int64_t)a.windows * a.slots;
-  const int64_t each = (tiles * blocks + 2047) / 2048;
+  const int64_t each = (tiles * blocks + 1023) / 1024;
   const dim3 grid((unsigned)blocks, (unsigned)((tiles + each - 1) / each));
   switch (a.dtype) {
-    case YTM_DTYPE_F16: up_kernel<W, YTM_DTYPE_F16><<<grid, kThreads, 0, s>>>(a); break;
-    case YTM_DTYPE_BF16: up_kernel<W, YTM_DTYPE_BF16><<<grid, kThreads, 0, s>>>(a); break;
-    default: up_kernel<W, YTM_DTYPE_F32><<<grid, kThreads, 0, s>>>(a); break;
+    case YTM_DTYPE_F16: return launch_up<W, YTM_DTYPE_F16>(a, grid, s);
+    case YTM_DTYPE_BF16: return launch_up<W, YTM_DTYPE_BF16>(a, grid, s);
+    default: return launch_up<W, YTM_DTYPE_F32>(a, grid, s);
   }
-  return hipGetLastError();
 }
 
 // A launch counts its threads in 32 bits: launch(first adapter or 0, blocks) for each of as many launches as
@@ -1147,6 +1219,7 @@ const char* wrong_operands(int dtype, int64_t stride, int64_t N, int64_t K, int 
   const int64_t apart[] = {stride, x_stride, down_adapter, down_rank, up_adapter, up_output};
   for (int64_t v : apart)
     if (v < 0 || v > kMostApart) return "rows are too far apart";
+  if (K > 1 && up_output > kMaxApart / 4) return "rows of up are at most 2097152 elements apart";
   if ((N > 1 && ((stride != 0 && stride < K) || (x_stride != 0 && x_stride < width))) ||
       (r > 1 && down_rank != 0 && down_rank < C) || (K > 1 && up_output != 0 && up_output < r) ||
       (M > 1 && ((down_adapter != 0 && down_adapter < C) || (up_adapter != 0 && up_adapter < r))))
