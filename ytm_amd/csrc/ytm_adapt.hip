@@ -287,7 +287,7 @@ __device__ __forceinline__ void write_part(const AdaptArgs& a, int p, int window
 template <int X, int W>
 constexpr bool kHalves = W != YTM_DTYPE_F32 && (X == W || X == YTM_DTYPE_BITS);
 template <int X, int W>
-constexpr int kChunk = kHalves<X, W> ? 128 : 64;  // clauses that a wave's lanes load at once, a quarter a lane
+constexpr int kChunk = kHalves<X, W> ? 128 : 64;  // clauses that a wave's lanes load at once, in four steps
 
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
@@ -320,12 +320,12 @@ __device__ __forceinline__ v4u load_halves(const T* p, int left) {
 }
 
 // Sums over a part of the clauses of 16 rows with 16 RT ranks of a segment's adapter.  Lane l has row l % 16, the
-// ranks RT (l % 16) + t and a quarter of a chunk's clauses in a row, all loaded before the first product; a
-// block's waves take chunks in turn.
+// ranks RT (l % 16) + t and 16 bytes of each 64 of a chunk, so that a load has whole lines of 16 rows; a block's
+// waves take chunks in turn, each with the next one's operands on their way.
 template <int X, int W, int RT>
 __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
   typedef typename Element<W>::type T;
-  constexpr int kOwn = kChunk<X, W> / 4;
+  constexpr int kOwn = kHalves<X, W> ? 8 : 4, kStep = 4 * kOwn;  // clauses of a lane and of the wave in a step
   __shared__ Order order;
   __shared__ v4f join[kWaves][RT][kWave];
   const int slot = blockIdx.x % a.slots, window = blockIdx.x / a.slots, p = blockIdx.y, ranks = blockIdx.z * RT * kTile;
@@ -345,32 +345,42 @@ __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
     // a chunk's operands, as they are in memory
     struct Operands {
       v4u x[kHalves<X, W> ? 4 : 1], w[kHalves<X, W> ? RT : 1][4];
-      uint32_t word;
+      uint32_t words[4];
       float fx[kHalves<X, W> ? 1 : 4][4], fw[kHalves<X, W> ? 1 : RT][4][4];
     };
     const auto load = [&](int at, auto all, Operands& o) {
       constexpr bool kWhole = decltype(all)::value;
       const int c = at * kChunk<X, W> + l / kTile * kOwn;
-      if constexpr (kHalves<X, W>) {
-        if constexpr (X == YTM_DTYPE_BITS) {
-          const int left = a.C - c;
-          o.word = kWhole || left > 0 ? ((const uint32_t*)a.x)[row * a.x_stride + c / 32] : 0u;
-          if (!kWhole && left > 0 && left < 32) o.word &= (1u << left) - 1u;
+      if constexpr (X == YTM_DTYPE_BITS) {
+        constexpr int kWords = kChunk<X, W> / 32;
+        const uint32_t* from = (const uint32_t*)a.x + row * a.x_stride + at * kWords;
+        if (kWhole) {
+          __builtin_memcpy(o.words, from, kWords * 4);
         } else {
 #pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            const int left = a.C - (at * kWords + i) * 32;
+            o.words[i] = left > 0 ? from[i] & (left < 32 ? (1u << left) - 1u : ~0u) : 0u;
+          }
+        }
+      }
+      if constexpr (kHalves<X, W>) {
+        if constexpr (X != YTM_DTYPE_BITS) {
+#pragma unroll
           for (int i = 0; i < 4; ++i)
-            o.x[i] = load_halves<T, kWhole>((const T*)a.x + row * a.x_stride + c + 8 * i, a.C - c - 8 * i);
+            o.x[i] = load_halves<T, kWhole>((const T*)a.x + row * a.x_stride + c + kStep * i, a.C - c - kStep * i);
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o.w[t][i] = load_halves<T, kWhole>(down[t] + c + 8 * i, a.C - c - 8 * i);
+          for (int i = 0; i < 4; ++i) o.w[t][i] = load_halves<T, kWhole>(down[t] + c + kStep * i, a.C - c - kStep * i);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          load_clauses<X, 4, kWhole>(a, row, c + 4 * i, o.fx[i]);
+          if constexpr (X != YTM_DTYPE_BITS) load_clauses<X, 4, kWhole>(a, row, c + kStep * i, o.fx[i]);
 #pragma unroll
-          for (int t = 0; t < RT; ++t) load_floats<4, kWhole>(down[t] + c + 4 * i, a.C - c - 4 * i, o.fw[t][i]);
+          for (int t = 0; t < RT; ++t)
+            load_floats<4, kWhole>(down[t] + c + kStep * i, a.C - c - kStep * i, o.fw[t][i]);
         }
       }
     };
@@ -383,7 +393,7 @@ __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
             constexpr uint32_t one = W == YTM_DTYPE_F16 ? 0x3C00u : 0x3F80u;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const uint32_t two = o.word >> (8 * i + 2 * q);
+              const uint32_t two = o.words[i] >> (l / kTile * 8 + 2 * q);
               x[q] = ((two & 1u) | (two & 2u) << 15) * one;
             }
           }
@@ -396,7 +406,14 @@ __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int t = 0; t < RT; ++t) sum[t] = product(o.fx[i][e], o.fw[t][i][e], sum[t]);
+            for (int t = 0; t < RT; ++t) {
+              float x;
+              if constexpr (X == YTM_DTYPE_BITS)
+                x = (float)(o.words[i / 2] >> (i % 2 * 16 + l / kTile * 4 + e) & 1u);
+              else
+                x = o.fx[i][e];
+              sum[t] = product(x, o.fw[t][i][e], sum[t]);
+            }
       }
     };
     const int whole = a.C / kChunk<X, W>, last = (p + 1) * a.part_steps < whole ? (p + 1) * a.part_steps : whole;
