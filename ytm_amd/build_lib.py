@@ -8,6 +8,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -25,7 +27,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "--offload-arch=gfx950",
     # exact IEEE semantics for the parity-critical float/double compares and updates
     "-ffp-contract=off",
@@ -60,15 +61,29 @@ def write_jit_sources() -> None:
         JIT_INC.write_text(text)
 
 
-def build(verbose: bool = False) -> Path:
-    write_jit_sources()
-    tmp = OUT.with_suffix(".so.tmp")
-    cmd = [hipcc(), *HIPCC_FLAGS, "-o", str(tmp), *map(str, SOURCES), "-lhiprtc"]
+def _run(cmd: list[str], verbose: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
     if verbose and res.stderr:
         print(res.stderr, file=sys.stderr)
+
+
+def build(verbose: bool = False) -> Path:
+    """Compiles each source to an object, several at once, and links them."""
+    write_jit_sources()
+    jobs = max(1, min(len(SOURCES), os.cpu_count() or 1, int(os.environ.get("MAX_JOBS", 8))))
+    with tempfile.TemporaryDirectory() as work:
+        objects = [Path(work) / f"{source.stem}.o" for source in SOURCES]
+        # the longest first
+        order = sorted(zip(SOURCES, objects), key=lambda pair: pair[0].stem not in ("ytm_kernels", "ytm_adapt"))
+        with ThreadPoolExecutor(jobs) as pool:
+            done = [pool.submit(_run, [hipcc(), *HIPCC_FLAGS, "-c", str(source), "-o", str(out)], verbose)
+                    for source, out in order]
+            for d in done:
+                d.result()
+        tmp = OUT.with_suffix(".so.tmp")
+        _run([hipcc(), "-shared", "-fPIC", "--offload-arch=gfx950", "-o", str(tmp), *map(str, objects), "-lhiprtc"], verbose)
     os.replace(tmp, OUT)
     return OUT
 

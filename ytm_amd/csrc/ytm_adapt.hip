@@ -71,6 +71,7 @@ struct AdaptArgs {
   uint32_t* order;  // [N], of more than kInline rows; then [begins] where adapters begin
   int begins;       // M + 1 where they are asked for
   int w_dtype;
+  int odd;  // 16-bit rows that do not all begin at multiples of 4
   int first;  // adapter of a launch of gradients
   RowWindows up_windows, down_windows;
 };
@@ -300,10 +301,22 @@ __device__ __forceinline__ v4f half_product(v4u x, v4u w, v4f d) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, x), __builtin_bit_cast(v8bf, w), d, 0, 0, 0);
 }
 
-// Eight 16-bit values at p, of which `left` are there.
-template <typename T, bool WHOLE>
+// Eight 16-bit values at p, of which `left` are there.  ODD: p is at any multiple of 2; lanes that read rows of
+// their own take such loads piece by piece (2048 rows of 10007 bfloat16, one pass: 37 us, at multiples of 4 22), so
+// the aligned words around them are read, all of which hold some of the eight, and shifted.
+template <typename T, bool WHOLE, bool ODD = false>
 __device__ __forceinline__ v4u load_halves(const T* p, int left) {
   v4u r;
+  if (WHOLE && ODD) {
+    const uintptr_t u = (uintptr_t)p;
+    const uint32_t shift = (uint32_t)(u & 2) * 8;
+    typedef uint32_t v4a __attribute__((ext_vector_type(4), aligned(4)));
+    const v4u v = *(const v4a*)(u & ~(uintptr_t)3);
+    const uint32_t last = *(const uint32_t*)(u + 14 & ~(uintptr_t)3);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) r[q] = __builtin_amdgcn_alignbit(q < 3 ? v[(q + 1) % 4] : last, v[q], shift);
+    return r;
+  }
   if (WHOLE || left >= 8) {
     __builtin_memcpy(&r, p, sizeof r);
     return r;
@@ -614,11 +627,11 @@ __device__ __forceinline__ void back_block(const AdaptArgs& a, int block, int p,
       uint16_t h[kHalf ? 8 : 1][RT];
       float g[kHalf ? 1 : 8], w[kHalf ? 1 : 8][RT];
     };
-    const auto load = [&](int step, auto all, Operands& v) {
+    const auto load = [&](int step, auto all, auto odd, Operands& v) {
       constexpr bool kWhole = decltype(all)::value;
       const int o = step * 32 + l / kTile * 8;
       if constexpr (kHalf) {
-        v.x = load_halves<S, kWhole>(grad + o, a.K - o);
+        v.x = load_halves<S, kWhole, decltype(odd)::value>(grad + o, a.K - o);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const T* from = up + (int64_t)(o + e) * a.up_output;
@@ -659,22 +672,30 @@ __device__ __forceinline__ void back_block(const AdaptArgs& a, int block, int p,
     const int steps = (a.K + 31) / 32, last = (p + 1) * a.part_steps < steps ? (p + 1) * a.part_steps : steps;
     const int whole = ranks + RT * kTile <= a.r ? (last < a.K / 32 ? last : a.K / 32) : 0;
     int step = p * a.part_steps + wave;
-    if (step < whole) {
-      Operands now;
-      load(step, std::true_type{}, now);
-      for (; step + kWaves < whole; step += kWaves) {
-        Operands next;
-        load(step + kWaves, std::true_type{}, next);
+    const auto pipeline = [&](auto odd) {
+      if (step >= whole) return;
+      Operands ring[3];  // two steps' operands are on their way
+      load(step, std::true_type{}, odd, ring[0]);
+      const int second = step + kWaves < whole ? step + kWaves : step;
+      load(second, std::true_type{}, odd, ring[1]);
+      for (;; step += kWaves) {
+        const int third = step + 2 * kWaves;
+        load(third < whole ? third : step, std::true_type{}, odd, ring[2]);
         loads_first();
-        multiply(now);
-        now = next;
+        multiply(ring[0]);
+        if (step + kWaves >= whole) break;
+        ring[0] = ring[1];
+        ring[1] = ring[2];
       }
-      multiply(now);
       step += kWaves;
-    }
+    };
+    if (kHalf && a.odd)
+      pipeline(std::true_type{});
+    else
+      pipeline(std::false_type{});
     for (; step < last; step += kWaves) {
       Operands now;
-      load(step, std::false_type{}, now);
+      load(step, std::false_type{}, std::false_type{}, now);
       multiply(now);
     }
     write_part<RT>(a, p, window, first, end, ranks, sum, join);
@@ -711,7 +732,7 @@ struct OuterShared {
   union {
     float values[kValues];
     uint16_t planes[2 * kValues];
-    v4f join[kWaves][8][kWave];
+    v4f join[kWaves][4][kWave];
   };
 };
 
@@ -798,7 +819,7 @@ __device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int ke
     v4u raw[PLANES && X != YTM_DTYPE_BITS ? 8 : 1];
     uint32_t bits[8];
     float v[PLANES ? 1 : 8][8];
-    const auto load = [&](auto all) {
+    const auto load = [&](auto all, auto odd) {
       constexpr bool kWhole = decltype(all)::value;
       const int last = row_of(code[rows - 1]);
 #pragma unroll
@@ -813,7 +834,7 @@ __device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int ke
           if (!kWhole && left > 0 && left < 8) bits[i] &= (1u << left) - 1u;
         } else if constexpr (PLANES > 0) {
           const bf16* from = UP ? (const bf16*)a.scores + row * a.stride : (const bf16*)a.x + row * a.x_stride;
-          raw[i] = load_halves<bf16, kWhole>(from + column, left);
+          raw[i] = load_halves<bf16, kWhole, decltype(odd)::value>(from + column, left);
         } else if constexpr (UP) {
           load_floats<8, kWhole>((const typename Element<X>::type*)a.scores + row * a.stride + column, left, v[i]);
         } else {
@@ -822,10 +843,12 @@ __device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int ke
       }
     };
     if (work) {
-      if (whole_tile && wave * 32 + 32 <= rows)
-        load(std::true_type{});
+      if (!whole_tile || wave * 32 + 32 > rows)
+        load(std::false_type{}, std::false_type{});
+      else if (PLANES > 0 && X == YTM_DTYPE_BF16 && a.odd)
+        load(std::true_type{}, std::true_type{});
       else
-        load(std::false_type{});
+        load(std::true_type{}, std::false_type{});
     }
     loads_first();
     // the rows' values at the ranks: two threads a row
@@ -909,15 +932,17 @@ __device__ __forceinline__ void outer_block(const AdaptArgs& a, int tile, int ke
   float total[RT][8];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sh.join[wave][e][l] = sum[t][e];
-    __syncthreads();
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
+      if (e % 4 == 0) {
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sh.join[wave][q][l] = sum[t][e + q];
+        __syncthreads();
+      }
       total[t][e] = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) total[t][e] += ((const float*)&sh.join[w][e][l])[wave];
+      for (int w = 0; w < kWaves; ++w) total[t][e] += ((const float*)&sh.join[w][e % 4][l])[wave];
       if (partial)
         partial[(t * 8 + e) * kThreads + threadIdx.x] = total[t][e];
       else
@@ -989,23 +1014,44 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AdaptArgs a) {
   }
 }
 
-// What reads the scores' gradient: the first blocks of a launch make back, the others the gradient of up.
+// Waves that a SIMD holds at once: what the sums of 16 RT ranks, and f32 operands, leave of its registers.
+constexpr int waves_of(int rt, int planes) { return planes ? (rt == 1 ? 4 : rt == 2 ? 3 : 2) : rt == 1 ? 3 : 2; }
+
+template <int G>
+constexpr int kGradPlanes = G == YTM_DTYPE_BF16 ? 3 : 0;
+
+// Of at most kInline rows both in one launch: the first blocks make back, the others the gradient of up.
 template <int G, int W, int RT>
-__global__ __launch_bounds__(kThreads) void grad_kernel(AdaptArgs a) {
-  constexpr int kPlanes = G == YTM_DTYPE_BF16 ? 3 : 0;
+__global__ __launch_bounds__(kThreads, waves_of(RT, kGradPlanes<G>)) void grad_kernel(AdaptArgs a) {
   __shared__ Order order;
-  __shared__ OuterShared<G, RT, kPlanes> sh;
+  __shared__ OuterShared<G, RT, kGradPlanes<G>> sh;
+  static_assert(sizeof sh.join >= sizeof(v4f[kWaves][RT][kWave]), "");
   const int back = a.windows * a.slots * a.parts, ranks = blockIdx.y * RT * kTile;
   if ((int)blockIdx.x < back) {
     const int p = blockIdx.x % a.parts;
     back_block<G, W, RT>(a, blockIdx.x / a.parts, p, ranks, order, (v4f(*)[RT][kWave])sh.join);
   } else {
-    outer_blocks<G, RT, true, kPlanes>(a, blockIdx.x - back, ranks, order, sh);
+    outer_blocks<G, RT, true, kGradPlanes<G>>(a, blockIdx.x - back, ranks, order, sh);
   }
 }
 
+// Of more two launches, so that back's blocks are as many as their registers allow (2048 rows of 10007 bfloat16, rank 32:
+// together 69 us).
+template <int G, int W, int RT>
+__global__ __launch_bounds__(kThreads) void back_kernel(AdaptArgs a) {
+  __shared__ Order order;
+  __shared__ v4f join[kWaves][RT][kWave];
+  back_block<G, W, RT>(a, blockIdx.x / a.parts, blockIdx.x % a.parts, blockIdx.y * RT * kTile, order, join);
+}
+template <int G, int RT>
+__global__ __launch_bounds__(kThreads, waves_of(RT, kGradPlanes<G>)) void outputs_kernel(AdaptArgs a) {
+  __shared__ Order order;
+  __shared__ OuterShared<G, RT, kGradPlanes<G>> sh;
+  outer_blocks<G, RT, true, kGradPlanes<G>>(a, blockIdx.x, blockIdx.y * RT * kTile, order, sh);
+}
+
 template <int X, int RT, int PLANES>
-__global__ __launch_bounds__(kThreads) void clauses_kernel(AdaptArgs a) {
+__global__ __launch_bounds__(kThreads, waves_of(RT, PLANES)) void clauses_kernel(AdaptArgs a) {
   __shared__ Order order;
   __shared__ OuterShared<X, RT, PLANES> sh;
   outer_blocks<X, RT, false, PLANES>(a, blockIdx.x, blockIdx.y * RT * kTile, order, sh);
@@ -1135,9 +1181,22 @@ hipError_t launch_outer(const AdaptArgs& a, int64_t columns, const RowWindows& w
   return hipSuccess;
 }
 
+template <int G, int W, int RT>
+hipError_t launch_many(const AdaptArgs& a, hipStream_t s) {
+  const unsigned ranks = (a.r + RT * kTile - 1) / (RT * kTile);
+  back_kernel<G, W, RT><<<dim3(a.windows * a.slots * a.parts, ranks), kThreads, 0, s>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.K == 0) return e;
+  return launch_outer(a, a.K, a.up_windows, [&](int, int64_t blocks) {
+    outputs_kernel<G, RT><<<dim3((unsigned)blocks, ranks), kThreads, 0, s>>>(a);
+    return hipGetLastError();
+  });
+}
+
 template <int G, int W>
 hipError_t launch_grad(AdaptArgs a, hipStream_t s) {
   const int t = rank_tiles(a.r);
+  if (a.N > kInline) return t == 1 ? launch_many<G, W, 1>(a, s) : t == 2 ? launch_many<G, W, 2>(a, s) : launch_many<G, W, 4>(a, s);
   return launch_outer(a, a.K, a.up_windows, [&](int first, int64_t blocks) {
     a.first = first;
     if (first) a.windows = 0;  // back is there
@@ -1401,6 +1460,10 @@ int ytm_adapt_gradient(const void* grad, int dtype, int64_t stride, int64_t N, i
   a.hidden = const_cast<float*>(hidden), a.hidden_stride = hidden_stride;
   a.out = d_up, a.d_up_adapter = d_up_adapter, a.d_up_output = d_up_output;
   a.d_down = d_down, a.d_down_adapter = d_down_adapter, a.d_down_rank = d_down_rank;
+  const auto odd = [](const void* p, int64_t rows, int64_t stride, int type) {
+    return ytm::size_of(type) == 2 && (((uintptr_t)p | (rows > 1 ? stride * 2 : 0)) & 2) != 0;
+  };
+  a.odd = odd(grad, N, stride, dtype) || odd(x, N, x_stride, x_dtype);
   const hipError_t e = ytm::launch_gradient(a, x_dtype, (hipStream_t)stream);
   if (e != hipSuccess) return fail(YTM_EHIP, std::string("adapt_gradient failed: ") + hipGetErrorString(e));
   return YTM_OK;
