@@ -355,7 +355,9 @@ def check_grad(got, scores, tokens, p, c, c_err, heat, eps, out):
     size = (one + p) * (np.abs(c) / heat)[:, None]
     rel, least = ROUND[out]
     bound = (one + p) * (c_err / heat)[:, None] + size * (eps + 2.0**-22 * (far + 4)) + rel * np.abs(want) * 1.01 + least
-    bound += (np.abs(c) / heat)[:, None] * 2.0**-126  # powers below the least normal number
+    # a power below the least normal number, 2^-126, is 0; it is divided by a sum of powers that is above 2^-24 2^-0.5 (one
+    # relative to a whole exponent near a score, taken where it is above 2^-24, or to the largest score itself)
+    bound += (np.abs(c) / heat)[:, None] * 2.0**(-126 + 24.5)
     err = np.abs(host(got) - want)
     err[np.isnan(err)] = np.inf
     assert (err <= bound).all(), (err / bound).max()
@@ -375,6 +377,32 @@ def policy_want(log, tokens, old, adv, ref, kl, low, high, w):
         loss, c = loss + kl * (np.expm1(far) - far), c - kl * np.expm1(far)
         size = size + kl * (np.exp(far) + np.abs(far) + 1)
     return tuple(np.where(there, v, 0.0) for v in (w * loss, w * c, w * size, lp))
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("N", [5, 600])
+def test_policy_scores_far_from_zero(N, kind):
+    """Whole rows at the ends of a type, masked beginnings of rows, temperatures of all sizes."""
+    rng = np.random.default_rng(N)
+    V, end = 3000, 6e4 if kind == "f16" else 3e38
+    s = rng.normal(0, 3, (N, V)).astype(np.float32)
+    s[0] = s[0] * 1e-3 - 200.0
+    s[1] = s[1] * 1e-3 + 300.0
+    s[2] = np.where(rng.random(V) < 0.5, end, -end)
+    s[3, :2900] = -np.inf
+    s[4, ::8] = -1e4  # each thread's first scores far below the others
+    temperature = np.ones(N, np.float32)
+    temperature[5:] = 10.0 ** rng.uniform(-3, 3, N - 5)
+    scores = gpu(s, kind)
+    log, p, heat, eps = log_softmax(host(scores), temperature)
+    tokens = np.where(np.arange(N) == 3, 2950, host(scores).argmax(1))
+    want = log[np.arange(N), tokens]
+    old = want.astype(np.float32)
+    losses, grad, lp = tune.policy_loss(scores, ints(tokens), gpu(old), gpu(np.full(N, 1.0)), weights=gpu(np.ones(N)),
+                                        temperature=gpu(temperature))
+    lp_err = eps + 2.0**-24 * np.abs(want) + 2.0**-22
+    assert (np.abs(host(lp) - want) <= lp_err).all()
+    check_grad(grad, host(scores), tokens, p, np.full(N, -1.0), np.full(N, 1.0) * (1.1 * lp_err + 2.0**-21), heat, eps, "f32")
 
 
 VOCABULARIES = [(1, 1), (5, 2), (3, 10), (7, 63), (4, 64), (300, 65), (2, 1000), (33, 4097), (1, 10000), (6, 32001),
@@ -857,6 +885,44 @@ def test_graph_replays(N, V, bits):
         torch.cuda.synchronize()
         for s, t in zip(captured + [c.down, c.up, opt.steps], eager + [e.down, e.up, e_opt.steps]):
             assert torch.equal(s.float(), t.float()), k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_learning_in_a_graph(bits):
+    """A whole step of Adapters captured: corrected scores, loss, gradient, optimiser, with users that change."""
+    C, K, N, users = 100, 40, 30, 4
+    rng = np.random.default_rng(0)
+    bits_in = decode.pack_outputs(rng.random((N, C)) < 0.3)
+    base, adv = gpu(rng.normal(0, 3, (N, K))), gpu(rng.normal(0, 1, N))
+    tokens, which, old = ints(rng.integers(0, K, N)), ints(rng.integers(0, users - 1, N)), gpu(np.full(N, -3.0))
+    models = [tune.Adapters(users, C, K, rank=5, bits=bits, seed=4) for _ in range(2)]
+
+    def step(m):
+        scores = base.clone()
+        hidden = m.adapt(scores, bits_in, which)
+        _, grad, lp = tune.policy_loss(scores, tokens, old, adv, out=scores)
+        m.learn(grad, bits_in, which, hidden, lr=0.05)
+        return lp
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(models[0])
+    torch.cuda.current_stream().wait_stream(stream)
+    step(models[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(models[0])
+    for k in range(3):
+        which.copy_(ints(rng.integers(-1, users - k, N)))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step(models[1])
+        torch.cuda.synchronize()
+        assert torch.equal(captured, eager)
+        for a, b in zip((models[0].down, models[0].up, models[0].optimizer.steps),
+                        (models[1].down, models[1].up, models[1].optimizer.steps)):
+            assert torch.equal(a, b), k
 
 
 def test_two_streams_at_once():

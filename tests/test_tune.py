@@ -114,6 +114,26 @@ def test_wrong_operands_are_refused(entries, name, operand, wrong, error):
     assert entries.launched == 0
 
 
+@pytest.mark.parametrize("name,wrong", [("adapt", dict(scale=float("nan"))), ("adapt_gradient", dict(scale=float("inf"))),
+                                        ("policy_loss", dict(kl=float("nan"))), ("policy_loss", dict(clip=float("inf"))),
+                                        ("policy_loss", dict(clip_high=float("nan"))),
+                                        ("preference_loss", dict(beta=float("inf"))),
+                                        ("preference_loss", dict(smoothing=float("nan")))])
+def test_numbers_that_are_not_finite_are_refused(entries, name, wrong):
+    function, base = CALLS[name]
+    with pytest.raises(ValueError, match="finite"):
+        function(**{**base, **wrong})
+    assert entries.launched == 0
+
+
+@pytest.mark.parametrize("name,numbers", [("adapt", dict(scale=np.float32(2))), ("policy_loss", dict(clip=np.float32(0.1))),
+                                          ("preference_loss", dict(beta=np.float64(0.1), smoothing=0))])
+def test_numbers_of_other_kinds_pass(entries, name, numbers):
+    function, base = CALLS[name]
+    function(**{**base, **numbers})
+    assert entries.launched == 1
+
+
 @pytest.mark.parametrize("name", list(CALLS))
 def test_tangents_are_refused(entries, name):
     function, base = CALLS[name]

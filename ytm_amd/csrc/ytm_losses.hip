@@ -149,8 +149,9 @@ struct Part {
   __device__ __forceinline__ static bool has(int r, int first, int last) { return first + r * (int)blockDim.x * E < last; }
 
   // The sum is made relative to the largest of the thread's first few scores, or to 0, in one pass and with one rounding
-  // of each exponent: score * scale less a whole number near that score's.  Where that loses it (a NaN, an
-  // infinity, scores far above or all far below: a sum above 2^60 or below 2^-60), relative to the largest.
+  // of each exponent: score * scale less a whole number near that score's.  Where that is not good enough (a NaN, an
+  // infinity, scores far above, whose exponents have fewer bits of fraction, or all far below: a sum above 2^24 or
+  // below 2^-24), relative to the largest.
   __device__ __forceinline__ Stats stats(int first, int last, float scale) {
     float near = -INFINITY;
 #pragma unroll
@@ -167,7 +168,7 @@ struct Part {
       }
     Stats s{near, ((sum[0] + sum[1]) + (sum[2] + sum[3])) * power(__builtin_fmaf(-near, scale, whole))};
     again();
-    if (s.sum > 0x1p-60f && s.sum < 0x1p60f && fabsf(whole) < kWholes) return s;
+    if (s.sum > 0x1p-24f && s.sum < 0x1p24f && fabsf(whole) < kWholes) return s;
     s = Stats{-INFINITY, 0.0f};
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -249,7 +250,7 @@ __device__ __forceinline__ Answer answer_of(const LossArgs& a, int n, float z, c
   r.cooling = cooling(a, n);
   r.there = t >= 0 && t < a.V && z > -INFINITY;
   r.lp = 0.0f;
-  if (r.there) r.lp = (float)((double)(z - all.max) * (double)r.cooling - log((double)all.sum));
+  if (r.there) r.lp = (float)(((double)z - (double)all.max) * (double)r.cooling - log((double)all.sum));
   return r;
 }
 

@@ -91,6 +91,7 @@ def adapt(scores: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.T
     three types, `scores` itself too (default: a new float32 tensor)."""
     if _forward_ad._current_level >= 0:
         _no_tangents(scores=scores, x=x, down=down, up=up, hidden=hidden, out=out)
+    scale = _number(scale, "scale")
     dtype, N, K, device = _rows_of(scores, "scores", _FLOATS)
     down_adapter, down_rank = _adapters(down, "down", None, None, device)
     M, r, C = down.shape
@@ -123,6 +124,7 @@ def adapt_gradient(grad: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: 
         _no_tangents(grad=grad, x=x, up=up, hidden=hidden)
         if out is not None:
             _no_tangents(down_gradient=out[0], up_gradient=out[1])
+    scale = _number(scale, "scale")
     dtype, N, K, device = _rows_of(grad, "grad", _FLOATS)
     _adapters(down, "down", None, None, device)
     M, r, C = down.shape
@@ -175,6 +177,8 @@ def policy_loss(scores: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, a
     reference = _per_row(reference, "reference", torch.float32, N, device)
     weights = _per_row(weights, "weights", torch.float32, N, device)
     temperature = _per_row(temperature, "temperature", torch.float32, N, device)
+    kl, clip = _number(kl, "kl"), _number(clip, "clip")
+    clip_high = clip if clip_high is None else _number(clip_high, "clip_high")
     if kl and reference is None:
         raise ValueError("kl needs a reference.")
     out, out_type = _result(out, (N, V), device)
@@ -183,7 +187,7 @@ def policy_loss(scores: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, a
     need = _bytes("ytm_policy_loss_workspace", N, V)
     workspace = torch.empty(need, dtype=torch.uint8, device=where) if need else None
     _call(lib.ytm_policy_loss, device, scores.data_ptr(), dtype, scores.stride(0), N, V, tokens, old, advantages,
-          reference, kl, clip, clip if clip_high is None else clip_high, weights, temperature, losses.data_ptr(),
+          reference, kl, clip, clip_high, weights, temperature, losses.data_ptr(),
           logprobs.data_ptr(), out.data_ptr(), out_type, out.stride(0), workspace.data_ptr() if need else None, need)
     return losses, out, logprobs
 
@@ -212,6 +216,7 @@ def preference_loss(scores: torch.Tensor, tokens: torch.Tensor, starts: torch.Te
     starts = _per_row(starts, "starts", torch.int32, 2 * pairs + 1, device)
     reference = _per_row(reference, "reference", torch.float32, 2 * pairs, device)
     temperature = _per_row(temperature, "temperature", torch.float32, N, device)
+    beta, smoothing = _number(beta, "beta"), _number(smoothing, "smoothing")
     out, out_type = _result(out, (N, V), device)
     where = scores.device
     losses, logprobs = (torch.empty(n, dtype=torch.float32, device=where) for n in (pairs, 2 * pairs))
@@ -350,7 +355,7 @@ class AdamW:
             flags = _per_row(active, "active", torch.bool, n, self._device)
         _changed(self._written)
         _call(lib.ytm_adamw, self._device, self._table.data_ptr(), n, self._chunks.value, self.bits,
-              self.steps.data_ptr(), flags, _number(lr, "lr"), rate_at, betas[0], betas[1], _number(eps, "eps"),
+              self.steps.data_ptr(), flags, _number(lr, "lr"), rate_at, float(betas[0]), float(betas[1]), _number(eps, "eps"),
               _number(weight_decay, "weight_decay"), self.seed)
 
 
