@@ -63,6 +63,8 @@ struct AdaptArgs {
   int64_t d_down_adapter, d_down_rank;
   int64_t d_up_adapter, d_up_output;
   int windows, slots;     // slots: blocks that share a window's segments
+  int tiles;              // blocks that share a window's outputs
+  bool tiles_first;       // whether these have numbers in a row
   int parts, part_steps;  // of a sum over clauses or outputs
   int padded;             // r, to whole tiles
   float* part;            // [parts][N in order][padded]
@@ -341,7 +343,9 @@ __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
   constexpr int kOwn = kHalves<X, W> ? 8 : 4, kStep = 4 * kOwn;  // clauses of a lane and of the wave in a step
   __shared__ Order order;
   __shared__ v4f join[kWaves][RT][kWave];
-  const int slot = blockIdx.x % a.slots, window = blockIdx.x / a.slots, p = blockIdx.y, ranks = blockIdx.z * RT * kTile;
+  // blocks of the same clauses are on the same XCD where there are 8 or 16 parts, and its L2 has their weights
+  // (512 rows, 8 adapters of 20000 x 32 bfloat16: 16.0 us, 16.7 the other way)
+  const int slot = blockIdx.y % a.slots, window = blockIdx.y / a.slots, p = blockIdx.x, ranks = blockIdx.z * RT * kTile;
   const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t row = row_of(code[l % kTile] == UINT32_MAX ? code[0] : code[l % kTile]);
@@ -464,7 +468,14 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
   __shared__ Order order;
   __shared__ __attribute__((aligned(16))) float hidden[kTile][RANKS + 4];
   __shared__ __attribute__((aligned(16))) float group_sums[kGroups > 1 ? kGroups : 1][kGroups > 1 ? kTile : 1][RANKS + 4];
-  const int slot = blockIdx.x % a.slots, window = blockIdx.x / a.slots;
+  // Few rows: blocks of the same outputs on the same XCD, which then reads their weights once (48 rows of some 30 adapters, 10000
+  // outputs, rank 16: 11.6 us, 12.9 the other way); many rows: those of the same rows one after the other (512 rows of
+  // 8 adapters, rank 32: 22.8 us, 27.0).
+  const int apart = a.tiles_first ? (a.tiles + 7) / 8 * 8 : a.windows * a.slots;
+  const int tile = a.tiles_first ? blockIdx.x % apart : blockIdx.x / apart;
+  const int rows = a.tiles_first ? blockIdx.x / apart : blockIdx.x % apart;
+  if (tile >= a.tiles) return;
+  const int slot = rows % a.slots, window = rows / a.slots;
   const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int at = l % kTile, four = l / kTile * 4;
@@ -538,7 +549,7 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
       store_floats<4>(a.out, row * a.out_stride + o0 + four, a.out_dtype, a.K - o0 - four, v);
     };
     const int whole = some && a.r % kTile == 0 ? a.K / kOutputs : 0;
-    int block = blockIdx.y * kWaves + wave;
+    int block = tile * kWaves + wave;
     Operands x;
     const bool early = block < whole;  // on their way beside the parts
     if (early) load(block * kOutputs, x);
@@ -576,14 +587,14 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
         }
         *(float4*)&hidden[n][j] = sum;
       }
-      if (a.hidden && blockIdx.y == 0 && n >= first && n < end) {
+      if (a.hidden && tile == 0 && n >= first && n < end) {
         float v[4];
         __builtin_memcpy(v, &hidden[n][j], sizeof v);
         store_floats<4>(a.hidden + row_of(code[n]) * a.hidden_stride + j, a.r - j, v);
       }
     }
     __syncthreads();
-    const int step = gridDim.y * kWaves;
+    const int step = a.tiles * kWaves;
     if (early)
       for (;;) {
         Operands next;
@@ -1127,7 +1138,7 @@ hipError_t launch_order(const AdaptArgs& a, hipStream_t s) {
 template <int X, int W>
 hipError_t launch_down(const AdaptArgs& a, hipStream_t s) {
   const int t = rank_tiles(a.r);
-  const dim3 grid(a.windows * a.slots, a.parts, (a.r + t * kTile - 1) / (t * kTile));
+  const dim3 grid(a.parts, a.windows * a.slots, (a.r + t * kTile - 1) / (t * kTile));
   switch (t) {
     case 1: down_kernel<X, W, 1><<<grid, kThreads, 0, s>>>(a); break;
     case 2: down_kernel<X, W, 2><<<grid, kThreads, 0, s>>>(a); break;
@@ -1147,7 +1158,7 @@ hipError_t launch_up(const AdaptArgs& a, dim3 grid, hipStream_t s) {
 }
 
 template <int W>
-hipError_t launch_adapt(const AdaptArgs& a, int x_dtype, hipStream_t s) {
+hipError_t launch_adapt(AdaptArgs a, int x_dtype, hipStream_t s) {
   hipError_t e = launch_order(a, s);
   if (e != hipSuccess) return e;
   switch (x_dtype) {
@@ -1160,7 +1171,9 @@ hipError_t launch_adapt(const AdaptArgs& a, int x_dtype, hipStream_t s) {
   // a block takes so many times 256 outputs that there are about 1024 of them
   const int64_t tiles = a.K > 0 ? (a.K + 255) / 256 : 1, blocks = (int64_t)a.windows * a.slots;
   const int64_t each = (tiles * blocks + 1023) / 1024;
-  const dim3 grid((unsigned)blocks, (unsigned)((tiles + each - 1) / each));
+  a.tiles = (int)((tiles + each - 1) / each);
+  a.tiles_first = a.windows < 16;
+  const dim3 grid((unsigned)(blocks * (a.tiles_first ? (a.tiles + 7) / 8 * 8 : a.tiles)));
   switch (a.dtype) {
     case YTM_DTYPE_F16: return launch_up<W, YTM_DTYPE_F16>(a, grid, s);
     case YTM_DTYPE_BF16: return launch_up<W, YTM_DTYPE_BF16>(a, grid, s);
