@@ -355,7 +355,8 @@ int ytm_adapt(const void *scores, int dtype, int64_t stride, int64_t N, int64_t 
 /* ytm_adapt_gradient: of a loss whose gradient by out is grad (N, K), with hidden as ytm_adapt gave it:
  *   d_up[a][o][j] = scale * sum over rows n of a of grad[n][o] * hidden[n][j]
  *   d_down[a][j][c] = sum over rows n of a of x[n][c] * scale * sum over o of grad[n][o] * up[a][o][j]
- * 0 for adapters that no row names.  (The gradient by scores is grad itself.)  d_down (M, r, C) and d_up
+ * 0 for adapters that no row names.  (The gradient by scores is grad itself.)  Sums with a value that is not
+ * finite are infinite or NaN.  d_down (M, r, C) and d_up
  * (M, K, r) are of w_dtype; grad F32, F16 or BF16.  Bounds and workspace as for ytm_adapt. */
 int ytm_adapt_gradient_workspace(int64_t N, int64_t C, int64_t K, int64_t M, int64_t r, int64_t *bytes);
 int ytm_adapt_gradient(const void *grad, int dtype, int64_t stride, int64_t N, int64_t K, const void *x, int x_dtype,

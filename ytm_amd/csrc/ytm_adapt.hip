@@ -7,9 +7,12 @@
 //
 // Rows are taken in the order of their adapters (ties in the order of rows), sixteen of that order,
 // a window, at a time: a window's rows of one adapter are a segment, whose weights are read once.
-// Sums run on the matrix cores in f32 with f32 operands, into which every type converts exactly; their
-// operands are one value a lane, so that products over rows need no transposition.  Sums over
-// clauses or outputs that several blocks share are joined in a fixed order.
+// Sums run on the matrix cores in f32 with exact operands: of one 16-bit type as they are, a f32 beside
+// values that bfloat16 holds as the sum of three of these, all else as f32, one value a lane.  Sums that
+// several blocks share are joined in a fixed order by a kernel that comes after.
+//
+// What bounds them is latency: a block's chain of waits (the order, the rows that it names, their values, the
+// parts' sums) takes 3 us at least, and memory is read and written at 1.6 to 3 TB/s.  Hence few launches, loads asked for before what they wait beside, and as many blocks a CU as the registers hold.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -238,7 +241,10 @@ struct Order {
     if (a.N > kInline) return __builtin_amdgcn_readfirstlane((int)a.order[a.N + key]);
     const uint32_t least = (uint32_t)key << 16;
     int before = 0;
-    for (int i = 0; i < a.N; i += kWave) before += __popcll(__ballot(i + threadIdx.x % kWave < a.N && code[(i + threadIdx.x % kWave) % kInline] < least));
+    for (int first = 0; first < a.N; first += kWave) {
+      const int i = first + (int)threadIdx.x % kWave;
+      before += __popcll(__ballot(i < a.N && code[i % kInline] < least));
+    }
     return before;
   }
 };
@@ -456,8 +462,9 @@ __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
   });
 }
 
-// 64 outputs a wave at a time of 16 rows.  Lane l has output l % 16 of a tile and row l % 16, and four ranks of
-// every 16; it gets sums of four outputs in a row of row l % 16.  RANKS: those of a.padded, or the most.
+// 64 outputs a wave at a time of 16 rows; f32 operands, since hidden is f32 and there are few products.
+// Lane l has output l % 16 of a tile and row l % 16, and four ranks of every 16; it gets sums of four outputs
+// in a row of row l % 16.  RANKS: those of a.padded, or the most.
 template <int W, int S, int RANKS>
 __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
   typedef typename Element<W>::type T;
@@ -468,9 +475,9 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
   __shared__ Order order;
   __shared__ __attribute__((aligned(16))) float hidden[kTile][RANKS + 4];
   __shared__ __attribute__((aligned(16))) float group_sums[kGroups > 1 ? kGroups : 1][kGroups > 1 ? kTile : 1][RANKS + 4];
-  // Few rows: blocks of the same outputs on the same XCD, which then reads their weights once (48 rows of some 30 adapters, 10000
-  // outputs, rank 16: 11.6 us, 12.9 the other way); many rows: those of the same rows one after the other (512 rows of
-  // 8 adapters, rank 32: 22.8 us, 27.0).
+  // Few rows: blocks of the same outputs on the same XCD, which then reads their weights once (48 rows of
+  // some 30 adapters, 10000 outputs, rank 16: 11.6 us, 12.9 the other way); many rows: those of the same rows
+  // one after the other (512 rows of 8 adapters, rank 32: 22.8 us, 27.0).
   const int apart = a.tiles_first ? (a.tiles + 7) / 8 * 8 : a.windows * a.slots;
   const int tile = a.tiles_first ? blockIdx.x % apart : blockIdx.x / apart;
   const int rows = a.tiles_first ? blockIdx.x / apart : blockIdx.x % apart;
@@ -747,7 +754,7 @@ struct OuterShared {
   };
 };
 
-// The 32 bits of a f32 as the sum of bfloat16: each cut, not rounded, so that nothing overflows; where the first is
+// The fraction of a f32 as the sum of bfloat16: each cut, not rounded, so that nothing overflows; where the first is
 // infinite or NaN the others are zero.
 template <int PLANES>
 __device__ __forceinline__ void split(float v, uint16_t (&part)[PLANES]) {
@@ -1047,7 +1054,7 @@ __global__ __launch_bounds__(kThreads, waves_of(RT, kGradPlanes<G>)) void grad_k
 }
 
 // Of more two launches, so that back's blocks are as many as their registers allow (2048 rows of 10007 bfloat16, rank 32:
-// together 69 us).
+// together 69 us; apart 27 and 37).
 template <int G, int W, int RT>
 __global__ __launch_bounds__(kThreads) void back_kernel(AdaptArgs a) {
   __shared__ Order order;
@@ -1209,7 +1216,10 @@ hipError_t launch_many(const AdaptArgs& a, hipStream_t s) {
 template <int G, int W>
 hipError_t launch_grad(AdaptArgs a, hipStream_t s) {
   const int t = rank_tiles(a.r);
-  if (a.N > kInline) return t == 1 ? launch_many<G, W, 1>(a, s) : t == 2 ? launch_many<G, W, 2>(a, s) : launch_many<G, W, 4>(a, s);
+  if (a.N > kInline) {
+    if (t == 1) return launch_many<G, W, 1>(a, s);
+    return t == 2 ? launch_many<G, W, 2>(a, s) : launch_many<G, W, 4>(a, s);
+  }
   return launch_outer(a, a.K, a.up_windows, [&](int first, int64_t blocks) {
     a.first = first;
     if (first) a.windows = 0;  // back is there
