@@ -316,6 +316,25 @@ def test_adapter_past_32_bits():
     np.testing.assert_array_equal(host(got[1]), host(torch.from_numpy(want[1]).to(torch.float16)))
 
 
+@pytest.mark.parametrize("N,M", [(65535, 4), (20000, 3000), (300, 65535)])
+def test_adapt_many_rows_and_adapters(N, M):
+    c = Case(N, 37, 5, 2, M)
+    out, hidden = c.adapt()
+    np.testing.assert_array_equal(host(hidden), c.hidden)
+    np.testing.assert_array_equal(host(out), c.out)
+    rng = np.random.default_rng(1)
+    grad, h = rng.integers(-1, 2, (N, 5)), rng.integers(-1, 2, (N, 2))
+    rows = np.flatnonzero(c.named)
+    at, u, xv = c.numbers[rows], host(c.up), c.xv[rows]
+    back = c.scale * np.einsum("no,noj->nj", grad[rows].astype(float), u[at])
+    d_down, d_up = np.zeros((M, 2, 37)), np.zeros((M, 5, 2))
+    np.add.at(d_down, at, back[:, :, None] * xv[:, None, :])
+    np.add.at(d_up, at, c.scale * grad[rows][:, :, None] * h[rows][:, None, :])
+    got = tune.adapt_gradient(gpu(grad), c.x, c.down, c.up, c.which, gpu(h), c.scale)
+    np.testing.assert_array_equal(host(got[0]), d_down)
+    np.testing.assert_array_equal(host(got[1]), d_up)
+
+
 # --------------------------------------------------------------------------------- losses
 def score_rows(rng, N, V, kind, masked=0.2):
     s = rng.normal(0, 3, (N, V)).astype(np.float32)
@@ -556,6 +575,36 @@ def test_losses_in_place_and_strides(N, V, kind):
             assert torch.equal(s, t)
 
 
+def test_losses_past_32_bits():
+    """The last rows of scores whose elements 32 bits do not count, in place."""
+    N, V, last = 17000, 131072, 3
+    rng = np.random.default_rng(0)
+    s = score_rows(rng, last, V, "bf16")
+    tokens = np.full(N, -1)
+    tokens[-last:] = rng.integers(0, V, last)
+    s[torch.arange(last), torch.from_numpy(tokens[-last:]).cuda()] = 1.0
+    old, adv = np.full(N, -12.0, np.float32), np.full(N, 0.5, np.float32)
+    want = tune.policy_loss(s, ints(tokens[-last:]), gpu(old[:last]), gpu(adv[:last]), weights=gpu(np.ones(last)),
+                            out=torch.empty_like(s))
+    pair = tune.preference_loss(s, ints(tokens[-last:]), ints([0, 1, last]), gpu([-12.0, -24.0]), out=torch.empty_like(s))
+    for call in ("policy", "preference"):
+        scores = torch.zeros(N, V, dtype=torch.bfloat16, device="cuda")
+        scores[-last:] = s
+        if call == "policy":
+            got = tune.policy_loss(scores, ints(tokens), gpu(old), gpu(adv), weights=gpu(np.ones(N)), out=scores)
+            assert bool((got[1][:-last] == 0).all())
+            # the rows alone are cut into slices, whose sums are joined
+            a, b = host(want[0]), host(got[0][-last:])
+            assert (np.abs(a - b) <= 2.0**-18 * np.abs(a)).all()
+            a, b = host(want[1]), host(got[1][-last:])
+        else:
+            got = tune.preference_loss(scores, ints(tokens), ints([N - last, N - last + 1, N]), gpu([-12.0, -24.0]), out=scores)
+            assert bool((got[1][:-last] == 0).all())
+            a, b = host(pair[1]), host(got[1][-last:])
+        assert (np.abs(a - b) <= 2.0**-7 * np.abs(a) + 2.0**-40).all() and np.abs(a).max() > 1e-3
+        del scores, got
+
+
 def test_policy_gradient_against_differences():
     rng = np.random.default_rng(4)
     N, V = 6, 12
@@ -736,6 +785,29 @@ def test_adamw_against_64_bits():
         x = x * (1 - lr * decay) - lr * (m / (1 - b1**k)) / (np.sqrt(v / (1 - b2**k)) + eps)
     # a step rounds p three times and the update, at most lr 10 here, some eight times
     assert (np.abs(host(p) - x) <= 10 * 2.0**-24 * (3 * (np.abs(x) + 0.5) + 8 * 10 * lr)).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_past_31_bits(bits):
+    """The last elements of a tensor whose elements 31 bits do not count."""
+    n, last = 2**31 + 999, 999
+    rng = np.random.default_rng(bits)
+    start = n - last - (n - last) % 256  # a block's first element
+    size = n - start
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    v, s = gpu(rng.normal(0, 0.1, size), "bf16"), gpu(rng.normal(0, 0.1, size), "bf16")
+    p[start:], g[start:] = v, s
+    a, m = tune.AdamW([p], [g], bits=bits, seed=9), Model(host(v), "bf16", bits)
+    for _ in range(2):
+        a.step(lr=0.01, betas=(0.9, 0.99), eps=1e-6, weight_decay=0.1)
+        m.step(host(s), start, 9, 0.01, 0.9, 0.99, 1e-6, 0.1)
+    off = np.abs(host(p[start:]) - m.p)
+    assert (off > 0).sum() <= 1 + 0.01 * off.size and (off <= 2.01 * ROUND["bf16"][0] * np.abs(m.p) + 2.0**-24).all()
+    first = host(a.first[0][start:])
+    if bits == 8:
+        first = first * host(a.first_scales[0][start // 256:]).repeat(256)[:size]
+    np.testing.assert_array_equal(first, m.m)
+    assert not bool(p[:start].any())
 
 
 def test_adamw_8_bits_keep_means():
