@@ -67,6 +67,7 @@ struct AdaptArgs {
   int64_t d_up_adapter, d_up_output;
   int windows, slots;     // slots: blocks that share a window's segments
   int tiles;              // blocks that share a window's outputs
+  int tile_blocks;        // blocks of 64 outputs of each
   bool tiles_first;       // whether these have numbers in a row
   int parts, part_steps;  // of a sum over clauses or outputs
   int padded;             // r, to whole tiles
@@ -250,7 +251,9 @@ struct Order {
 };
 
 // The segments of a window that block `slot` of `slots` takes: body(key, first place, end).  A place begins one
-// where its key is not that of the place before.
+// where its key is not that of the place before.  Blocks of the same slot have numbers in a row: those of later
+// slots often find nothing, and by turns they would leave every other XCD without work (4096 rows of one
+// adapter, 20000 clauses, 10000 outputs, rank 32: 312 us, 188 in a row).
 template <typename Body>
 __device__ __forceinline__ void segments(const uint32_t* code, int slot, int slots, Body body) {
   const int i = threadIdx.x % kTile;
@@ -351,7 +354,7 @@ __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
   __shared__ v4f join[kWaves][RT][kWave];
   // blocks of the same clauses are on the same XCD where there are 8 or 16 parts, and its L2 has their weights
   // (512 rows, 8 adapters of 20000 x 32 bfloat16: 16.0 us, 16.7 the other way)
-  const int slot = blockIdx.y % a.slots, window = blockIdx.y / a.slots, p = blockIdx.x, ranks = blockIdx.z * RT * kTile;
+  const int slot = blockIdx.y / a.windows, window = blockIdx.y % a.windows, p = blockIdx.x, ranks = blockIdx.z * RT * kTile;
   const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t row = row_of(code[l % kTile] == UINT32_MAX ? code[0] : code[l % kTile]);
@@ -482,7 +485,7 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
   const int tile = a.tiles_first ? blockIdx.x % apart : blockIdx.x / apart;
   const int rows = a.tiles_first ? blockIdx.x / apart : blockIdx.x % apart;
   if (tile >= a.tiles) return;
-  const int slot = rows % a.slots, window = rows / a.slots;
+  const int slot = rows / a.windows, window = rows % a.windows;
   const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int at = l % kTile, four = l / kTile * 4;
@@ -556,9 +559,12 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
       store_floats<4>(a.out, row * a.out_stride + o0 + four, a.out_dtype, a.K - o0 - four, v);
     };
     const int whole = some && a.r % kTile == 0 ? a.K / kOutputs : 0;
-    int block = tile * kWaves + wave;
+    // a block's outputs are in a row
+    int block = tile * a.tile_blocks + wave;
+    const int past = (tile + 1) * a.tile_blocks, last = (a.K + kOutputs - 1) / kOutputs;
+    const int end_block = past < last ? past : last;
     Operands x;
-    const bool early = block < whole;  // on their way beside the parts
+    const bool early = block < whole && block < end_block;  // on their way beside the parts
     if (early) load(block * kOutputs, x);
     loads_first();
     __syncthreads();
@@ -601,19 +607,18 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
       }
     }
     __syncthreads();
-    const int step = a.tiles * kWaves;
     if (early)
       for (;;) {
         Operands next;
-        const bool more = block + step < whole;
-        if (more) load((block + step) * kOutputs, next);
+        const bool more = block + kWaves < whole && block + kWaves < end_block;
+        if (more) load((block + kWaves) * kOutputs, next);
         loads_first();
         finish(block * kOutputs, x);
-        block += step;
+        block += kWaves;
         if (!more) break;
         x = next;
       }
-    for (; block * kOutputs < a.K; block += step)
+    for (; block < end_block; block += kWaves)
       for (int o0 = block * kOutputs; o0 < a.K && o0 < (block + 1) * kOutputs; o0 += kTile) guarded(o0);
   });
 }
@@ -628,7 +633,7 @@ __device__ __forceinline__ void back_block(const AdaptArgs& a, int block, int p,
   typedef typename Element<W>::type T;
   typedef typename Element<G>::type S;
   constexpr bool kHalf = G == W && W != YTM_DTYPE_F32;
-  const int slot = block % a.slots, window = block / a.slots;
+  const int slot = block / a.windows, window = block % a.windows;
   const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t row = row_of(code[l % kTile] == UINT32_MAX ? code[0] : code[l % kTile]);
@@ -986,9 +991,9 @@ __device__ __forceinline__ void outer_blocks(const AdaptArgs& a, int block, int 
     return;
   }
   const RowWindows& w = UP ? a.up_windows : a.down_windows;
-  const int window = block / w.slots, from = window * w.rows, to = from + w.rows < a.N ? from + w.rows : a.N;
+  const int window = block % w.count, from = window * w.rows, to = from + w.rows < a.N ? from + w.rows : a.N;
   const int first = key_of(a.order[from]), last = key_of(a.order[to - 1]);
-  for (int key = first + block % w.slots; key <= last && key < a.M; key += w.slots) {
+  for (int key = first + block / w.count; key <= last && key < a.M; key += w.slots) {
     const int begin = order.begin(a, key), end = order.begin(a, key + 1);
     if (begin == end) continue;
     float* partial = nullptr;
@@ -1080,20 +1085,21 @@ struct Split {
   int windows, slots, parts, part_steps;
 };
 
-// Parts of a sum over `steps` (of `block` rows in a row), so that about 512 blocks share it, each with a step a
+// Parts of a sum over `steps` (of `block` rows in a row), so that about 1024 blocks share it, each with a step a
 // wave at least, and slots that share a window's segments where there are still few blocks.
 Split split_of(int64_t N, int64_t M, int64_t steps, int64_t most_parts) {
   Split s;
   s.windows = (int)((N + kTile - 1) / kTile);
   const int64_t most = steps > kWaves ? (steps + kWaves - 1) / kWaves : 1;
-  int64_t parts = 512 / s.windows;
+  int64_t parts = 1024 / s.windows;
   parts = parts < 1 ? 1 : parts > most_parts ? most_parts : parts;
   parts = parts < most ? parts : most;
   s.part_steps = (int)((steps + parts - 1) / parts);
   s.part_steps = s.part_steps ? s.part_steps : 1;
   s.parts = steps ? (int)((steps + s.part_steps - 1) / s.part_steps) : 1;
   int64_t slots = 1024 / ((int64_t)s.windows * s.parts);
-  const int64_t segments = M + 1 < kTile ? M + 1 : kTile;
+  int64_t segments = M + 1 < kTile ? M + 1 : kTile;  // of a window, at most
+  segments = N < segments ? N : segments;
   slots = slots < 1 ? 1 : slots < segments ? slots : segments;
   s.slots = (int)slots;
   return s;
@@ -1175,11 +1181,13 @@ hipError_t launch_adapt(AdaptArgs a, int x_dtype, hipStream_t s) {
     default: e = launch_down<YTM_DTYPE_F32, W>(a, s); break;
   }
   if (e != hipSuccess) return e;
-  // a block takes so many times 256 outputs that there are about 1024 of them
-  const int64_t tiles = a.K > 0 ? (a.K + 255) / 256 : 1, blocks = (int64_t)a.windows * a.slots;
-  const int64_t each = (tiles * blocks + 1023) / 1024;
-  a.tiles = (int)((tiles + each - 1) / each);
+  // A block takes so many times 256 outputs that there are about 1024 of them, or 2048 for many rows (4096 rows of 8
+  // adapters: 205 us, with 1024 230; 48 rows of some 30 adapters: 19.3 us, with 1024 18.8).
   a.tiles_first = a.windows < 16;
+  const int64_t tiles = a.K > 0 ? (a.K + 255) / 256 : 1, blocks = (int64_t)a.windows * a.slots;
+  const int64_t most = a.tiles_first ? 1024 : 2048, each = (tiles * blocks + most - 1) / most;
+  a.tiles = (int)((tiles + each - 1) / each);
+  a.tile_blocks = (int)(each * kWaves);
   const dim3 grid((unsigned)(blocks * (a.tiles_first ? (a.tiles + 7) / 8 * 8 : a.tiles)));
   switch (a.dtype) {
     case YTM_DTYPE_F16: return launch_up<W, YTM_DTYPE_F16>(a, grid, s);
