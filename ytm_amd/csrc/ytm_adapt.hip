@@ -253,7 +253,7 @@ struct Order {
 // The segments of a window that block `slot` of `slots` takes: body(key, first place, end).  A place begins one
 // where its key is not that of the place before.  Blocks of the same slot have numbers in a row: those of later
 // slots often find nothing, and by turns they would leave every other XCD without work (4096 rows of one
-// adapter, 20000 clauses, 10000 outputs, rank 32: 312 us, 188 in a row).
+// adapter, 20000 clauses, 10000 outputs, rank 32: 312 us, 196 in a row).
 template <typename Body>
 __device__ __forceinline__ void segments(const uint32_t* code, int slot, int slots, Body body) {
   const int i = threadIdx.x % kTile;
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(kThreads) void down_kernel(AdaptArgs a) {
   __shared__ Order order;
   __shared__ v4f join[kWaves][RT][kWave];
   // blocks of the same clauses are on the same XCD where there are 8 or 16 parts, and its L2 has their weights
-  // (512 rows, 8 adapters of 20000 x 32 bfloat16: 16.0 us, 16.7 the other way)
+  // (512 rows, 8 adapters of 20000 x 32 bfloat16: 30 MB read, 58 the other way)
   const int slot = blockIdx.y / a.windows, window = blockIdx.y % a.windows, p = blockIdx.x, ranks = blockIdx.z * RT * kTile;
   const uint32_t* code = order.window(a, window);
   const int l = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -1059,7 +1059,7 @@ __global__ __launch_bounds__(kThreads, waves_of(RT, kGradPlanes<G>)) void grad_k
 }
 
 // Of more two launches, so that back's blocks are as many as their registers allow (2048 rows of 10007 bfloat16, rank 32:
-// together 69 us; apart 27 and 37).
+// together 69 us; apart 20 and 38).
 template <int G, int W, int RT>
 __global__ __launch_bounds__(kThreads) void back_kernel(AdaptArgs a) {
   __shared__ Order order;
