@@ -1,0 +1,35 @@
+"""The adapting and learning operators at the ends of their ranges: memory that is not an operand's own, numbers at
+the ends of their types, what is left out, and objects that are copied."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+ytm_amd = pytest.importorskip("ytm_amd")
+from ytm_amd import tune  # noqa: E402
+
+from test_gpu_tune import TYPES, Case, gpu, host, ints  # noqa: E402
+
+
+# ------------------------------------------------------------------------------- adapters
+@pytest.mark.parametrize("w", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("N,K,r", [(20, 128, 48), (300, 64, 48), (17, 192, 80), (5, 64, 112), (40, 130, 144), (9, 64, 240),
+                                   (20, 128, 64), (20, 128, 32)])
+def test_adapt_reads_no_weights_behind_a_row(N, K, r, w):
+    """Ranks of whole 16s: NaN between the rows of up and in the adapters between those that rows name."""
+    c = Case(N, 100, K, r, 3, "bits", w, which=np.arange(N) % 4 - 1)
+    memory = torch.full((5, K, r + 19), float("nan"), dtype=TYPES[w], device="cuda")
+    up = memory[::2, :, :r]
+    up.copy_(c.up)
+    memory[::2, :, r:] = float("nan")
+    hidden = torch.empty(N, r, device="cuda")
+    out = tune.adapt(c.scores, c.x, c.down, up, c.which, c.scale, hidden=hidden)
+    np.testing.assert_array_equal(host(hidden), c.hidden)
+    np.testing.assert_array_equal(host(out), c.out)
+    # rows one after the other: what follows one is the next output's, which is not finite
+    c.up[:, 1::2] = float("inf")
+    c.up[1] = float("nan")
+    out = host(tune.adapt(c.scores, c.x, c.down, c.up, c.which, c.scale))
+    clean = c.numbers != 1
+    np.testing.assert_array_equal(out[clean][:, 0::2], c.out[clean][:, 0::2])

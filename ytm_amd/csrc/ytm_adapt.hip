@@ -526,7 +526,8 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
       for (int t = 0; t < kTiles; ++t) sum[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) multiply(s * kTile, x.w[s], sum);
-      for (int j = kSteps * kTile; RANKS > 32 && j < padded; j += kTile) {
+      // up to r, a multiple of 16 here, and not to `padded`: what follows a row of up is not its own
+      for (int j = kSteps * kTile; RANKS > 32 && j < a.r; j += kTile) {
         T w[kTiles][4];
         weights(o0, j, w);
         multiply(j, w, sum);
