@@ -33,3 +33,30 @@ def test_adapt_reads_no_weights_behind_a_row(N, K, r, w):
     out = host(tune.adapt(c.scores, c.x, c.down, c.up, c.which, c.scale))
     clean = c.numbers != 1
     np.testing.assert_array_equal(out[clean][:, 0::2], c.out[clean][:, 0::2])
+
+
+@pytest.fixture
+def other_defaults():
+    torch.set_default_device("cuda")
+    torch.set_default_dtype(torch.bfloat16)
+    yield
+    torch.set_default_device(None)
+    torch.set_default_dtype(torch.float32)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_torchs_defaults_change_nothing(bits, request):
+    def learnt():
+        rng = np.random.default_rng(0)
+        a = tune.Adapters(3, 50, 20, rank=4, bits=bits, seed=2)
+        scores, which = gpu(rng.normal(0, 1, (30, 20))), ints(np.arange(30) % 3 - 1)
+        x = gpu(rng.normal(0, 1, (30, 50)))
+        hidden = a.adapt(scores, x, which)
+        _, grad, lp = tune.policy_loss(scores, ints(np.arange(30) % 20), gpu(np.zeros(30)), gpu(np.ones(30)))
+        a.learn(grad, x, which, hidden)
+        return [a.down, a.up, hidden, grad, lp]
+
+    want = learnt()
+    request.getfixturevalue("other_defaults")
+    for s, t in zip(want, learnt()):
+        assert s.dtype == t.dtype and torch.equal(s, t)

@@ -330,7 +330,7 @@ class AdamW:
                 setattr(row, name, getattr(self, name)[i].data_ptr())
         size, self._chunks = ctypes.c_int64(), ctypes.c_int64()
         check(lib.ytm_adamw_table(rows, n, self.bits, None, size, self._chunks))
-        host = torch.empty(size.value, dtype=torch.uint8)
+        host = torch.empty(size.value, dtype=torch.uint8, device="cpu")  # whatever torch's default is
         check(lib.ytm_adamw_table(rows, n, self.bits, host.data_ptr(), size, self._chunks))
         self._table = host.to(self.parameters[0].device)
         # the memory that the table's addresses mean
@@ -376,7 +376,8 @@ class Adapters:
             raise TypeError("adapters are float32, float16 or bfloat16.")
         g = torch.Generator(device=device).manual_seed(int(seed))
         self.count, self.scale = int(count), _number(scale, "scale")
-        self.down = torch.empty(count, rank, clauses, device=device).normal_(0.0, clauses ** -0.5, generator=g).to(dtype)
+        down = torch.empty(count, rank, clauses, dtype=torch.float32, device=device)
+        self.down = down.normal_(0.0, clauses ** -0.5, generator=g).to(dtype)
         self.up = torch.zeros(count, outputs, rank, dtype=dtype, device=device)
         self.gradients = torch.zeros_like(self.down), torch.zeros_like(self.up)
         each = lambda down, up: [t for a in range(count) for t in (down[a], up[a])]  # noqa: E731
@@ -384,7 +385,7 @@ class Adapters:
 
     def adapt(self, scores: torch.Tensor, x: torch.Tensor, which: torch.Tensor) -> torch.Tensor:
         """Corrects scores (N, K) in place, each row by its adapter, and returns what learn() needs (N, rank)."""
-        hidden = torch.empty(which.shape[0], self.down.shape[1], device=self.down.device)
+        hidden = torch.empty(which.shape[0], self.down.shape[1], dtype=torch.float32, device=self.down.device)
         adapt(scores, x, self.down, self.up, which, self.scale, hidden=hidden, out=scores)
         return hidden
 
