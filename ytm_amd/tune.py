@@ -385,7 +385,8 @@ class Adapters:
 
     def adapt(self, scores: torch.Tensor, x: torch.Tensor, which: torch.Tensor) -> torch.Tensor:
         """Corrects scores (N, K) in place, each row by its adapter, and returns what learn() needs (N, rank)."""
-        hidden = torch.empty(which.shape[0], self.down.shape[1], dtype=torch.float32, device=self.down.device)
+        rows = which.shape[0] if isinstance(which, _Tensor) and which.dim() == 1 else 0  # adapt says what is wrong
+        hidden = torch.empty(rows, self.down.shape[1], dtype=torch.float32, device=self.down.device)
         adapt(scores, x, self.down, self.up, which, self.scale, hidden=hidden, out=scores)
         return hidden
 
