@@ -1,5 +1,9 @@
 """The adapting and learning operators at the ends of their ranges: memory that is not an operand's own, numbers at
 the ends of their types, what is left out, and objects that are copied."""
+import copy
+import io
+import pickle
+
 import numpy as np
 import pytest
 
@@ -60,3 +64,48 @@ def test_torchs_defaults_change_nothing(bits, request):
     request.getfixturevalue("other_defaults")
     for s, t in zip(want, learnt()):
         assert s.dtype == t.dtype and torch.equal(s, t)
+
+
+# --------------------------------------------------------------------------------- copies
+def saved(a):
+    f = io.BytesIO()
+    torch.save(a, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)  # what this test wrote itself
+
+
+def learn(a, seed):
+    rng = np.random.default_rng(seed)
+    x, which, grad = gpu(rng.normal(0, 1, (30, 50))), ints(rng.integers(-1, 3, 30)), gpu(rng.normal(0, 1, (30, 20)))
+    hidden = a.adapt(gpu(np.zeros((30, 20))), x, which)
+    a.learn(grad, x, which, hidden, lr=0.05)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda a: pickle.loads(pickle.dumps(a)), saved])
+def test_copies_of_adapters_learn_apart(copied, bits):
+    a = tune.Adapters(3, 50, 20, rank=4, bits=bits, seed=2, scale=0.5)
+    learn(a, 1)
+    frozen = [t.clone() for t in (a.down, a.up, *a.optimizer.first)]
+    b = copied(a)
+    learn(b, 2)
+    for s, t in zip(frozen, (a.down, a.up, *a.optimizer.first)):
+        assert torch.equal(s.float(), t.float())
+    assert not torch.equal(b.up, a.up) and not torch.equal(b.down, a.down)
+    learn(a, 2)  # the same step from the same states
+    for s, t in zip((a.down, a.up, *a.optimizer.first, *a.optimizer.second, a.optimizer.steps),
+                    (b.down, b.up, *b.optimizer.first, *b.optimizer.second, b.optimizer.steps)):
+        assert torch.equal(s.float(), t.float())
+    del a
+    learn(b, 3)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_of_adamw_step_their_own(bits):
+    a = tune.AdamW([gpu(np.ones(500))], [gpu(np.ones(500))], bits=bits, seed=1)
+    a.step(0.1)
+    was, b = a.parameters[0].clone(), copy.deepcopy(a)
+    b.step(0.1)
+    assert torch.equal(a.parameters[0], was) and not torch.equal(b.parameters[0], was)
+    a.step(0.1)
+    assert torch.equal(a.parameters[0], b.parameters[0]) and a.steps.tolist() == b.steps.tolist() == [2]

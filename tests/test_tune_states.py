@@ -1,12 +1,16 @@
 """What AdamW and Adapters make of their surroundings and of what they are given, without a GPU: tensors that say that
 they are on one, and entries that count their calls (as in test_tune.py)."""
+import copy
+import io
+import pickle
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 from ytm_amd import tune  # noqa: E402
 
-from test_tune import I32, entries, on_gpu  # noqa: E402, F401
+from test_tune import I32, OnGpu, entries, on_gpu  # noqa: E402, F401
 
 
 def test_tables_are_made_on_the_host(entries):  # noqa: F811
@@ -23,3 +27,45 @@ def test_adapters_say_what_is_wrong(entries, which):  # noqa: F811
     with pytest.raises((TypeError, ValueError), match="which"):
         a.adapt(on_gpu(4, 6), on_gpu(4, 2, dtype=I32), which)
     assert entries.launched == 0
+
+
+class Copied(OnGpu):
+    def __deepcopy__(self, memo):
+        return memo.setdefault(id(self), self.clone())
+
+
+def copied_on_gpu(n, dtype=torch.float32):
+    return on_gpu(n, dtype=dtype).as_subclass(Copied)
+
+
+def addresses(a):
+    """The parameters' addresses in an AdamW's table, whose rows are 136 bytes or more, each parameter's first."""
+    words = a._table[:a._table.numel() // 8 * 8].view(torch.int64).tolist()
+    return [t.data_ptr() in words for t in (*a.parameters, *a.gradients, *a.first, *a.second)], words
+
+
+def saved(a):
+    f = io.BytesIO()
+    torch.save(a, f)
+    f.seek(0)
+    return torch.load(f, weights_only=False)  # what this test wrote itself
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda a: pickle.loads(pickle.dumps(a)), saved])
+def test_copies_have_addresses_of_their_own(copied, bits):
+    sizes, state = (300, 7), torch.float32 if bits == 32 else torch.float8_e4m3fn
+    states = {name: [copied_on_gpu(n, dtype=state) for n in sizes] for name in ("first", "second")}
+    if bits == 8:
+        states |= {name: [copied_on_gpu(-(-n // 256)) for n in sizes] for name in ("first_scales", "second_scales")}
+    a = tune.AdamW([copied_on_gpu(n) for n in sizes], [copied_on_gpu(n) for n in sizes], bits=bits, states=states, steps=5, seed=3)
+    b = copied(a)
+    assert (b.bits, b.seed, b.steps.tolist()) == (bits, 3, [5, 5])
+    for one, other in ((a, b), (b, a)):
+        there, words = addresses(one)
+        assert all(there)
+        assert not any(t.data_ptr() in words for t in (*other.parameters, *other.gradients, *other.first, *other.second))
+    b.steps += 1
+    assert a.steps.tolist() == [5, 5]
+    c = copy.copy(a)
+    assert all(addresses(c)[0]) and c.parameters[0] is a.parameters[0] and c.steps is a.steps

@@ -243,7 +243,9 @@ class AdamW:
     average that moves by a thousandth a step would never leave an 8-bit number's neighbourhood otherwise.
 
     states: first, second (and the scales) to go on with, as `states()` gives them, and steps the number of
-    steps made, a number or a tensor of one for each parameter; by default all begin at 0."""
+    steps made, a number or a tensor of one for each parameter; by default all begin at 0.
+
+    A copy (copy.deepcopy, pickle, torch.save) steps the copied tensors, a shallow one the same as its original."""
 
     def __init__(self, parameters: list[torch.Tensor], gradients: list[torch.Tensor], bits: int = 32,
                  states: dict[str, list[torch.Tensor]] | None = None, steps: int | torch.Tensor = 0, seed: int = 0):
@@ -336,6 +338,20 @@ class AdamW:
         # the memory that the table's addresses mean
         self._held = [t.detach() for t in (*self._written, *self.gradients)]
 
+    def __getstate__(self) -> dict:
+        # the table's addresses are those of this object's tensors; pickle alone does not know float8
+        state = {k: v for k, v in self.__dict__.items() if k not in ("_table", "_chunks", "_held", "_written")}
+        if self.bits == 8:
+            state |= {name: [t.view(torch.uint8) for t in state[name]] for name in ("first", "second")}
+        return state
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        if self.bits == 8:
+            self.first, self.second = ([t.view(torch.float8_e4m3fn) for t in s] for s in (self.first, self.second))
+        AdamW.__init__(self, self.parameters, self.gradients, self.bits, self.states(), self.steps, self.seed)
+        self.steps = state["steps"]
+
     def states(self) -> dict[str, list[torch.Tensor]]:
         """The states, to go on with: AdamW(..., states=a.states(), steps=a.steps)."""
         return {name: getattr(self, name) for name in self._names}
@@ -364,7 +380,8 @@ class Adapters:
 
     down (count, rank, clauses) starts as small random numbers, up (count, outputs, rank) as 0, so that nothing
     changes before something is learnt.  gradients: those of the last learn().  optimizer: an AdamW whose tensors
-    are down[a] and up[a] of each adapter a, in turn, with states of `bits` bits."""
+    are down[a] and up[a] of each adapter a, in turn, with states of `bits` bits.  A copy (copy.deepcopy, pickle,
+    torch.save) has adapters, states and step counts of its own."""
 
     def __init__(self, count: int, clauses: int, outputs: int, rank: int = 16, scale: float = 1.0,
                  dtype: torch.dtype = torch.float32, bits: int = 32, device: str | torch.device = "cuda", seed: int = 0):
@@ -380,8 +397,23 @@ class Adapters:
         self.down = down.normal_(0.0, clauses ** -0.5, generator=g).to(dtype)
         self.up = torch.zeros(count, outputs, rank, dtype=dtype, device=device)
         self.gradients = torch.zeros_like(self.down), torch.zeros_like(self.up)
-        each = lambda down, up: [t for a in range(count) for t in (down[a], up[a])]  # noqa: E731
-        self.optimizer = AdamW(each(self.down, self.up), each(*self.gradients), bits=bits, seed=seed)
+        self.optimizer = AdamW(*self._each(), bits=bits, seed=seed)
+
+    def _each(self) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
+        each = lambda down, up: [t for a in range(self.count) for t in (down[a], up[a])]  # noqa: E731
+        return each(self.down, self.up), each(*self.gradients)
+
+    def __getstate__(self) -> dict:
+        # the optimiser's parameters and gradients are parts of this object's tensors, which pickle would part
+        optimizer = self.optimizer.__getstate__()
+        del optimizer["parameters"], optimizer["gradients"]
+        return dict(self.__dict__, optimizer=optimizer)
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        parameters, gradients = self._each()
+        self.optimizer = AdamW.__new__(AdamW)
+        self.optimizer.__setstate__(dict(state["optimizer"], parameters=parameters, gradients=gradients))
 
     def adapt(self, scores: torch.Tensor, x: torch.Tensor, which: torch.Tensor) -> torch.Tensor:
         """Corrects scores (N, K) in place, each row by its adapter, and returns what learn() needs (N, rank)."""
