@@ -405,7 +405,7 @@ int ytm_preference_loss(const void *scores, int dtype, int64_t stride, int64_t N
  *   m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2
  *   p = (1 - rate decay) p - rate / (1 - beta1^k) * m / (sqrt(v / (1 - beta2^k)) + eps)
  * and none where active[i] (NULL: all are) is 0.  rate_at (or NULL) has the rate instead of `rate`.
- * steps, active, rate_at: device.  The tensors are in a table
+ * steps (0 or more before the step), active, rate_at: device.  The tensors are in a table
  * that ytm_adamw_table writes to host memory (NULL: says only its bytes and its chunks, which ytm_adamw
  * takes) and that the caller copies to device memory at a multiple of 16 bytes; ytm_adamw writes to it,
  * so two steps of one table follow each other.  parameter: F32, F16 or BF16; gradient: of the same type or

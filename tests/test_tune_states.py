@@ -69,3 +69,10 @@ def test_copies_have_addresses_of_their_own(copied, bits):
     assert a.steps.tolist() == [5, 5]
     c = copy.copy(a)
     assert all(addresses(c)[0]) and c.parameters[0] is a.parameters[0] and c.steps is a.steps
+
+
+@pytest.mark.parametrize("steps", [-1, torch.tensor([0, -1]), torch.tensor([-(2**40), 3])])
+def test_steps_before_the_first_are_refused(entries, steps):  # noqa: F811
+    with pytest.raises(ValueError, match="0 or more"):
+        tune.AdamW([on_gpu(3), on_gpu(4)], [on_gpu(3), on_gpu(4)], steps=steps)
+    tune.AdamW([on_gpu(3), on_gpu(4)], [on_gpu(3), on_gpu(4)], steps=torch.tensor([0, 2**40]))

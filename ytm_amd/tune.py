@@ -283,8 +283,12 @@ class AdamW:
         if isinstance(steps, _Tensor):
             if steps.shape != (len(self.parameters),) or steps.is_floating_point():
                 raise ValueError(f"steps must be whole numbers of shape ({len(self.parameters)},).")
+            if bool((steps < 0).any()):
+                raise ValueError("steps must be 0 or more.")
             self.steps = steps.detach().to(device=first.device, dtype=torch.int64, copy=True).contiguous()
         else:
+            if steps < 0:
+                raise ValueError("steps must be 0 or more.")
             self.steps = torch.full((len(self.parameters),), int(steps), dtype=torch.int64, device=first.device)
         self._names = names
         self._written = tuple(t for name in ("parameters", *names) for t in getattr(self, name))
