@@ -411,7 +411,7 @@ int ytm_preference_loss(const void *scores, int dtype, int64_t stride, int64_t N
  * so two steps of one table follow each other.  parameter: F32, F16 or BF16; gradient: of the same type or
  * F32.  With bits 32 first (m) and second (v) are f32.  With bits 8 they are E4M3 floats (sign, four bits
  * of exponent with bias 7, three of fraction, 127 a NaN) times a power of two for each 256 elements in a
- * row, m itself and v as its root.  What is stored in fewer bits than f32 is rounded up or down at random,
+ * row (2^-98 or more; of roots 2^-54 or more but for zeros alone), m itself and v as its root.  What is stored in fewer bits than f32 is rounded up or down at random,
  * with the chances that keep the mean of parameters, of m and of v, from `seed`, the step and the
  * element's place (each tensor before it counts as a multiple of 256 long); a v above 0 stays above 0, what is
  * not finite becomes NaN in 8 bits.  The operands of different tensors must not overlap. */

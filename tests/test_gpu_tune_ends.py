@@ -66,6 +66,35 @@ def test_torchs_defaults_change_nothing(bits, request):
         assert s.dtype == t.dtype and torch.equal(s, t)
 
 
+# ---------------------------------------------------------------------------------- AdamW
+@pytest.mark.parametrize("size", [1e-10, 1e-14, 1e-17, 1e-18])
+def test_second_states_above_zero_stay_above_it(size):
+    """8 bits, eps 0: gradients whose squares float32 holds, of very different sizes in a block, and none after."""
+    rng = np.random.default_rng(0)
+    n = 256 * 6 + 100
+    g = gpu(size * 10.0 ** rng.uniform(-1, 0, n) * rng.choice([-1, 1], n))
+    g[::256] *= 1.0 / 16  # codes that are next to 0
+    p = gpu(np.ones(n))
+    a = tune.AdamW([p], [g], bits=8, seed=3)
+    root = lambda: host(a.second[0]) * host(a.second_scales[0]).repeat(256)[:n]  # noqa: E731
+    for k in range(4):
+        a.step(0.01, eps=0.0)
+        assert bool(torch.isfinite(p).all()) and (root() > 0).all(), k
+        assert (np.float32(root()) ** 2 >= 2.0**-126).all() and float(a.second_scales[0].min()) >= 2.0**-54, k
+        assert float((p - 1).abs().max()) <= 4 * 0.011 * (k + 1), k
+        if k == 0:
+            g.zero_()
+
+
+def test_blocks_of_zeros_keep_their_scale():
+    p, g = gpu(np.ones(600)), gpu(np.zeros(600))
+    g[300] = 1.0
+    a = tune.AdamW([p], [g], bits=8)
+    a.step(0.01)
+    assert a.second_scales[0].tolist()[::2] == a.first_scales[0].tolist()[::2] == [2.0**-98] * 2
+    assert float(a.second_scales[0][1]) > 2.0**-54 and not bool(a.second[0][:256].float().any())
+
+
 # --------------------------------------------------------------------------------- copies
 def saved(a):
     f = io.BytesIO()

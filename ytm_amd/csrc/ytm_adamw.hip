@@ -238,7 +238,9 @@ __device__ __forceinline__ void roots_of(const float (&v)[kEach], float (&root)[
 }
 
 // Exponents of a block's two scales: 2^e 448 is the least such number that its largest magnitude does not
-// pass, and at least 2^-98, so that no product leaves what float32 holds.  What is not finite has no part.
+// pass, at least 2^-98, so that no product leaves what float32 holds, and of roots at least 2^-54, so that the square
+// of the least code, 2^-9 of it, is a normal float and not 0 (a block of zeros alone has 2^-98).  What is not finite
+// has no part.
 typedef uint16_t v2h __attribute__((ext_vector_type(2)));
 template <int CONTROL>
 __device__ __forceinline__ v2h larger_of_row(v2h v) {
@@ -264,7 +266,6 @@ __device__ __forceinline__ void exponents_of(const float (&m)[kEach], const floa
   }
   // the exponent of what comes after 1.75 times a power of two is the next
   v2h v = {(uint16_t)(most[0] + 0x1FFFFFu >> 23), (uint16_t)(most[1] + 0x1FFFFFu >> 23)};
-  v = __builtin_elementwise_max(v, (v2h{37, 37}));
   v = larger_of_row<0x128>(v);  // of the 16 lanes of a row, turned by 8, 4, 2 and 1
   v = larger_of_row<0x124>(v);
   v = larger_of_row<0x122>(v);
@@ -276,6 +277,8 @@ __device__ __forceinline__ void exponents_of(const float (&m)[kEach], const floa
   const auto halves = __builtin_amdgcn_permlane32_swap(w, w, false, false);
   v = __builtin_elementwise_max(__builtin_bit_cast(v2h, (uint32_t)halves[0]),
                                 __builtin_bit_cast(v2h, (uint32_t)halves[1]));
+  // the root of any float above 0 is 2^-75 or more: a 0 here is a block of zeros
+  v = __builtin_elementwise_max(v, (v2h{37, (uint16_t)(v[1] ? 81 : 37)}));
   first = (int)v[0] - 135, second = (int)v[1] - 135;
 }
 
