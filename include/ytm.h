@@ -356,8 +356,10 @@ int ytm_adapt(const void *scores, int dtype, int64_t stride, int64_t N, int64_t 
  *   d_up[a][o][j] = scale * sum over rows n of a of grad[n][o] * hidden[n][j]
  *   d_down[a][j][c] = sum over rows n of a of x[n][c] * scale * sum over o of grad[n][o] * up[a][o][j]
  * 0 for adapters that no row names.  (The gradient by scores is grad itself.)  Sums with a value that is not
- * finite are infinite or NaN.  d_down (M, r, C) and d_up
- * (M, K, r) are of w_dtype; grad F32, F16 or BF16.  Bounds and workspace as for ytm_adapt. */
+ * finite are infinite or NaN.  d_down (M, r, C) and d_up (M, K, r) are of w_dtype; grad F32, F16 or BF16.
+ * Bounds and workspace as for ytm_adapt.
+ * ytm_adapt_gradient_as: the same with d_down and d_up of d_dtype, which is w_dtype or F32: the sums of a batch
+ * are often less than the 2^-24 that float16 holds. */
 int ytm_adapt_gradient_workspace(int64_t N, int64_t C, int64_t K, int64_t M, int64_t r, int64_t *bytes);
 int ytm_adapt_gradient(const void *grad, int dtype, int64_t stride, int64_t N, int64_t K, const void *x, int x_dtype,
                        int64_t x_stride, int64_t C, const void *up, int64_t up_adapter, int64_t up_output, int w_dtype,
@@ -365,6 +367,12 @@ int ytm_adapt_gradient(const void *grad, int dtype, int64_t stride, int64_t N, i
                        int64_t hidden_stride, void *d_down, int64_t d_down_adapter, int64_t d_down_rank, void *d_up,
                        int64_t d_up_adapter, int64_t d_up_output, void *workspace, int64_t workspace_bytes,
                        void *stream);
+int ytm_adapt_gradient_as(const void *grad, int dtype, int64_t stride, int64_t N, int64_t K, const void *x, int x_dtype,
+                          int64_t x_stride, int64_t C, const void *up, int64_t up_adapter, int64_t up_output,
+                          int w_dtype, int64_t M, int64_t r, const int32_t *which, float scale, const float *hidden,
+                          int64_t hidden_stride, int d_dtype, void *d_down, int64_t d_down_adapter, int64_t d_down_rank,
+                          void *d_up, int64_t d_up_adapter, int64_t d_up_output, void *workspace,
+                          int64_t workspace_bytes, void *stream);
 
 /* Both losses take N rows (at most 65535) of V scores (8388608), F32, F16 or BF16, the answer tokens[n]
  * of each, and a temperature (NULL: 1; 0 or less counts as 1, less than the smallest normal float or NaN
@@ -411,10 +419,11 @@ int ytm_preference_loss(const void *scores, int dtype, int64_t stride, int64_t N
  * so two steps of one table follow each other.  parameter: F32, F16 or BF16; gradient: of the same type or
  * F32.  With bits 32 first (m) and second (v) are f32.  With bits 8 they are E4M3 floats (sign, four bits
  * of exponent with bias 7, three of fraction, 127 a NaN) times a power of two for each 256 elements in a
- * row (2^-98 or more; of roots 2^-54 or more but for zeros alone), m itself and v as its root.  What is stored in fewer bits than f32 is rounded up or down at random,
- * with the chances that keep the mean of parameters, of m and of v, from `seed`, the step and the
- * element's place (each tensor before it counts as a multiple of 256 long); a v above 0 stays above 0, what is
- * not finite becomes NaN in 8 bits.  The operands of different tensors must not overlap. */
+ * row (2^-98 or more; of roots 2^-54 or more but for zeros alone), m itself and v as its root.  What is stored
+ * in fewer bits than f32 is rounded up or down at random, with the chances that keep the mean of parameters, of
+ * m and of v, from `seed`, the step and the element's place (each tensor before it counts as a multiple of 256
+ * long); a v above 0 stays above 0, what is not finite becomes NaN in 8 bits.  The operands of different tensors
+ * must not overlap. */
 typedef struct {
   void *parameter;
   const void *gradient;

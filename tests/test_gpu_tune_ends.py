@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 ytm_amd = pytest.importorskip("ytm_amd")
 from ytm_amd import tune  # noqa: E402
 
-from test_gpu_tune import TYPES, Case, gpu, host, ints  # noqa: E402
+from test_gpu_tune import TYPES, Case, gpu, host, ints, spread, untouched, within  # noqa: E402
 
 
 # ------------------------------------------------------------------------------- adapters
@@ -64,6 +64,45 @@ def test_torchs_defaults_change_nothing(bits, request):
     request.getfixturevalue("other_defaults")
     for s, t in zip(want, learnt()):
         assert s.dtype == t.dtype and torch.equal(s, t)
+
+
+@pytest.mark.parametrize("w,kind", [("f16", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("N,C,K,r,M", [(1, 500, 40, 4, 1), (40, 777, 129, 16, 9), (300, 333, 65, 40, 4), (700, 130, 90, 8, 300)])
+def test_float32_gradients_of_16_bit_adapters(N, C, K, r, M, w, kind):
+    """Sums that 16 bits hold nothing, or a bit or two, of."""
+    c = Case(N, C, K, r, M, "bits", w, exact=False)
+    rng = np.random.default_rng(2)
+    grad = gpu(rng.normal(0, 1e-8, (N, K)), kind if kind == "bf16" else "f32")
+    hidden = gpu(rng.normal(0, 1, (N, r)))
+    want, size = c.gradients(host(grad), host(hidden))
+    to = tuple(spread(torch.zeros(*t.shape, device="cuda"), 3, 1) for t in (c.down, c.up))
+    got = tune.adapt_gradient(grad, c.x, c.down, c.up, c.which, hidden, c.scale, out=to)
+    assert got[0] is to[0] and got[1] is to[1] and untouched(to[0], 3, 1) and untouched(to[1], 3, 1)
+    within(got[0], want[0], size[0], N + K + 1, "f32")
+    within(got[1], want[1], size[1], N + 1, "f32")
+    narrow = tune.adapt_gradient(grad, c.x, c.down, c.up, c.which, hidden, c.scale)
+    for s, t in zip(got, narrow):
+        assert t.dtype is TYPES[w] and torch.equal(s.to(t.dtype), t)
+
+
+def test_float16_adapters_learn_from_unlikely_answers():
+    """A mean over a batch and many outputs, some of whose sums float16 makes 0.  An answer's probability is
+    exp(3 z) / (5000 exp(9 / 2)), z normal, so the sums of 64 rows' are a few 10^-6 in the median, and a few in a
+    thousand of the 20000 are below 2^-25."""
+    N, C, K, r = 64, 100, 5000, 4
+    rng = np.random.default_rng(0)
+    a = tune.Adapters(1, C, K, rank=r, dtype=torch.float16)
+    scores, x = gpu(rng.normal(0, 3, (N, K))), gpu(rng.normal(0, 1, (N, C)), "f16")
+    which = ints(np.zeros(N))
+    hidden = a.adapt(scores, x, which)
+    tokens = ints(rng.integers(0, 10, N))
+    _, grad, lp = tune.policy_loss(scores, tokens, gpu(np.zeros(N)), gpu(np.ones(N)))
+    _, grad, _ = tune.policy_loss(scores, tokens, lp, gpu(np.ones(N)))
+    a.learn(grad, x, which, hidden, lr=0.01, eps=1e-15, weight_decay=0.0)
+    sums = a.gradients[1][0]
+    assert sums.dtype is torch.float32 and bool((sums.abs() < 2.0**-25).any())
+    # the first step is as long for all, against the gradient
+    assert bool((a.up[0].float() * sums < 0).all()) and float((a.up[0].float().abs() - 0.01).abs().max()) < 2e-5
 
 
 # ---------------------------------------------------------------------------------- AdamW

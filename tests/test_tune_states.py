@@ -8,9 +8,9 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from ytm_amd import tune  # noqa: E402
+from ytm_amd import _lib, tune  # noqa: E402
 
-from test_tune import I32, OnGpu, entries, on_gpu  # noqa: E402, F401
+from test_tune import C_GRADIENT, F16, GRADIENT, I32, OnGpu, entries, on_gpu  # noqa: E402, F401
 
 
 def test_tables_are_made_on_the_host(entries):  # noqa: F811
@@ -76,3 +76,35 @@ def test_steps_before_the_first_are_refused(entries, steps):  # noqa: F811
     with pytest.raises(ValueError, match="0 or more"):
         tune.AdamW([on_gpu(3), on_gpu(4)], [on_gpu(3), on_gpu(4)], steps=steps)
     tune.AdamW([on_gpu(3), on_gpu(4)], [on_gpu(3), on_gpu(4)], steps=torch.tensor([0, 2**40]))
+
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("w,kinds,error", [(F16, (F16, F16), None), (F16, (F32, F32), None), (BF16, (F32, F32), None),
+                                           (F32, (F32, F32), None), (F16, (F32, F16), TypeError),
+                                           (F16, (F16, F32), TypeError), (F16, (BF16, BF16), TypeError),
+                                           (F32, (F16, F16), TypeError)])
+def test_types_of_adapters_gradients(entries, w, kinds, error):  # noqa: F811
+    down, up = (on_gpu(*GRADIENT[t].shape, dtype=w) for t in ("down", "up"))
+    operands = {**GRADIENT, "down": down, "up": up, "out": (on_gpu(*down.shape, dtype=kinds[0]), on_gpu(*up.shape, dtype=kinds[1]))}
+    if error:
+        with pytest.raises(error):
+            tune.adapt_gradient(**operands)
+        assert entries.launched == 0
+    else:
+        assert tune.adapt_gradient(**operands)[0].dtype is kinds[0] and entries.launched == 1
+
+
+@pytest.mark.parametrize("w,d", [(7, 9), (9, 10), (10, 9), (9, 11), (7, 8)])
+def test_types_of_adapters_gradients_at_the_boundary(w, d):
+    operands = {}
+    for name, v in dict(C_GRADIENT, w_dtype=w).items():
+        if name == "d_down":
+            operands["d_dtype"] = d
+        operands[name] = v
+    assert _lib.lib.ytm_adapt_gradient_as(*operands.values()) == _lib.YTM_EINVAL
+    # where the wider gradients reach what a narrower one would not
+    operands |= dict(w_dtype=9, d_dtype=7, d_down=C_GRADIENT["d_up"] - 4 * 200)
+    assert _lib.lib.ytm_adapt_gradient_as(*operands.values()) == _lib.YTM_EINVAL
+    assert b"overlap" in _lib.lib.ytm_last_error()

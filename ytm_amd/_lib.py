@@ -113,6 +113,9 @@ SIGNATURES = {
     "ytm_adapt_gradient": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, ctypes.c_int, _I64, _I64, _P, _I64,
                                           _I64, ctypes.c_int, _I64, _I64, _P, ctypes.c_float, _P, _I64, _P, _I64, _I64,
                                           _P, _I64, _I64, _P, _I64, _P]),
+    "ytm_adapt_gradient_as": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, ctypes.c_int, _I64, _I64, _P, _I64,
+                                             _I64, ctypes.c_int, _I64, _I64, _P, ctypes.c_float, _P, _I64, ctypes.c_int,
+                                             _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P]),
     "ytm_policy_loss_workspace": (ctypes.c_int, [_I64, _I64, ctypes.POINTER(_I64)]),
     "ytm_policy_loss": (ctypes.c_int, [_P, ctypes.c_int, _I64, _I64, _I64, _P, _P, _P, _P, ctypes.c_float,
                                        ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _P, ctypes.c_int, _I64, _P, _I64,

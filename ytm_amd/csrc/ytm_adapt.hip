@@ -77,6 +77,7 @@ struct AdaptArgs {
   uint32_t* order;  // [N], of more than kInline rows; then [begins] where adapters begin
   int begins;       // M + 1 where they are asked for
   int w_dtype;
+  int d_dtype;  // of the gradients: w_dtype, or float32 where that one's range is too small for them
   int odd;  // 16-bit rows that do not all begin at multiples of 4
   int first;  // adapter of a launch of gradients
   RowWindows up_windows, down_windows;
@@ -790,7 +791,7 @@ __device__ __forceinline__ void store_outer(const AdaptArgs& a, int tile, int ke
 #pragma unroll
       for (int t = 0; t < RT; ++t) v[t] = total[t][e];
       if (o < a.K && j < a.r)
-        store_floats<RT>(a.out, key * a.d_up_adapter + o * a.d_up_output + j, a.w_dtype, a.r - j, v);
+        store_floats<RT>(a.out, key * a.d_up_adapter + o * a.d_up_output + j, a.d_dtype, a.r - j, v);
     }
   } else {
     const int column = tile * kColumns + l % kTile * 8;
@@ -798,7 +799,7 @@ __device__ __forceinline__ void store_outer(const AdaptArgs& a, int tile, int ke
     for (int t = 0; t < RT; ++t) {
       const int rank = ranks + (l / kTile * 4 + wave) * RT + t;
       if (rank < a.r && column < a.C)
-        store_floats<8>(a.d_down, key * a.d_down_adapter + rank * a.d_down_rank + column, a.w_dtype, a.C - column,
+        store_floats<8>(a.d_down, key * a.d_down_adapter + rank * a.d_down_rank + column, a.d_dtype, a.C - column,
                         total[t]);
     }
   }
@@ -1438,9 +1439,22 @@ int ytm_adapt_gradient(const void* grad, int dtype, int64_t stride, int64_t N, i
                        int64_t hidden_stride, void* d_down, int64_t d_down_adapter, int64_t d_down_rank, void* d_up,
                        int64_t d_up_adapter, int64_t d_up_output, void* workspace, int64_t workspace_bytes,
                        void* stream) {
+  return ytm_adapt_gradient_as(grad, dtype, stride, N, K, x, x_dtype, x_stride, C, up, up_adapter, up_output, w_dtype, M,
+                               r, which, scale, hidden, hidden_stride, w_dtype, d_down, d_down_adapter, d_down_rank, d_up,
+                               d_up_adapter, d_up_output, workspace, workspace_bytes, stream);
+}
+
+int ytm_adapt_gradient_as(const void* grad, int dtype, int64_t stride, int64_t N, int64_t K, const void* x, int x_dtype,
+                          int64_t x_stride, int64_t C, const void* up, int64_t up_adapter, int64_t up_output,
+                          int w_dtype, int64_t M, int64_t r, const int32_t* which, float scale, const float* hidden,
+                          int64_t hidden_stride, int d_dtype, void* d_down, int64_t d_down_adapter, int64_t d_down_rank,
+                          void* d_up, int64_t d_up_adapter, int64_t d_up_output, void* workspace,
+                          int64_t workspace_bytes, void* stream) {
   if (const char* wrong = ytm::wrong_operands(dtype, stride, N, K, x_dtype, x_stride, C, d_down_adapter, d_down_rank,
                                               up_adapter, up_output, w_dtype, M, r, scale))
     return fail(YTM_EINVAL, std::string("adapt_gradient: ") + wrong);
+  if (d_dtype != w_dtype && d_dtype != YTM_DTYPE_F32)
+    return fail(YTM_EINVAL, "adapt_gradient: gradients are of the adapters' type or float32");
   if (M == 0) return YTM_OK;
   if ((C > 0 && !d_down) || (K > 0 && !d_up) ||
       (N > 0 && (!which || !hidden || (K > 0 && (!grad || !up)) || (C > 0 && !x))))
@@ -1456,9 +1470,9 @@ int ytm_adapt_gradient(const void* grad, int dtype, int64_t stride, int64_t N, i
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
     return fail(YTM_EINVAL, "adapt_gradient: the workspace is too small or not at a multiple of 16 bytes");
   const int64_t width = x_dtype == YTM_DTYPE_BITS ? (C + 31) / 32 : C;
-  const int size = ytm::size_of(w_dtype);
-  const ytm::Rows written[] = {ytm::parts_of(d_down, M, r, C, d_down_adapter, d_down_rank, size),
-                               ytm::parts_of(d_up, M, K, r, d_up_adapter, d_up_output, size),
+  const int size = ytm::size_of(w_dtype), d_size = ytm::size_of(d_dtype);
+  const ytm::Rows written[] = {ytm::parts_of(d_down, M, r, C, d_down_adapter, d_down_rank, d_size),
+                               ytm::parts_of(d_up, M, K, r, d_up_adapter, d_up_output, d_size),
                                ytm::block_of(workspace, need)};
   const ytm::Rows read[] = {ytm::rows_of(grad, N, K, stride, ytm::size_of(dtype)),
                             ytm::rows_of(x, N, width, x_stride, ytm::size_of(x_dtype)),
@@ -1488,7 +1502,7 @@ int ytm_adapt_gradient(const void* grad, int dtype, int64_t stride, int64_t N, i
   a.scores = grad, a.dtype = dtype, a.stride = stride, a.N = (int)N, a.K = (int)K;
   a.x = x, a.x_stride = x_stride, a.C = (int)C;
   a.up = up, a.up_adapter = up_adapter, a.up_output = up_output;
-  a.M = (int)M, a.r = (int)r, a.w_dtype = w_dtype, a.which = which, a.scale = scale;
+  a.M = (int)M, a.r = (int)r, a.w_dtype = w_dtype, a.d_dtype = d_dtype, a.which = which, a.scale = scale;
   a.hidden = const_cast<float*>(hidden), a.hidden_stride = hidden_stride;
   a.out = d_up, a.d_up_adapter = d_up_adapter, a.d_up_output = d_up_output;
   a.d_down = d_down, a.d_down_adapter = d_down_adapter, a.d_down_rank = d_down_rank;

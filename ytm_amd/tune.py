@@ -119,7 +119,8 @@ def adapt_gradient(grad: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: 
     """The gradients (M, r, C) of down and (M, K, r) of up, where grad (N, K) is that of adapt's output and
     hidden what adapt gave; the other operands are adapt's.  Adapters that no row names get 0.  The gradient
     of adapt's scores is grad itself; clause outputs have none.
-    out: where the two go, of the adapters' type (default: new tensors)."""
+    out: where the two go, both of the adapters' type (default: new tensors) or both float32, for sums below what
+    float16 holds."""
     if _forward_ad._current_level >= 0:
         _no_tangents(grad=grad, x=x, up=up, hidden=hidden)
         if out is not None:
@@ -138,15 +139,16 @@ def adapt_gradient(grad: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: 
     if out is None:
         out = torch.empty((M, r, C), dtype=w, device=grad.device), torch.empty((M, K, r), dtype=w, device=grad.device)
     d_down, d_up = out
-    d_down_adapter, d_down_rank = _adapters(d_down, "out[0]", w, (M, r, C), device)
-    d_up_adapter, d_up_output = _adapters(d_up, "out[1]", w, (M, K, r), device)
+    kind = torch.float32 if isinstance(d_down, _Tensor) and d_down.dtype is torch.float32 else w
+    d_down_adapter, d_down_rank = _adapters(d_down, "out[0]", kind, (M, r, C), device)
+    d_up_adapter, d_up_output = _adapters(d_up, "out[1]", kind, (M, K, r), device)
     _changed((d_down, d_up))
     need = _bytes("ytm_adapt_gradient_workspace", N, C, K, M, r)
     workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
-    _call(lib.ytm_adapt_gradient, device, grad.data_ptr(), dtype, grad.stride(0), N, K, x.data_ptr(), x_type,
+    _call(lib.ytm_adapt_gradient_as, device, grad.data_ptr(), dtype, grad.stride(0), N, K, x.data_ptr(), x_type,
           x.stride(0), C, up.data_ptr(), up_adapter, up_output, _FLOATS[w], M, r, which, scale, hidden.data_ptr(),
-          hidden.stride(0), d_down.data_ptr(), d_down_adapter, d_down_rank, d_up.data_ptr(), d_up_adapter, d_up_output,
-          workspace.data_ptr() if need else None, need)
+          hidden.stride(0), _FLOATS[kind], d_down.data_ptr(), d_down_adapter, d_down_rank, d_up.data_ptr(), d_up_adapter,
+          d_up_output, workspace.data_ptr() if need else None, need)
     return d_down, d_up
 
 
@@ -383,7 +385,8 @@ class Adapters:
     """Low-rank adapters of many users beside one model's readout, and what they learn with.
 
     down (count, rank, clauses) starts as small random numbers, up (count, outputs, rank) as 0, so that nothing
-    changes before something is learnt.  gradients: those of the last learn().  optimizer: an AdamW whose tensors
+    changes before something is learnt.  gradients: those of the last learn(), float32 where the adapters are float16,
+    which holds nothing below 6e-8: a mean over a batch and many outputs is often less.  optimizer: an AdamW whose tensors
     are down[a] and up[a] of each adapter a, in turn, with states of `bits` bits.  A copy (copy.deepcopy, pickle,
     torch.save) has adapters, states and step counts of its own."""
 
@@ -400,7 +403,8 @@ class Adapters:
         down = torch.empty(count, rank, clauses, dtype=torch.float32, device=device)
         self.down = down.normal_(0.0, clauses ** -0.5, generator=g).to(dtype)
         self.up = torch.zeros(count, outputs, rank, dtype=dtype, device=device)
-        self.gradients = torch.zeros_like(self.down), torch.zeros_like(self.up)
+        kind = torch.float32 if dtype is torch.float16 else dtype
+        self.gradients = torch.zeros_like(self.down, dtype=kind), torch.zeros_like(self.up, dtype=kind)
         self.optimizer = AdamW(*self._each(), bits=bits, seed=seed)
 
     def _each(self) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
