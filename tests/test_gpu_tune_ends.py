@@ -177,3 +177,36 @@ def test_copies_of_adamw_step_their_own(bits):
     assert torch.equal(a.parameters[0], was) and not torch.equal(b.parameters[0], was)
     a.step(0.1)
     assert torch.equal(a.parameters[0], b.parameters[0]) and a.steps.tolist() == b.steps.tolist() == [2]
+
+
+# ---------------------------------------------------------------------------------- graphs
+def test_learning_of_many_rows_in_a_graph():
+    """More rows than one block sees, replayed with users that change and eager work between the replays."""
+    C, K, N, users = 64, 12, 20000, 40
+    rng = np.random.default_rng(0)
+    x, grad = gpu(rng.normal(0, 1, (N, C))), gpu(rng.normal(0, 1, (N, K)))
+    which = ints(rng.integers(0, 10, N))
+    models = [tune.Adapters(users, C, K, rank=3, seed=4) for _ in range(2)]
+
+    def step(m):
+        hidden = m.adapt(torch.zeros(N, K, device="cuda"), x, which)
+        m.learn(grad, x, which, hidden, lr=0.05)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(models[0])
+    torch.cuda.current_stream().wait_stream(stream)
+    step(models[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(models[0])
+    for k in range(4):
+        which.copy_(ints(rng.integers(10 * k - 3, 10 * k + 10, N)))
+        graph.replay()
+        torch.cuda.synchronize()
+        step(models[1])
+        torch.cuda.synchronize()
+        for s, t in zip((models[0].down, models[0].up, models[0].optimizer.steps),
+                        (models[1].down, models[1].up, models[1].optimizer.steps)):
+            assert torch.equal(s, t), k

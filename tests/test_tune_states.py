@@ -108,3 +108,38 @@ def test_types_of_adapters_gradients_at_the_boundary(w, d):
     operands |= dict(w_dtype=9, d_dtype=7, d_down=C_GRADIENT["d_up"] - 4 * 200)
     assert _lib.lib.ytm_adapt_gradient_as(*operands.values()) == _lib.YTM_EINVAL
     assert b"overlap" in _lib.lib.ytm_last_error()
+
+
+@pytest.mark.parametrize("which", [[], [0], [3, 0, 3, 3], [-1, 4, 2**31 - 1, -(2**31), 1], [-5, 9]])
+def test_adapters_step_those_that_a_batch_names(monkeypatch, which):
+    a, said = object.__new__(tune.Adapters), []
+    a.count, a.scale, a.down, a.up, a.gradients = 4, 1.0, None, None, None
+    a.optimizer = type("Optimizer", (), {"step": lambda self, *args, active: said.append(active)})()
+    monkeypatch.setattr(tune, "adapt_gradient", lambda *args, **kw: None)
+    a.learn(None, None, torch.tensor(which, dtype=I32), None)
+    assert said[0].dtype is torch.bool and said[0].is_contiguous()
+    assert said[0].tolist() == [n in which for n in range(4) for _ in range(2)]
+
+
+def test_adapters_find_those_named_without_a_table_of_rows_and_adapters(monkeypatch):
+    """As many rows and adapters as the entries take: what it needs is counted in either, not in their product."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Sizes(TorchDispatchMode):
+        largest = 0
+
+        def __torch_dispatch__(self, function, types, args=(), kwargs=None):
+            out = function(*args, **(kwargs or {}))
+            for t in out if isinstance(out, (tuple, list)) else (out,):
+                if isinstance(t, torch.Tensor):
+                    Sizes.largest = max(Sizes.largest, t.numel())
+            return out
+
+    a = object.__new__(tune.Adapters)
+    a.count, a.scale, a.down, a.up, a.gradients = 3000, 1.0, None, None, None
+    a.optimizer = type("Optimizer", (), {"step": lambda self, *args, active: None})()
+    monkeypatch.setattr(tune, "adapt_gradient", lambda *args, **kw: None)
+    which = torch.arange(5000, dtype=I32)
+    with Sizes():
+        a.learn(None, None, which, None)
+    assert Sizes.largest <= 2 * (3000 + 2) + 5000

@@ -435,5 +435,7 @@ class Adapters:
               weight_decay: float = 0.01) -> None:
         """A step of the adapters that `which` names, by the gradient (N, K) of the scores that adapt() made."""
         adapt_gradient(grad, x, self.down, self.up, which, hidden, self.scale, out=self.gradients)
-        named = (which[:, None] == torch.arange(self.count, dtype=torch.int32, device=which.device)).any(0)
-        self.optimizer.step(lr, betas, eps, weight_decay, active=named.repeat_interleave(2))
+        # a row's adapter at 1 .. count, rows without one at the ends
+        at = which.long().add_(1).clamp_(0, self.count + 1)
+        named = torch.zeros(self.count + 2, 2, dtype=torch.bool, device=which.device).index_fill_(0, at, True)
+        self.optimizer.step(lr, betas, eps, weight_decay, active=named[1:-1].view(-1))
