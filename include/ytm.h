@@ -376,7 +376,7 @@ int ytm_adapt_gradient_as(const void *grad, int dtype, int64_t stride, int64_t N
 
 /* Both losses take N rows (at most 65535) of V scores (8388608), F32, F16 or BF16, the answer tokens[n]
  * of each, and a temperature (NULL: 1; 0 or less counts as 1, less than the smallest normal float or NaN
- * as that).  A score that is NaN counts as -inf, one of +inf as the largest float.  With p = softmax(score
+ * as that, an infinite one as the largest float).  A score that is NaN counts as -inf, one of +inf as the largest float.  With p = softmax(score
  * / temperature) and lp = log p[tokens[n]], grad (F32, F16 or BF16; scores itself too, with elements of the
  * same size and rows of the same distance) becomes the gradient of the losses' sum by the scores.  A
  * row whose answer is outside 0..V-1 or has a score of -inf is left out: its lp and loss are 0, and so is

@@ -105,6 +105,34 @@ def test_float16_adapters_learn_from_unlikely_answers():
     assert bool((a.up[0].float() * sums < 0).all()) and float((a.up[0].float().abs() - 0.01).abs().max()) < 2e-5
 
 
+# --------------------------------------------------------------------------------- losses
+def both_losses(scores, tokens, **kw):
+    """(losses, gradient, log probabilities) of the policy's loss, gradient and log probabilities of a preference's."""
+    N = scores.shape[0]
+    policy = tune.policy_loss(scores, ints(tokens), gpu(np.zeros(N)), gpu(np.ones(N)), weights=gpu(np.ones(N)), **kw)
+    starts, reference = ints([0, *[1] * (N > 1), N, *[N] * (N < 2)]), gpu([0.0, 0.0])
+    return policy + tune.preference_loss(scores, ints(tokens), starts, reference, **kw)[1:]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("N,V", [(2, 40), (2, 5000), (300, 4100), (2, 70000)])
+def test_an_infinite_temperature_leaves_masks_in_place(N, V, kind):
+    """All answers that are not masked are alike; a probability is 1 / V to the rounding of a sum of V ones."""
+    s = np.random.default_rng(0).normal(0, 3, (N, V))
+    s[:, ::3] = -np.inf
+    s[1, :3] = np.nan, 2.0, 6e4
+    scores, tokens = gpu(s, kind), np.full(N, 2)
+    heat = np.full(N, np.inf)
+    losses, grad, lp, pair_grad, said = both_losses(scores, tokens, temperature=gpu(heat))
+    count = np.isfinite(s).sum(1)
+    # 16 units: of a sum of ones in chains of at most V / 64 + 64 that are exact below 2^24, of its logarithm, two
+    # powers and three products
+    assert (np.abs(host(lp) + np.log(count)) <= 2.0**-20 * np.log(count)).all()
+    assert bool(torch.isfinite(grad).all()) and bool(torch.isfinite(pair_grad).all()) and bool(torch.isfinite(said).all())
+    assert not bool(grad[:, ::3].any()) and not bool(pair_grad[:, ::3].any())
+    assert float(grad[0].abs().max()) < 1e-38  # nothing that is divided by an infinite temperature is left
+
+
 # ---------------------------------------------------------------------------------- AdamW
 @pytest.mark.parametrize("size", [1e-10, 1e-14, 1e-17, 1e-18])
 def test_second_states_above_zero_stay_above_it(size):

@@ -66,11 +66,12 @@ __device__ __forceinline__ float score_of(In v) {
 // 2^x, to one unit in its last place; what is less than the smallest normal float is 0.
 __device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 1 / temperature as choose() takes it: 0 or less counts as 1, less than the smallest normal float or NaN as that.
+// 1 / temperature as choose() takes it: 0 or less counts as 1, less than the smallest normal float or NaN as that, and an
+// infinite one as the largest float, beside which a score of -inf stays -inf.
 __device__ __forceinline__ float cooling(const LossArgs& a, int n) {
   if (!a.temperature) return 1.0f;
   const float t = a.temperature[n];
-  return t <= 0.0f ? 1.0f : 1.0f / (t >= FLT_MIN ? t : FLT_MIN);
+  return t <= 0.0f ? 1.0f : 1.0f / (t >= FLT_MIN ? fminf(t, FLT_MAX) : FLT_MIN);
 }
 
 // Of some of a row's scores: one of them, or near them, and their sum of exp((score - it) / temperature), in powers of
