@@ -133,6 +133,30 @@ def test_an_infinite_temperature_leaves_masks_in_place(N, V, kind):
     assert float(grad[0].abs().max()) < 1e-38  # nothing that is divided by an infinite temperature is left
 
 
+@pytest.mark.parametrize("N,V", [(8, 40), (8, 5000), (8, 70000)])
+def test_rows_of_weight_0_are_left_out(N, V):
+    """Rows that fill a batch, with numbers whose ratio or distance is infinite or NaN."""
+    rng = np.random.default_rng(0)
+    scores, tokens = gpu(rng.normal(0, 3, (N, V))), rng.integers(0, V, N)
+    old, adv, reference, weights = np.full(N, -4.0), np.ones(N), np.full(N, -5.0), np.full(N, 0.25)
+    old[1], old[2], adv[3], reference[4], reference[5] = -1e4, np.nan, np.nan, 1e4, np.inf
+    old[6], adv[6] = -np.inf, -1.0
+    weights[1:7] = 0.0
+    weights[6] = -0.0
+    losses, grad, lp = tune.policy_loss(scores, ints(tokens), gpu(old), gpu(adv), reference=gpu(reference), kl=0.1,
+                                        weights=gpu(weights))
+    assert not bool(losses[1:7].any()) and not bool(grad[1:7].any())
+    assert bool((lp < 0).all()) and bool(torch.isfinite(grad).all())
+    # the others, as if they were alone
+    ends = [0, 7]
+    want = tune.policy_loss(scores[::7], ints(tokens[ends]), gpu(old[ends]), gpu(adv[ends]),
+                            reference=gpu(reference[ends]), kl=0.1, weights=gpu(weights[ends]))
+    for s, t in zip((losses, grad, lp), want):
+        # rows longer than a slice are cut otherwise, and joined: sums of exponentials to 2^-20, the log's to 2^-22
+        assert float((s[::7] - t).abs().max()) <= 2.0**-18 * (1 if V >= 32768 else 0)
+        assert float(t.abs().max()) > 1e-5
+
+
 # ---------------------------------------------------------------------------------- AdamW
 @pytest.mark.parametrize("size", [1e-10, 1e-14, 1e-17, 1e-18])
 def test_second_states_above_zero_stay_above_it(size):

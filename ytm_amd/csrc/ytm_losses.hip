@@ -268,13 +268,13 @@ __device__ __forceinline__ Answer answer_of(const LossArgs& a, int n) {
   return answer_of(a, n, t >= 0 && t < a.V ? a.at[n] : -INFINITY, all);
 }
 
-// The policy loss of a row and its derivative by lp.
+// The policy loss of a row and its derivative by lp; 0 where its weight is, whatever fills such a row.
 struct Loss {
   float value, slope;
 };
 __device__ __forceinline__ Loss policy(const LossArgs& a, int n, const Answer& r) {
-  if (!r.there) return Loss{0.0f, 0.0f};
   const float w = a.weights ? a.weights[n] : 1.0f / (float)a.N, adv = a.advantages[n];
+  if (!r.there || w == 0.0f) return Loss{0.0f, 0.0f};
   const float ratio = expf(r.lp - a.old[n]);
   const float free = ratio * adv, held = fminf(fmaxf(ratio, a.low), a.high) * adv;
   float value = -fminf(free, held), slope = free <= held ? -free : 0.0f;

@@ -164,8 +164,9 @@ def policy_loss(scores: torch.Tensor, tokens: torch.Tensor, old: torch.Tensor, a
     out.  old: float32 (N,), their log probabilities when they were drawn, as choose gives them (without
     filters).  advantages: float32 (N,), what they were worth.  The ratio of the probabilities counts up
     to 1 + clip_high (default: clip) and down to 1 - clip.  reference: float32 (N,), their log probabilities by
-    the model that kl draws the answers towards.  weights: float32 (N,), each row's (default 1 / N).
-    temperature: float32 (N,), as for choose.
+    the model that kl draws the answers towards.  weights: float32 (N,), each row's (default 1 / N; a row of 0,
+    such as one that fills a batch, has a loss and gradient of 0 whatever its other numbers).  temperature:
+    float32 (N,), as for choose.
     out: where the gradient goes, any of the three types, `scores` itself too (default: a new float32 tensor)."""
     if _forward_ad._current_level >= 0:
         _no_tangents(scores=scores, old=old, advantages=advantages, reference=reference, weights=weights,
