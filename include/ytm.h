@@ -386,7 +386,8 @@ int ytm_adapt_gradient_as(const void *grad, int dtype, int64_t stride, int64_t N
  *   losses[n] = weights[n] * (kl * (exp(d) - d - 1)
  *               - min(ratio * advantages[n], clamp(ratio, 1 - low, 1 + high) * advantages[n]))
  * (where the two are equal, the first counts); weights NULL: 1 / N; 0: the row has a loss and gradient of 0,
- * whatever its other numbers; reference NULL: kl must be 0.
+ * whatever its other numbers; reference NULL: kl must be 0.  Of other rows a number that is NaN makes loss and
+ * gradient NaN.
  * logprobs[n] = lp.
  *
  * ytm_preference_loss: rows starts[s] .. starts[s + 1] - 1 are sequence s of 2 pairs (at most 65535),

@@ -157,6 +157,26 @@ def test_rows_of_weight_0_are_left_out(N, V):
         assert float(t.abs().max()) > 1e-5
 
 
+@pytest.mark.parametrize("V", [40, 5000, 70000])
+def test_numbers_that_are_nan_are_not_hidden(V):
+    """And stay in their rows; a ratio past float32 of an advantage of 0 is none."""
+    N = 6
+    rng = np.random.default_rng(0)
+    scores, tokens = gpu(rng.normal(0, 3, (N, V))), rng.integers(0, V, N)
+    old, adv, reference = np.full(N, -4.0), np.ones(N), np.full(N, -5.0)
+    old[1], adv[2], reference[3] = np.nan, np.nan, np.nan
+    old[4], adv[4] = -1e4, 0.0
+    for kl in (0.0, 0.1):
+        losses, grad, lp = tune.policy_loss(scores, ints(tokens), gpu(old), gpu(adv), reference=gpu(reference), kl=kl)
+        bad = [1, 2] + [3] * (kl > 0)
+        good = [n for n in range(N) if n not in bad]
+        assert bool(torch.isnan(losses[bad]).all()) and bool(torch.isnan(grad[bad]).all())
+        assert bool(torch.isfinite(losses[good]).all()) and bool(torch.isfinite(grad[good]).all())
+        assert bool(torch.isfinite(lp).all())
+        if not kl:
+            assert float(losses[4]) == 0.0 and not bool(grad[4].any())
+
+
 # ---------------------------------------------------------------------------------- AdamW
 @pytest.mark.parametrize("size", [1e-10, 1e-14, 1e-17, 1e-18])
 def test_second_states_above_zero_stay_above_it(size):

@@ -276,8 +276,11 @@ __device__ __forceinline__ Loss policy(const LossArgs& a, int n, const Answer& r
   const float w = a.weights ? a.weights[n] : 1.0f / (float)a.N, adv = a.advantages[n];
   if (!r.there || w == 0.0f) return Loss{0.0f, 0.0f};
   const float ratio = expf(r.lp - a.old[n]);
-  const float free = ratio * adv, held = fminf(fmaxf(ratio, a.low), a.high) * adv;
-  float value = -fminf(free, held), slope = free <= held ? -free : 0.0f;
+  // an advantage of 0 makes nothing of a ratio past float32; what is NaN makes the comparison false and goes on
+  const float free = adv == 0.0f && ratio == INFINITY ? 0.0f : ratio * adv;
+  const float held = fminf(fmaxf(ratio, a.low), a.high) * adv;
+  const bool outside = free > held;
+  float value = outside ? -held : -free, slope = outside ? 0.0f : -free;
   if (a.kl != 0.0f) {
     const float far = a.reference[n] - r.lp, up = expm1f(far);
     value += a.kl * (up - far);
