@@ -395,7 +395,7 @@ int ytm_adapt_gradient_as(const void *grad, int dtype, int64_t stride, int64_t N
  * results are unspecified).  With l[s] the sum of its rows' lp, of pair p
  *   m = beta * ((l[2p] - reference[2p]) - (l[2p+1] - reference[2p+1]))
  *   losses[p] = ((1 - smoothing) * log(1 + exp(-m)) + smoothing * log(1 + exp(m))) / pairs
- * logprobs[s] = l[s].  Rows of no sequence are left out.
+ * where 0 times an infinity is 0 (a reference of -inf).  logprobs[s] = l[s].  Rows of no sequence are left out.
  *
  * workspace: device memory of the _workspace's bytes at a multiple of 16 bytes, for the time of the
  * call's work (NULL where that is 0). */

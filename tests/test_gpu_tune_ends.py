@@ -177,6 +177,23 @@ def test_numbers_that_are_nan_are_not_hidden(V):
             assert float(losses[4]) == 0.0 and not bool(grad[4].any())
 
 
+@pytest.mark.parametrize("pairs,V", [(3, 40), (200, 300), (3, 40000)])
+def test_references_that_a_mask_made_infinite(pairs, V):
+    """A sequence that the reference cannot say: preferred, its pair is won and its loss 0; the other way it is lost."""
+    N = 2 * pairs
+    scores, tokens = gpu(np.random.default_rng(0).normal(0, 3, (N, V))), ints(np.arange(N) % V)
+    reference = np.full(N, -5.0)
+    reference[0] = reference[3] = -np.inf
+    starts = ints(np.arange(N + 1))
+    for smoothing, won, lost in ((0.0, 0.0, np.inf), (1.0, np.inf, 0.0), (0.5, np.inf, np.inf)):
+        losses, grad, _ = tune.preference_loss(scores, tokens, starts, gpu(reference), smoothing=smoothing)
+        assert float(losses[0]) == won and float(losses[1]) == lost
+        assert bool(torch.isfinite(losses[2:]).all()) and bool(torch.isfinite(grad).all())
+        # a loss that is as small as it gets has no slope
+        assert not bool(grad[:2].any()) if won == 0.0 else bool(grad[:2].any())
+        assert not bool(grad[2:4].any()) if lost == 0.0 else bool(grad[2:4].any())
+
+
 # ---------------------------------------------------------------------------------- AdamW
 @pytest.mark.parametrize("size", [1e-10, 1e-14, 1e-17, 1e-18])
 def test_second_states_above_zero_stay_above_it(size):

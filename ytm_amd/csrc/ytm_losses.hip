@@ -400,7 +400,10 @@ struct Pair {
     const float share = 1.0f / (float)a.pairs, log1 = log1pf(small);
     const float won = (m >= 0.0f ? 1.0f : small) / (1.0f + small), lost = (m >= 0.0f ? small : 1.0f) / (1.0f + small);
     slope = share * a.beta * (a.smoothing * won - (1.0f - a.smoothing) * lost);
-    loss = share * ((1.0f - a.smoothing) * (fmaxf(-m, 0.0f) + log1) + a.smoothing * (fmaxf(m, 0.0f) + log1));
+    // what has no part may be infinite
+    const float right = a.smoothing == 1.0f ? 0.0f : (1.0f - a.smoothing) * (fmaxf(-m, 0.0f) + log1);
+    const float wrong = a.smoothing == 0.0f ? 0.0f : a.smoothing * (fmaxf(m, 0.0f) + log1);
+    loss = share * (right + wrong);
   }
   __device__ __forceinline__ void write(const LossArgs& a, int pair) const {
     if (threadIdx.x != 0) return;
