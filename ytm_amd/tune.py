@@ -436,7 +436,7 @@ class Adapters:
               weight_decay: float = 0.01) -> None:
         """A step of the adapters that `which` names, by the gradient (N, K) of the scores that adapt() made."""
         adapt_gradient(grad, x, self.down, self.up, which, hidden, self.scale, out=self.gradients)
-        # a row's adapter at 1 .. count, rows without one at the ends
-        at = which.long().add_(1).clamp_(0, self.count + 1)
-        named = torch.zeros(self.count + 2, 2, dtype=torch.bool, device=which.device).index_fill_(0, at, True)
-        self.optimizer.step(lr, betas, eps, weight_decay, active=named[1:-1].view(-1))
+        # rows without an adapter, -1 and count, mark what is after the last
+        named = torch.zeros(self.count + 1, 2, dtype=torch.bool, device=which.device)
+        named.index_fill_(0, which.clamp(-1, self.count).long(), True)
+        self.optimizer.step(lr, betas, eps, weight_decay, active=named.view(-1)[:-2])
