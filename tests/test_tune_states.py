@@ -143,3 +143,15 @@ def test_adapters_find_those_named_without_a_table_of_rows_and_adapters(monkeypa
     with Sizes():
         a.learn(None, None, which, None)
     assert Sizes.largest <= 2 * (3000 + 2) + 5000
+
+
+def test_a_step_takes_the_tensors_of_its_table(monkeypatch):
+    """Also where somebody has put more into the lists, of which it has no rows."""
+    calls = []
+    monkeypatch.setattr(tune, "_call", lambda function, device, *args: calls.append(args))
+    a = tune.AdamW([on_gpu(3), on_gpu(4)], [on_gpu(3), on_gpu(4)])
+    a.parameters.append(on_gpu(5))
+    a.step()
+    assert calls[0][1] == 2
+    with pytest.raises(ValueError, match="active"):
+        a.step(active=on_gpu(3, dtype=torch.bool))

@@ -337,7 +337,7 @@ class AdamW:
             row.parameter_dtype, row.gradient_dtype = _FLOATS[p.dtype], _FLOATS[g.dtype]
             for name in self._names:
                 setattr(row, name, getattr(self, name)[i].data_ptr())
-        size, self._chunks = ctypes.c_int64(), ctypes.c_int64()
+        size, self._chunks, self._count = ctypes.c_int64(), ctypes.c_int64(), n
         check(lib.ytm_adamw_table(rows, n, self.bits, None, size, self._chunks))
         host = torch.empty(size.value, dtype=torch.uint8, device="cpu")  # whatever torch's default is
         check(lib.ytm_adamw_table(rows, n, self.bits, host.data_ptr(), size, self._chunks))
@@ -369,7 +369,7 @@ class AdamW:
 
         lr: a number, or a float32 tensor () on the GPU, which a captured graph reads again at each replay.
         active: bool, one for each tensor, on the GPU; the tensors for which it is false stay as they are."""
-        n, rate_at, flags = len(self.parameters), None, None
+        n, rate_at, flags = self._count, None, None  # as many as the table has
         if isinstance(lr, _Tensor):
             if lr.dtype is not torch.float32 or lr.numel() != 1 or lr.get_device() != self._device:
                 raise ValueError(f"lr must be a number or one float32 on cuda:{self._device}.")
