@@ -65,7 +65,7 @@ def test_copies_have_addresses_of_their_own(copied, bits):
         there, words = addresses(one)
         assert all(there)
         assert not any(t.data_ptr() in words for t in (*other.parameters, *other.gradients, *other.first, *other.second))
-    b.steps += 1
+    b.steps.add_(1)
     assert a.steps.tolist() == [5, 5]
     c = copy.copy(a)
     assert all(addresses(c)[0]) and c.parameters[0] is a.parameters[0] and c.steps is a.steps
@@ -155,3 +155,16 @@ def test_a_step_takes_the_tensors_of_its_table(monkeypatch):
     assert calls[0][1] == 2
     with pytest.raises(ValueError, match="active"):
         a.step(active=on_gpu(3, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("steps,error", [(torch.zeros(2, dtype=torch.int64), ValueError), (on_gpu(2, dtype=I32), TypeError),
+                                         (on_gpu(3, dtype=torch.int64), ValueError), (3, TypeError), (None, TypeError),
+                                         (on_gpu(4, dtype=torch.int64)[::2], ValueError)])
+def test_steps_that_a_step_cannot_count_are_refused(entries, steps, error):  # noqa: F811
+    a = tune.AdamW([on_gpu(3), on_gpu(4)], [on_gpu(3), on_gpu(4)])
+    was = a.steps
+    with pytest.raises(error, match="steps"):
+        a.steps = steps
+    assert a.steps is was
+    a.steps = good = on_gpu(2, dtype=torch.int64)
+    assert a.steps is good

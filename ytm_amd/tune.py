@@ -288,11 +288,11 @@ class AdamW:
                 raise ValueError(f"steps must be whole numbers of shape ({len(self.parameters)},).")
             if bool((steps < 0).any()):
                 raise ValueError("steps must be 0 or more.")
-            self.steps = steps.detach().to(device=first.device, dtype=torch.int64, copy=True).contiguous()
+            self._steps = steps.detach().to(device=first.device, dtype=torch.int64, copy=True).contiguous()
         else:
             if steps < 0:
                 raise ValueError("steps must be 0 or more.")
-            self.steps = torch.full((len(self.parameters),), int(steps), dtype=torch.int64, device=first.device)
+            self._steps = torch.full((len(self.parameters),), int(steps), dtype=torch.int64, device=first.device)
         self._names = names
         self._written = tuple(t for name in ("parameters", *names) for t in getattr(self, name))
         self._apart()
@@ -357,7 +357,17 @@ class AdamW:
         if self.bits == 8:
             self.first, self.second = ([t.view(torch.float8_e4m3fn) for t in s] for s in (self.first, self.second))
         AdamW.__init__(self, self.parameters, self.gradients, self.bits, self.states(), self.steps, self.seed)
-        self.steps = state["steps"]
+        self._steps = state["_steps"]
+
+    @property
+    def steps(self) -> torch.Tensor:
+        return self._steps
+
+    @steps.setter
+    def steps(self, steps: torch.Tensor) -> None:
+        if _per_row(steps, "steps", torch.int64, self._count, self._device) is None:
+            raise TypeError("steps must be a torch tensor.")
+        self._steps = steps
 
     def states(self) -> dict[str, list[torch.Tensor]]:
         """The states, to go on with: AdamW(..., states=a.states(), steps=a.steps)."""
@@ -378,7 +388,7 @@ class AdamW:
             flags = _per_row(active, "active", torch.bool, n, self._device)
         _changed(self._written)
         _call(lib.ytm_adamw, self._device, self._table.data_ptr(), n, self._chunks.value, self.bits,
-              self.steps.data_ptr(), flags, _number(lr, "lr"), rate_at, float(betas[0]), float(betas[1]), _number(eps, "eps"),
+              self._steps.data_ptr(), flags, _number(lr, "lr"), rate_at, float(betas[0]), float(betas[1]), _number(eps, "eps"),
               _number(weight_decay, "weight_decay"), self.seed)
 
 
