@@ -110,12 +110,21 @@ def test_types_of_adapters_gradients_at_the_boundary(w, d):
     assert b"overlap" in _lib.lib.ytm_last_error()
 
 
+def adapters(monkeypatch, count):
+    """Adapters whose optimiser only notes which of its tensors it should step, and these notes."""
+    a, said = object.__new__(tune.Adapters), []
+    a.count, a.scale, a.down, a.up = count, 1.0, on_gpu(count, 2, 3), on_gpu(count, 5, 2)
+    a.gradients = on_gpu(count, 2, 3), on_gpu(count, 5, 2)
+    parameters, gradients = a._each()
+    a.optimizer = type("Optimizer", (), {"step": lambda self, *args, active: said.append(active)})()
+    a.optimizer.parameters, a.optimizer.gradients = parameters, gradients
+    monkeypatch.setattr(tune, "adapt_gradient", lambda *args, **kw: None)
+    return a, said
+
+
 @pytest.mark.parametrize("which", [[], [0], [3, 0, 3, 3], [-1, 4, 2**31 - 1, -(2**31), 1], [-5, 9]])
 def test_adapters_step_those_that_a_batch_names(monkeypatch, which):
-    a, said = object.__new__(tune.Adapters), []
-    a.count, a.scale, a.down, a.up, a.gradients = 4, 1.0, None, None, None
-    a.optimizer = type("Optimizer", (), {"step": lambda self, *args, active: said.append(active)})()
-    monkeypatch.setattr(tune, "adapt_gradient", lambda *args, **kw: None)
+    a, said = adapters(monkeypatch, 4)
     a.learn(None, None, torch.tensor(which, dtype=I32), None)
     assert said[0].dtype is torch.bool and said[0].is_contiguous()
     assert said[0].tolist() == [n in which for n in range(4) for _ in range(2)]
@@ -135,10 +144,7 @@ def test_adapters_find_those_named_without_a_table_of_rows_and_adapters(monkeypa
                     Sizes.largest = max(Sizes.largest, t.numel())
             return out
 
-    a = object.__new__(tune.Adapters)
-    a.count, a.scale, a.down, a.up, a.gradients = 3000, 1.0, None, None, None
-    a.optimizer = type("Optimizer", (), {"step": lambda self, *args, active: None})()
-    monkeypatch.setattr(tune, "adapt_gradient", lambda *args, **kw: None)
+    a, _ = adapters(monkeypatch, 3000)
     which = torch.arange(5000, dtype=I32)
     with Sizes():
         a.learn(None, None, which, None)
@@ -168,3 +174,18 @@ def test_steps_that_a_step_cannot_count_are_refused(entries, steps, error):  # n
     assert a.steps is was
     a.steps = good = on_gpu(2, dtype=torch.int64)
     assert a.steps is good
+
+
+@pytest.mark.parametrize("name", ["down", "up", "gradients"])
+def test_adapters_refuse_tensors_that_their_optimiser_does_not_step(monkeypatch, name):
+    a, said = adapters(monkeypatch, 3)
+    which = torch.zeros(2, dtype=I32)
+    a.learn(None, None, which, None)
+    held = getattr(a, name)
+    setattr(a, name, tuple(t.clone() for t in held) if isinstance(held, tuple) else held.clone())
+    with pytest.raises(ValueError, match="copy into"):
+        a.learn(None, None, which, None)
+    assert len(said) == 1
+    a.optimizer.parameters, a.optimizer.gradients = a._each()  # one that does
+    a.learn(None, None, which, None)
+    assert len(said) == 2

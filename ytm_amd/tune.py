@@ -399,7 +399,8 @@ class Adapters:
     changes before something is learnt.  gradients: those of the last learn(), float32 where the adapters are float16,
     which holds nothing below 6e-8: a mean over a batch and many outputs is often less.  optimizer: an AdamW whose tensors
     are down[a] and up[a] of each adapter a, in turn, with states of `bits` bits.  A copy (copy.deepcopy, pickle,
-    torch.save) has adapters, states and step counts of its own."""
+    torch.save) has adapters, states and step counts of its own.  down, up and gradients stay where they are: what
+    is to be in them is copied into them."""
 
     def __init__(self, count: int, clauses: int, outputs: int, rank: int = 16, scale: float = 1.0,
                  dtype: torch.dtype = torch.float32, bits: int = 32, device: str | torch.device = "cuda", seed: int = 0):
@@ -445,8 +446,12 @@ class Adapters:
               lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
               weight_decay: float = 0.01) -> None:
         """A step of the adapters that `which` names, by the gradient (N, K) of the scores that adapt() made."""
+        o = self.optimizer
+        if [t.data_ptr() for t in (self.down, self.up, *self.gradients)] != [
+                t.data_ptr() for t in (*o.parameters[:2], *o.gradients[:2])]:
+            raise ValueError("down, up and gradients must be the tensors that the optimizer steps; copy into them.")
         adapt_gradient(grad, x, self.down, self.up, which, hidden, self.scale, out=self.gradients)
         # rows without an adapter, -1 and count, mark what is after the last
         named = torch.zeros(self.count + 1, 2, dtype=torch.bool, device=which.device)
         named.index_fill_(0, which.clamp(-1, self.count).long(), True)
-        self.optimizer.step(lr, betas, eps, weight_decay, active=named.view(-1)[:-2])
+        o.step(lr, betas, eps, weight_decay, active=named.view(-1)[:-2])
