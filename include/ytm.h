@@ -424,8 +424,9 @@ int ytm_preference_loss(const void *scores, int dtype, int64_t stride, int64_t N
  * row (2^-98 or more; of roots 2^-54 or more but for zeros alone), m itself and v as its root.  What is stored
  * in fewer bits than f32 is rounded up or down at random, with the chances that keep the mean of parameters, of
  * m and of v, from `seed`, the step and the element's place (each tensor before it counts as a multiple of 256
- * long); a v above 0 stays above 0, what is not finite becomes NaN in 8 bits.  The operands of different tensors
- * must not overlap. */
+ * long); a v above 0 stays above 0, what is not finite becomes NaN in 8 bits.  Operations are f32,
+ * each rounded (of the rate and of k in f64, rounded once), but with bits 8 the quotient, which is within two
+ * units in its last place.  The operands of different tensors must not overlap. */
 typedef struct {
   void *parameter;
   const void *gradient;

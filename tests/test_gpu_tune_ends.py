@@ -223,6 +223,20 @@ def test_blocks_of_zeros_keep_their_scale():
     assert float(a.second_scales[0][1]) > 2.0**-54 and not bool(a.second[0][:256].float().any())
 
 
+def test_float32_steps_are_rounded_as_they_are_written():
+    """The first step of parameters that are 0, in numpy's float32."""
+    F, n = np.float32, 100003
+    rng = np.random.default_rng(0)
+    g = (rng.normal(0, 1, n) * np.exp(rng.normal(0, 5, n))).astype(F)
+    p, slopes = gpu(np.zeros(n)), gpu(g)
+    a = tune.AdamW([p], [slopes])
+    a.step(lr=0.01, betas=(0.9, 0.99), eps=1e-6, weight_decay=0.1)
+    m, v = F(1 - 0.9) * g, F(1 - 0.99) * (g * g)
+    by = np.sqrt(v) * F(1 / np.sqrt(1 - 0.99)) + F(1e-6)
+    want = F(0) * F(1 - 0.01 * 0.1) - F(0.01 / (1 - 0.9)) * m / by
+    np.testing.assert_array_equal(p.cpu().numpy(), want)
+
+
 # --------------------------------------------------------------------------------- copies
 def saved(a):
     f = io.BytesIO()

@@ -241,7 +241,8 @@ class AdamW:
     float32 powers of two for each 256 elements in a row, and second is held as its root.  steps: int64, the
     steps that each tensor has made.
 
-    Sums and states are float32 while a step is made.  What is stored in fewer bits, 16-bit parameters too, is
+    Sums and states are float32 while a step is made (with bits=8 m / (sqrt(v) + eps) to two units in its last
+    place).  What is stored in fewer bits, 16-bit parameters too, is
     rounded up or down at random with the chances that keep its mean, the same ones for the same `seed`: an
     average that moves by a thousandth a step would never leave an 8-bit number's neighbourhood otherwise.
 
