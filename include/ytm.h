@@ -358,8 +358,8 @@ int ytm_adapt(const void *scores, int dtype, int64_t stride, int64_t N, int64_t 
  * 0 for adapters that no row names.  (The gradient by scores is grad itself.)  Sums with a value that is not
  * finite are infinite or NaN.  d_down (M, r, C) and d_up (M, K, r) are of w_dtype; grad F32, F16 or BF16.
  * Bounds and workspace as for ytm_adapt.
- * ytm_adapt_gradient_as: the same with d_down and d_up of d_dtype, which is w_dtype or F32: the sums of a batch
- * are often less than the 2^-24 that float16 holds. */
+ * ytm_adapt_gradient_as: the same with d_down and d_up of d_dtype, which is w_dtype or F32: means over a batch
+ * of unlikely answers are less than the 2^-24 that float16 holds. */
 int ytm_adapt_gradient_workspace(int64_t N, int64_t C, int64_t K, int64_t M, int64_t r, int64_t *bytes);
 int ytm_adapt_gradient(const void *grad, int dtype, int64_t stride, int64_t N, int64_t K, const void *x, int x_dtype,
                        int64_t x_stride, int64_t C, const void *up, int64_t up_adapter, int64_t up_output, int w_dtype,

@@ -9,8 +9,8 @@
 // down at random with the chances that keep its mean: a step of 1 - beta2 of the state is less than
 // half the distance of two codes, so that the nearest one would stay for ever.
 //
-// Bound by memory: 61 M bfloat16 parameters with f32 states (1.35 GB) 271 us, 5.0 TB/s.  With states in 8 bits the
-// coding takes 72% of the vector units' time: 20.6 M f32 parameters (330 MB) 75 us, 4.4 TB/s; in f32 125.
+// Bound by memory: 62.1 M bfloat16 parameters with f32 states (1.37 GB) 269 us, 5.1 TB/s.  With states in 8 bits the
+// coding takes 72% of the vector units' time: 21.1 M f32 parameters (339 MB) 75 us, 4.5 TB/s; in f32 (592 MB) 120.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -12,7 +12,8 @@
 // several blocks share are joined in a fixed order by a kernel that comes after.
 //
 // What bounds them is latency: a block's chain of waits (the order, the rows that it names, their values, the
-// parts' sums) takes 3 us at least, and memory is read and written at 1.6 to 3 TB/s.  Hence few launches, loads asked for before what they wait beside, and as many blocks a CU as the registers hold.
+// parts' sums) takes 3 us at least, and memory is read and written at 1.6 to 3 TB/s.  Hence few launches, loads
+// asked for before what they wait beside, and as many blocks a CU as the registers hold.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -253,8 +254,8 @@ struct Order {
 
 // The segments of a window that block `slot` of `slots` takes: body(key, first place, end).  A place begins one
 // where its key is not that of the place before.  Blocks of the same slot have numbers in a row: those of later
-// slots often find nothing, and by turns they would leave every other XCD without work (4096 rows of one
-// adapter, 20000 clauses, 10000 outputs, rank 32: 312 us, 196 in a row).
+// slots often find nothing, and by turns they would leave every other XCD without work (adapt of 512 rows of
+// one adapter, 20000 clauses, 10000 outputs, rank 32: 39.9 us, 33.1 in a row).
 template <typename Body>
 __device__ __forceinline__ void segments(const uint32_t* code, int slot, int slots, Body body) {
   const int i = threadIdx.x % kTile;
@@ -480,8 +481,9 @@ __global__ __launch_bounds__(kThreads) void up_kernel(AdaptArgs a) {
   __shared__ __attribute__((aligned(16))) float hidden[kTile][RANKS + 4];
   __shared__ __attribute__((aligned(16))) float group_sums[kGroups > 1 ? kGroups : 1][kGroups > 1 ? kTile : 1][RANKS + 4];
   // Few rows: blocks of the same outputs on the same XCD, which then reads their weights once (48 rows of
-  // some 30 adapters, 10000 outputs, rank 16: 11.6 us, 12.9 the other way); many rows: those of the same rows
-  // one after the other (512 rows of 8 adapters, rank 32: 22.8 us, 27.0).
+  // some 30 adapters, 10000 outputs, rank 16: 12.3 us, 16.0 the other way); many rows: those of the same rows
+  // one after the other (4096 rows of 8 adapters, rank 32: 106 us, 182; 512 rows 22.2, where the other way
+  // takes 19.6).
   const int apart = a.tiles_first ? (a.tiles + 7) / 8 * 8 : a.windows * a.slots;
   const int tile = a.tiles_first ? blockIdx.x % apart : blockIdx.x / apart;
   const int rows = a.tiles_first ? blockIdx.x / apart : blockIdx.x % apart;
@@ -752,7 +754,9 @@ __global__ __launch_bounds__(kThreads) void back_join_kernel(AdaptArgs a) {
 constexpr int kColumns = 128, kBatch = 128;
 template <int X, int RT, int PLANES>
 struct OuterShared {
-  static constexpr int kPitch = kBatch + 8;  // of a rank's rows, so that 16 ranks' are in different banks
+  // Of a rank's rows, so that neighbouring ranks' are in different banks.  Lanes read every RT-th rank: with RT 2
+  // two of them meet in a bank, with RT 4 four, and a float of four in `join` meets three others at any RT.
+  static constexpr int kPitch = kBatch + 8;
   static constexpr int kValues = PLANES ? PLANES * RT * kTile * kPitch / 2 : kBatch * (RT * kTile + 4);
   union {
     float values[kValues];
@@ -1039,7 +1043,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AdaptArgs a) {
   }
 }
 
-// Waves that a SIMD holds at once: what the sums of 16 RT ranks, and f32 operands, leave of its registers.
+// Waves that a SIMD holds at once: what the sums of 16 RT ranks, and f32 operands, leave of its registers.  With RT 4 they
+// leave too few: 28 bytes of scratch a lane in the gradient of up by f32 and f16 gradients, 36 to 180 in that of down
+// (bits 36, bf16 76, f16 156, f32 180); bf16 clause outputs take 12 at smaller RT too.
 constexpr int waves_of(int rt, int planes) { return planes ? (rt == 1 ? 4 : rt == 2 ? 3 : 2) : rt == 1 ? 3 : 2; }
 
 template <int G>
@@ -1184,7 +1190,7 @@ hipError_t launch_adapt(AdaptArgs a, int x_dtype, hipStream_t s) {
   }
   if (e != hipSuccess) return e;
   // A block takes so many times 256 outputs that there are about 1024 of them, or 2048 for many rows (4096 rows of 8
-  // adapters: 205 us, with 1024 230; 48 rows of some 30 adapters: 19.3 us, with 1024 18.8).
+  // adapters, rank 32: 106 us, with 1024 126; 48 rows of some 30 adapters, rank 16: 12.3 us, with 2048 13.3).
   a.tiles_first = a.windows < 16;
   const int64_t tiles = a.K > 0 ? (a.K + 255) / 256 : 1, blocks = (int64_t)a.windows * a.slots;
   const int64_t most = a.tiles_first ? 1024 : 2048, each = (tiles * blocks + most - 1) / most;

