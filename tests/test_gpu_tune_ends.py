@@ -39,6 +39,38 @@ def test_adapt_reads_no_weights_behind_a_row(N, K, r, w):
     np.testing.assert_array_equal(out[clean][:, 0::2], c.out[clean][:, 0::2])
 
 
+def among_nan(t, pad, offset):
+    """The same tensor with NaN between its rows and around it."""
+    *front, width = t.shape
+    rows = int(np.prod(front))
+    memory = torch.full((rows * (width + pad) + offset + 8,), float("nan"), dtype=t.dtype, device="cuda")
+    out = memory[offset:offset + rows * (width + pad)].view(*front, width + pad)[..., :width]
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("x,w,kind", [("bits", "f32", "f32"), ("f32", "f32", "bf16"), ("f16", "f16", "f16"),
+                                      ("bf16", "bf16", "bf16"), ("f32", "bf16", "f32")])
+@pytest.mark.parametrize("N,C,K,r,M,pad,offset", [(1, 7, 3, 1, 1, 1, 1), (33, 130, 64, 16, 3, 5, 3), (20, 259, 129, 48, 2, 3, 0),
+                                                  (300, 65, 192, 33, 9, 1, 7), (700, 128, 70, 112, 40, 8, 8),
+                                                  (260, 200, 100, 24, 1, 2, 5)])
+def test_what_lies_between_rows_is_not_used(N, C, K, r, M, pad, offset, x, w, kind):
+    c = Case(N, C, K, r, M, x, w)
+    rng = np.random.default_rng(3)
+    grad, h = rng.integers(-1, 2, (N, K)).astype(float), rng.integers(-2, 3, (N, r)).astype(float)
+    clauses = c.x if x == "bits" else among_nan(c.x, pad, offset)
+    down, up, scores = (among_nan(t, pad, offset) for t in (c.down, c.up, c.scores))
+    hidden = torch.empty(N, r, device="cuda")
+    out = tune.adapt(scores, clauses, down, up, c.which, c.scale, hidden=hidden)
+    np.testing.assert_array_equal(host(hidden), c.hidden)
+    np.testing.assert_array_equal(host(out), c.out)
+    wants, _ = c.gradients(grad, h)
+    got = tune.adapt_gradient(among_nan(gpu(grad, kind), pad, offset), clauses, down, up, c.which,
+                              among_nan(gpu(h), pad, offset), c.scale)
+    for t, want in zip(got, wants):
+        np.testing.assert_array_equal(host(t), host(torch.from_numpy(want).float().to(TYPES[w])))
+
+
 @pytest.fixture
 def other_defaults():
     torch.set_default_device("cuda")
