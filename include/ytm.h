@@ -376,11 +376,11 @@ int ytm_adapt_gradient_as(const void *grad, int dtype, int64_t stride, int64_t N
 
 /* Both losses take N rows (at most 65535) of V scores (8388608), F32, F16 or BF16, the answer tokens[n]
  * of each, and a temperature (NULL: 1; 0 or less counts as 1, less than the smallest normal float or NaN
- * as that, an infinite one as the largest float).  A score that is NaN counts as -inf, one of +inf as the largest float.  With p = softmax(score
- * / temperature) and lp = log p[tokens[n]], grad (F32, F16 or BF16; scores itself too, with elements of the
- * same size and rows of the same distance) becomes the gradient of the losses' sum by the scores.  A
- * row whose answer is outside 0..V-1 or has a score of -inf is left out: its lp and loss are 0, and so is
- * its gradient.
+ * as that, an infinite one as the largest float).  A score that is NaN counts as -inf, one of +inf as the
+ * largest float.  With p = softmax(score / temperature) and lp = log p[tokens[n]], grad (F32, F16 or BF16;
+ * scores itself too, with elements of the same size and rows of the same distance) becomes the gradient of the
+ * losses' sum by the scores.  A row whose answer is outside 0..V-1 or has a score of -inf is left out: its lp
+ * and loss are 0, and so is its gradient.
  *
  * ytm_policy_loss: with ratio = exp(lp - old[n]), d = reference[n] - lp,
  *   losses[n] = weights[n] * (kl * (exp(d) - d - 1)
@@ -395,7 +395,7 @@ int ytm_adapt_gradient_as(const void *grad, int dtype, int64_t stride, int64_t N
  * results are unspecified).  With l[s] the sum of its rows' lp, of pair p
  *   m = beta * ((l[2p] - reference[2p]) - (l[2p+1] - reference[2p+1]))
  *   losses[p] = ((1 - smoothing) * log(1 + exp(-m)) + smoothing * log(1 + exp(m))) / pairs
- * where 0 times an infinity is 0 (a reference of -inf).  logprobs[s] = l[s].  Rows of no sequence are left out.
+ * in which 0 times an infinity (from a reference of -inf) is 0.  logprobs[s] = l[s].  Rows of no sequence are left out.
  *
  * workspace: device memory of the _workspace's bytes at a multiple of 16 bytes, for the time of the
  * call's work (NULL where that is 0). */
@@ -424,9 +424,9 @@ int ytm_preference_loss(const void *scores, int dtype, int64_t stride, int64_t N
  * row (2^-98 or more; of roots 2^-54 or more but for zeros alone), m itself and v as its root.  What is stored
  * in fewer bits than f32 is rounded up or down at random, with the chances that keep the mean of parameters, of
  * m and of v, from `seed`, the step and the element's place (each tensor before it counts as a multiple of 256
- * long); a v above 0 stays above 0, what is not finite becomes NaN in 8 bits.  Operations are f32,
- * each rounded (of the rate and of k in f64, rounded once), but with bits 8 the quotient, which is within two
- * units in its last place.  The operands of different tensors must not overlap. */
+ * long); a v above 0 stays above 0, what is not finite becomes NaN in 8 bits.  Operations are f32, each rounded
+ * (of the rate and of k in f64, rounded once), but with bits 8 the quotient, which is within two units in its
+ * last place.  The operands of different tensors must not overlap. */
 typedef struct {
   void *parameter;
   const void *gradient;

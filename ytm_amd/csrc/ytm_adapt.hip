@@ -1043,9 +1043,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(AdaptArgs a) {
   }
 }
 
-// Waves that a SIMD holds at once: what the sums of 16 RT ranks, and f32 operands, leave of its registers.  With RT 4 they
-// leave too few: 28 bytes of scratch a lane in the gradient of up by f32 and f16 gradients, 36 to 180 in that of down
-// (bits 36, bf16 76, f16 156, f32 180); bf16 clause outputs take 12 at smaller RT too.
+// Waves that a SIMD holds at once: what the sums of 16 RT ranks, and f32 operands, leave of its registers.  With
+// RT 4 they leave too few: 28 bytes of scratch a lane in the gradient of up by f32 and f16 gradients, 36 to 180 in
+// that of down (bits 36, bf16 76, f16 156, f32 180); bf16 clause outputs take 12 at smaller RT too.
 constexpr int waves_of(int rt, int planes) { return planes ? (rt == 1 ? 4 : rt == 2 ? 3 : 2) : rt == 1 ? 3 : 2; }
 
 template <int G>

@@ -66,8 +66,8 @@ __device__ __forceinline__ float score_of(In v) {
 // 2^x, to one unit in its last place; what is less than the smallest normal float is 0.
 __device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 1 / temperature as choose() takes it: 0 or less counts as 1, less than the smallest normal float or NaN as that, and an
-// infinite one as the largest float, beside which a score of -inf stays -inf.
+// 1 / temperature as choose() takes it: 0 or less counts as 1, less than the smallest normal float or NaN as that,
+// and an infinite one as the largest float, beside which a score of -inf stays -inf.
 __device__ __forceinline__ float cooling(const LossArgs& a, int n) {
   if (!a.temperature) return 1.0f;
   const float t = a.temperature[n];
@@ -152,10 +152,10 @@ struct Part {
   __device__ __forceinline__ static bool has(int r, int first, int last) { return first + r * (int)blockDim.x * E < last; }
 
   // The sum is made relative to the largest of the thread's first few scores, or to 0, in one pass: each exponent is
-  // score * scale less a whole number near that score's, rounded once beside the rounding that all share in scale, and the
-  // power to that whole number comes as one more factor.  (Of all gradients of 64 rows of 10000 normal scores, times
-  // 3, the mean error is 6.9 units of 2^-24 and the largest 32; of differences to the maximum, powers and a quotient,
-  // each rounded, 9.0 and 48.)  Where that is not good enough (a NaN, an
+  // score * scale less a whole number near that score's, rounded once beside the rounding that all share in scale,
+  // and the power to that whole number comes as one more factor.  (Of all gradients of 64 rows of 10000 scores of
+  // deviation 3 the mean error is 6.9 units of 2^-24 and the largest 32; of differences to the maximum, powers and
+  // a quotient, each rounded, 9.0 and 48.)  Where that is not good enough (a NaN, an
   // infinity, scores far above, whose exponents have fewer bits of fraction, or all far below: a sum above 2^24 or
   // below 2^-24), relative to the largest.
   __device__ __forceinline__ Stats stats(int first, int last, float scale) {
